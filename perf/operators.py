@@ -7,8 +7,9 @@ A case is one call on one batch that is already on the GPU.  `path` names the ca
   norm_train    the same with its backward pass: y and the gradients of x, w and b
   linear        y = x8 w8^T + b from a quantised weight that the program keeps; x is quantised within the call
   norm_linear   the norm, its output quantised without being stored, and the product with a quantised weight
-  linear_train  from a weight in bf16 or f32, with its backward pass, all three products in e4m3: y and the gradients of
-                x, w and b
+  linear_train  from a weight in bf16, with its backward pass, all three products in e4m3: y and the gradients of x, w and b
+
+Products of e4m3 operands come out in bf16, whatever the type of the rows that were quantised.
 
 Quantisation.  Over a block, m = max |x| and e is the smallest integer, -127 at least, with m <= 448 * 2^e; the block
 holds x * 2^-e rounded to e4m3 and the byte e + 127.  Blocks are 1 x 128 along the axis that the product sums over, and
@@ -47,7 +48,7 @@ def listed():
       # Wan-1.3B at 480p: modulated norm and q|k|v projection
       dict(name="norm_linear_wan1.3b", path="norm_linear", batch=1, tokens=32760, channels=1536, outer=4608, x="bf16", w="f32", modulated=True),
       # a small head in training with sizes that nothing divides
-      dict(name="linear_odd_train", path="linear_train", batch=3, tokens=111, inner=1000, outer=333, x="bf16", w="f32"),
+      dict(name="linear_odd_train", path="linear_train", batch=3, tokens=111, inner=1000, outer=333, x="bf16", w="bf16"),
       # training one rank of Wan-14B: its q|k|v projection over a quarter of the tokens, the largest product
       dict(name="linear_wan14b_train", path="linear_train", batch=1, tokens=18900, inner=5120, outer=15360, x="bf16", w="bf16"),
   ]
@@ -79,7 +80,7 @@ def draw(rng):
     if "linear" in path:
       c["outer"] = _width(rng, 16, 30720)
     if path == "linear_train":
-      c["w"] = rng.choice(["bf16", "f32"])
+      c["x"] = "bf16"
     w = work(c)
     if c["batch"] * c["tokens"] <= 75600 and w["flops"] <= most and w["bytes"] <= 2.5e9:
       return c
@@ -151,17 +152,13 @@ def prepare(case, seed):
     values = v[:N].view(torch.uint8).contiguous()
     scales = torch.nn.functional.pad(byte, (0, -byte.shape[1] % 4)).contiguous()
     s.update(values=values, scales=scales, out_bias=normal(N, std=0.2, dtype=torch.bfloat16))
-    if own:
-      from maxdiffusion_amd import ops
-      s["w8"] = ops.BlockQuant(values, scales, N, C, 128)
   elif path == "linear_train":
     N = c["outer"]
     s.update(weight=normal(N, C, std=C**-0.5).to(wt), bias=normal(N, std=0.2).to(wt))
   if path.endswith("train"):
     s["dy"] = normal(B, T, c.get("outer", C), std=1e-3).to(xt)
-    if own:  # what a training program asks gradients of
-      for n in ("x", "weight", "bias"):
-        s[n].requires_grad_(True)
+    for n in ("x", "weight", "bias"):  # what a training program asks gradients of
+      s[n].requires_grad_(True)
   return s
 
 
@@ -172,14 +169,17 @@ def _offset(c):
 # ------------------------------------------------------------------------------------------------ one pass
 def _run_own(s):
   from maxdiffusion_amd import layer_op as L
+  from maxdiffusion_amd import ops
 
   c, path = s["case"], s["case"]["path"]
+  if "values" in s:
+    w8 = ops.BlockQuant(s["values"], s["scales"], c["outer"], c.get("channels", c.get("inner")), 128)
   if path == "linear":
     with torch.no_grad():
-      return L.hip_linear_fp8(s["x"], s["w8"], s["out_bias"])
+      return L.hip_linear_fp8(s["x"], w8, s["out_bias"])
   if path == "norm_linear":
     with torch.no_grad():
-      return L.hip_layer_norm_linear_fp8(s["x"], s["weight"], s["bias"], s["w8"], s["out_bias"], eps=EPS, weight_offset=_offset(c))
+      return L.hip_layer_norm_linear_fp8(s["x"], s["weight"], s["bias"], w8, s["out_bias"], eps=EPS, weight_offset=_offset(c))
   if path == "norm":
     with torch.no_grad():
       return L.hip_layer_norm(s["x"], s["weight"], s["bias"], eps=EPS, weight_offset=_offset(c))
@@ -203,6 +203,7 @@ def _plain_norm(x, weight, bias, offset):
   return h * (_rows(weight) + offset) + _rows(bias), h, r
 
 
+@torch.no_grad()
 def _run_plain(s):
   c, path = s["case"], s["case"]["path"]
   x = s["x"].float()
@@ -249,23 +250,16 @@ def _exact_blocks(x, block_rows):
   """x [R, C] in 64 bits as its blocks hold it: each block divided by its power of two, rounded to three bits behind the
   leading one (multiples of 2^-9 below 2^-6), half to even, and multiplied back."""
   R, C = x.shape
-  out = torch.empty_like(x)
-  step = max(block_rows, (1 << 26) // C // block_rows * block_rows)
-  for r in range(0, R, step):
-    part = x[r:r + step]
-    rows = part.shape[0]
-    t = torch.zeros((-(-rows // block_rows) * block_rows, -(-C // 128) * 128), dtype=torch.float64, device=x.device)
-    t[:rows, :C] = part
-    t = t.reshape(-1, block_rows, t.shape[1] // 128, 128)
-    m = t.abs().amax(dim=(1, 3), keepdim=True)
-    e = torch.ceil(torch.log2(m / 448)).clamp(min=-127)
-    e = torch.where(448 * torch.exp2(e - 1) >= m, e - 1, e)  # a logarithm that came out a little too high or low
-    e = torch.where(448 * torch.exp2(e) < m, e + 1, e).clamp(min=-127)
-    t = t / torch.exp2(e)
-    grid = torch.exp2(torch.floor(torch.log2(t.abs().clamp(min=2.0**-6))) - 3)
-    t = torch.round(t / grid) * grid * torch.exp2(e)
-    out[r:r + step] = t.reshape(-1, t.shape[2] * 128)[:rows, :C]
-  return out
+  t = torch.nn.functional.pad(x, (0, -C % 128, 0, -R % block_rows))
+  t = t.reshape(-1, block_rows, t.shape[1] // 128, 128)
+  m = t.abs().amax(dim=(1, 3), keepdim=True)
+  e = torch.ceil(torch.log2(m / 448)).clamp(min=-127)
+  e = torch.where(448 * torch.exp2(e - 1) >= m, e - 1, e)  # a logarithm that came out a little too high or low
+  e = torch.where(448 * torch.exp2(e) < m, e + 1, e).clamp(min=-127)
+  t = t / torch.exp2(e)
+  grid = torch.exp2(torch.floor(torch.log2(t.abs().clamp(min=2.0**-6))) - 3)
+  t = torch.round(t / grid) * grid * torch.exp2(e)
+  return t.reshape(-1, t.shape[2] * 128)[:R, :C]
 
 
 def exact(case, seed):
