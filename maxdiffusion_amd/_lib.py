@@ -1,4 +1,4 @@
-"""ctypes binding of libmdattn.so (the C ABI declared in include/mdattn.h).
+"""ctypes binding of libmdattn.so (the C ABI declared in include/mdattn.h and include/mdlayers.h).
 
 There is no fallback: when the library is missing or a call fails this module raises.
 """
@@ -59,6 +59,18 @@ SIGNATURES = {
     "mdattn_finalize": ([_P, _P, _P, _L], _I),
 }
 
+# symbol -> argtypes; every symbol include/mdlayers.h declares
+LAYER_SIGNATURES = {
+    "mdattn_layer_norm": ([_P, _P, _I, _P, _I, _P, _P, _I, _L, _L, _I, _L, _L, _L, _L, _L, _F, _F], _I),
+    "mdattn_layer_norm_e4m3": ([_P, _P, _I, _P, _P, _P, _P, _I, _L, _L, _I, _L, _L, _L, _F, _F], _I),
+    "mdattn_layer_norm_bwd_workspace_floats": ([_L, _L, _I], _L),
+    "mdattn_layer_norm_bwd": ([_P, _P, _I, _P, _P, _P, _P, _P, _I, _L, _L, _I, _L, _L, _L, _L, _L, _L, _L, _F, _F, _P, _L], _I),
+    "mdattn_quant_block_e4m3": ([_P, _P, _I, _L, _L, _L, _I, _P, _P, _P, _P, _P], _I),
+    "mdattn_sum_rows": ([_P, _P, _L, _L, _P, _I], _I),
+    "mdattn_matmul_fp8_block_workspace_floats": ([_L, _L, _L], _L),
+    "mdattn_matmul_fp8_block": ([_P, _P, _P, _P, _P, _I, _P, _I, _P, _L, _L, _L, _L, _P, _L], _I),
+}
+
 # what csrc/mdattn_host.h declares: entry points for this package's own host side
 HOST_SIGNATURES = {
     "mdattn_bwd_split_workspace_floats": ([_I, _I, _I, _I, _I], _L),
@@ -84,7 +96,7 @@ def load() -> ctypes.CDLL:
           f"{LIB_PATH} is missing: build it with `python -m maxdiffusion_amd.build` "
           "(there is no non-HIP fallback for this path)")
     lib = ctypes.CDLL(LIB_PATH)
-    for name, (argtypes, restype) in {**SIGNATURES, **HOST_SIGNATURES}.items():
+    for name, (argtypes, restype) in {**SIGNATURES, **LAYER_SIGNATURES, **HOST_SIGNATURES}.items():
       fn = getattr(lib, name)
       fn.argtypes = argtypes
       fn.restype = restype

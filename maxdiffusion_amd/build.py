@@ -18,7 +18,8 @@ FFI_LIB_PATH = os.path.join(PKG_DIR, "libmdattn_ffi.so")
 HOST_EXT_NAME = "_mdattn_torch"
 HOST_EXT_PATH = os.path.join(PKG_DIR, HOST_EXT_NAME + ".so")  # the torch-side host path in C++ (csrc/host/torch_host.cc)
 
-SOURCES = ["mdattn_api.hip", "norm_rope.hip", "norm_rope_bwd.hip", "attn_fwd_bf16.hip", "attn_fwd_fp8.hip", "attn_bwd_bf16.hip", "merge_quant.hip", "probes.hip",
+SOURCES = ["mdattn_api.hip", "norm_rope.hip", "norm_rope_bwd.hip", "attn_fwd_bf16.hip", "attn_fwd_fp8.hip", "attn_bwd_bf16.hip", "merge_quant.hip", "layer_norm.hip", "quant_block.hip",
+           "matmul_fp8.hip", "probes.hip",
            # the bodies of the XLA custom-call handlers on plain structs (no XLA header): part of the library
            os.path.join("ffi", "mdattn_marshal.cc")]
 
@@ -94,7 +95,7 @@ def source_id() -> str:
 
   h = hashlib.sha256(" ".join(HIPCC_FLAGS).encode())
   files = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".hip", ".h"))]
-  for path in files + [os.path.join(CSRC, "ffi", "mdattn_marshal.cc"), os.path.join(CSRC, "host", "torch_host.cc"), os.path.join(INCLUDE, "mdattn.h"), os.path.join(INCLUDE, "mdattn_marshal.h")]:
+  for path in files + [os.path.join(CSRC, "ffi", "mdattn_marshal.cc"), os.path.join(CSRC, "host", "torch_host.cc"), os.path.join(INCLUDE, "mdattn.h"), os.path.join(INCLUDE, "mdlayers.h"), os.path.join(INCLUDE, "mdattn_marshal.h")]:
     h.update(os.path.basename(path).encode())
     with open(path, "rb") as f:
       h.update(f.read())

@@ -1,0 +1,502 @@
+// Layer norm (plain, affine, modulated per batch element) with its backward pass, and with its output quantised to e4m3.
+//
+//   mean = sum x / C,  var = sum (x - mean)^2 / C,  r = (var + eps)^-1/2,  h = (x - mean) r,  y = h (o + w) + b
+//   a = g (o + w),  dx = r (a - mean a - h mean(a h)),  dw = sum over rows g h,  db = sum over rows g
+//
+// One pass over the data: a workgroup owns whole rows, a thread the same few chunks of 8 channels in each of its rows, so that w, b and
+// the sums of dw and db stay in its registers while the rows pass by, the next row already on its way.  A wave makes the mean of
+// its own part and the squares around that mean; the parts join as  M2 = sum M2_w + n_w (mean_w - mean)^2  (Chan et al., Updating
+// formulae and a pairwise algorithm for computing sample variances, 1979), which loses nothing where the mean is large against the
+// deviation, and takes one exchange through LDS, and one barrier, per row.
+#include "mdattn_common.h"
+#include "mdlayers.h"
+#include "quant_block.h"
+
+namespace mdattn {
+namespace {
+
+constexpr int kMaxWaves = 16;
+
+__device__ __forceinline__ float wave_sum(float x) {
+  x = row16_sum(x);
+  const u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return xhalf_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// eight channels of a row as they are loaded
+template <typename T>
+struct Chunk;
+template <>
+struct Chunk<__bf16> {
+  u32x4 u;
+  __device__ __forceinline__ void load(const __bf16* p) { u = *reinterpret_cast<const u32x4_any*>(p); }
+  __device__ __forceinline__ void load_some(const __bf16* p, int n) {
+    unsigned short e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = i < n ? reinterpret_cast<const unsigned short*>(p)[i] : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = e[2 * i] | (unsigned)e[2 * i + 1] << 16;
+  }
+  __device__ __forceinline__ void zero() { u = u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(u[i] << 16);
+      f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+  }
+};
+template <>
+struct Chunk<float> {
+  f32x4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const f32x4_any*>(p);
+    b = *reinterpret_cast<const f32x4_any*>(p + 4);
+  }
+  __device__ __forceinline__ void load_some(const float* p, int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = i < n ? p[i] : 0.f;
+      b[i] = i + 4 < n ? p[i + 4] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void zero() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[i] = a[i]; f[i + 4] = b[i]; }
+  }
+};
+
+__device__ __forceinline__ void store8(__bf16* p, const float* f) {
+  const uint4 u = pack8(f);
+  *reinterpret_cast<u32x4_any*>(p) = u32x4{u.x, u.y, u.z, u.w};
+}
+__device__ __forceinline__ void store8(float* p, const float* f) {
+  *reinterpret_cast<f32x4_any*>(p) = f32x4{f[0], f[1], f[2], f[3]};
+  *reinterpret_cast<f32x4_any*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
+}
+
+// A row of C channels dealt to the threads of a workgroup: slot j of a thread is chunk j * blockDim.x + threadIdx.x.  TAIL: C is
+// not a multiple of 8, and the last chunk is walked by elements.
+template <int NV, bool TAIL>
+struct Deal {
+  int c[NV];  // first channel of each slot
+  int C;
+  __device__ __forceinline__ explicit Deal(int C_) : C(C_) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) c[j] = (j * (int)blockDim.x + (int)threadIdx.x) * 8;
+  }
+  __device__ __forceinline__ bool has(int j) const { return c[j] < C; }
+  __device__ __forceinline__ bool has(int j, int e) const { return TAIL ? c[j] + e < C : c[j] < C; }
+  template <typename T>
+  __device__ __forceinline__ void load(Chunk<T> (&x)[NV], const T* row) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (TAIL ? c[j] + 8 <= C : c[j] < C) x[j].load(row + c[j]);
+      else if (TAIL && c[j] < C) x[j].load_some(row + c[j], C - c[j]);
+      else x[j].zero();
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(int j, T* row, const float* f) const {
+    if (TAIL ? c[j] + 8 <= C : c[j] < C) {
+      store8(row + c[j], f);
+    } else if (TAIL && c[j] < C) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c[j] + e < C) row[c[j] + e] = (T)f[e];
+    }
+  }
+  // w or b of one group as f32; `none` where there is none or no channel
+  __device__ __forceinline__ void vector(float (&v)[NV][8], const void* p, int is_f32, int64_t at, float none) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[j][e] = none;
+      if (p == nullptr) continue;
+      if (is_f32) {
+        Chunk<float> x[NV];
+        load(x, static_cast<const float*>(p) + at);
+        x[j].get(v[j]);
+      } else {
+        Chunk<__bf16> x[NV];
+        load(x, static_cast<const __bf16*>(p) + at);
+        x[j].get(v[j]);
+      }
+    }
+  }
+  // channels that the slots of wave `w` hold
+  __device__ __forceinline__ float count(int w) const {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) n += min(max(C - (j * (int)blockDim.x + w * 64) * 8, 0), 512);
+    return (float)n;
+  }
+};
+
+struct NormArgs {
+  const void* x;
+  void* y;
+  const void *w, *b;
+  uint8_t* scales;
+  int64_t rows, wb_stride;                // rows of a group
+  int64_t x_sg, x_sr, y_sg, y_sr;
+  int64_t scale_stride;
+  int C, wb_f32, blocks, rows_per_block;  // workgroups of a group, and the rows of each
+  float eps, offset;
+};
+
+enum { kToBf16 = 0, kToF32 = 1, kToE4m3 = 2 };
+
+template <typename T, int OUT, int NV, bool TAIL>
+__global__ __launch_bounds__(1024) void layer_norm_kernel(NormArgs a) {
+  __shared__ float2 part[2][kMaxWaves];
+  const int group = blockIdx.x / a.blocks, block = blockIdx.x - group * a.blocks;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const Deal<NV, TAIL> deal(a.C);
+  const int64_t first = (int64_t)block * a.rows_per_block, last = min(first + a.rows_per_block, a.rows);
+  const T* x = static_cast<const T*>(a.x) + group * a.x_sg;
+  Chunk<T> now[NV], next[NV];
+  deal.load(next, x + first * a.x_sr);
+  float w[NV][8], b[NV][8];
+  deal.vector(w, a.w, a.wb_f32, group * a.wb_stride, 1.f - a.offset);
+  deal.vector(b, a.b, a.wb_f32, group * a.wb_stride, 0.f);
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[j][e] += a.offset;
+  const float inv_c = 1.f / a.C, n_wave = deal.count(wave);
+  const float inv_n = n_wave > 0.f ? 1.f / n_wave : 0.f;
+
+  for (int64_t row = first; row < last; ++row) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) now[j] = next[j];
+    if (row + 1 < last) deal.load(next, x + (row + 1) * a.x_sr);
+    float f[NV][8], sum = 0.f, sq = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      now[j].get(f[j]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += f[j][e];
+    }
+    float mean = wave_sum(sum) * inv_n;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = deal.has(j, e) ? f[j][e] - mean : 0.f;
+        sq += d * d;
+      }
+    float m2 = wave_sum(sq);
+    if (waves > 1) {
+      float2* slot = part[(row - first) & 1];  // the other slot is read until the next barrier
+      if ((threadIdx.x & 63) == 0) slot[wave] = make_float2(mean, m2);
+      __syncthreads();
+      float all = 0.f;
+      for (int i = 0; i < waves; ++i) all += slot[i].x * deal.count(i);
+      all *= inv_c;
+      m2 = 0.f;
+      for (int i = 0; i < waves; ++i) {
+        const float d = slot[i].x - all;
+        m2 += slot[i].y + deal.count(i) * d * d;
+      }
+      mean = all;
+    }
+    const float r = rsqrtf(m2 * inv_c + a.eps);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[j][e] = (f[j][e] - mean) * r * w[j][e] + b[j][e];
+      if constexpr (OUT == kToE4m3) {
+        unsigned m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (!deal.has(j, e)) f[j][e] = 0.f;
+          m = max(m, __float_as_uint(f[j][e]) & 0x7FFFFFFFu);
+        }
+        const unsigned byte = scale_byte(row16_umax(m));  // 16 lanes hold a block of 128
+        const int64_t at = group * a.rows + row, ld = (a.C + 127) / 128 * 128;
+        if (deal.c[j] < ld) {
+          *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.y) + at * ld + deal.c[j]) = to_e4m3x8(f[j], scale_inverse(byte), byte);
+          if ((threadIdx.x & 15) == 0) a.scales[at * a.scale_stride + deal.c[j] / 128] = (uint8_t)byte;
+        }
+      } else if constexpr (OUT == kToF32) {
+        deal.store(j, static_cast<float*>(a.y) + group * a.y_sg + row * a.y_sr, f[j]);
+      } else {
+        deal.store(j, static_cast<__bf16*>(a.y) + group * a.y_sg + row * a.y_sr, f[j]);
+      }
+    }
+  }
+}
+
+struct NormBwdArgs {
+  const void *x, *g, *w;
+  void* dx;
+  float* part;  // [workgroup][2][C]: its rows' dw and db; null: neither is wanted
+  int64_t rows, wb_stride;
+  int64_t x_sg, x_sr, g_sg, g_sr, d_sg, d_sr;
+  int C, wb_f32, blocks, rows_per_block;
+  float eps, offset;
+};
+
+template <typename T, int NV, bool TAIL>
+__global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(NormBwdArgs a) {
+  __shared__ float4 part[2][kMaxWaves];
+  const int group = blockIdx.x / a.blocks, block = blockIdx.x - group * a.blocks;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const Deal<NV, TAIL> deal(a.C);
+  const int64_t first = (int64_t)block * a.rows_per_block, last = min(first + a.rows_per_block, a.rows);
+  const T* x = static_cast<const T*>(a.x) + group * a.x_sg;
+  const T* g = static_cast<const T*>(a.g) + group * a.g_sg;
+  T* dx = static_cast<T*>(a.dx) + group * a.d_sg;
+  Chunk<T> xn[NV], gn[NV];
+  if (first < last) {
+    deal.load(xn, x + first * a.x_sr);
+    deal.load(gn, g + first * a.g_sr);
+  }
+  float w[NV][8], dw[NV][8], db[NV][8];
+  deal.vector(w, a.w, a.wb_f32, group * a.wb_stride, 1.f - a.offset);
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[j][e] += a.offset;
+      dw[j][e] = db[j][e] = 0.f;
+    }
+  const float inv_c = 1.f / a.C, n_wave = deal.count(wave);
+  const float inv_n = n_wave > 0.f ? 1.f / n_wave : 0.f;
+
+  for (int64_t row = first; row < last; ++row) {
+    float f[NV][8], q[NV][8], sum = 0.f, sq = 0.f, sa = 0.f, sad = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      xn[j].get(f[j]);
+      gn[j].get(q[j]);
+    }
+    if (row + 1 < last) {
+      deal.load(xn, x + (row + 1) * a.x_sr);
+      deal.load(gn, g + (row + 1) * a.g_sr);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sum += f[j][e];
+        sa += q[j][e] * w[j][e];  // (g is 0 where there is no channel)
+      }
+    float mean = wave_sum(sum) * inv_n;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = deal.has(j, e) ? f[j][e] - mean : 0.f;
+        sq += d * d;
+        sad += q[j][e] * w[j][e] * d;
+      }
+    float m2 = wave_sum(sq);
+    sa = wave_sum(sa);
+    sad = wave_sum(sad);
+    if (waves > 1) {
+      float4* slot = part[(row - first) & 1];
+      if ((threadIdx.x & 63) == 0) slot[wave] = make_float4(mean, m2, sa, sad);
+      __syncthreads();
+      float all = 0.f;
+      for (int i = 0; i < waves; ++i) all += slot[i].x * deal.count(i);
+      all *= inv_c;
+      m2 = sa = sad = 0.f;
+      for (int i = 0; i < waves; ++i) {
+        const float4 p = slot[i];
+        const float d = p.x - all;
+        m2 += p.y + deal.count(i) * d * d;
+        sa += p.z;
+        sad += p.w + p.z * d;  // the sum of a (x - mean) around the common mean
+      }
+      mean = all;
+    }
+    const float r = rsqrtf(m2 * inv_c + a.eps);
+    const float c1 = sa * inv_c, c2 = sad * inv_c * r;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float h = (f[j][e] - mean) * r;
+        dw[j][e] += q[j][e] * h;
+        db[j][e] += q[j][e];
+        o[e] = r * (q[j][e] * w[j][e] - c1 - h * c2);
+      }
+      deal.store(j, dx + row * a.d_sr, o);
+    }
+  }
+  if (a.part) {
+    float* p = a.part + (int64_t)blockIdx.x * 2 * a.C;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      deal.store(j, p, dw[j]);
+      deal.store(j, p + a.C, db[j]);
+    }
+  }
+}
+
+// out[g][c] = sum over i < n of part[g * n + i][plane][c], plane 0 to dw, 1 to db.  32 columns per workgroup, 32 partial sums each.
+struct SumArgs {
+  const float* part;
+  void *out0, *out1;
+  int64_t n, row_stride, plane_stride;
+  int64_t C;
+  int f32;
+};
+__global__ __launch_bounds__(1024) void sum_rows_kernel(SumArgs a) {
+  __shared__ float part[32][33];
+  const int lane = threadIdx.x & 31, i0 = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  void* out = blockIdx.y ? a.out1 : a.out0;
+  if (out == nullptr) return;
+  const float* p = a.part + blockIdx.z * a.n * a.row_stride + blockIdx.y * a.plane_stride + c;
+  float s = 0.f;
+  if (c < a.C)
+    for (int64_t i = i0; i < a.n; i += 32) s += p[i * a.row_stride];
+  part[i0][lane] = s;
+  __syncthreads();
+  if (i0 == 0 && c < a.C) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += part[i][lane];
+    const int64_t at = blockIdx.z * a.C + c;
+    if (a.f32) static_cast<float*>(out)[at] = s;
+    else static_cast<__bf16*>(out)[at] = (__bf16)s;
+  }
+}
+
+constexpr int kMaxC = 16384;
+// How a row is dealt: chunks per thread and threads.
+struct Shape {
+  int nv, threads;
+};
+Shape shape_of(int C) {
+  const int chunks = (C + 7) / 8;
+  return chunks <= 64 ? Shape{1, 64} : Shape{2, (chunks + 127) / 128 * 64};
+}
+// Workgroups of one group, and the rows of each
+void split_rows(int64_t groups, int64_t rows, int64_t target, int* blocks, int* rows_per_block) {
+  int64_t per = (groups * rows + target - 1) / target;
+  if (per > rows) per = rows;
+  *rows_per_block = (int)per;
+  *blocks = (int)((rows + per - 1) / per);
+}
+int64_t fwd_target(const Shape& s) { return 256 * (1536 / s.threads); }
+int64_t bwd_target(const Shape& s) { return 256 * (768 / s.threads > 0 ? 768 / s.threads : 1); }
+
+bool sizes_ok(int64_t groups, int64_t rows, int C) {
+  return groups > 0 && rows > 0 && C > 0 && rows < ((int64_t)1 << 40) / groups;
+}
+bool elem_aligned(const void* p, int is_f32) { return (reinterpret_cast<uintptr_t>(p) & (is_f32 ? 3u : 1u)) == 0; }
+
+template <typename T, int OUT>
+int launch_norm(hipStream_t st, const NormArgs& a, const Shape& s, unsigned grid) {
+#define MDATTN_NORM(NV)                                                                                              \
+  if (s.nv == NV) {                                                                                                  \
+    if (a.C % 8) MDATTN_LAUNCH((layer_norm_kernel<T, OUT, NV, true>), dim3(grid), dim3(s.threads), 0, st, a);      \
+    else MDATTN_LAUNCH((layer_norm_kernel<T, OUT, NV, false>), dim3(grid), dim3(s.threads), 0, st, a);             \
+  }
+  MDATTN_NORM(1) MDATTN_NORM(2)
+#undef MDATTN_NORM
+  return launch_status();
+}
+
+int norm(hipStream_t st, NormArgs& a, int x_is_f32, int out, int64_t groups) {
+  const Shape s = shape_of(a.C);
+  split_rows(groups, a.rows, fwd_target(s), &a.blocks, &a.rows_per_block);
+  const int64_t grid = groups * a.blocks;
+  if (grid > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
+  if (x_is_f32) {
+    if (out == kToE4m3) return launch_norm<float, kToE4m3>(st, a, s, (unsigned)grid);
+    return out == kToF32 ? launch_norm<float, kToF32>(st, a, s, (unsigned)grid) : launch_norm<float, kToBf16>(st, a, s, (unsigned)grid);
+  }
+  if (out == kToE4m3) return launch_norm<__bf16, kToE4m3>(st, a, s, (unsigned)grid);
+  return out == kToF32 ? launch_norm<__bf16, kToF32>(st, a, s, (unsigned)grid) : launch_norm<__bf16, kToBf16>(st, a, s, (unsigned)grid);
+}
+
+}  // namespace
+}  // namespace mdattn
+
+using namespace mdattn;
+
+extern "C" int mdattn_layer_norm(void* stream, const void* x, int x_is_f32, void* y, int y_is_f32, const void* w, const void* b, int wb_is_f32,
+                                 int64_t groups, int64_t rows, int C, int64_t x_stride_group, int64_t x_stride_row, int64_t y_stride_group,
+                                 int64_t y_stride_row, int64_t wb_stride, float eps, float w_offset) {
+  if (!x || !y || !sizes_ok(groups, rows, C) || !(eps >= 0.f) || !(w_offset == w_offset)) return MDATTN_E_BADARG;
+  if (C > kMaxC) return MDATTN_E_UNSUPPORTED;
+  if (!elem_aligned(x, x_is_f32) || !elem_aligned(y, y_is_f32) || !elem_aligned(w, wb_is_f32) || !elem_aligned(b, wb_is_f32)) return MDATTN_E_ALIGN;
+  NormArgs a{};
+  a.x = x; a.y = y; a.w = w; a.b = b;
+  a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w_offset;
+  a.x_sg = x_stride_group; a.x_sr = x_stride_row; a.y_sg = y_stride_group; a.y_sr = y_stride_row;
+  return norm((hipStream_t)stream, a, x_is_f32, y_is_f32 ? kToF32 : kToBf16, groups);
+}
+
+extern "C" int mdattn_layer_norm_e4m3(void* stream, const void* x, int x_is_f32, void* q, void* scales, const void* w, const void* b, int wb_is_f32,
+                                      int64_t groups, int64_t rows, int C, int64_t x_stride_group, int64_t x_stride_row, int64_t wb_stride,
+                                      float eps, float w_offset) {
+  if (!x || !q || !scales || !sizes_ok(groups, rows, C) || !(eps >= 0.f) || !(w_offset == w_offset)) return MDATTN_E_BADARG;
+  if (C > kMaxC) return MDATTN_E_UNSUPPORTED;
+  if (!elem_aligned(x, x_is_f32) || !aligned16(q) || !elem_aligned(w, wb_is_f32) || !elem_aligned(b, wb_is_f32)) return MDATTN_E_ALIGN;
+  NormArgs a{};
+  a.x = x; a.y = q; a.scales = static_cast<uint8_t*>(scales); a.w = w; a.b = b;
+  a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w_offset;
+  a.x_sg = x_stride_group; a.x_sr = x_stride_row; a.scale_stride = scale_stride(C);
+  return norm((hipStream_t)stream, a, x_is_f32, kToE4m3, groups);
+}
+
+extern "C" int64_t mdattn_layer_norm_bwd_workspace_floats(int64_t groups, int64_t rows, int C) {
+  if (!sizes_ok(groups, rows, C) || C > kMaxC) return 0;
+  int blocks, per;
+  split_rows(groups, rows, bwd_target(shape_of(C)), &blocks, &per);
+  return groups * blocks * 2 * C;
+}
+
+extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, const void* g, void* dx, const void* w, void* dw, void* db,
+                                     int wb_is_f32, int64_t groups, int64_t rows, int C, int64_t x_stride_group, int64_t x_stride_row,
+                                     int64_t g_stride_group, int64_t g_stride_row, int64_t dx_stride_group, int64_t dx_stride_row,
+                                     int64_t wb_stride, float eps, float w_offset, float* workspace, int64_t workspace_floats) {
+  if (!x || !g || !dx || !sizes_ok(groups, rows, C) || !(eps >= 0.f) || !(w_offset == w_offset) || (dw && !w)) return MDATTN_E_BADARG;
+  if (C > kMaxC) return MDATTN_E_UNSUPPORTED;
+  const bool sums = dw || db;
+  if (sums && (!workspace || workspace_floats < mdattn_layer_norm_bwd_workspace_floats(groups, rows, C))) return MDATTN_E_BADARG;
+  if (!elem_aligned(x, x_is_f32) || !elem_aligned(g, x_is_f32) || !elem_aligned(dx, x_is_f32) || !elem_aligned(w, wb_is_f32) ||
+      !elem_aligned(dw, wb_is_f32) || !elem_aligned(db, wb_is_f32) || !elem_aligned(workspace, 1))
+    return MDATTN_E_ALIGN;
+  const Shape s = shape_of(C);
+  NormBwdArgs a{};
+  a.x = x; a.g = g; a.w = w; a.dx = dx; a.part = sums ? workspace : nullptr;
+  a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w_offset;
+  a.x_sg = x_stride_group; a.x_sr = x_stride_row; a.g_sg = g_stride_group; a.g_sr = g_stride_row; a.d_sg = dx_stride_group; a.d_sr = dx_stride_row;
+  split_rows(groups, rows, bwd_target(s), &a.blocks, &a.rows_per_block);
+  const int64_t grid = groups * a.blocks;
+  if (grid > 0x7FFFFFFF || groups > 65535) return MDATTN_E_UNSUPPORTED;
+  hipStream_t st = (hipStream_t)stream;
+#define MDATTN_NORM(T, NV)                                                                                                    \
+  if (s.nv == NV) {                                                                                                           \
+    if (C % 8) MDATTN_LAUNCH((layer_norm_bwd_kernel<T, NV, true>), dim3((unsigned)grid), dim3(s.threads), 0, st, a);        \
+    else MDATTN_LAUNCH((layer_norm_bwd_kernel<T, NV, false>), dim3((unsigned)grid), dim3(s.threads), 0, st, a);             \
+  }
+  if (x_is_f32) { MDATTN_NORM(float, 1) MDATTN_NORM(float, 2) }
+  else { MDATTN_NORM(__bf16, 1) MDATTN_NORM(__bf16, 2) }
+#undef MDATTN_NORM
+  const int rc = launch_status();
+  if (rc != MDATTN_OK || !sums) return rc;
+  // shared w and b: one sum over the workgroups of all groups
+  const int64_t out_groups = wb_stride ? groups : 1;
+  const SumArgs r{workspace, dw, db, wb_stride ? a.blocks : grid, 2 * (int64_t)C, C, C, wb_is_f32};
+  MDATTN_LAUNCH(sum_rows_kernel, dim3((C + 31) / 32, 2, (unsigned)out_groups), dim3(1024), 0, st, r);
+  return launch_status();
+}
+
+extern "C" int mdattn_sum_rows(void* stream, const float* rows, int64_t n, int64_t C, void* out, int out_is_f32) {
+  if (!rows || !out || n <= 0 || C <= 0) return MDATTN_E_BADARG;
+  if ((C + 31) / 32 > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
+  if (!elem_aligned(rows, 1) || !elem_aligned(out, out_is_f32)) return MDATTN_E_ALIGN;
+  const SumArgs r{rows, out, nullptr, n, C, 0, C, out_is_f32};
+  MDATTN_LAUNCH(sum_rows_kernel, dim3((unsigned)((C + 31) / 32)), dim3(1024), 0, (hipStream_t)stream, r);
+  return launch_status();
+}

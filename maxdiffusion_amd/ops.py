@@ -18,6 +18,7 @@ from ._lib import Strides
 __all__ = [
     "norm_rope_fullrow", "norm_rope_qkv", "norm_rope_perhead", "norm_rope_rows",
     "norm_rope_fullrow_backward", "norm_rope_perhead_backward", "norm_rope_rows_backward", "flash_attention", "flash_attention_backward", "flash_attention_backward_static", "flash_attention_fp8", "quant_e4m3", "key_mask_bias",
+    "layer_norm", "layer_norm_quant", "layer_norm_backward", "BlockQuant", "quant_block_e4m3", "sum_rows", "matmul_fp8_block",
     "merge_partial", "flash_attention_merge", "finalize", "new_merge_state", "LSE_INIT", "FOLDED_SCALE", "folded_q_mul", "set_fwd_schedule", "FWD_SCHEDULES", "FP8_SOFTMAX_MODES",
 ]
 
@@ -585,4 +586,197 @@ def finalize(o_run: torch.Tensor) -> torch.Tensor:
     raise ValueError("finalize needs a dense tensor")
   rc = _lib.load().mdattn_finalize(_stream(), _ptr(o_run), _ptr(out), o_run.numel())
   _lib.check(rc, "mdattn_finalize")
+  return out
+
+
+# ------------------------------------------------------------------------------------------------ the layers beside attention
+def _float_kind(t, name):
+  """1 for f32, 0 for bf16."""
+  if t.dtype not in (torch.bfloat16, torch.float32):
+    raise ValueError(f"{name} must be bf16 or f32, got {t.dtype}")
+  return int(t.dtype == torch.float32)
+
+
+def _norm_rows(x, name="x"):
+  """(groups, rows of a group, C, stride of a group, stride of a row) of x [..., C]: the first axis and the ones between."""
+  if x.dim() < 2 or (x.stride(-1) != 1 and x.shape[-1] > 1):
+    raise ValueError(f"{name} must have shape [..., C] with a contiguous last axis, got {tuple(x.shape)} strides {x.stride()}")
+  if x.dim() == 2:
+    return 1, x.shape[0], x.shape[1], 0, x.stride(0)
+  if x.dim() == 3:
+    return x.shape[0], x.shape[1], x.shape[2], x.stride(0), x.stride(1)
+  for i in range(1, x.dim() - 2):
+    if x.stride(i) != x.stride(i + 1) * x.shape[i + 1]:
+      raise ValueError(f"the axes of {name} between the first and the last must be dense, got {tuple(x.shape)} strides {x.stride()}")
+  return x.shape[0], math.prod(x.shape[1:-1]), x.shape[-1], x.stride(0), x.stride(-2)
+
+
+def _norm_vectors(weight, bias, groups, c):
+  """(elements between the groups' vectors, is f32) of weight and bias, each [C], [B, C], [B, 1, C] or None."""
+  stride, f32 = None, 0
+  for name, t in (("weight", weight), ("bias", bias)):
+    if t is None:
+      continue
+    shape = tuple(t.shape)
+    if t.dim() == 3 and shape[1] == 1:
+      shape = (shape[0], shape[2])
+    if shape not in ((c,), (groups, c)) or not t.is_contiguous():
+      raise ValueError(f"{name} must be a contiguous tensor of shape [{c}], [{groups}, {c}] or [{groups}, 1, {c}], got {tuple(t.shape)} strides {t.stride()}")
+    mine = c if len(shape) == 2 else 0
+    if stride is None:
+      stride, f32 = mine, _float_kind(t, name)
+    elif stride != mine or f32 != _float_kind(t, name):
+      raise ValueError("weight and bias must agree in dtype, and in whether they are per batch element")
+  return stride or 0, f32
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-6, weight_offset: float = 0.0, out_dtype=None):
+  """h * (weight_offset + weight) + bias with h = (x - mean) / sqrt(var + eps) over the last axis of x [..., C], bf16 or f32.
+
+  weight, bias: bf16 or f32, [C], or one per element of x's first axis, [B, C] or [B, 1, C] (adaLN's scale and shift, with
+  weight_offset 1); None: h (+ bias), h * (weight_offset + weight).  Statistics and arithmetic in f32, rounded once to out_dtype (x's)."""
+  _check_dev(x, weight, bias)
+  x_f32 = _float_kind(x, "x")
+  groups, rows, c, sg, sr = _norm_rows(x)
+  stride, wb_f32 = _norm_vectors(weight, bias, groups, c)
+  out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+  y_f32 = _float_kind(out, "out_dtype")
+  if out.numel():
+    rc = _lib.load().mdattn_layer_norm(_stream(), _ptr(x), x_f32, _ptr(out), y_f32, _ptr(weight), _ptr(bias), wb_f32, groups, rows, c, sg, sr,
+                                       rows * c, c, stride, float(eps), float(weight_offset))
+    _lib.check(rc, "mdattn_layer_norm")
+  return out
+
+
+def layer_norm_quant(x, weight=None, bias=None, eps: float = 1e-6, weight_offset: float = 0.0):
+  """`layer_norm` with its unrounded rows quantised (`quant_block_e4m3`, blocks of 1 x 128) instead of stored: a BlockQuant of
+  as many rows as x [..., C] has."""
+  _check_dev(x, weight, bias)
+  x_f32 = _float_kind(x, "x")
+  groups, rows, c, sg, sr = _norm_rows(x)
+  stride, wb_f32 = _norm_vectors(weight, bias, groups, c)
+  out = _new_quant(groups * rows, c, 1, x.device)
+  if x.numel():
+    rc = _lib.load().mdattn_layer_norm_e4m3(_stream(), _ptr(x), x_f32, _ptr(out.values), _ptr(out.scales), _ptr(weight), _ptr(bias), wb_f32, groups,
+                                            rows, c, sg, sr, stride, float(eps), float(weight_offset))
+    _lib.check(rc, "mdattn_layer_norm_e4m3")
+  return out
+
+
+def layer_norm_backward(x, weight, bias, g, eps: float = 1e-6, weight_offset: float = 0.0, needs_vectors: bool = True):
+  """Backward of `layer_norm`: x, weight, bias as the forward had them (of bias only whether there is one, its shape and dtype),
+  g the gradient of its output, in x's dtype.  Returns (dx, dweight, dbias) in their tensors' shapes and dtypes, None for what
+  there is not, or for the last two with needs_vectors False."""
+  _check_dev(x, weight, bias, g)
+  x_f32 = _float_kind(x, "x")
+  groups, rows, c, sg, sr = _norm_rows(x)
+  stride, wb_f32 = _norm_vectors(weight, bias, groups, c)
+  if g.shape != x.shape or g.dtype != x.dtype:
+    raise ValueError(f"g must be shaped and typed like x, {tuple(x.shape)} {x.dtype}, got {tuple(g.shape)} {g.dtype}")
+  _, _, _, gg, gr = _norm_rows(g, "g")
+  dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+  dw = torch.empty_like(weight) if weight is not None and needs_vectors else None
+  db = torch.empty_like(bias) if bias is not None and needs_vectors else None
+  if not x.numel():
+    return dx, *(None if t is None else t.zero_() for t in (dw, db))
+  lib = _lib.load()
+  nws = lib.mdattn_layer_norm_bwd_workspace_floats(groups, rows, c) if dw is not None or db is not None else 0
+  ws = torch.empty(nws, dtype=torch.float32, device=x.device) if nws else None
+  rc = lib.mdattn_layer_norm_bwd(_stream(), _ptr(x), x_f32, _ptr(g), _ptr(dx), _ptr(weight), _ptr(dw), _ptr(db), wb_f32, groups, rows, c, sg, sr,
+                                 gg, gr, rows * c, c, stride, float(eps), float(weight_offset), _ptr(ws), nws)
+  _lib.check(rc, "mdattn_layer_norm_bwd")
+  return dx, dw, db
+
+
+class BlockQuant:
+  """A matrix [rows, cols] held as e4m3 with one power-of-two scale per block of block_rows x 128.
+
+  values: uint8 [rows, cols rounded up to 128], the padding zero.  scales: uint8 [ceil(rows / block_rows), blocks of a row
+  rounded up to 4], the exponents with a bias of 127 (0xFF: a block that is not finite).  Both dense."""
+  __slots__ = ("values", "scales", "rows", "cols", "block_rows")
+
+  def __init__(self, values, scales, rows: int, cols: int, block_rows: int):
+    want = ((rows, -(-cols // 128) * 128), (-(-rows // block_rows), -(-cols // 512) * 4)) if block_rows in (1, 128) else None
+    if want is None or (tuple(values.shape), tuple(scales.shape)) != want or values.dtype != torch.uint8 or scales.dtype != torch.uint8 or \
+        not values.is_contiguous() or not scales.is_contiguous():
+      raise ValueError(f"a BlockQuant of {rows} x {cols} in blocks of {block_rows} x 128 (1 or 128) has dense uint8 values and scales of shapes "
+                       f"{want}, got {tuple(values.shape)} {values.dtype} and {tuple(scales.shape)} {scales.dtype}")
+    self.values, self.scales, self.rows, self.cols, self.block_rows = values, scales, rows, cols, block_rows
+
+  def dequantize(self, dtype=torch.float32):
+    """The numbers that it stands for, [rows, cols] (plain torch, for inspection)."""
+    v = self.values.view(torch.float8_e4m3fn).to(torch.float32)
+    s = torch.exp2(self.scales.to(torch.float32) - 127).masked_fill_(self.scales == 255, math.nan)
+    s = s.repeat_interleave(self.block_rows, 0)[:self.rows].repeat_interleave(128, 1)[:, :v.shape[1]]
+    return (v * s)[:, :self.cols].to(dtype)
+
+
+def _new_quant(rows, cols, block_rows, device):
+  u8 = dict(dtype=torch.uint8, device=device)
+  return BlockQuant(torch.empty((rows, -(-cols // 128) * 128), **u8), torch.empty((-(-rows // block_rows), -(-cols // 512) * 4), **u8), rows, cols,
+                    block_rows)
+
+
+def quant_block_e4m3(x, block_rows: int = 1, plain: bool = True, transposed: bool = False, sums: bool = False):
+  """x [R, C] (bf16 or f32, C contiguous) to e4m3 with one power-of-two scale per block of block_rows x 128 (1 or 128): the smallest
+  power of two, 2^-127 at least, with which a block's largest magnitude is at most 448.
+
+  Returns what is asked for, one BlockQuant or a tuple: of x (`plain`), of its transpose [C, R] in blocks of block_rows x 128 of that
+  (`transposed`), and f32 [ceil(R / 128), C], the sums of each column over 128 rows each (`sums`; see `sum_rows`)."""
+  _check_dev(x)
+  if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+    raise ValueError(f"quant_block_e4m3 needs a matrix with contiguous rows, got {tuple(x.shape)} strides {x.stride()}")
+  if block_rows not in (1, 128):
+    raise ValueError(f"block_rows={block_rows!r} not supported. Choose between 1 and 128.")
+  if not plain and not transposed:
+    raise ValueError("neither the matrix nor its transpose is asked for")
+  x_f32 = _float_kind(x, "x")
+  r, c = x.shape
+  q = _new_quant(r, c, block_rows, x.device) if plain else None
+  qt = _new_quant(c, r, block_rows, x.device) if transposed else None
+  part = torch.empty((-(-r // 128), c), dtype=torch.float32, device=x.device) if sums else None
+  if x.numel():
+    rc = _lib.load().mdattn_quant_block_e4m3(_stream(), _ptr(x), x_f32, r, c, x.stride(0), block_rows, _ptr(q.values if q else None),
+                                             _ptr(q.scales if q else None), _ptr(qt.values if qt else None), _ptr(qt.scales if qt else None), _ptr(part))
+    _lib.check(rc, "mdattn_quant_block_e4m3")
+  out = tuple(t for t in (q, qt, part) if t is not None)
+  return out[0] if len(out) == 1 else out
+
+
+def sum_rows(rows, out_dtype=torch.float32):
+  """f32 [n, C] -> [C], summed in a fixed order."""
+  _check_dev(rows)
+  if rows.dim() != 2 or rows.dtype != torch.float32 or not rows.is_contiguous():
+    raise ValueError("sum_rows needs a contiguous f32 matrix")
+  out = torch.empty(rows.shape[1], dtype=out_dtype, device=rows.device)
+  kind = _float_kind(out, "out_dtype")
+  if not rows.numel():
+    return out.zero_()
+  _lib.check(_lib.load().mdattn_sum_rows(_stream(), _ptr(rows), rows.shape[0], rows.shape[1], _ptr(out), kind), "mdattn_sum_rows")
+  return out
+
+
+def matmul_fp8_block(a: BlockQuant, b: BlockQuant, bias=None):
+  """a b^T + bias in bf16: a [M, K] in blocks of 1 x 128, b [N, K] in blocks of 1 x 128 or 128 x 128; bias bf16 or f32 [N] or None.
+  Sums in f32 on the matrix cores, whose 8-bit products are added eight at a time with 14 bits below the largest of them; rounded once."""
+  _check_dev(a.values, a.scales, b.values, b.scales, bias)
+  if a.block_rows != 1:
+    raise ValueError("the first operand's blocks must be 1 x 128")
+  if a.cols != b.cols:
+    raise ValueError(f"inner dims differ: {a.cols} and {b.cols}")
+  if bias is not None and (bias.dim() != 1 or bias.shape[0] != b.rows or not bias.is_contiguous()):
+    raise ValueError(f"bias must be a contiguous tensor of shape [{b.rows}], got {tuple(bias.shape)}")
+  bias_f32 = 0 if bias is None else _float_kind(bias, "bias")
+  m, n, k = a.rows, b.rows, a.cols
+  out = torch.empty((m, n), dtype=torch.bfloat16, device=a.values.device)
+  if not out.numel():
+    return out
+  if not k:
+    return out.zero_() if bias is None else out.copy_(bias.expand(m, n))
+  lib = _lib.load()
+  nws = lib.mdattn_matmul_fp8_block_workspace_floats(m, n, k)
+  ws = torch.empty(nws, dtype=torch.float32, device=out.device) if nws else None
+  rc = lib.mdattn_matmul_fp8_block(_stream(), _ptr(a.values), _ptr(a.scales), _ptr(b.values), _ptr(b.scales), b.block_rows, _ptr(bias), bias_f32,
+                                   _ptr(out), n, m, n, k, _ptr(ws), nws)
+  _lib.check(rc, "mdattn_matmul_fp8_block")
   return out
