@@ -1,12 +1,29 @@
 // c [M, N] = a b^T + bias over e4m3 operands with one power-of-two scale per block of 128 along K:
 //   c[m, n] = sum over k-blocks 2^(ea[m, kb] + eb[n, kb]) sum over k in kb qa[m, k] qb[n, k]
 // The scales are operands of the matrix cores' scaled product (32 x 32 x 64): a block costs no instruction but the read of its byte.
+#include <type_traits>
+
 #include "mdattn_common.h"
 #include "mdlayers.h"
 #include "quant_block.h"
 
 namespace mdattn {
 namespace {
+
+// acc += a b^T of 32 x 32 x 64, scaled by byte PH of sa and of sb.  As one statement with the accumulator in the accumulation registers, where
+// the 256 of a wave's 128 x 128 just fit: the compiler's own form moved them about, and spilled.  The statement hides what
+// it is from the compiler, so that the waits are here: two cycles between the vector ALU's write of an operand and its read (they cost
+// nothing, the pipe being busy with the product before), and the ones after the last product.
+template <int PH>
+__device__ __forceinline__ void mfma(f32x16& acc, const i32x8& a, const i32x8& b, int sa, int sb) {
+#define MDATTN_MFMA(SEL) \
+  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
+  if constexpr (PH == 0) MDATTN_MFMA("op_sel_hi:[0,0,0]");
+  if constexpr (PH == 1) MDATTN_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
+  if constexpr (PH == 2) MDATTN_MFMA("op_sel_hi:[1,1,0]");
+  if constexpr (PH == 3) MDATTN_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
+#undef MDATTN_MFMA
+}
 
 struct MatmulArgs {
   const uint8_t *a, *b, *sa, *sb;
@@ -25,15 +42,18 @@ __device__ __forceinline__ float bias_at(const void* p, int f32, int64_t i) {
 }
 
 // One workgroup, four waves in 2 x 2, computes BM x BN.  A stage of LDS holds 128 bytes of each row of both tiles, written by
-// direct loads; 16-byte chunk c of row r sits at c ^ ((r >> 1) & 7), which spreads 16 rows' reads of one chunk over all banks.  While a stage is
-// multiplied the next one is on its way: one barrier per 128 of K, behind which the first half of the next stage's fragments are read
-// under the second half's products.
+// direct loads; 16-byte chunk c of row r sits at c ^ ((r >> 1) & 7), which spreads 16 rows' reads of one chunk over all banks.  A step
+// multiplies a stage in two halves of K: under the products of the first half the second half's fragments are read; then the one barrier
+// of the step, by which the next stage has landed and this one has been read; under the products of the second half the next stage's first
+// fragments are read and the stage after it is requested into the place of this one.  A matrix instruction keeps its pipe busy for 64
+// cycles, in which the wave issues the reads and requests that stand behind it: their order is the program's (sched_barrier).
 template <int BM, int BN>
 __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
-  constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
+  constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32, kProducts = TM * TN;
   constexpr int kStage = (BM + BN) * 128, kScales = (BM + BN) * 4;
   constexpr int kLoads = (BM + BN) / 32;  // direct loads of a stage by one wave: 8 rows each
   constexpr int kScaleLoads = (BM + BN) / 256;
+  constexpr int kLoadsPer = kLoads / kProducts;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, hh = lane >> 5, wm = wave & 1, wn = wave >> 1;
@@ -52,10 +72,9 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   const uint8_t* b_at = p.b + n0 * p.ld + (int64_t)kb0 * 128;
   unsigned from[kLoads], from_s[kScaleLoads];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int r = (wave + 4 * i) * 8 + (lane >> 3);  // row of the stage: a's, then b's
-    const int64_t left = r < BM ? p.M - 1 - m0 : p.N - 1 - n0;
-    const int64_t row = min((int64_t)(r < BM ? r : r - BM), left);
+  for (int i = 0; i < kLoads; ++i) {  // the first half of them are a's rows
+    const int r = (wave + 4 * i) * 8 + (lane >> 3);
+    const int64_t row = i < kLoads * BM / (BM + BN) ? min((int64_t)r, p.M - 1 - m0) : min((int64_t)r - BM, p.N - 1 - n0);
     from[i] = (unsigned)(row * p.ld + ((lane & 7) ^ ((r >> 1) & 7)) * 16);
   }
   const uint8_t* sa_at = p.sa + m0 * p.ls + kb0;
@@ -67,81 +86,119 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     else from_s[i] = (unsigned)(((min(n0 + r - BM, p.N - 1) >> p.b_shift) - (n0 >> p.b_shift)) * p.ls);
   }
   const unsigned lds = lds_addr_of(smem);
-  auto request = [&](int k) {  // stage k, and the scales of the four stages that begin with it
-    const unsigned to = lds + (k & 1) * kStage + wave * 1024;
+  auto request = [&](int stage, int i) {  // the i-th load of the next stage
+    lds_dma16(i < kLoads * BM / (BM + BN) ? a_at : b_at, from[i], lds + stage * kStage + wave * 1024 + i * 4096);
+  };
+  int ahead = nk - 1;  // stages that are not requested yet; past the last one it is requested again, and not read
+  auto requested = [&] {
+    const int by = ahead > 0 ? 128 : 0;
+    a_at += by;
+    b_at += by;
+    --ahead;
+  };
+  int scale_slot = 0;
+  auto request_scales = [&] {  // of the next four stages, or the last ones again
+    const unsigned to = __builtin_amdgcn_readfirstlane(lds + 2 * kStage + scale_slot * kScales + wave * 256);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) lds_dma16((wave + 4 * i) * 8 < BM ? a_at : b_at, from[i], to + i * 4096);
-    a_at += 128;
-    b_at += 128;
-    if ((k & 3) == 0) {
-      const unsigned to_s = lds + 2 * kStage + ((k >> 2) & 1) * kScales + wave * 256;
-#pragma unroll
-      for (int i = 0; i < kScaleLoads; ++i) lds_dma4((wave + 4 * i) * 64 < BM ? sa_at : sb_at, from_s[i], to_s + i * 1024);
-      sa_at += 4;
-      sb_at += 4;
-    }
+    for (int i = 0; i < kScaleLoads; ++i) lds_dma4((wave + 4 * i) * 64 < BM ? sa_at : sb_at, from_s[i], to + i * 1024);
+    const int by = ahead > 3 ? 4 : 0;
+    sa_at += by;
+    sb_at += by;
+    scale_slot ^= 1;
   };
 
-  f32x16 acc[TN][TM];
+  f32x16 acc[TN][TM];  // zeros, made where they stay: from the vector registers they would be copied in every pass of the loop
 #pragma unroll
   for (int n = 0; n < TN; ++n)
 #pragma unroll
     for (int m = 0; m < TM; ++m)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[n][m][i] = 0.f;
+      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_fp8_fp8 %0, %1, %1, 0" : "=a"(acc[n][m]) : "v"(0l));
   i32x8 fa[2][TM], fb[2][TN];
-  int sa[TM], sb[TN], sa_next[TM], sb_next[TN];
-  const char* ra = smem + (wm * WM + l32) * 128;
-  const char* rb = smem + (BM + wn * WN + l32) * 128;
-  const int swz = (l32 >> 1) & 7;
-  auto fragment = [&](const char* at, int j) {
-    const u32x4 lo = *reinterpret_cast<const u32x4*>(at + (((4 * j + 2 * hh) ^ swz) * 16));
-    const u32x4 hi = *reinterpret_cast<const u32x4*>(at + (((4 * j + 2 * hh + 1) ^ swz) * 16));
+  int sa[TM], sb[TN];  // four stages' scale bytes
+  // where this lane's 16-byte chunks of a fragment begin, by stage and half: the rest of an address is a constant of the instruction
+  typedef const char __attribute__((address_space(3))) * Lds;
+  Lds ra[2][2][2], rb[2][2][2];
+#pragma unroll
+  for (int stage = 0; stage < 2; ++stage)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int chunk = ((4 * j + 2 * hh + q) ^ ((l32 >> 1) & 7)) * 16 + stage * kStage;
+        ra[stage][j][q] = (Lds)smem + (wm * WM + l32) * 128 + chunk;
+        rb[stage][j][q] = (Lds)smem + (BM + wn * WN + l32) * 128 + chunk;
+        asm volatile("" : "+v"(ra[stage][j][q]), "+v"(rb[stage][j][q]));
+      }
+  auto fragment = [&](const Lds (&at)[2], int off) {
+    typedef const u32x4 __attribute__((address_space(3))) * Chunk;
+    const u32x4 lo = *(Chunk)(at[0] + off), hi = *(Chunk)(at[1] + off);
     return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
   };
-  auto read_half = [&](int k, int j) {
-    const int s = (k & 1) * kStage;
-#pragma unroll
-    for (int m = 0; m < TM; ++m) fa[j][m] = fragment(ra + s + m * 4096, j);
-#pragma unroll
-    for (int n = 0; n < TN; ++n) fb[j][n] = fragment(rb + s + n * 4096, j);
+  // the i-th fragment of half j, in the order in which the products want them
+  auto read = [&](int stage, int j, int i) {
+    if (i == 0) fb[j][0] = fragment(rb[stage][j], 0);
+    else if (i <= TM) fa[j][i - 1] = fragment(ra[stage][j], (i - 1) * 4096);
+    else fb[j][i - TM] = fragment(rb[stage][j], (i - TM) * 4096);
   };
-  auto read_scales = [&](int k) {
-    const char* s = smem + 2 * kStage + ((k >> 2) & 1) * kScales + (k & 3);
+  auto read_scales = [&](int slot) {
+    const char* s = smem + 2 * kStage + slot * kScales;
 #pragma unroll
-    for (int m = 0; m < TM; ++m) sa_next[m] = *reinterpret_cast<const uint8_t*>(s + (wm * WM + m * 32 + l32) * 4);
+    for (int m = 0; m < TM; ++m) sa[m] = *reinterpret_cast<const int*>(s + (wm * WM + m * 32 + l32) * 4);
 #pragma unroll
-    for (int n = 0; n < TN; ++n) sb_next[n] = *reinterpret_cast<const uint8_t*>(s + (BM + wn * WN + n * 32 + l32) * 4);
-  };
-  auto multiply = [&](int j) {
-#pragma unroll
-    for (int n = 0; n < TN; ++n)
-#pragma unroll
-      for (int m = 0; m < TM; ++m)
-        acc[n][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j][n], fa[j][m], acc[n][m], 0, 0, 0, sb[n], 0, sa[m]);
+    for (int n = 0; n < TN; ++n) sb[n] = *reinterpret_cast<const int*>(s + (BM + wn * WN + n * 32 + l32) * 4);
   };
   auto everyone_has_it = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-
-  request(0);
-  everyone_has_it();
-  if (nk > 1) request(1);
-  read_scales(0);
-  read_half(0, 0);
-  for (int k = 0; k < nk; ++k) {
+  // step k, PH = k & 3
+  auto step = [&](auto ph) __attribute__((always_inline)) {
+    constexpr int PH = decltype(ph)::value, kNow = PH & 1;
 #pragma unroll
-    for (int m = 0; m < TM; ++m) sa[m] = sa_next[m];
-#pragma unroll
-    for (int n = 0; n < TN; ++n) sb[n] = sb_next[n];
-    read_half(k, 1);
-    multiply(0);
-    everyone_has_it();  // stage k is read, stage k + 1 has landed
-    if (k + 2 < nk) request(k + 2);
-    if (k + 1 < nk) {
-      read_scales(k + 1);
-      read_half(k + 1, 0);
+    for (int i = 0; i < kProducts; ++i) {
+      const int n = i / TM, m = i % TM;
+      mfma<PH>(acc[n][m], fb[0][n], fa[0][m], sb[n], sa[m]);
+      if (i < TM + TN) read(kNow, 1, i);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    multiply(1);
+    everyone_has_it();
+#pragma unroll
+    for (int i = 0; i < kProducts; ++i) {
+      const int n = i / TM, m = i % TM;
+      mfma<PH>(acc[n][m], fb[1][n], fa[1][m], sb[n], sa[m]);
+      if (i < TM + TN) read(kNow ^ 1, 0, i);
+#pragma unroll
+      for (int l = 0; l < kLoadsPer; ++l) request(kNow, i * kLoadsPer + l);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (PH == 2) request_scales();
+    requested();
+    if (PH == 3) read_scales(scale_slot ^ 1);
+  };
+
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) request(0, i);
+  request_scales();
+  requested();
+  everyone_has_it();
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) request(1, i);
+  requested();
+  read_scales(0);
+#pragma unroll
+  for (int i = 0; i < TM + TN; ++i) read(0, 0, i);
+  for (int left = nk;; left -= 4) {
+    step(std::integral_constant<int, 0>{});
+    if (left == 1) break;
+    step(std::integral_constant<int, 1>{});
+    if (left == 2) break;
+    step(std::integral_constant<int, 2>{});
+    if (left == 3) break;
+    step(std::integral_constant<int, 3>{});
+    if (left == 4) break;
   }
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");  // (the last product's result: 16 passes and a few)
+#pragma unroll
+  for (int n = 0; n < TN; ++n)
+#pragma unroll
+    for (int m = 0; m < TM; ++m) asm volatile("" : "+a"(acc[n][m]));  // nothing reads it above this
 
   // lane l32 holds output row m0 + .. + l32; register i of it column (i & 3) + 8 (i >> 2) + 4 hh of 32
 #pragma unroll
@@ -195,7 +252,8 @@ struct Plan {
 };
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
   const int kb = (int)((K + 127) / 128);
-  return {128, 1, (kb + 3) / 4 * 4};
+  const int64_t big = (M + 255) / 256 * ((N + 255) / 256);
+  return {big >= 192 ? 256 : 128, 1, (kb + 3) / 4 * 4};
 }
 int64_t floats_of(const Plan& p, int64_t M, int64_t N) { return p.pieces > 1 ? p.pieces * M * N : 0; }
 
@@ -245,7 +303,7 @@ extern "C" int mdattn_matmul_fp8_block(void* stream, const void* a, const void* 
   p.kb_piece = plan.kb_piece;
   p.part = plan.pieces > 1 ? workspace : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  const int rc = launch<128, 128>(st, p, plan.pieces);
+  const int rc = plan.tile == 256 ? launch<256, 256>(st, p, plan.pieces) : launch<128, 128>(st, p, plan.pieces);
   if (rc != MDATTN_OK || plan.pieces == 1) return rc;
   const int64_t groups = (M * N + 255) / 256;
   MDATTN_LAUNCH(join_pieces_kernel, dim3((unsigned)(groups < 65536 ? groups : 65536)), dim3(256), 0, st, workspace, plan.pieces, bias, bias_is_f32,
