@@ -37,6 +37,12 @@ struct MatmulArgs {
   int mt, nt, total, chunk;
 };
 
+// a pointer that is the same in all lanes, in scalar registers whatever the compiler makes of the branches around it
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u), hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));
+  return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ float bias_at(const void* p, int f32, int64_t i) {
   return f32 ? static_cast<const float*>(p)[i] : (float)static_cast<const __bf16*>(p)[i];
 }
@@ -68,8 +74,8 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   const int kb0 = piece * p.kb_piece, nk = min(p.kb_piece, p.kb - kb0);
 
   // what this lane loads: byte offsets from the tile's first row (rows past the end read the last one; they are not stored)
-  const uint8_t* a_at = p.a + m0 * p.ld + (int64_t)kb0 * 128;
-  const uint8_t* b_at = p.b + n0 * p.ld + (int64_t)kb0 * 128;
+  const uint8_t* a_at = uniform(p.a + m0 * p.ld + (int64_t)kb0 * 128);
+  const uint8_t* b_at = uniform(p.b + n0 * p.ld + (int64_t)kb0 * 128);
   unsigned from[kLoads], from_s[kScaleLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {  // the first half of them are a's rows
@@ -77,8 +83,8 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     const int64_t row = i < kLoads * BM / (BM + BN) ? min((int64_t)r, p.M - 1 - m0) : min((int64_t)r - BM, p.N - 1 - n0);
     from[i] = (unsigned)(row * p.ld + ((lane & 7) ^ ((r >> 1) & 7)) * 16);
   }
-  const uint8_t* sa_at = p.sa + m0 * p.ls + kb0;
-  const uint8_t* sb_at = p.sb + (n0 >> p.b_shift) * p.ls + kb0;
+  const uint8_t* sa_at = uniform(p.sa + m0 * p.ls + kb0);
+  const uint8_t* sb_at = uniform(p.sb + (n0 >> p.b_shift) * p.ls + kb0);
 #pragma unroll
   for (int i = 0; i < kScaleLoads; ++i) {
     const int r = (wave + 4 * i) * 64 + lane;
@@ -92,8 +98,8 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   int ahead = nk - 1;  // stages that are not requested yet; past the last one it is requested again, and not read
   auto requested = [&] {
     const int by = ahead > 0 ? 128 : 0;
-    a_at += by;
-    b_at += by;
+    a_at = uniform(a_at + by);
+    b_at = uniform(b_at + by);
     --ahead;
   };
   int scale_slot = 0;
@@ -102,8 +108,8 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
 #pragma unroll
     for (int i = 0; i < kScaleLoads; ++i) lds_dma4((wave + 4 * i) * 64 < BM ? sa_at : sb_at, from_s[i], to + i * 1024);
     const int by = ahead > 3 ? 4 : 0;
-    sa_at += by;
-    sb_at += by;
+    sa_at = uniform(sa_at + by);
+    sb_at = uniform(sb_at + by);
     scale_slot ^= 1;
   };
 
@@ -176,6 +182,8 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) request(0, i);
   request_scales();
+  float* bias = reinterpret_cast<float*>(smem + 2 * (kStage + kScales));  // of the tile's columns, for the end
+  if ((int)threadIdx.x < BN) bias[threadIdx.x] = p.bias && n0 + threadIdx.x < p.N ? bias_at(p.bias, p.bias_f32, n0 + threadIdx.x) : 0.f;
   requested();
   everyone_has_it();
 #pragma unroll
@@ -201,35 +209,59 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     for (int m = 0; m < TM; ++m) asm volatile("" : "+a"(acc[n][m]));  // nothing reads it above this
 
   // lane l32 holds output row m0 + .. + l32; register i of it column (i & 3) + 8 (i >> 2) + 4 hh of 32
+  if (p.part) {
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+      const int64_t row = m0 + wm * WM + m * 32 + l32;
+      if (row >= p.M) continue;
+      float* o = p.part + ((int64_t)piece * p.M + row) * p.N;
+#pragma unroll
+      for (int n = 0; n < TN; ++n) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t col = n0 + wn * WN + n * 32 + 8 * q + 4 * hh;
+          if (col + 4 <= p.N) {
+            *reinterpret_cast<f32x4_any*>(o + col) = f32x4{acc[n][m][4 * q], acc[n][m][4 * q + 1], acc[n][m][4 * q + 2], acc[n][m][4 * q + 3]};
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < p.N) o[col + e] = acc[n][m][4 * q + e];
+          }
+        }
+      }
+    }
+    return;
+  }
+  // The outputs by whole rows, through LDS: 32 rows of the wave at a time in a place of its own, the 16-byte chunk c of row r at
+  // c ^ (r & (kChunks - 1)).  (Stored from the registers, 16 bytes of a row at a time, they took as long as 20 steps.)
+  constexpr int kChunks = WN / 8;
+  __syncthreads();
+  char* mine = smem + wave * (32 * WN * 2);
+  const bool wide = p.c_stride % 8 == 0 && p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
 #pragma unroll
   for (int m = 0; m < TM; ++m) {
-    const int64_t row = m0 + wm * WM + m * 32 + l32;
-    if (row >= p.M) continue;
 #pragma unroll
     for (int n = 0; n < TN; ++n) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int64_t col = n0 + wn * WN + n * 32 + 8 * q + 4 * hh;
-        float v[4];
+        const float4 b = *reinterpret_cast<const float4*>(bias + wn * WN + n * 32 + 8 * q + 4 * hh);
+        const u32x2 v{pack2(acc[n][m][4 * q] + b.x, acc[n][m][4 * q + 1] + b.y), pack2(acc[n][m][4 * q + 2] + b.z, acc[n][m][4 * q + 3] + b.w)};
+        *reinterpret_cast<u32x2*>(mine + l32 * (WN * 2) + (((n * 4 + q) ^ (l32 & (kChunks - 1))) * 16) + hh * 8) = v;
+      }
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = acc[n][m][4 * q + e];
-          if (p.bias && !p.part && col + e < p.N) v[e] += bias_at(p.bias, p.bias_f32, col + e);
-        }
-        if (p.part) {
-          float* o = p.part + ((int64_t)piece * p.M + row) * p.N + col;
-          if (col + 4 <= p.N) *reinterpret_cast<f32x4_any*>(o) = f32x4{v[0], v[1], v[2], v[3]};
-          else
-            for (int e = 0; e < 4; ++e)
-              if (col + e < p.N) o[e] = v[e];
-        } else {
-          __bf16* o = p.c + row * p.c_stride + col;
-          typedef u32x2 u32x2_half __attribute__((aligned(2)));
-          if (col + 4 <= p.N) *reinterpret_cast<u32x2_half*>(o) = u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])};
-          else
-            for (int e = 0; e < 4; ++e)
-              if (col + e < p.N) o[e] = (__bf16)v[e];
-        }
+    for (int i = 0; i < kChunks / 2; ++i) {
+      const int r = i * (64 / kChunks) + lane / kChunks, c = lane % kChunks;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * (WN * 2) + ((c ^ (r & (kChunks - 1))) * 16));
+      const int64_t row = m0 + wm * WM + m * 32 + r, col = n0 + wn * WN + c * 8;
+      if (row >= p.M) continue;
+      __bf16* o = p.c + row * p.c_stride + col;
+      if (wide) {
+        if (col < p.N) *reinterpret_cast<u32x4*>(o) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (col + e < p.N) reinterpret_cast<unsigned short*>(o)[e] = (unsigned short)(v[e / 2] >> (16 * (e & 1)));
       }
     }
   }
@@ -263,7 +295,7 @@ bool sizes_ok(int64_t M, int64_t N, int64_t K) {
 
 template <int BM, int BN>
 int launch(hipStream_t st, MatmulArgs& a, int pieces) {
-  constexpr int kBytes = 2 * ((BM + BN) * 128 + (BM + BN) * 4);
+  constexpr int kBytes = 2 * ((BM + BN) * 128 + (BM + BN) * 4) + BN * 4;
   static LdsOptIn flag;
   const int rc = lds_opt_in(flag, reinterpret_cast<const void*>(&matmul_fp8_kernel<BM, BN>), kBytes);
   if (rc != MDATTN_OK) return rc;
