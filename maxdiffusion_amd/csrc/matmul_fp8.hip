@@ -10,31 +10,30 @@
 namespace mdattn {
 namespace {
 
-// acc += a b^T of 32 x 32 x 64, scaled by byte PH of sa and of sb.  As one statement with the accumulator in the accumulation registers, where
+// acc += a b^T of 32 x 32 x 64, scaled by the low bytes of sa and sb.  As one statement with the accumulator in the accumulation registers, where
 // the 256 of a wave's 128 x 128 just fit: the compiler's own form moved them about, and spilled.  The statement hides what
 // it is from the compiler, so that the waits are here: two cycles between the vector ALU's write of an operand and its read (they cost
 // nothing, the pipe being busy with the product before), and the ones after the last product.
-template <int PH>
 __device__ __forceinline__ void mfma(f32x16& acc, const i32x8& a, const i32x8& b, int sa, int sb) {
-#define MDATTN_MFMA(SEL) \
-  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
-  if constexpr (PH == 0) MDATTN_MFMA("op_sel_hi:[0,0,0]");
-  if constexpr (PH == 1) MDATTN_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
-  if constexpr (PH == 2) MDATTN_MFMA("op_sel_hi:[1,1,0]");
-  if constexpr (PH == 3) MDATTN_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
-#undef MDATTN_MFMA
+  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb));
+}
+// nothing reads a sum above this, not even to move it to a vector register
+__device__ __forceinline__ void pin(f32x16& acc) { asm volatile("" : "+a"(acc)); }
+__device__ __forceinline__ void mfma_zero(f32x16& acc) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_fp8_fp8 %0, %1, %1, 0" : "=a"(acc) : "v"(0l));
 }
 
 struct MatmulArgs {
   const uint8_t *a, *b, *sa, *sb;
   const void* bias;
   __bf16* c;
-  float* part;       // split over K: f32 sums [piece][M][N]
+  float* part;       // split over K: each piece's f32 sums
   int64_t c_stride, M, N;
   int64_t ld, ls;    // bytes of an operand's row, and of a row of scales
   int b_shift, bias_f32;
   int kb, kb_piece;  // k-blocks, and those of a piece (a multiple of 4)
   int mt, nt, total, chunk;
+  int wide;          // 16-byte stores of c
 };
 
 // a pointer that is the same in all lanes, in scalar registers whatever the compiler makes of the branches around it
@@ -47,235 +46,335 @@ __device__ __forceinline__ float bias_at(const void* p, int f32, int64_t i) {
   return f32 ? static_cast<const float*>(p)[i] : (float)static_cast<const __bf16*>(p)[i];
 }
 
-// One workgroup, four waves in 2 x 2, computes BM x BN.  A stage of LDS holds 128 bytes of each row of both tiles, written by
-// direct loads; 16-byte chunk c of row r sits at c ^ ((r >> 1) & 7), which spreads 16 rows' reads of one chunk over all banks.  A step
-// multiplies a stage in two halves of K: under the products of the first half the second half's fragments are read; then the one barrier
-// of the step, by which the next stage has landed and this one has been read; under the products of the second half the next stage's first
-// fragments are read and the stage after it is requested into the place of this one.  A matrix instruction keeps its pipe busy for 64
-// cycles, in which the wave issues the reads and requests that stand behind it: their order is the program's (sched_barrier).
+// What a workgroup keeps in LDS: two stages, two sets of scale words, each wave's bias values and a place to turn its outputs
 template <int BM, int BN>
+struct Layout {
+  static constexpr int kStage = (BM + BN) * 128, kScales = (BM + BN) * 4;
+  static constexpr int kScaleAt = 2 * kStage;  // (stages, and sets of scales, change places by an exclusive or)
+  static constexpr int kBiasAt = kScaleAt + 2 * kScales;
+  static constexpr int kCols = BN >= 256 ? 64 : 32;  // columns that are turned at a time
+  static constexpr int kTurnAt = kBiasAt + 4 * (BN / 2) * 4;
+  static constexpr int kBytes = kTurnAt + 4 * 32 * kCols * 2;
+};
+
+// A wave's sums to memory: lane l holds row l % 32 of each 32 x 32, register i of it column (i & 3) + 8 (i >> 2) + 4 (l / 32).  By whole
+// rows, through LDS: 32 rows x kCols columns at a time, 16-byte chunk c of row r at c ^ ((r >> 1) & (chunks - 1)).  (Stored from the
+// registers, 16 bytes of a row at a time, they took as long as 20 steps.)
+template <int BM, int BN, int TM, int TN>
+__device__ __forceinline__ void store_rows(const MatmulArgs& p, f32x16 (&acc)[TN][TM], char* smem, int64_t m0, int64_t n0, int lane, int wave) {
+  using L = Layout<BM, BN>;
+  constexpr int WM = BM / 2, WN = BN / 2;
+  const int l32 = lane & 31, hh = lane >> 5;
+  m0 += (wave & 1) * WM;
+  n0 += (wave >> 1) * WN;
+  // LDS serves a wave's requests in order: a block's writes, its reads and the next block's writes follow one another unwaited, and a
+  // block is stored while the next is turned.
+  constexpr int kChunks = L::kCols / 8, kPasses = 32 * kChunks / 64, kRows = 64 / kChunks, kPart = L::kCols / 32, kBlocks = TM * TN / kPart;
+  float* bias = reinterpret_cast<float*>(smem + L::kBiasAt) + wave * WN;
+#pragma unroll
+  for (int i = 0; i < WN; i += 64) bias[i + lane] = p.bias && n0 + i + lane < p.N ? bias_at(p.bias, p.bias_f32, n0 + i + lane) : 0.f;
+  char* mine = smem + L::kTurnAt + wave * (32 * L::kCols * 2);
+  char* put = mine + l32 * (L::kCols * 2) + hh * 8;
+  const int r0 = lane / kChunks, c0 = lane % kChunks, swap = (l32 >> 1) & (kChunks - 1);
+  const char* get = mine + r0 * (L::kCols * 2);
+  const int rows = (int)min(p.M - m0, (int64_t)WM), cols = (int)min(p.N - n0, (int64_t)WN);
+  __bf16* out = p.c + (m0 + r0) * p.c_stride + n0 + c0 * 8;
+  u32x4 v[2][kPasses];
+  auto store = [&](int block) __attribute__((always_inline)) {
+    const int m = block % TM, col = block / TM * L::kCols;
+    const int left = c0 * 8 + col < cols ? rows - r0 - m * 32 : 0;  // rows of this lane's columns from here on
+    __bf16* o = out + m * 32 * p.c_stride + col;
+    if (p.wide) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+        if (i * kRows < left) __builtin_nontemporal_store(v[block & 1][i], reinterpret_cast<u32x4*>(o + i * kRows * p.c_stride));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const u32x4 x = v[block & 1][i];
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          const unsigned word = e < 4 ? (e < 2 ? x[0] : x[1]) : (e < 6 ? x[2] : x[3]);
+          if (i * kRows < left && c0 * 8 + col + e < cols)
+            reinterpret_cast<unsigned short*>(o + i * kRows * p.c_stride)[e] = (unsigned short)(word >> (16 * (e & 1)));
+        }
+      }
+    }
+  };
+  float4 b[kPart][4];
+#pragma unroll
+  for (int block = 0; block < kBlocks; ++block) {
+    const int m = block % TM, n1 = block / TM * kPart;
+    if (m == 0) {
+#pragma unroll
+      for (int n = 0; n < kPart; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) b[n][q] = *reinterpret_cast<const float4*>(bias + (n1 + n) * 32 + 8 * q + 4 * hh);
+    }
+#pragma unroll
+    for (int n = 0; n < kPart; ++n) {
+      f32x16& f = acc[n1 + n][m];
+      pin(f);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<u32x2*>(put + ((n * 4 + q) ^ swap) * 16) =
+            u32x2{pack2(f[4 * q] + b[n][q].x, f[4 * q + 1] + b[n][q].y), pack2(f[4 * q + 2] + b[n][q].z, f[4 * q + 3] + b[n][q].w)};
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+      v[block & 1][i] = *reinterpret_cast<const u32x4*>(get + i * (kRows * L::kCols * 2) + ((c0 ^ (((i * kRows + r0) >> 1) & (kChunks - 1))) * 16));
+    if (block) store(block - 1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  store(kBlocks - 1);
+}
+
+// A piece's sums in the order of the registers, whole and in f32: [piece][tile][wave][n][m][q][lane], four columns each (join_pieces_kernel)
+template <int BM, int BN, int TM, int TN>
+__device__ __forceinline__ void store_piece(const MatmulArgs& p, f32x16 (&acc)[TN][TM], int tile, int piece, int lane, int wave) {
+  f32x4* o = reinterpret_cast<f32x4*>(p.part) + ((int64_t)piece * (p.mt * p.nt) + tile) * (BM * BN / 4) + wave * (BM * BN / 16) + lane;
+#pragma unroll
+  for (int n = 0; n < TN; ++n)
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+      pin(acc[n][m]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        o[((n * TM + m) * 4 + q) * 64] = f32x4{acc[n][m][4 * q], acc[n][m][4 * q + 1], acc[n][m][4 * q + 2], acc[n][m][4 * q + 3]};
+    }
+}
+
+// A workgroup of four waves in 2 x 2 computes BM x BN at a time, and as many such tiles as it takes for the resident workgroups to get through
+// all of them.  A stage of LDS holds 128 bytes of each row of both operands, written by direct loads; 16-byte chunk c of row r sits at
+// c ^ ((r >> 1) & 7), which spreads 16 rows' reads of one chunk over all banks.  A step multiplies a stage in two halves of K: under the
+// products of the first half the second half's fragments are read; then the one barrier of the step, by which the next stage has landed and
+// this one has been read; under the products of the second half the next stage's first fragments are read and the stage after it is
+// requested into the place of this one.  A matrix instruction keeps its pipe busy for 64 cycles, in which the wave issues the reads and
+// requests that stand behind it: their order is the program's (sched_barrier).  The stages are one stream over a workgroup's tiles: while the
+// outputs of one tile are stored, the first stages of the next are on their way.
+template <int BM, int BN, bool PIECES>
 __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
+  using L = Layout<BM, BN>;
   constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32, kProducts = TM * TN;
-  constexpr int kStage = (BM + BN) * 128, kScales = (BM + BN) * 4;
-  constexpr int kLoads = (BM + BN) / 32;  // direct loads of a stage by one wave: 8 rows each
+  constexpr int kStage = L::kStage, kScales = L::kScales;
+  constexpr int kLoads = (BM + BN) / 32;  // direct loads of a stage by one wave: 8 rows each; the first of them a's rows
+  constexpr int kLoadsA = BM / 32;
   constexpr int kScaleLoads = (BM + BN) / 256;
   constexpr int kLoadsPer = kLoads / kProducts;
+  constexpr int kReads = 2 * (TM + TN);  // LDS reads of half a stage's fragments
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, hh = lane >> 5, wm = wave & 1, wn = wave >> 1;
 
-  // neighbouring workgroups sit on different dies: each die takes a contiguous piece of the tiles, in groups of 8 rows of them
-  int id = (blockIdx.x & 7) * p.chunk + (blockIdx.x >> 3);
-  if (id >= p.total) return;
-  const int piece = id / (p.mt * p.nt);
-  id -= piece * p.mt * p.nt;
-  const int band = id / (8 * p.nt), rows = min(p.mt - band * 8, 8), in = id - band * 8 * p.nt;
-  const int64_t m0 = (int64_t)(band * 8 + in % rows) * BM, n0 = (int64_t)(in / rows) * BN;
-  const int kb0 = piece * p.kb_piece, nk = min(p.kb_piece, p.kb - kb0);
+  // Neighbouring workgroups sit on different dies: each die takes a contiguous piece of the tiles, in groups of 8 rows of them.
+  struct Tile {
+    int64_t m0, n0;
+    int tile, piece, kb0, nk;
+  };
+  const int per_die = gridDim.x >> 3, die = blockIdx.x & 7;
+  auto tile_at = [&](int i) {  // i-th of the die
+    int id = min(die * p.chunk + min(i, p.chunk - 1), p.total - 1);
+    Tile t;
+    t.piece = id / (p.mt * p.nt);
+    id -= t.piece * p.mt * p.nt;
+    t.tile = id;
+    const int band = id / (8 * p.nt), rows = min(p.mt - band * 8, 8), in = id - band * 8 * p.nt;
+    t.m0 = (int64_t)(band * 8 + in % rows) * BM;
+    t.n0 = (int64_t)(in / rows) * BN;
+    t.kb0 = t.piece * p.kb_piece;
+    t.nk = min(p.kb_piece, p.kb - t.kb0);
+    return t;
+  };
+  const int last = min(p.chunk, p.total - die * p.chunk);  // tiles of this die
+  int index = blockIdx.x >> 3;
+  if (index >= last) return;
 
   // what this lane loads: byte offsets from the tile's first row (rows past the end read the last one; they are not stored)
-  const uint8_t* a_at = uniform(p.a + m0 * p.ld + (int64_t)kb0 * 128);
-  const uint8_t* b_at = uniform(p.b + n0 * p.ld + (int64_t)kb0 * 128);
   unsigned from[kLoads], from_s[kScaleLoads];
+  const uint8_t *a_at, *b_at, *sa_at, *sb_at;
+  int to_request, requested_of_tile;
+  auto aim = [&](const Tile& t) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {  // the first half of them are a's rows
-    const int r = (wave + 4 * i) * 8 + (lane >> 3);
-    const int64_t row = i < kLoads * BM / (BM + BN) ? min((int64_t)r, p.M - 1 - m0) : min((int64_t)r - BM, p.N - 1 - n0);
-    from[i] = (unsigned)(row * p.ld + ((lane & 7) ^ ((r >> 1) & 7)) * 16);
-  }
-  const uint8_t* sa_at = uniform(p.sa + m0 * p.ls + kb0);
-  const uint8_t* sb_at = uniform(p.sb + (n0 >> p.b_shift) * p.ls + kb0);
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = (wave + 4 * i) * 8 + (lane >> 3);
+      const int row = i < kLoadsA ? min(r, (int)min(p.M - 1 - t.m0, (int64_t)BM)) : min(r - BM, (int)min(p.N - 1 - t.n0, (int64_t)BN));
+      from[i] = (unsigned)row * (unsigned)p.ld + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+    }
 #pragma unroll
-  for (int i = 0; i < kScaleLoads; ++i) {
-    const int r = (wave + 4 * i) * 64 + lane;
-    if (r < BM) from_s[i] = (unsigned)(min((int64_t)r, p.M - 1 - m0) * p.ls);
-    else from_s[i] = (unsigned)(((min(n0 + r - BM, p.N - 1) >> p.b_shift) - (n0 >> p.b_shift)) * p.ls);
-  }
+    for (int i = 0; i < kScaleLoads; ++i) {
+      const int r = (wave + 4 * i) * 64 + lane;
+      const int row = r < BM ? min(r, (int)min(p.M - 1 - t.m0, (int64_t)BM))
+                             : (min(r - BM, (int)min(p.N - 1 - t.n0, (int64_t)BN)) + (int)(t.n0 & ((1 << p.b_shift) - 1))) >> p.b_shift;
+      from_s[i] = (unsigned)row * (unsigned)p.ls;
+    }
+    a_at = uniform(p.a + t.m0 * p.ld + (int64_t)t.kb0 * 128);
+    b_at = uniform(p.b + t.n0 * p.ld + (int64_t)t.kb0 * 128);
+    sa_at = uniform(p.sa + t.m0 * p.ls + t.kb0);
+    sb_at = uniform(p.sb + (t.n0 >> p.b_shift) * p.ls + t.kb0);
+    to_request = t.nk;
+    requested_of_tile = 0;
+  };
   const unsigned lds = lds_addr_of(smem);
-  auto request = [&](int stage, int i) {  // the i-th load of the next stage
-    lds_dma16(i < kLoads * BM / (BM + BN) ? a_at : b_at, from[i], lds + stage * kStage + wave * 1024 + i * 4096);
+  unsigned place = lds + wave * 1024;  // of the stage that is requested next
+  auto request = [&](int i) {  // its i-th load
+    lds_dma16(i < kLoadsA ? a_at : b_at, from[i], (unsigned)__builtin_amdgcn_readfirstlane(place + i * 4096));
   };
-  int ahead = nk - 1;  // stages that are not requested yet; past the last one it is requested again, and not read
+  unsigned scale_place = lds + L::kScaleAt + wave * 256;
+  int aimed = index;  // the tile whose stages are being requested; past the die's last one, that one again
   auto requested = [&] {
-    const int by = ahead > 0 ? 128 : 0;
-    a_at = uniform(a_at + by);
-    b_at = uniform(b_at + by);
-    --ahead;
-  };
-  int scale_slot = 0;
-  auto request_scales = [&] {  // of the next four stages, or the last ones again
-    const unsigned to = __builtin_amdgcn_readfirstlane(lds + 2 * kStage + scale_slot * kScales + wave * 256);
+    if ((requested_of_tile & 3) == 0) {  // the scales of four stages, with the first of them
 #pragma unroll
-    for (int i = 0; i < kScaleLoads; ++i) lds_dma4((wave + 4 * i) * 64 < BM ? sa_at : sb_at, from_s[i], to + i * 1024);
-    const int by = ahead > 3 ? 4 : 0;
-    sa_at = uniform(sa_at + by);
-    sb_at = uniform(sb_at + by);
-    scale_slot ^= 1;
+      for (int i = 0; i < kScaleLoads; ++i)
+        lds_dma4((wave + 4 * i) * 64 < BM ? sa_at : sb_at, from_s[i], (unsigned)__builtin_amdgcn_readfirstlane(scale_place + i * 1024));
+      sa_at = uniform(sa_at + 4);
+      sb_at = uniform(sb_at + 4);
+      scale_place ^= kScales;
+    }
+    a_at = uniform(a_at + 128);
+    b_at = uniform(b_at + 128);
+    place ^= kStage;
+    ++requested_of_tile;
+    if (--to_request == 0) {
+      aimed += per_die;
+      aim(tile_at(min(aimed, last - 1)));
+    }
   };
 
-  f32x16 acc[TN][TM];  // zeros, made where they stay: from the vector registers they would be copied in every pass of the loop
-#pragma unroll
-  for (int n = 0; n < TN; ++n)
-#pragma unroll
-    for (int m = 0; m < TM; ++m)
-      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_fp8_fp8 %0, %1, %1, 0" : "=a"(acc[n][m]) : "v"(0l));
+  f32x16 acc[TN][TM];
   i32x8 fa[2][TM], fb[2][TN];
-  int sa[TM], sb[TN];  // four stages' scale bytes
-  // where this lane's 16-byte chunks of a fragment begin, by stage and half: the rest of an address is a constant of the instruction
+  int sa[TM], sb[TN], sa_next[TM], sb_next[TN];
+  // where this lane's 16-byte chunks of a fragment begin in the stage that is read, by half: the rest of an address is a constant of the
+  // instruction.  The two stages are kStage apart, a power of two.
   typedef const char __attribute__((address_space(3))) * Lds;
-  Lds ra[2][2][2], rb[2][2][2];
+  unsigned ra[2][2], rb[2][2];
 #pragma unroll
-  for (int stage = 0; stage < 2; ++stage)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int chunk = ((4 * j + 2 * hh + q) ^ ((l32 >> 1) & 7)) * 16 + stage * kStage;
-        ra[stage][j][q] = (Lds)smem + (wm * WM + l32) * 128 + chunk;
-        rb[stage][j][q] = (Lds)smem + (BM + wn * WN + l32) * 128 + chunk;
-        asm volatile("" : "+v"(ra[stage][j][q]), "+v"(rb[stage][j][q]));
-      }
-  auto fragment = [&](const Lds (&at)[2], int off) {
+    for (int q = 0; q < 2; ++q) {
+      const int chunk = ((4 * j + 2 * hh + q) ^ ((l32 >> 1) & 7)) * 16;
+      ra[j][q] = lds + (wm * WM + l32) * 128 + chunk;
+      rb[j][q] = lds + (BM + wn * WN + l32) * 128 + chunk;
+    }
+  // read i of half j (two for each fragment), in the order in which the products want them
+  auto read = [&](int j, int i) {
     typedef const u32x4 __attribute__((address_space(3))) * Chunk;
-    const u32x4 lo = *(Chunk)(at[0] + off), hi = *(Chunk)(at[1] + off);
-    return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-  };
-  // the i-th fragment of half j, in the order in which the products want them
-  auto read = [&](int stage, int j, int i) {
-    if (i == 0) fb[j][0] = fragment(rb[stage][j], 0);
-    else if (i <= TM) fa[j][i - 1] = fragment(ra[stage][j], (i - 1) * 4096);
-    else fb[j][i - TM] = fragment(rb[stage][j], (i - TM) * 4096);
-  };
-  auto read_scales = [&](int slot) {
-    const char* s = smem + 2 * kStage + slot * kScales;
+    const int f = i >> 1, q = i & 1;
+    const bool of_a = f >= 1 && f <= TM;
+    const int t = of_a ? f - 1 : f == 0 ? 0 : f - TM;
+    const u32x4 v = *(Chunk)((Lds)(uintptr_t)(of_a ? ra : rb)[j][q] + t * 4096);
+    i32x8& to = of_a ? fa[j][t] : fb[j][t];
 #pragma unroll
-    for (int m = 0; m < TM; ++m) sa[m] = *reinterpret_cast<const int*>(s + (wm * WM + m * 32 + l32) * 4);
+    for (int e = 0; e < 4; ++e) to[4 * q + e] = (int)v[e];
+  };
+  unsigned rsa = lds + L::kScaleAt + (wm * WM + l32) * 4, rsb = lds + L::kScaleAt + (BM + wn * WN + l32) * 4;
+  auto read_scales = [&](int k) {  // of step k of a tile
+    typedef const uint8_t __attribute__((address_space(3))) * Byte;
+    const unsigned at = k & 3;
 #pragma unroll
-    for (int n = 0; n < TN; ++n) sb[n] = *reinterpret_cast<const int*>(s + (BM + wn * WN + n * 32 + l32) * 4);
+    for (int m = 0; m < TM; ++m) sa_next[m] = *((Byte)(uintptr_t)(rsa + at) + m * 128);
+#pragma unroll
+    for (int n = 0; n < TN; ++n) sb_next[n] = *((Byte)(uintptr_t)(rsb + at) + n * 128);
   };
   auto everyone_has_it = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-  // step k, PH = k & 3
-  auto step = [&](auto ph) __attribute__((always_inline)) {
-    constexpr int PH = decltype(ph)::value, kNow = PH & 1;
-#pragma unroll
-    for (int i = 0; i < kProducts; ++i) {
-      const int n = i / TM, m = i % TM;
-      mfma<PH>(acc[n][m], fb[0][n], fa[0][m], sb[n], sa[m]);
-      if (i < TM + TN) read(kNow, 1, i);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    everyone_has_it();
-#pragma unroll
-    for (int i = 0; i < kProducts; ++i) {
-      const int n = i / TM, m = i % TM;
-      mfma<PH>(acc[n][m], fb[1][n], fa[1][m], sb[n], sa[m]);
-      if (i < TM + TN) read(kNow ^ 1, 0, i);
-#pragma unroll
-      for (int l = 0; l < kLoadsPer; ++l) request(kNow, i * kLoadsPer + l);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (PH == 2) request_scales();
-    requested();
-    if (PH == 3) read_scales(scale_slot ^ 1);
-  };
 
+  Tile t = tile_at(index);
+  aim(t);
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) request(0, i);
-  request_scales();
-  float* bias = reinterpret_cast<float*>(smem + 2 * (kStage + kScales));  // of the tile's columns, for the end
-  if ((int)threadIdx.x < BN) bias[threadIdx.x] = p.bias && n0 + threadIdx.x < p.N ? bias_at(p.bias, p.bias_f32, n0 + threadIdx.x) : 0.f;
+  for (int i = 0; i < kLoads; ++i) request(i);
   requested();
   everyone_has_it();
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) request(1, i);
+  for (int i = 0; i < kLoads; ++i) request(i);
   requested();
   read_scales(0);
 #pragma unroll
-  for (int i = 0; i < TM + TN; ++i) read(0, 0, i);
-  for (int left = nk;; left -= 4) {
-    step(std::integral_constant<int, 0>{});
-    if (left == 1) break;
-    step(std::integral_constant<int, 1>{});
-    if (left == 2) break;
-    step(std::integral_constant<int, 2>{});
-    if (left == 3) break;
-    step(std::integral_constant<int, 3>{});
-    if (left == 4) break;
-  }
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");  // (the last product's result: 16 passes and a few)
+  for (int i = 0; i < kReads; ++i) read(0, i);
+  for (;;) {
+    // zeros, made where they stay: from the vector registers they would be copied in every pass of the loop
 #pragma unroll
-  for (int n = 0; n < TN; ++n)
+    for (int n = 0; n < TN; ++n)
 #pragma unroll
-    for (int m = 0; m < TM; ++m) asm volatile("" : "+a"(acc[n][m]));  // nothing reads it above this
-
-  // lane l32 holds output row m0 + .. + l32; register i of it column (i & 3) + 8 (i >> 2) + 4 hh of 32
-  if (p.part) {
+      for (int m = 0; m < TM; ++m) mfma_zero(acc[n][m]);
+#pragma unroll 1
+    for (int k = 0; k < t.nk; ++k) {
 #pragma unroll
-    for (int m = 0; m < TM; ++m) {
-      const int64_t row = m0 + wm * WM + m * 32 + l32;
-      if (row >= p.M) continue;
-      float* o = p.part + ((int64_t)piece * p.M + row) * p.N;
+      for (int m = 0; m < TM; ++m) sa[m] = sa_next[m];
 #pragma unroll
-      for (int n = 0; n < TN; ++n) {
+      for (int n = 0; n < TN; ++n) sb[n] = sb_next[n];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int64_t col = n0 + wn * WN + n * 32 + 8 * q + 4 * hh;
-          if (col + 4 <= p.N) {
-            *reinterpret_cast<f32x4_any*>(o + col) = f32x4{acc[n][m][4 * q], acc[n][m][4 * q + 1], acc[n][m][4 * q + 2], acc[n][m][4 * q + 3]};
-          } else {
+      for (int i = 0; i < kProducts; ++i) {
+        const int n = i / TM, m = i % TM;
+        mfma(acc[n][m], fb[0][n], fa[0][m], sb[n], sa[m]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (col + e < p.N) o[col + e] = acc[n][m][4 * q + e];
-          }
+        for (int r = 0; r < kReads; ++r)
+          if (r * 3 * kProducts / 4 / kReads == i) read(1, r);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      everyone_has_it();
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          ra[j][q] ^= kStage;
+          rb[j][q] ^= kStage;
         }
+      const bool next_four = k + 1 == t.nk || (k & 3) == 3;
+      if (next_four) {
+        rsa ^= kScales;
+        rsb ^= kScales;
       }
+      read_scales(next_four ? 0 : k + 1);
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i) {
+        const int n = i / TM, m = i % TM;
+        mfma(acc[n][m], fb[1][n], fa[1][m], sb[n], sa[m]);
+#pragma unroll
+        for (int r = 0; r < kReads; ++r)
+          if (r * kProducts / kReads == i) read(0, r);
+#pragma unroll
+        for (int l = 0; l < kLoadsPer; ++l) request(i * kLoadsPer + l);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      requested();
     }
-    return;
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // (the last product's result: 16 passes and a few)
+    if constexpr (PIECES) {
+      store_piece<BM, BN>(p, acc, t.tile, t.piece, lane, wave);
+    } else {
+      store_rows<BM, BN>(p, acc, smem, t.m0, t.n0, lane, wave);
+    }
+    index += per_die;
+    if (index >= last) break;
+    t = tile_at(index);
   }
-  // The outputs by whole rows, through LDS: 32 rows of the wave at a time in a place of its own, the 16-byte chunk c of row r at
-  // c ^ (r & (kChunks - 1)).  (Stored from the registers, 16 bytes of a row at a time, they took as long as 20 steps.)
-  constexpr int kChunks = WN / 8;
-  __syncthreads();
-  char* mine = smem + wave * (32 * WN * 2);
-  const bool wide = p.c_stride % 8 == 0 && p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
-#pragma unroll
-  for (int m = 0; m < TM; ++m) {
-#pragma unroll
-    for (int n = 0; n < TN; ++n) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 b = *reinterpret_cast<const float4*>(bias + wn * WN + n * 32 + 8 * q + 4 * hh);
-        const u32x2 v{pack2(acc[n][m][4 * q] + b.x, acc[n][m][4 * q + 1] + b.y), pack2(acc[n][m][4 * q + 2] + b.z, acc[n][m][4 * q + 3] + b.w)};
-        *reinterpret_cast<u32x2*>(mine + l32 * (WN * 2) + (((n * 4 + q) ^ (l32 & (kChunks - 1))) * 16) + hh * 8) = v;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kChunks / 2; ++i) {
-      const int r = i * (64 / kChunks) + lane / kChunks, c = lane % kChunks;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * (WN * 2) + ((c ^ (r & (kChunks - 1))) * 16));
-      const int64_t row = m0 + wm * WM + m * 32 + r, col = n0 + wn * WN + c * 8;
-      if (row >= p.M) continue;
-      __bf16* o = p.c + row * p.c_stride + col;
-      if (wide) {
-        if (col < p.N) *reinterpret_cast<u32x4*>(o) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (col + e < p.N) reinterpret_cast<unsigned short*>(o)[e] = (unsigned short)(v[e / 2] >> (16 * (e & 1)));
-      }
-    }
-  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was requested past the end
 }
 
-// the pieces of a product that was split over K, in their order, then the bias
-__global__ __launch_bounds__(256) void join_pieces_kernel(const float* part, int pieces, const void* bias, int bias_f32, __bf16* c, int64_t c_stride,
-                                                          int64_t M, int64_t N) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < M * N; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / N, col = i - row * N;
-    float s = 0.f;
-    for (int j = 0; j < pieces; ++j) s += part[j * M * N + i];
-    if (bias) s += bias_at(bias, bias_f32, col);
-    c[row * c_stride + col] = (__bf16)s;
+// the pieces of a product that was split over K, in their order, then the bias.  A thread takes four columns of a row in each piece, 16
+// bytes where store_piece left them.
+template <int BM, int BN>
+__global__ __launch_bounds__(256) void join_pieces_kernel(MatmulArgs p, int pieces) {
+  constexpr int TM = BM / 64;
+  const int tile = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
+  const int lane = i & 63, q = (i >> 6) & 3, m = (i >> 8) % TM, n = (i >> 8) / TM % (BN / 64), wave = i / (BM * BN / 16);
+  const int band = tile / (8 * p.nt), rows = min(p.mt - band * 8, 8), in = tile - band * 8 * p.nt;
+  const int64_t row = (int64_t)(band * 8 + in % rows) * BM + (wave & 1) * (BM / 2) + m * 32 + (lane & 31);
+  const int64_t col = (int64_t)(in / rows) * BN + (wave >> 1) * (BN / 2) + n * 32 + 8 * q + 4 * (lane >> 5);
+  if (row >= p.M || col >= p.N) return;
+  const f32x4* at = reinterpret_cast<const f32x4*>(p.part) + (int64_t)tile * (BM * BN / 4) + i;
+  const int64_t step = (int64_t)p.mt * p.nt * (BM * BN / 4);
+  f32x4 s = at[0];
+  for (int j = 1; j < pieces; ++j) s += at[j * step];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (p.bias && col + e < p.N) s[e] += bias_at(p.bias, p.bias_f32, col + e);
+  __bf16* o = p.c + row * p.c_stride + col;
+  if (p.wide) {
+    *reinterpret_cast<u32x2*>(o) = u32x2{pack2(s[0], s[1]), pack2(s[2], s[3])};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < p.N) o[e] = (__bf16)s[e];
   }
 }
 
@@ -287,23 +386,32 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
   const int64_t big = (M + 255) / 256 * ((N + 255) / 256);
   return {big >= 192 ? 256 : 128, 1, (kb + 3) / 4 * 4};
 }
-int64_t floats_of(const Plan& p, int64_t M, int64_t N) { return p.pieces > 1 ? p.pieces * M * N : 0; }
+int64_t floats_of(const Plan& p, int64_t M, int64_t N) { return p.pieces > 1 ? p.pieces * ceil_to(M, p.tile) * ceil_to(N, p.tile) : 0; }
 
 bool sizes_ok(int64_t M, int64_t N, int64_t K) {
   return M > 0 && N > 0 && K > 0 && M < ((int64_t)1 << 31) && N < ((int64_t)1 << 31) && K <= (1 << 23) && (M + 127) / 128 * ((N + 127) / 128) < (1 << 27);
 }
 
-template <int BM, int BN>
-int launch(hipStream_t st, MatmulArgs& a, int pieces) {
-  constexpr int kBytes = 2 * ((BM + BN) * 128 + (BM + BN) * 4) + BN * 4;
+template <int BM, int BN, bool PIECES>
+int launch(hipStream_t st, const MatmulArgs& a) {
+  constexpr int kBytes = Layout<BM, BN>::kBytes, kResident = 256 * (160 * 1024 / kBytes);
   static LdsOptIn flag;
-  const int rc = lds_opt_in(flag, reinterpret_cast<const void*>(&matmul_fp8_kernel<BM, BN>), kBytes);
+  const int rc = lds_opt_in(flag, reinterpret_cast<const void*>(&matmul_fp8_kernel<BM, BN, PIECES>), kBytes);
   if (rc != MDATTN_OK) return rc;
+  const int grid = a.chunk * 8 < kResident ? a.chunk * 8 : kResident;
+  MDATTN_LAUNCH((matmul_fp8_kernel<BM, BN, PIECES>), dim3((unsigned)grid), dim3(256), kBytes, st, a);
+  return launch_status();
+}
+template <int BM, int BN>
+int launch_tiles(hipStream_t st, MatmulArgs& a, int pieces) {
   a.mt = (int)((a.M + BM - 1) / BM);
   a.nt = (int)((a.N + BN - 1) / BN);
   a.total = a.mt * a.nt * pieces;
   a.chunk = (a.total + 7) / 8;
-  MDATTN_LAUNCH((matmul_fp8_kernel<BM, BN>), dim3((unsigned)(a.chunk * 8)), dim3(256), kBytes, st, a);
+  if (pieces == 1) return launch<BM, BN, false>(st, a);
+  const int rc = launch<BM, BN, true>(st, a);
+  if (rc != MDATTN_OK) return rc;
+  MDATTN_LAUNCH((join_pieces_kernel<BM, BN>), dim3(BM * BN / 1024, (unsigned)(a.mt * a.nt)), dim3(256), 0, st, a, pieces);
   return launch_status();
 }
 
@@ -331,14 +439,10 @@ extern "C" int mdattn_matmul_fp8_block(void* stream, const void* a, const void* 
   p.bias = bias; p.bias_f32 = bias_is_f32; p.c = (__bf16*)c; p.c_stride = c_stride; p.M = M; p.N = N;
   p.ld = ceil_to(K, 128); p.ls = scale_stride(K); p.b_shift = b_block_rows == 128 ? 7 : 0;
   p.kb = (int)(p.ld / 128);
+  p.wide = c_stride % 8 == 0 && N % 8 == 0 && aligned16(c);
   if (plan.pieces > 1 && (!workspace || workspace_floats < floats_of(plan, M, N))) plan.pieces = 1, plan.kb_piece = (p.kb + 3) / 4 * 4;
   p.kb_piece = plan.kb_piece;
   p.part = plan.pieces > 1 ? workspace : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  const int rc = plan.tile == 256 ? launch<256, 256>(st, p, plan.pieces) : launch<128, 128>(st, p, plan.pieces);
-  if (rc != MDATTN_OK || plan.pieces == 1) return rc;
-  const int64_t groups = (M * N + 255) / 256;
-  MDATTN_LAUNCH(join_pieces_kernel, dim3((unsigned)(groups < 65536 ? groups : 65536)), dim3(256), 0, st, workspace, plan.pieces, bias, bias_is_f32,
-                (__bf16*)c, c_stride, M, N);
-  return launch_status();
+  return plan.tile == 256 ? launch_tiles<256, 256>(st, p, plan.pieces) : launch_tiles<128, 128>(st, p, plan.pieces);
 }
