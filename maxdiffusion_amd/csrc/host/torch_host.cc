@@ -21,6 +21,7 @@
 
 #include "mdattn.h"
 #include "mdattn_host.h"
+#include "mdlayers.h"
 
 namespace {
 
@@ -693,6 +694,243 @@ std::optional<variable_list> norm_rope_rows(const Tensor& q, const OptTensor& k_
   return out;
 }
 
+// ------------------------------------------------------------------------------------------------ the layers beside attention
+// (layer_op.py, ops.py.)  An undefined tensor is a missing one.
+bool float_on(const Tensor& t, const Tensor& ref) {
+  return t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) && t.get_device() == ref.get_device() && !t.is_neg();
+}
+int is_f32(const Tensor& t) { return t.defined() && t.scalar_type() == at::kFloat; }
+
+// x [..., C] as the norm walks it: the first axis, and the ones between it and the last, which have to be dense
+struct Rows3 {
+  int64_t groups = 0, rows = 0, c = 0, sg = 0, sr = 0;
+  int64_t all() const { return groups * rows; }
+};
+std::optional<Rows3> as_rows(const Tensor& x) {
+  const int64_t n = x.dim();
+  if (n < 2 || x.numel() == 0 || x.stride(n - 1) != 1) return std::nullopt;
+  for (int64_t i = 1; i < n - 2; ++i)
+    if (x.stride(i) != x.stride(i + 1) * x.size(i + 1)) return std::nullopt;
+  Rows3 r;
+  r.c = x.size(n - 1);
+  r.sr = x.stride(n - 2);
+  r.groups = n == 2 ? 1 : x.size(0);
+  r.sg = n == 2 ? 0 : x.stride(0);
+  r.rows = x.numel() / r.c / r.groups;
+  if (r.c > 16384) return std::nullopt;
+  return r;
+}
+// elements between the groups' vectors of w and b, which have to agree; false: the Python path says what is wrong
+bool norm_vectors(const Tensor& x, const Rows3& r, const Tensor& w, const Tensor& b, int64_t& stride, int& f32) {
+  stride = -1;
+  f32 = 0;
+  for (const Tensor* t : {&w, &b}) {
+    if (!t->defined()) continue;
+    if (!float_on(*t, x) || !t->is_contiguous() || t->numel() == 0 || t->size(t->dim() - 1) != r.c) return false;
+    const bool per_group = (t->dim() == 2 && t->size(0) == r.groups) || (t->dim() == 3 && t->size(0) == r.groups && t->size(1) == 1);
+    if (!per_group && t->dim() != 1) return false;
+    const int64_t mine = per_group ? r.c : 0;
+    if (stride >= 0 && (stride != mine || f32 != is_f32(*t))) return false;
+    stride = mine;
+    f32 = is_f32(*t);
+  }
+  if (stride < 0) stride = 0;
+  return true;
+}
+
+Tensor norm_run(const Tensor& x, const Rows3& r, const Tensor& w, const Tensor& b, int64_t stride, int f32, double eps, double offset) {
+  Tensor y = at::empty(x.sizes(), x.options());
+  const int rc = mdattn_layer_norm(stream(), ptr(x), is_f32(x), mut(y), is_f32(x), ptr(w), ptr(b), f32, r.groups, r.rows, (int)r.c, r.sg, r.sr, r.rows * r.c,
+                                   r.c, stride, (float)eps, (float)offset);
+  return rc == MDATTN_OK ? y : Tensor();
+}
+// Saved for the backward: x and w; of b only its shape and type.
+struct NormFn : torch::autograd::Function<NormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w_, const OptTensor& b_, double eps, double offset) {
+    const Tensor w = value(w_), b = value(b_);
+    const Rows3 r = *as_rows(x);
+    int64_t stride;
+    int f32;
+    norm_vectors(x, r, w, b, stride, f32);
+    Tensor y = norm_run(x, r, w, b, stride, f32, eps, offset);
+    if (!y.defined()) throw Refused{};
+    ctx->save_for_backward({x, w});
+    ctx->saved_data["f"] = c10::List<double>({eps, offset});
+    ctx->saved_data["i"] = c10::List<int64_t>({stride, f32, w.defined(), b.defined(), (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())});
+    ctx->saved_data["wshape"] = w.defined() ? w.sizes().vec() : std::vector<int64_t>{};
+    ctx->saved_data["bshape"] = b.defined() ? b.sizes().vec() : std::vector<int64_t>{};
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto f = ctx->saved_data["f"].toDoubleVector();
+    const auto i = ctx->saved_data["i"].toIntVector();
+    const Tensor &x = saved[0], &w = saved[1];
+    Tensor g = grads[0];
+    const auto r = as_rows(x);
+    unpacked(r && float_on(x, x) && x.sizes() == g.sizes() && w.defined() == (bool)i[2] &&
+             (!w.defined() || (float_on(w, x) && is_f32(w) == (int)i[1] && w.is_contiguous() && w.sizes() == at::IntArrayRef(ctx->saved_data["wshape"].toIntVector()))));
+    if (g.scalar_type() != x.scalar_type()) g = g.to(x.scalar_type());
+    auto rg = as_rows(g);
+    if (!rg || g.is_neg()) {
+      g = g.contiguous();
+      rg = as_rows(g);
+    }
+    const bool vectors = i[4];
+    const auto vec = x.options().dtype(i[1] ? at::kFloat : at::kBFloat16);
+    Tensor dx = at::empty(x.sizes(), x.options());
+    Tensor dw = vectors && i[2] ? at::empty(ctx->saved_data["wshape"].toIntVector(), vec) : Tensor();
+    Tensor db = vectors && i[3] ? at::empty(ctx->saved_data["bshape"].toIntVector(), vec) : Tensor();
+    const int64_t nws = dw.defined() || db.defined() ? mdattn_layer_norm_bwd_workspace_floats(r->groups, r->rows, (int)r->c) : 0;
+    const Tensor ws = nws ? at::empty({nws}, x.options().dtype(at::kFloat)) : Tensor();
+    must(mdattn_layer_norm_bwd(stream(), ptr(x), is_f32(x), ptr(g), mut(dx), ptr(w), mut(dw), mut(db), (int)i[1], r->groups, r->rows, (int)r->c, r->sg, r->sr,
+                               rg->sg, rg->sr, r->rows * r->c, r->c, i[0], (float)f[0], (float)f[1], f32(ws), nws),
+         "mdattn_layer_norm_bwd");
+    return {dx, dw, db, Tensor(), Tensor()};
+  }
+};
+OptTensor layer_norm(const Tensor& x, const OptTensor& w_, const OptTensor& b_, double eps, double offset) {
+  const Tensor w = value(w_), b = value(b_);
+  int64_t stride;
+  int f32;
+  if (!x.is_cuda() || !float_on(x, x)) return std::nullopt;
+  const auto r = as_rows(x);
+  if (!r || !norm_vectors(x, *r, w, b, stride, f32)) return std::nullopt;
+  if (wants_grad({&x, &w, &b})) return unless_refused([&] { return NormFn::apply(x, w_, b_, eps, offset); });
+  at::NoGradGuard guard;
+  const Tensor y = norm_run(x, *r, w, b, stride, f32, eps, offset);
+  return opt(y);
+}
+
+// [rows, cols] in blocks of e4m3 (ops.BlockQuant), in one buffer: the values, then the scales
+struct Blocks {
+  Tensor buf;
+  int64_t rows, cols, block_rows;
+  static int64_t values_bytes(int64_t rows, int64_t cols) { return rows * ((cols + 127) / 128 * 128); }
+  static int64_t bytes(int64_t rows, int64_t cols, int64_t block_rows) {
+    return values_bytes(rows, cols) + (rows + block_rows - 1) / block_rows * ((cols + 511) / 512 * 4);
+  }
+  Blocks(const Tensor& like, int64_t r, int64_t c, int64_t br) : buf(at::empty({bytes(r, c, br)}, like.options().dtype(at::kByte))), rows(r), cols(c), block_rows(br) {}
+  Blocks(const Tensor& saved, int64_t r, int64_t c, int64_t br, const Tensor& ref) : buf(saved), rows(r), cols(c), block_rows(br) {
+    unpacked(buf.is_cuda() && buf.get_device() == ref.get_device() && buf.scalar_type() == at::kByte && buf.is_contiguous() && buf.numel() == bytes(r, c, br) && aligned(buf));
+  }
+  uint8_t* values() const { return static_cast<uint8_t*>(buf.data_ptr()); }
+  uint8_t* scales() const { return values() + values_bytes(rows, cols); }
+};
+// x [..., K] as a matrix of contiguous rows with one stride, or undefined
+Tensor as_matrix(const Tensor& x) {
+  const int64_t k = x.size(-1);
+  if (x.is_contiguous()) return x.view({x.numel() / k, k});
+  if (x.dim() == 2 && x.stride(1) == 1) return x;
+  return Tensor();
+}
+int quant(const Tensor& x, int64_t block_rows, const Blocks* q, const Blocks* qt, const Tensor& sums) {
+  return mdattn_quant_block_e4m3(stream(), ptr(x), is_f32(x), x.size(0), x.size(1), x.stride(0), (int)block_rows, q ? q->values() : nullptr,
+                                 q ? q->scales() : nullptr, qt ? qt->values() : nullptr, qt ? qt->scales() : nullptr, f32(sums));
+}
+int product(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t* sb, int64_t b_block_rows, const Tensor& bias, const Tensor& out, int64_t k) {
+  const int64_t m = out.size(0), n = out.size(1), nws = mdattn_matmul_fp8_block_workspace_floats(m, n, k);
+  const Tensor ws = nws ? at::empty({nws}, out.options().dtype(at::kFloat)) : Tensor();
+  return mdattn_matmul_fp8_block(stream(), a, sa, b, sb, (int)b_block_rows, ptr(bias), is_f32(bias), mut(out), n, m, n, k, f32(ws), nws);
+}
+std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
+  auto v = x.sizes().vec();
+  v.back() = n;
+  return v;
+}
+bool bias_ok(const Tensor& b, int64_t n, const Tensor& ref) { return !b.defined() || (float_on(b, ref) && b.dim() == 1 && b.size(0) == n && b.is_contiguous()); }
+
+// From a weight that the program keeps quantised; with a norm in front where `norm` says so (rows by `r`)
+OptTensor linear_quantized(const Tensor& x, const Tensor& values, const Tensor& scales, int64_t n, int64_t k, int64_t block_rows, const OptTensor& bias_, bool norm,
+                           const OptTensor& w_, const OptTensor& b_, double eps, double offset) {
+  const Tensor bias = value(bias_), w = value(w_), b = value(b_);
+  if (!x.is_cuda() || !float_on(x, x) || x.dim() < 1 || x.size(-1) != k || x.numel() == 0 || k <= 0 || n <= 0 || !values.is_cuda() ||
+      values.get_device() != x.get_device() || scales.get_device() != x.get_device() || !bias_ok(bias, n, x) || wants_grad({&x, &bias, &w, &b}))
+    return std::nullopt;
+  at::NoGradGuard guard;
+  std::optional<Rows3> r;
+  Tensor rows;
+  int64_t stride = 0;
+  int f32 = 0;
+  if (norm) {
+    r = as_rows(x);
+    if (!r || !norm_vectors(x, *r, w, b, stride, f32)) return std::nullopt;
+  } else {
+    rows = as_matrix(x);
+    if (!rows.defined()) return std::nullopt;
+  }
+  const int64_t m = norm ? r->all() : rows.size(0);
+  const Blocks q(x, m, k, 1);
+  const int rc = norm ? mdattn_layer_norm_e4m3(stream(), ptr(x), is_f32(x), q.values(), q.scales(), ptr(w), ptr(b), f32, r->groups, r->rows, (int)r->c, r->sg, r->sr,
+                                               stride, (float)eps, (float)offset)
+                      : quant(rows, 1, &q, nullptr, Tensor());
+  if (rc != MDATTN_OK) return std::nullopt;
+  Tensor y = at::empty({m, n}, x.options().dtype(at::kBFloat16));
+  if (product(q.values(), q.scales(), static_cast<const uint8_t*>(ptr(values)), static_cast<const uint8_t*>(ptr(scales)), block_rows, bias, y, k) != MDATTN_OK)
+    return std::nullopt;
+  return x.dim() == 2 ? y : y.view(with_last(x, n));
+}
+
+// y = x8 w8^T + b, dx = dy8 w8, dw = dy8'^T x8', ' quantised along the tokens.  Saved: x and w in e4m3, transposed, from one read of each.
+struct LinearFn : torch::autograd::Function<LinearFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias_) {
+    const Tensor bias = value(bias_), rows = as_matrix(x);
+    const bool need_dx = x.requires_grad(), need_dw = w.requires_grad(), need_db = bias.defined() && bias.requires_grad();
+    const int64_t m = rows.size(0), k = rows.size(1), n = w.size(0);
+    const Blocks xq(x, m, k, 1), wq(x, n, k, 128);
+    std::optional<Blocks> xt, wt;
+    if (need_dw) xt.emplace(x, k, m, 1);
+    if (need_dx) wt.emplace(x, k, n, 128);
+    if (quant(rows, 1, &xq, xt ? &*xt : nullptr, Tensor()) != MDATTN_OK || quant(w, 128, &wq, wt ? &*wt : nullptr, Tensor()) != MDATTN_OK) throw Refused{};
+    Tensor y = at::empty({m, n}, x.options());
+    if (product(xq.values(), xq.scales(), wq.values(), wq.scales(), 128, bias, y, k) != MDATTN_OK) throw Refused{};
+    ctx->save_for_backward({xt ? xt->buf : Tensor(), wt ? wt->buf : Tensor()});
+    ctx->saved_data["i"] = c10::List<int64_t>({m, n, k, need_dx, need_dw, need_db, is_f32(bias)});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return x.dim() == 2 ? y : y.view(with_last(x, n));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto i = ctx->saved_data["i"].toIntVector();
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const int64_t m = i[0], n = i[1], k = i[2];
+    Tensor g = grads[0];
+    if (g.scalar_type() != at::kBFloat16) g = g.to(at::kBFloat16);
+    if (g.is_neg()) g = g.resolve_neg();
+    Tensor rows = as_matrix(g);
+    if (!rows.defined()) rows = as_matrix(g = g.contiguous());
+    std::optional<Blocks> xt, wt, gq, gt;
+    if (i[4]) xt.emplace(saved[0], k, m, 1, rows);
+    if (i[3]) wt.emplace(saved[1], k, n, 128, rows);
+    if (i[3] || !i[4]) gq.emplace(rows, m, n, 1);
+    if (i[4]) gt.emplace(rows, n, m, 1);
+    const Tensor sums = i[5] ? at::empty({(m + 127) / 128, n}, rows.options().dtype(at::kFloat)) : Tensor();
+    must(quant(rows, 1, gq ? &*gq : nullptr, gt ? &*gt : nullptr, sums), "mdattn_quant_block_e4m3");
+    Tensor dx, dw, db;
+    if (i[3]) {
+      dx = at::empty({m, k}, rows.options());
+      must(product(gq->values(), gq->scales(), wt->values(), wt->scales(), 128, Tensor(), dx, n), "mdattn_matmul_fp8_block");
+      dx = dx.view(shape);
+    }
+    if (i[4]) {
+      dw = at::empty({n, k}, rows.options());
+      must(product(gt->values(), gt->scales(), xt->values(), xt->scales(), 1, Tensor(), dw, m), "mdattn_matmul_fp8_block");
+    }
+    if (i[5]) {
+      db = at::empty({n}, rows.options().dtype(i[6] ? at::kFloat : at::kBFloat16));
+      must(mdattn_sum_rows(stream(), f32(sums), sums.size(0), n, mut(db), (int)i[6]), "mdattn_sum_rows");
+    }
+    return {dx, dw, db};
+  }
+};
+OptTensor linear_autograd(const Tensor& x, const Tensor& w, const OptTensor& bias_) {
+  const Tensor bias = value(bias_);
+  if (!x.is_cuda() || !bf16_on(x, x) || !bf16_on(w, x) || x.dim() < 1 || w.dim() != 2 || x.numel() == 0 || w.numel() == 0 || x.size(-1) != w.size(1) || w.stride(1) != 1 ||
+      !bias_ok(bias, w.size(0), x) || !as_matrix(x).defined())
+    return std::nullopt;
+  return unless_refused([&] { return LinearFn::apply(x, w, bias_); });
+}
+
 // the id of the sources, behind the marker that build.py finds in the file (as in libmdattn.so)
 const char kBuildIdRecord[] = "mdattn-build-id:" MDATTN_BUILD_ID;
 
@@ -711,4 +949,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("norm_rope_perhead", &norm_rope_perhead, Unlocked());
   m.def("norm_rope_qkv", &norm_rope_qkv, Unlocked());
   m.def("norm_rope_rows", &norm_rope_rows, Unlocked());
+  m.def("layer_norm", &layer_norm, Unlocked());
+  m.def("linear_quantized", &linear_quantized, Unlocked());
+  m.def("linear_autograd", &linear_autograd, Unlocked());
 }

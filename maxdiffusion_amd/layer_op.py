@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from . import _lib, ops
 from .ops import BlockQuant
 
 __all__ = ["hip_layer_norm", "hip_linear_fp8", "hip_layer_norm_linear_fp8", "quantize_weight", "BlockQuant"]
@@ -48,6 +48,11 @@ def hip_layer_norm(x, weight=None, bias=None, eps: float = 1e-6, weight_offset: 
   """x [..., C], bf16 or f32 -> the same: h * (weight_offset + weight) + bias, h the row less its mean, over its deviation.
 
   weight and bias [C], or per element of x's first axis [B, C] or [B, 1, C]: adaLN is (scale, shift, weight_offset=1)."""
+  if x.is_cuda:
+    y = _lib.host().layer_norm(x, weight, bias, eps, weight_offset)
+    if y is not None:
+      return y
+  # what the native path leaves: views to be copied, nothing to compute, and every error
   weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
   if _wants_grad(x, weight, bias):
     return _HipLayerNorm.apply(_rows(x), weight, bias, eps, weight_offset)
@@ -107,11 +112,19 @@ def hip_linear_fp8(x, weight, bias=None):
   weight: a BlockQuant (`quantize_weight`), which a program keeps between calls, or, for training, a bf16 [N, K] tensor, quantised in
   every call.  bias bf16 or f32 [N], or None.  Differentiable with a bf16 x and weight; all three products run on e4m3 operands."""
   if isinstance(weight, BlockQuant):
+    if x.is_cuda:
+      y = _lib.host().linear_quantized(x, weight.values, weight.scales, weight.rows, weight.cols, weight.block_rows, bias, False, None, None, 0.0, 0.0)
+      if y is not None:
+        return y
     if _wants_grad(x, bias):
       raise NotImplementedError("hip_linear_fp8 has no gradient through a quantised weight: give the weight itself, or call it under torch.no_grad()")
     rows = x.reshape(-1, x.shape[-1])
     rows = rows if rows.stride(1) == 1 else rows.contiguous()
     return ops.matmul_fp8_block(ops.quant_block_e4m3(rows), weight, bias).view(*x.shape[:-1], weight.rows)
+  if x.is_cuda and _wants_grad(x, weight, bias):
+    y = _lib.host().linear_autograd(x, weight, bias)
+    if y is not None:
+      return y
   if weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
     raise ValueError(f"weight must be a BlockQuant or a [N, {x.shape[-1]}] tensor, got {tuple(weight.shape)}")
   x, weight = (t if t.stride(-1) == 1 else t.contiguous() for t in (x, weight))
@@ -125,6 +138,10 @@ def hip_linear_fp8(x, weight, bias=None):
 def hip_layer_norm_linear_fp8(x, weight, bias, w8: BlockQuant, out_bias=None, eps: float = 1e-6, weight_offset: float = 0.0):
   """`hip_linear_fp8(hip_layer_norm(x, weight, bias, eps, weight_offset), w8, out_bias)` with the norm's f32 rows quantised where they are
   made: x is read once, and what the product reads is written once, a byte per channel.  Inference only."""
+  if x.is_cuda:
+    y = _lib.host().linear_quantized(x, w8.values, w8.scales, w8.rows, w8.cols, w8.block_rows, out_bias, True, weight, bias, eps, weight_offset)
+    if y is not None:
+      return y
   if _wants_grad(x, weight, bias, out_bias):
     raise NotImplementedError("hip_layer_norm_linear_fp8 has no backward pass: use hip_layer_norm and hip_linear_fp8 for training")
   weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
