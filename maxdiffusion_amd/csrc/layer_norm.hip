@@ -3,8 +3,9 @@
 //   mean = sum x / C,  var = sum (x - mean)^2 / C,  r = (var + eps)^-1/2,  h = (x - mean) r,  y = h (o + w) + b
 //   a = g (o + w),  dx = r (a - mean a - h mean(a h)),  dw = sum over rows g h,  db = sum over rows g
 //
-// One pass over the data: a workgroup owns whole rows, a thread the same few chunks of 8 channels in each of its rows, so that w, b and
-// the sums of dw and db stay in its registers while the rows pass by, the next row already on its way.  A wave makes the mean of
+// One pass over the data: a team of threads owns whole rows, a thread the same few chunks of 8 channels in each of its rows, so that w, b and
+// the sums of dw and db stay in its registers while the rows pass by, the next row already on its way.  All teams together walk a window of
+// neighbouring rows (75,600 x 5,120 with a stretch of rows each: 8 % slower).  A wave makes the mean of
 // its own part and the squares around that mean; the parts join as  M2 = sum M2_w + n_w (mean_w - mean)^2  (Chan et al., Updating
 // formulae and a pairwise algorithm for computing sample variances, 1979), which loses nothing where the mean is large against the
 // deviation, and takes one exchange through LDS, and one barrier, per row.
@@ -69,24 +70,23 @@ struct Chunk<float> {
 
 __device__ __forceinline__ void store8(__bf16* p, const float* f) {
   const uint4 u = pack8(f);
-  *reinterpret_cast<u32x4_any*>(p) = u32x4{u.x, u.y, u.z, u.w};
+  __builtin_nontemporal_store(u32x4{u.x, u.y, u.z, u.w}, reinterpret_cast<u32x4_any*>(p));
 }
 __device__ __forceinline__ void store8(float* p, const float* f) {
-  *reinterpret_cast<f32x4_any*>(p) = f32x4{f[0], f[1], f[2], f[3]};
-  *reinterpret_cast<f32x4_any*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
+  __builtin_nontemporal_store(f32x4{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32x4_any*>(p));
+  __builtin_nontemporal_store(f32x4{f[4], f[5], f[6], f[7]}, reinterpret_cast<f32x4_any*>(p + 4));
 }
 
-// A row of C channels dealt to the threads of a workgroup: slot j of a thread is chunk j * blockDim.x + threadIdx.x.  TAIL: C is
-// not a multiple of 8, and the last chunk is walked by elements.
+// A row of C channels dealt to a team of threads: slot j of a thread is chunk j * team + tid.  TAIL: C is not a multiple of 8, and the
+// last chunk is walked by elements.
 template <int NV, bool TAIL>
 struct Deal {
   int c[NV];  // first channel of each slot
-  int C;
-  __device__ __forceinline__ explicit Deal(int C_) : C(C_) {
+  int C, team;
+  __device__ __forceinline__ Deal(int C_, int tid, int team_) : C(C_), team(team_) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) c[j] = (j * (int)blockDim.x + (int)threadIdx.x) * 8;
+    for (int j = 0; j < NV; ++j) c[j] = (j * team + tid) * 8;
   }
-  __device__ __forceinline__ bool has(int j) const { return c[j] < C; }
   __device__ __forceinline__ bool has(int j, int e) const { return TAIL ? c[j] + e < C : c[j] < C; }
   template <typename T>
   __device__ __forceinline__ void load(Chunk<T> (&x)[NV], const T* row) const {
@@ -107,6 +107,17 @@ struct Deal {
         if (c[j] + e < C) row[c[j] + e] = (T)f[e];
     }
   }
+  // f32 that is read again soon
+  __device__ __forceinline__ void keep(int j, float* row, const float* f) const {
+    if (TAIL ? c[j] + 8 <= C : c[j] < C) {
+      *reinterpret_cast<f32x4_any*>(row + c[j]) = f32x4{f[0], f[1], f[2], f[3]};
+      *reinterpret_cast<f32x4_any*>(row + c[j] + 4) = f32x4{f[4], f[5], f[6], f[7]};
+    } else if (TAIL && c[j] < C) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c[j] + e < C) row[c[j] + e] = f[e];
+    }
+  }
   // w or b of one group as f32; `none` where there is none or no channel
   __device__ __forceinline__ void vector(float (&v)[NV][8], const void* p, int is_f32, int64_t at, float none) const {
 #pragma unroll
@@ -125,11 +136,11 @@ struct Deal {
       }
     }
   }
-  // channels that the slots of wave `w` hold
+  // channels that the slots of the team's wave `w` hold
   __device__ __forceinline__ float count(int w) const {
     int n = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) n += min(max(C - (j * (int)blockDim.x + w * 64) * 8, 0), 512);
+    for (int j = 0; j < NV; ++j) n += min(max(C - (j * team + w * 64) * 8, 0), 512);
     return (float)n;
   }
 };
@@ -142,22 +153,21 @@ struct NormArgs {
   int64_t rows, wb_stride;                // rows of a group
   int64_t x_sg, x_sr, y_sg, y_sr;
   int64_t scale_stride;
-  int C, wb_f32, blocks, rows_per_block;  // workgroups of a group, and the rows of each
+  int C, wb_f32, blocks;                  // workgroups of a group
   float eps, offset;
 };
 
 enum { kToBf16 = 0, kToF32 = 1, kToE4m3 = 2 };
 
-template <typename T, int OUT, int NV, bool TAIL>
-__global__ __launch_bounds__(1024) void layer_norm_kernel(NormArgs a) {
+template <typename T, int OUT, int NV, int MAXT, bool TAIL>
+__global__ __launch_bounds__(MAXT) void layer_norm_kernel(NormArgs a) {
   __shared__ float2 part[2][kMaxWaves];
   const int group = blockIdx.x / a.blocks, block = blockIdx.x - group * a.blocks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const Deal<NV, TAIL> deal(a.C);
-  const int64_t first = (int64_t)block * a.rows_per_block, last = min(first + a.rows_per_block, a.rows);
+  const Deal<NV, TAIL> deal(a.C, threadIdx.x, blockDim.x);
   const T* x = static_cast<const T*>(a.x) + group * a.x_sg;
   Chunk<T> now[NV], next[NV];
-  deal.load(next, x + first * a.x_sr);
+  deal.load(next, x + block * a.x_sr);
   float w[NV][8], b[NV][8];
   deal.vector(w, a.w, a.wb_f32, group * a.wb_stride, 1.f - a.offset);
   deal.vector(b, a.b, a.wb_f32, group * a.wb_stride, 0.f);
@@ -168,10 +178,11 @@ __global__ __launch_bounds__(1024) void layer_norm_kernel(NormArgs a) {
   const float inv_c = 1.f / a.C, n_wave = deal.count(wave);
   const float inv_n = n_wave > 0.f ? 1.f / n_wave : 0.f;
 
-  for (int64_t row = first; row < last; ++row) {
+  int odd = 0;
+  for (int64_t row = block; row < a.rows; row += a.blocks, odd ^= 1) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) now[j] = next[j];
-    if (row + 1 < last) deal.load(next, x + (row + 1) * a.x_sr);
+    if (row + a.blocks < a.rows) deal.load(next, x + (row + a.blocks) * a.x_sr);
     float f[NV][8], sum = 0.f, sq = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -189,7 +200,7 @@ __global__ __launch_bounds__(1024) void layer_norm_kernel(NormArgs a) {
       }
     float m2 = wave_sum(sq);
     if (waves > 1) {
-      float2* slot = part[(row - first) & 1];  // the other slot is read until the next barrier
+      float2* slot = part[odd];  // the other one is read until the next barrier
       if ((threadIdx.x & 63) == 0) slot[wave] = make_float2(mean, m2);
       __syncthreads();
       float all = 0.f;
@@ -235,24 +246,30 @@ struct NormBwdArgs {
   float* part;  // [workgroup][2][C]: its rows' dw and db; null: neither is wanted
   int64_t rows, wb_stride;
   int64_t x_sg, x_sr, g_sg, g_sr, d_sg, d_sr;
-  int C, wb_f32, blocks, rows_per_block;
+  int C, wb_f32, blocks, team;  // workgroups of a group; threads of a team
   float eps, offset;
 };
 
-template <typename T, int NV, bool TAIL>
-__global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(NormBwdArgs a) {
+// A workgroup is one team or several, which walk a row each and add up their dw and db at the end, in their order: the sums of all
+// workgroups are written and read once more.
+template <typename T, int NV, int MAXT, bool TAIL>
+__global__ __launch_bounds__(MAXT) void layer_norm_bwd_kernel(NormBwdArgs a) {
   __shared__ float4 part[2][kMaxWaves];
+  extern __shared__ float sums[];  // [2][C], of several teams
   const int group = blockIdx.x / a.blocks, block = blockIdx.x - group * a.blocks;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const Deal<NV, TAIL> deal(a.C);
-  const int64_t first = (int64_t)block * a.rows_per_block, last = min(first + a.rows_per_block, a.rows);
+  const int teams = blockDim.x / a.team, waves = a.team >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave / waves, first_wave = mine * waves;
+  const Deal<NV, TAIL> deal(a.C, threadIdx.x - first_wave * 64, a.team);
   const T* x = static_cast<const T*>(a.x) + group * a.x_sg;
   const T* g = static_cast<const T*>(a.g) + group * a.g_sg;
   T* dx = static_cast<T*>(a.dx) + group * a.d_sg;
+  const int64_t step = (int64_t)a.blocks * teams;
+  int64_t row = (int64_t)block * teams + mine;
   Chunk<T> xn[NV], gn[NV];
-  if (first < last) {
-    deal.load(xn, x + first * a.x_sr);
-    deal.load(gn, g + first * a.g_sr);
+  {
+    const int64_t at = min(row, a.rows - 1);
+    deal.load(xn, x + at * a.x_sr);
+    deal.load(gn, g + at * a.g_sr);
   }
   float w[NV][8], dw[NV][8], db[NV][8];
   deal.vector(w, a.w, a.wb_f32, group * a.wb_stride, 1.f - a.offset);
@@ -263,19 +280,20 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(NormBwdArgs a) {
       w[j][e] += a.offset;
       dw[j][e] = db[j][e] = 0.f;
     }
-  const float inv_c = 1.f / a.C, n_wave = deal.count(wave);
+  const float inv_c = 1.f / a.C, n_wave = deal.count(wave - first_wave);
   const float inv_n = n_wave > 0.f ? 1.f / n_wave : 0.f;
 
-  for (int64_t row = first; row < last; ++row) {
+  int odd = 0;
+  for (int64_t row0 = (int64_t)block * teams; row0 < a.rows; row0 += step, row += step, odd ^= 1) {  // all teams as often: they share the barrier
     float f[NV][8], q[NV][8], sum = 0.f, sq = 0.f, sa = 0.f, sad = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       xn[j].get(f[j]);
       gn[j].get(q[j]);
     }
-    if (row + 1 < last) {
-      deal.load(xn, x + (row + 1) * a.x_sr);
-      deal.load(gn, g + (row + 1) * a.g_sr);
+    if (row + step < a.rows) {
+      deal.load(xn, x + (row + step) * a.x_sr);
+      deal.load(gn, g + (row + step) * a.g_sr);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -297,15 +315,15 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(NormBwdArgs a) {
     sa = wave_sum(sa);
     sad = wave_sum(sad);
     if (waves > 1) {
-      float4* slot = part[(row - first) & 1];
+      float4* slot = part[odd];
       if ((threadIdx.x & 63) == 0) slot[wave] = make_float4(mean, m2, sa, sad);
       __syncthreads();
       float all = 0.f;
-      for (int i = 0; i < waves; ++i) all += slot[i].x * deal.count(i);
+      for (int i = 0; i < waves; ++i) all += slot[first_wave + i].x * deal.count(i);
       all *= inv_c;
       m2 = sa = sad = 0.f;
       for (int i = 0; i < waves; ++i) {
-        const float4 p = slot[i];
+        const float4 p = slot[first_wave + i];
         const float d = p.x - all;
         m2 += p.y + deal.count(i) * d * d;
         sa += p.z;
@@ -313,6 +331,7 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(NormBwdArgs a) {
       }
       mean = all;
     }
+    if (row >= a.rows) continue;
     const float r = rsqrtf(m2 * inv_c + a.eps);
     const float c1 = sa * inv_c, c2 = sad * inv_c * r;
 #pragma unroll
@@ -328,17 +347,41 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(NormBwdArgs a) {
       deal.store(j, dx + row * a.d_sr, o);
     }
   }
-  if (a.part) {
-    float* p = a.part + (int64_t)blockIdx.x * 2 * a.C;
+  if (a.part == nullptr) return;
+  for (int i = 1; i < teams; ++i) {  // team 0 takes over the others', one after the other
+    __syncthreads();
+    if (mine == i) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      deal.store(j, p, dw[j]);
-      deal.store(j, p + a.C, db[j]);
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (deal.has(j, e)) {
+            sums[deal.c[j] + e] = dw[j][e];
+            sums[a.C + deal.c[j] + e] = db[j][e];
+          }
     }
+    __syncthreads();
+    if (mine == 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (deal.has(j, e)) {
+            dw[j][e] += sums[deal.c[j] + e];
+            db[j][e] += sums[a.C + deal.c[j] + e];
+          }
+    }
+  }
+  if (mine != 0) return;
+  float* p = a.part + (int64_t)blockIdx.x * 2 * a.C;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    deal.keep(j, p, dw[j]);
+    deal.keep(j, p + a.C, db[j]);
   }
 }
 
-// out[g][c] = sum over i < n of part[g * n + i][plane][c], plane 0 to dw, 1 to db.  32 columns per workgroup, 32 partial sums each.
+// out[g][c] = sum over i < n of part[g * n + i][plane][c], plane 0 to dw, 1 to db.  64 columns per workgroup, 16 partial sums each.
 struct SumArgs {
   const float* part;
   void *out0, *out1;
@@ -347,21 +390,28 @@ struct SumArgs {
   int f32;
 };
 __global__ __launch_bounds__(1024) void sum_rows_kernel(SumArgs a) {
-  __shared__ float part[32][33];
-  const int lane = threadIdx.x & 31, i0 = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  __shared__ float part[16][64];
+  const int lane = threadIdx.x & 63, i0 = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
   void* out = blockIdx.y ? a.out1 : a.out0;
   if (out == nullptr) return;
-  const float* p = a.part + blockIdx.z * a.n * a.row_stride + blockIdx.y * a.plane_stride + c;
+  const float* p = a.part + blockIdx.z * a.n * a.row_stride + blockIdx.y * a.plane_stride + (c < a.C ? c : a.C - 1);
   float s = 0.f;
-  if (c < a.C)
-    for (int64_t i = i0; i < a.n; i += 32) s += p[i * a.row_stride];
+  int64_t i = i0;
+  for (; i + 112 < a.n; i += 128) {  // eight loads on their way
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = p[(i + 16 * j) * a.row_stride];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += v[j];
+  }
+  for (; i < a.n; i += 16) s += p[i * a.row_stride];
   part[i0][lane] = s;
   __syncthreads();
   if (i0 == 0 && c < a.C) {
     s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) s += part[i][lane];
+    for (int j = 0; j < 16; ++j) s += part[j][lane];
     const int64_t at = blockIdx.z * a.C + c;
     if (a.f32) static_cast<float*>(out)[at] = s;
     else static_cast<__bf16*>(out)[at] = (__bf16)s;
@@ -369,23 +419,41 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(SumArgs a) {
 }
 
 constexpr int kMaxC = 16384;
-// How a row is dealt: chunks per thread and threads.
+// How a row is dealt: chunks per thread and threads of a team.  The fewest places that hold a row, with a power of two of threads: teams of
+// five or six waves sit unevenly on the four SIMDs of a CU (quantised rows of 5,120: 320 threads 2.6 TB/s, 256 with a sixth of the places
+// empty 4.5).
 struct Shape {
   int nv, threads;
 };
 Shape shape_of(int C) {
   const int chunks = (C + 7) / 8;
-  return chunks <= 64 ? Shape{1, 64} : Shape{2, (chunks + 127) / 128 * 64};
+  Shape best{0, 0};
+  for (int t = 64; t <= 1024; t *= 2)
+    for (int nv = 1; nv <= 3; ++nv)
+      if (nv * t >= chunks && (best.nv == 0 || nv * t < best.nv * best.threads || (nv * t == best.nv * best.threads && nv > best.nv))) best = {nv, t};
+  return best;
 }
-// Workgroups of one group, and the rows of each
-void split_rows(int64_t groups, int64_t rows, int64_t target, int* blocks, int* rows_per_block) {
-  int64_t per = (groups * rows + target - 1) / target;
-  if (per > rows) per = rows;
-  *rows_per_block = (int)per;
-  *blocks = (int)((rows + per - 1) / per);
+// Rows in flight on a CU, by their bytes: enough to keep the memory busy, and no more, which would make the rows' pages compete.  16 KB of
+// rows forward (8,192 channels: one row 5.8 TB/s, four 5.4; 2,048: four 5.8, sixteen 5.4), 36 with a quantised output, whose arithmetic needs
+// more waves (5,120: two 3.4, four 4.5), 32 of x and g backward (2,048: four 4.9, twelve 3.8; 5,120: two 5.2, four 4.4).
+int rows_per_cu(int64_t row_bytes, int64_t in_flight, int least) { return (int)((in_flight + row_bytes / 2) / row_bytes < least ? least : (in_flight + row_bytes / 2) / row_bytes); }
+// Workgroups of one group of so many rows, of all groups' `target`
+int blocks_of(int64_t groups, int64_t rows, int64_t target) {
+  const int64_t n = (target + groups - 1) / groups;
+  return (int)(n < rows ? n : rows);
 }
-int64_t fwd_target(const Shape& s) { return 256 * (1536 / s.threads); }
-int64_t bwd_target(const Shape& s) { return 256 * (768 / s.threads > 0 ? 768 / s.threads : 1); }
+struct BwdShape {
+  Shape s;
+  int teams, blocks;
+};
+// Several teams to a workgroup of up to 256 threads: their dw and db leave it as one row of sums.
+BwdShape bwd_shape(int64_t groups, int64_t rows, int C, int x_is_f32) {
+  BwdShape b{shape_of(C), 1, 0};
+  if (b.s.threads < 256) b.teams = 256 / b.s.threads;
+  const int per_cu = rows_per_cu((int64_t)C * (x_is_f32 ? 8 : 4), 32768, 1);
+  b.blocks = blocks_of(groups, (rows + b.teams - 1) / b.teams, 256 * (int64_t)((per_cu + b.teams - 1) / b.teams));
+  return b;
+}
 
 bool sizes_ok(int64_t groups, int64_t rows, int C) {
   return groups > 0 && rows > 0 && C > 0 && rows < ((int64_t)1 << 40) / groups;
@@ -394,19 +462,20 @@ bool elem_aligned(const void* p, int is_f32) { return (reinterpret_cast<uintptr_
 
 template <typename T, int OUT>
 int launch_norm(hipStream_t st, const NormArgs& a, const Shape& s, unsigned grid) {
-#define MDATTN_NORM(NV)                                                                                              \
-  if (s.nv == NV) {                                                                                                  \
-    if (a.C % 8) MDATTN_LAUNCH((layer_norm_kernel<T, OUT, NV, true>), dim3(grid), dim3(s.threads), 0, st, a);      \
-    else MDATTN_LAUNCH((layer_norm_kernel<T, OUT, NV, false>), dim3(grid), dim3(s.threads), 0, st, a);             \
+#define MDATTN_NORM(NV, MAXT)                                                                                              \
+  if (s.nv == NV && (s.threads <= 256 ? 256 : s.threads) == MAXT) {                                                              \
+    if (a.C % 8) MDATTN_LAUNCH((layer_norm_kernel<T, OUT, NV, MAXT, true>), dim3(grid), dim3(s.threads), 0, st, a);      \
+    else MDATTN_LAUNCH((layer_norm_kernel<T, OUT, NV, MAXT, false>), dim3(grid), dim3(s.threads), 0, st, a);             \
   }
-  MDATTN_NORM(1) MDATTN_NORM(2)
+  MDATTN_NORM(1, 256) MDATTN_NORM(2, 256) MDATTN_NORM(3, 256) MDATTN_NORM(2, 512) MDATTN_NORM(3, 512) MDATTN_NORM(2, 1024)
 #undef MDATTN_NORM
   return launch_status();
 }
 
 int norm(hipStream_t st, NormArgs& a, int x_is_f32, int out, int64_t groups) {
   const Shape s = shape_of(a.C);
-  split_rows(groups, a.rows, fwd_target(s), &a.blocks, &a.rows_per_block);
+  const int64_t row_bytes = (int64_t)a.C * (x_is_f32 ? 4 : 2);
+  a.blocks = blocks_of(groups, a.rows, 256 * (int64_t)(out == kToE4m3 ? rows_per_cu(row_bytes, 36864, 2) : rows_per_cu(row_bytes, 18432, 1)));
   const int64_t grid = groups * a.blocks;
   if (grid > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
   if (x_is_f32) {
@@ -450,9 +519,7 @@ extern "C" int mdattn_layer_norm_e4m3(void* stream, const void* x, int x_is_f32,
 
 extern "C" int64_t mdattn_layer_norm_bwd_workspace_floats(int64_t groups, int64_t rows, int C) {
   if (!sizes_ok(groups, rows, C) || C > kMaxC) return 0;
-  int blocks, per;
-  split_rows(groups, rows, bwd_target(shape_of(C)), &blocks, &per);
-  return groups * blocks * 2 * C;
+  return groups * bwd_shape(groups, rows, C, 0).blocks * 2 * C;  // (bf16 rows: as many workgroups as f32 ones, or more)
 }
 
 extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, const void* g, void* dx, const void* w, void* dw, void* db,
@@ -466,37 +533,41 @@ extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, 
   if (!elem_aligned(x, x_is_f32) || !elem_aligned(g, x_is_f32) || !elem_aligned(dx, x_is_f32) || !elem_aligned(w, wb_is_f32) ||
       !elem_aligned(dw, wb_is_f32) || !elem_aligned(db, wb_is_f32) || !elem_aligned(workspace, 1))
     return MDATTN_E_ALIGN;
-  const Shape s = shape_of(C);
+  const BwdShape b = bwd_shape(groups, rows, C, x_is_f32);
   NormBwdArgs a{};
   a.x = x; a.g = g; a.w = w; a.dx = dx; a.part = sums ? workspace : nullptr;
   a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w_offset;
   a.x_sg = x_stride_group; a.x_sr = x_stride_row; a.g_sg = g_stride_group; a.g_sr = g_stride_row; a.d_sg = dx_stride_group; a.d_sr = dx_stride_row;
-  split_rows(groups, rows, bwd_target(s), &a.blocks, &a.rows_per_block);
+  a.blocks = b.blocks;
+  a.team = b.s.threads;
   const int64_t grid = groups * a.blocks;
   if (grid > 0x7FFFFFFF || groups > 65535) return MDATTN_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
-#define MDATTN_NORM(T, NV)                                                                                                    \
-  if (s.nv == NV) {                                                                                                           \
-    if (C % 8) MDATTN_LAUNCH((layer_norm_bwd_kernel<T, NV, true>), dim3((unsigned)grid), dim3(s.threads), 0, st, a);        \
-    else MDATTN_LAUNCH((layer_norm_bwd_kernel<T, NV, false>), dim3((unsigned)grid), dim3(s.threads), 0, st, a);             \
+  const unsigned threads = (unsigned)(b.s.threads * b.teams), lds = b.teams > 1 ? 8u * C : 0u;
+#define MDATTN_NORM(T, NV, MAXT)                                                                                                      \
+  if (b.s.nv == NV && (threads <= 256 ? 256 : threads) == MAXT) {                                                                         \
+    if (C % 8) MDATTN_LAUNCH((layer_norm_bwd_kernel<T, NV, MAXT, true>), dim3((unsigned)grid), dim3(threads), lds, st, a);          \
+    else MDATTN_LAUNCH((layer_norm_bwd_kernel<T, NV, MAXT, false>), dim3((unsigned)grid), dim3(threads), lds, st, a);               \
   }
-  if (x_is_f32) { MDATTN_NORM(float, 1) MDATTN_NORM(float, 2) }
-  else { MDATTN_NORM(__bf16, 1) MDATTN_NORM(__bf16, 2) }
+#define MDATTN_NORMS(T) MDATTN_NORM(T, 1, 256) MDATTN_NORM(T, 2, 256) MDATTN_NORM(T, 3, 256) MDATTN_NORM(T, 2, 512) MDATTN_NORM(T, 3, 512) MDATTN_NORM(T, 2, 1024)
+  if (x_is_f32) { MDATTN_NORMS(float) }
+  else { MDATTN_NORMS(__bf16) }
+#undef MDATTN_NORMS
 #undef MDATTN_NORM
   const int rc = launch_status();
   if (rc != MDATTN_OK || !sums) return rc;
   // shared w and b: one sum over the workgroups of all groups
   const int64_t out_groups = wb_stride ? groups : 1;
   const SumArgs r{workspace, dw, db, wb_stride ? a.blocks : grid, 2 * (int64_t)C, C, C, wb_is_f32};
-  MDATTN_LAUNCH(sum_rows_kernel, dim3((C + 31) / 32, 2, (unsigned)out_groups), dim3(1024), 0, st, r);
+  MDATTN_LAUNCH(sum_rows_kernel, dim3((C + 63) / 64, 2, (unsigned)out_groups), dim3(1024), 0, st, r);
   return launch_status();
 }
 
 extern "C" int mdattn_sum_rows(void* stream, const float* rows, int64_t n, int64_t C, void* out, int out_is_f32) {
   if (!rows || !out || n <= 0 || C <= 0) return MDATTN_E_BADARG;
-  if ((C + 31) / 32 > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
+  if ((C + 63) / 64 > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
   if (!elem_aligned(rows, 1) || !elem_aligned(out, out_is_f32)) return MDATTN_E_ALIGN;
   const SumArgs r{rows, out, nullptr, n, C, 0, C, out_is_f32};
-  MDATTN_LAUNCH(sum_rows_kernel, dim3((unsigned)((C + 31) / 32)), dim3(1024), 0, (hipStream_t)stream, r);
+  MDATTN_LAUNCH(sum_rows_kernel, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, (hipStream_t)stream, r);
   return launch_status();
 }
