@@ -24,50 +24,6 @@ __device__ __forceinline__ float wave_sum(float x) {
   return xhalf_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// eight channels of a row as they are loaded
-template <typename T>
-struct Chunk;
-template <>
-struct Chunk<__bf16> {
-  u32x4 u;
-  __device__ __forceinline__ void load(const __bf16* p) { u = *reinterpret_cast<const u32x4_any*>(p); }
-  __device__ __forceinline__ void load_some(const __bf16* p, int n) {
-    unsigned short e[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < n ? reinterpret_cast<const unsigned short*>(p)[i] : 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = e[2 * i] | (unsigned)e[2 * i + 1] << 16;
-  }
-  __device__ __forceinline__ void zero() { u = u32x4{0, 0, 0, 0}; }
-  __device__ __forceinline__ void get(float* f) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(u[i] << 16);
-      f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-    }
-  }
-};
-template <>
-struct Chunk<float> {
-  f32x4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = *reinterpret_cast<const f32x4_any*>(p);
-    b = *reinterpret_cast<const f32x4_any*>(p + 4);
-  }
-  __device__ __forceinline__ void load_some(const float* p, int n) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = i < n ? p[i] : 0.f;
-      b[i] = i + 4 < n ? p[i + 4] : 0.f;
-    }
-  }
-  __device__ __forceinline__ void zero() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
-  __device__ __forceinline__ void get(float* f) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { f[i] = a[i]; f[i + 4] = b[i]; }
-  }
-};
-
 __device__ __forceinline__ void store8(__bf16* p, const float* f) {
   const uint4 u = pack8(f);
   __builtin_nontemporal_store(u32x4{u.x, u.y, u.z, u.w}, reinterpret_cast<u32x4_any*>(p));

@@ -10,17 +10,18 @@
 namespace mdattn {
 namespace {
 
-// acc += a b^T of 32 x 32 x 64, scaled by the low bytes of sa and sb.  As one statement with the accumulator in the accumulation registers, where
-// the 256 of a wave's 128 x 128 just fit: the compiler's own form moved them about, and spilled.  The statement hides what
-// it is from the compiler, so that the waits are here: two cycles between the vector ALU's write of an operand and its read (they cost
-// nothing, the pipe being busy with the product before), and the ones after the last product.
-__device__ __forceinline__ void mfma(f32x16& acc, const i32x8& a, const i32x8& b, int sa, int sb) {
-  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb));
+// acc += a b^T of 16 x 16 x 128, scaled by the low bytes of sa and of sb.  As one statement with the accumulator in the accumulation registers,
+// where the 256 of a wave's 128 x 128 just fit: the compiler's own form moved them about, and spilled.  The statement hides what it is from
+// the compiler, so that the waits are here: two cycles between the vector ALU's write of an operand and its read (they cost nothing, the
+// pipe being busy with the product before), and the ones after the last product.  (32 x 32 x 64 draws 5 % more power, which is what bounds a
+// large product: 4.15 against 4.37 PFLOP/s from registers.)
+__device__ __forceinline__ void mfma(f32x4& acc, const i32x8& a, const i32x8& b, int sa, int sb) {
+  asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb));
 }
 // nothing reads a sum above this, not even to move it to a vector register
-__device__ __forceinline__ void pin(f32x16& acc) { asm volatile("" : "+a"(acc)); }
-__device__ __forceinline__ void mfma_zero(f32x16& acc) {
-  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_fp8_fp8 %0, %1, %1, 0" : "=a"(acc) : "v"(0l));
+__device__ __forceinline__ void pin(f32x4& acc) { asm volatile("" : "+a"(acc)); }
+__device__ __forceinline__ void mfma_zero(f32x4& acc) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_fp8_fp8 %0, %1, %1, 0" : "=a"(acc) : "v"(0l));
 }
 
 struct MatmulArgs {
@@ -57,31 +58,31 @@ struct Layout {
   static constexpr int kBytes = kTurnAt + 4 * 32 * kCols * 2;
 };
 
-// A wave's sums to memory: lane l holds row l % 32 of each 32 x 32, register i of it column (i & 3) + 8 (i >> 2) + 4 (l / 32).  By whole
-// rows, through LDS: 32 rows x kCols columns at a time, 16-byte chunk c of row r at c ^ ((r >> 1) & (chunks - 1)).  (Stored from the
-// registers, 16 bytes of a row at a time, they took as long as 20 steps.)
+// A wave's sums to memory: of each 16 x 16, lane l holds row l % 16 and columns 4 (l / 16) to + 3.  By whole rows, through LDS: 32 rows x kCols
+// columns at a time, 16-byte chunk c of row r at c ^ ((r >> 1) & (chunks - 1)).  (Stored from the registers, 16 bytes of a row at a time, they
+// took as long as 20 steps.)
 template <int BM, int BN, int TM, int TN>
-__device__ __forceinline__ void store_rows(const MatmulArgs& p, f32x16 (&acc)[TN][TM], char* smem, int64_t m0, int64_t n0, int lane, int wave) {
+__device__ __forceinline__ void store_rows(const MatmulArgs& p, f32x4 (&acc)[TN][TM], char* smem, int64_t m0, int64_t n0, int lane, int wave) {
   using L = Layout<BM, BN>;
   constexpr int WM = BM / 2, WN = BN / 2;
-  const int l32 = lane & 31, hh = lane >> 5;
+  const int l16 = lane & 15, h = lane >> 4;
   m0 += (wave & 1) * WM;
   n0 += (wave >> 1) * WN;
   // LDS serves a wave's requests in order: a block's writes, its reads and the next block's writes follow one another unwaited, and a
   // block is stored while the next is turned.
-  constexpr int kChunks = L::kCols / 8, kPasses = 32 * kChunks / 64, kRows = 64 / kChunks, kPart = L::kCols / 32, kBlocks = TM * TN / kPart;
+  constexpr int kChunks = L::kCols / 8, kPasses = 32 * kChunks / 64, kRows = 64 / kChunks, kPart = L::kCols / 16, kDown = TM / 2, kBlocks = kDown * TN / kPart;
   float* bias = reinterpret_cast<float*>(smem + L::kBiasAt) + wave * WN;
 #pragma unroll
   for (int i = 0; i < WN; i += 64) bias[i + lane] = p.bias && n0 + i + lane < p.N ? bias_at(p.bias, p.bias_f32, n0 + i + lane) : 0.f;
   char* mine = smem + L::kTurnAt + wave * (32 * L::kCols * 2);
-  char* put = mine + l32 * (L::kCols * 2) + hh * 8;
-  const int r0 = lane / kChunks, c0 = lane % kChunks, swap = (l32 >> 1) & (kChunks - 1);
+  char* put = mine + l16 * (L::kCols * 2) + (h & 1) * 8;
+  const int r0 = lane / kChunks, c0 = lane % kChunks, swap = (l16 >> 1) & (kChunks - 1);
   const char* get = mine + r0 * (L::kCols * 2);
   const int rows = (int)min(p.M - m0, (int64_t)WM), cols = (int)min(p.N - n0, (int64_t)WN);
   __bf16* out = p.c + (m0 + r0) * p.c_stride + n0 + c0 * 8;
   u32x4 v[2][kPasses];
   auto store = [&](int block) __attribute__((always_inline)) {
-    const int m = block % TM, col = block / TM * L::kCols;
+    const int m = block % kDown, col = block / kDown * L::kCols;
     const int left = c0 * 8 + col < cols ? rows - r0 - m * 32 : 0;  // rows of this lane's columns from here on
     __bf16* o = out + m * 32 * p.c_stride + col;
     if (p.wide) {
@@ -101,25 +102,23 @@ __device__ __forceinline__ void store_rows(const MatmulArgs& p, f32x16 (&acc)[TN
       }
     }
   };
-  float4 b[kPart][4];
+  float4 b[kPart];
 #pragma unroll
   for (int block = 0; block < kBlocks; ++block) {
-    const int m = block % TM, n1 = block / TM * kPart;
-    if (m == 0) {
+    const int m0s = block % kDown * 2, n1 = block / kDown * kPart;
+    if (m0s == 0) {
 #pragma unroll
-      for (int n = 0; n < kPart; ++n)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) b[n][q] = *reinterpret_cast<const float4*>(bias + (n1 + n) * 32 + 8 * q + 4 * hh);
+      for (int n = 0; n < kPart; ++n) b[n] = *reinterpret_cast<const float4*>(bias + (n1 + n) * 16 + 4 * h);
     }
 #pragma unroll
-    for (int n = 0; n < kPart; ++n) {
-      f32x16& f = acc[n1 + n][m];
-      pin(f);
+    for (int n = 0; n < kPart; ++n)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<u32x2*>(put + ((n * 4 + q) ^ swap) * 16) =
-            u32x2{pack2(f[4 * q] + b[n][q].x, f[4 * q + 1] + b[n][q].y), pack2(f[4 * q + 2] + b[n][q].z, f[4 * q + 3] + b[n][q].w)};
-    }
+      for (int m = 0; m < 2; ++m) {
+        f32x4& f = acc[n1 + n][m0s + m];
+        pin(f);
+        *reinterpret_cast<u32x2*>(put + m * (16 * L::kCols * 2) + ((n * 2 + (h >> 1)) ^ swap) * 16) =
+            u32x2{pack2(f[0] + b[n].x, f[1] + b[n].y), pack2(f[2] + b[n].z, f[3] + b[n].w)};
+      }
 #pragma unroll
     for (int i = 0; i < kPasses; ++i)
       v[block & 1][i] = *reinterpret_cast<const u32x4*>(get + i * (kRows * L::kCols * 2) + ((c0 ^ (((i * kRows + r0) >> 1) & (kChunks - 1))) * 16));
@@ -129,42 +128,40 @@ __device__ __forceinline__ void store_rows(const MatmulArgs& p, f32x16 (&acc)[TN
   store(kBlocks - 1);
 }
 
-// A piece's sums in the order of the registers, whole and in f32: [piece][tile][wave][n][m][q][lane], four columns each (join_pieces_kernel)
+// A piece's sums in the order of the registers, whole and in f32: [piece][tile][wave][n][m][lane], four columns each (join_pieces_kernel)
 template <int BM, int BN, int TM, int TN>
-__device__ __forceinline__ void store_piece(const MatmulArgs& p, f32x16 (&acc)[TN][TM], int tile, int piece, int lane, int wave) {
+__device__ __forceinline__ void store_piece(const MatmulArgs& p, f32x4 (&acc)[TN][TM], int tile, int piece, int lane, int wave) {
   f32x4* o = reinterpret_cast<f32x4*>(p.part) + ((int64_t)piece * (p.mt * p.nt) + tile) * (BM * BN / 4) + wave * (BM * BN / 16) + lane;
 #pragma unroll
   for (int n = 0; n < TN; ++n)
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
       pin(acc[n][m]);
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        o[((n * TM + m) * 4 + q) * 64] = f32x4{acc[n][m][4 * q], acc[n][m][4 * q + 1], acc[n][m][4 * q + 2], acc[n][m][4 * q + 3]};
+      o[(n * TM + m) * 64] = acc[n][m];
     }
 }
 
 // A workgroup of four waves in 2 x 2 computes BM x BN at a time, and as many such tiles as it takes for the resident workgroups to get through
 // all of them.  A stage of LDS holds 128 bytes of each row of both operands, written by direct loads; 16-byte chunk c of row r sits at
-// c ^ ((r >> 1) & 7), which spreads 16 rows' reads of one chunk over all banks.  A step multiplies a stage in two halves of K: under the
-// products of the first half the second half's fragments are read; then the one barrier of the step, by which the next stage has landed and
-// this one has been read; under the products of the second half the next stage's first fragments are read and the stage after it is
-// requested into the place of this one.  A matrix instruction keeps its pipe busy for 64 cycles, in which the wave issues the reads and
+// c ^ ((r >> 1) & 7), which spreads 16 rows' reads of one chunk over all banks.  A step multiplies all of a wave's rows of a with the
+// first half of its rows of b, then with the second.  Under the products of the first half the stage's remaining fragments are read (the second
+// halves of a and b); then the one barrier of the step, by which the next stage has landed and this one has been read; under the products of
+// the second half the next stage's first fragments are read, each into the registers of one that has been used up, and the stage after it is
+// requested into the place of this one.  A matrix instruction keeps its pipe busy for 32 cycles, in which the wave issues the reads and
 // requests that stand behind it: their order is the program's (sched_barrier).  The stages are one stream over a workgroup's tiles: while the
 // outputs of one tile are stored, the first stages of the next are on their way.
 template <int BM, int BN, bool PIECES>
 __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   using L = Layout<BM, BN>;
-  constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32, kProducts = TM * TN;
+  constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16, HM = TM / 2, HN = TN / 2, kProducts = TM * HN;
   constexpr int kStage = L::kStage, kScales = L::kScales;
   constexpr int kLoads = (BM + BN) / 32;  // direct loads of a stage by one wave: 8 rows each; the first of them a's rows
   constexpr int kLoadsA = BM / 32;
   constexpr int kScaleLoads = (BM + BN) / 256;
-  constexpr int kLoadsPer = kLoads / kProducts;
-  constexpr int kReads = 2 * (TM + TN);  // LDS reads of half a stage's fragments
+  constexpr int kReads = HM + HN;         // fragments that are read under half a step's products
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int l32 = lane & 31, hh = lane >> 5, wm = wave & 1, wn = wave >> 1;
+  const int l16 = lane & 15, h = lane >> 4, wm = wave & 1, wn = wave >> 1;
 
   // Neighbouring workgroups sit on different dies: each die takes a contiguous piece of the tiles, in groups of 8 rows of them.
   struct Tile {
@@ -240,40 +237,31 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     }
   };
 
-  f32x16 acc[TN][TM];
-  i32x8 fa[2][TM], fb[2][TN];
-  int sa[TM], sb[TN], sa_next[TM], sb_next[TN];
-  // where this lane's 16-byte chunks of a fragment begin in the stage that is read, by half: the rest of an address is a constant of the
-  // instruction.  The two stages are kStage apart, a power of two.
+  f32x4 acc[TN][TM];
+  i32x8 fa[TM], fb[TN];
+  int sa[TM], sb[TN];
+  // where this lane's two 16-byte chunks of a fragment, and its scale, are in the stage that is read: the rest of an address is a constant of
+  // the instruction.  The two stages are kStage apart, a power of two.
   typedef const char __attribute__((address_space(3))) * Lds;
-  unsigned ra[2][2], rb[2][2];
+  typedef const u32x4 __attribute__((address_space(3))) * Quad;
+  typedef const uint8_t __attribute__((address_space(3))) * Byte;
+  unsigned ra[2], rb[2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int chunk = ((4 * j + 2 * hh + q) ^ ((l32 >> 1) & 7)) * 16;
-      ra[j][q] = lds + (wm * WM + l32) * 128 + chunk;
-      rb[j][q] = lds + (BM + wn * WN + l32) * 128 + chunk;
-    }
-  // read i of half j (two for each fragment), in the order in which the products want them
-  auto read = [&](int j, int i) {
-    typedef const u32x4 __attribute__((address_space(3))) * Chunk;
-    const int f = i >> 1, q = i & 1;
-    const bool of_a = f >= 1 && f <= TM;
-    const int t = of_a ? f - 1 : f == 0 ? 0 : f - TM;
-    const u32x4 v = *(Chunk)((Lds)(uintptr_t)(of_a ? ra : rb)[j][q] + t * 4096);
-    i32x8& to = of_a ? fa[j][t] : fb[j][t];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) to[4 * q + e] = (int)v[e];
+  for (int q = 0; q < 2; ++q) {
+    const int chunk = ((2 * h + q) ^ ((l16 >> 1) & 7)) * 16;
+    ra[q] = lds + (wm * WM + l16) * 128 + chunk;
+    rb[q] = lds + (BM + wn * WN + l16) * 128 + chunk;
+  }
+  unsigned rsa = lds + L::kScaleAt + (wm * WM + l16) * 4, rsb = lds + L::kScaleAt + (BM + wn * WN + l16) * 4;
+  auto read_a = [&](int m, unsigned k) {  // k: the step's place among the four of a scale word
+    const u32x4 lo = *(Quad)((Lds)(uintptr_t)ra[0] + m * 2048), hi = *(Quad)((Lds)(uintptr_t)ra[1] + m * 2048);
+    fa[m] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+    sa[m] = *((Byte)(uintptr_t)(rsa + k) + m * 64);
   };
-  unsigned rsa = lds + L::kScaleAt + (wm * WM + l32) * 4, rsb = lds + L::kScaleAt + (BM + wn * WN + l32) * 4;
-  auto read_scales = [&](int k) {  // of step k of a tile
-    typedef const uint8_t __attribute__((address_space(3))) * Byte;
-    const unsigned at = k & 3;
-#pragma unroll
-    for (int m = 0; m < TM; ++m) sa_next[m] = *((Byte)(uintptr_t)(rsa + at) + m * 128);
-#pragma unroll
-    for (int n = 0; n < TN; ++n) sb_next[n] = *((Byte)(uintptr_t)(rsb + at) + n * 128);
+  auto read_b = [&](int n, unsigned k) {
+    const u32x4 lo = *(Quad)((Lds)(uintptr_t)rb[0] + n * 2048), hi = *(Quad)((Lds)(uintptr_t)rb[1] + n * 2048);
+    fb[n] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+    sb[n] = *((Byte)(uintptr_t)(rsb + k) + n * 64);
   };
   auto everyone_has_it = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
@@ -286,9 +274,10 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) request(i);
   requested();
-  read_scales(0);
 #pragma unroll
-  for (int i = 0; i < kReads; ++i) read(0, i);
+  for (int m = 0; m < HM; ++m) read_a(m, 0);
+#pragma unroll
+  for (int n = 0; n < HN; ++n) read_b(n, 0);
   for (;;) {
     // zeros, made where they stay: from the vector registers they would be copied in every pass of the loop
 #pragma unroll
@@ -298,41 +287,42 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
 #pragma unroll 1
     for (int k = 0; k < t.nk; ++k) {
 #pragma unroll
-      for (int m = 0; m < TM; ++m) sa[m] = sa_next[m];
-#pragma unroll
-      for (int n = 0; n < TN; ++n) sb[n] = sb_next[n];
-#pragma unroll
       for (int i = 0; i < kProducts; ++i) {
-        const int n = i / TM, m = i % TM;
-        mfma(acc[n][m], fb[0][n], fa[0][m], sb[n], sa[m]);
+        const int m = i / HN, n = i % HN;
+        mfma(acc[n][m], fb[n], fa[m], sb[n], sa[m]);
 #pragma unroll
-        for (int r = 0; r < kReads; ++r)
-          if (r * 3 * kProducts / 4 / kReads == i) read(1, r);
+        for (int r = 0; r < kReads; ++r)  // a's first: their products come in this half.  Done by three quarters: the barrier waits for them
+          if (r * 3 * kProducts / 4 / kReads == i) {
+            if (r < HM) read_a(HM + r, k & 3);
+            else read_b(HN + r - HM, k & 3);
+          }
         __builtin_amdgcn_sched_barrier(0);
       }
       everyone_has_it();
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          ra[j][q] ^= kStage;
-          rb[j][q] ^= kStage;
-        }
+      for (int q = 0; q < 2; ++q) {
+        ra[q] ^= kStage;
+        rb[q] ^= kStage;
+      }
       const bool next_four = k + 1 == t.nk || (k & 3) == 3;
       if (next_four) {
         rsa ^= kScales;
         rsb ^= kScales;
       }
-      read_scales(next_four ? 0 : k + 1);
+      const unsigned next = next_four ? 0 : (k + 1) & 3;
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
-        const int n = i / TM, m = i % TM;
-        mfma(acc[n][m], fb[1][n], fa[1][m], sb[n], sa[m]);
+        const int m = i / HN, n = HN + i % HN;
+        mfma(acc[n][m], fb[n], fa[m], sb[n], sa[m]);
 #pragma unroll
-        for (int r = 0; r < kReads; ++r)
-          if (r * kProducts / kReads == i) read(0, r);
+        for (int r = 0; r < kReads; ++r)  // b's and a's in turn, a's behind the products that use up what was there
+          if (r * kProducts / kReads == i) {
+            if (r % 2 == 0) read_b(r / 2, next);
+            else read_a(r / 2, next);
+          }
 #pragma unroll
-        for (int l = 0; l < kLoadsPer; ++l) request(i * kLoadsPer + l);
+        for (int l = 0; l < kLoads; ++l)
+          if (l * kProducts / kLoads == i) request(l);
         __builtin_amdgcn_sched_barrier(0);
       }
       requested();
@@ -354,12 +344,12 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
 // bytes where store_piece left them.
 template <int BM, int BN>
 __global__ __launch_bounds__(256) void join_pieces_kernel(MatmulArgs p, int pieces) {
-  constexpr int TM = BM / 64;
+  constexpr int TM = BM / 32, TN = BN / 32;
   const int tile = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
-  const int lane = i & 63, q = (i >> 6) & 3, m = (i >> 8) % TM, n = (i >> 8) / TM % (BN / 64), wave = i / (BM * BN / 16);
+  const int lane = i & 63, m = (i >> 6) % TM, n = (i >> 6) / TM % TN, wave = i / (BM * BN / 16);
   const int band = tile / (8 * p.nt), rows = min(p.mt - band * 8, 8), in = tile - band * 8 * p.nt;
-  const int64_t row = (int64_t)(band * 8 + in % rows) * BM + (wave & 1) * (BM / 2) + m * 32 + (lane & 31);
-  const int64_t col = (int64_t)(in / rows) * BN + (wave >> 1) * (BN / 2) + n * 32 + 8 * q + 4 * (lane >> 5);
+  const int64_t row = (int64_t)(band * 8 + in % rows) * BM + (wave & 1) * (BM / 2) + m * 16 + (lane & 15);
+  const int64_t col = (int64_t)(in / rows) * BN + (wave >> 1) * (BN / 2) + n * 16 + 4 * (lane >> 4);
   if (row >= p.M || col >= p.N) return;
   const f32x4* at = reinterpret_cast<const f32x4*>(p.part) + (int64_t)tile * (BM * BN / 4) + i;
   const int64_t step = (int64_t)p.mt * p.nt * (BM * BN / 4);

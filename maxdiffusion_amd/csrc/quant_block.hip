@@ -11,29 +11,12 @@
 namespace mdattn {
 namespace {
 
-// eight channels from c on as f32; zeros past C
-__device__ __forceinline__ void load8(const __bf16* row, int64_t c, int64_t C, float* f) {
-  if (c + 8 <= C) {
-    const u32x4 u = *reinterpret_cast<const u32x4_any*>(row + c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(u[i] << 16);
-      f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = c + i < C ? (float)row[c + i] : 0.f;
-  }
-}
-__device__ __forceinline__ void load8(const float* row, int64_t c, int64_t C, float* f) {
-  if (c + 8 <= C) {
-    const f32x4 a = *reinterpret_cast<const f32x4_any*>(row + c), b = *reinterpret_cast<const f32x4_any*>(row + c + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { f[i] = a[i]; f[i + 4] = b[i]; }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = c + i < C ? row[c + i] : 0.f;
-  }
+// eight channels from c on; zeros past C
+template <typename T>
+__device__ __forceinline__ void load8(Chunk<T>& x, const T* row, int64_t c, int64_t C) {
+  if (c + 8 <= C) x.load(row + c);
+  else if (c < C) x.load_some(row + c, (int)(C - c));
+  else x.zero();
 }
 __device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
@@ -53,22 +36,24 @@ template <typename T>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
   const int l16 = threadIdx.x & 15;
   const int64_t u0 = (int64_t)blockIdx.x * (16 * kUnits) + (threadIdx.x >> 4);
-  float f[kUnits][8];
+  Chunk<T> x[kUnits];
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
     const int64_t u = min(u0 + 16 * i, a.units - 1), row = u / a.blocks;
-    load8(static_cast<const T*>(a.x) + row * a.x_stride, (u - row * a.blocks) * 128 + l16 * 8, a.C, f[i]);
+    load8(x[i], static_cast<const T*>(a.x) + row * a.x_stride, (u - row * a.blocks) * 128 + l16 * 8, a.C);
   }
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
     const int64_t u = u0 + 16 * i;
     if (u >= a.units) break;
     const int64_t row = u / a.blocks, block = u - row * a.blocks;
+    float f[8];
+    x[i].get(f);
     unsigned m = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, magnitude(f[i][e]));
+    for (int e = 0; e < 8; ++e) m = max(m, magnitude(f[e]));
     const unsigned byte = scale_byte(row16_umax(m));
-    *reinterpret_cast<u32x2*>(a.q + row * a.ldq + block * 128 + l16 * 8) = to_e4m3x8(f[i], scale_inverse(byte), byte);
+    *reinterpret_cast<u32x2*>(a.q + row * a.ldq + block * 128 + l16 * 8) = to_e4m3x8(f, scale_inverse(byte), byte);
     if (l16 == 0) a.s[row * a.lds + block] = (uint8_t)byte;
   }
 }
@@ -84,99 +69,107 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
   const int tid = threadIdx.x, l16 = tid & 15, g = tid >> 4, wave = tid >> 6;
   const int64_t rb = blockIdx.x / a.blocks, cb = blockIdx.x - rb * a.blocks;
   const int64_t r0 = rb * 128 + g * 8, c0 = cb * 128 + l16 * 8;
-  float f[8][8];
+  Chunk<T> x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    if (r0 + i < a.R) {
-      load8(static_cast<const T*>(a.x) + (r0 + i) * a.x_stride, c0, a.C, f[i]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
-    }
+    if (r0 + i < a.R) load8(x[i], static_cast<const T*>(a.x) + (r0 + i) * a.x_stride, c0, a.C);
+    else x[i].zero();
   }
-  unsigned cm[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    cm[e] = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) cm[e] = max(cm[e], magnitude(f[i][e]));
-  }
+  unsigned cm[8] = {};
+  float cs[8] = {};
   unsigned block_byte = 0;
-  if constexpr (BLOCK_ROWS == 128) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float f[8];
+    x[i].get(f);
     unsigned m = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, cm[e]);
-    col_max[0][tid & 127] = 0;
-    __syncthreads();
-    atomicMax(&col_max[0][0], m);  // (of whole numbers: the order does not matter)
-    __syncthreads();
-    block_byte = scale_byte(col_max[0][0]);
-    if (tid == 0) {
-      if (a.s) a.s[rb * a.lds + cb] = (uint8_t)block_byte;
-      if (a.st) a.st[cb * a.ldst + rb] = (uint8_t)block_byte;
-    }
-  } else {
-    // the four row groups of a wave, then the four waves
-#pragma unroll
     for (int e = 0; e < 8; ++e) {
-      unsigned m = cm[e];
-      const u32x2 p = __builtin_amdgcn_permlane16_swap(m, m, false, false);
-      m = max(p[0], p[1]);
-      const u32x2 h = __builtin_amdgcn_permlane32_swap(m, m, false, false);
-      m = max(h[0], h[1]);
-      if ((tid & 48) == 0) col_max[wave][l16 * 8 + e] = m;
+      cm[e] = max(cm[e], magnitude(f[e]));
+      cs[e] += f[e];
+      m = max(m, magnitude(f[e]));
     }
+    if (BLOCK_ROWS == 1 && a.q) {
+      const unsigned byte = scale_byte(row16_umax(m));
+      if (r0 + i < a.R) {
+        *reinterpret_cast<u32x2*>(a.q + (r0 + i) * a.ldq + c0) = to_e4m3x8(f, scale_inverse(byte), byte);
+        if (l16 == 0) a.s[(r0 + i) * a.lds + cb] = (uint8_t)byte;
+      }
+    }
+  }
+  // over the four row groups of a wave, then over the four waves
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const u32x2 p = __builtin_amdgcn_permlane16_swap(cm[e], cm[e], false, false);
+    const unsigned m = max(p[0], p[1]);
+    const u32x2 h = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    if ((tid & 48) == 0) col_max[wave][l16 * 8 + e] = max(h[0], h[1]);
   }
   if (a.colsum) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s += f[i][e];
-      const u32x2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
-      s = xhalf_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+      const u32x2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(cs[e]), __float_as_uint(cs[e]), false, false);
+      const float s = xhalf_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
       if ((tid & 48) == 0) col_sum[wave][l16 * 8 + e] = s;
     }
   }
-  if (a.q) {
+  __syncthreads();
+  if (a.colsum && tid < 128 && cb * 128 + tid < a.C)
+    a.colsum[rb * a.C + cb * 128 + tid] = (col_sum[0][tid] + col_sum[1][tid]) + (col_sum[2][tid] + col_sum[3][tid]);
+  if constexpr (BLOCK_ROWS == 128) {
+    unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      unsigned byte = block_byte;
-      if constexpr (BLOCK_ROWS == 1) {
-        unsigned m = 0;
+    for (int e = 0; e < 8; ++e) {
+      const int c = l16 * 8 + e;
+      m = max(m, max(max(col_max[0][c], col_max[1][c]), max(col_max[2][c], col_max[3][c])));
+    }
+    block_byte = scale_byte(row16_umax(m));
+    if (tid == 0) {
+      if (a.s) a.s[rb * a.lds + cb] = (uint8_t)block_byte;
+      if (a.st) a.st[cb * a.ldst + rb] = (uint8_t)block_byte;
+    }
+    if (a.q) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = max(m, magnitude(f[i][e]));
-        byte = scale_byte(row16_umax(m));
-      }
-      if (r0 + i < a.R) {
-        *reinterpret_cast<u32x2*>(a.q + (r0 + i) * a.ldq + c0) = to_e4m3x8(f[i], scale_inverse(byte), byte);
-        if (BLOCK_ROWS == 1 && l16 == 0) a.s[(r0 + i) * a.lds + cb] = (uint8_t)byte;
+      for (int i = 0; i < 8; ++i) {
+        float f[8];
+        x[i].get(f);
+        if (r0 + i < a.R) *reinterpret_cast<u32x2*>(a.q + (r0 + i) * a.ldq + c0) = to_e4m3x8(f, scale_inverse(block_byte), block_byte);
       }
     }
   }
-  if (BLOCK_ROWS == 1 || a.colsum) __syncthreads();
-  if (a.colsum && tid < 128 && cb * 128 + tid < a.C)
-    a.colsum[rb * a.C + cb * 128 + tid] = (col_sum[0][tid] + col_sum[1][tid]) + (col_sum[2][tid] + col_sum[3][tid]);
   if (!a.qt) return;
+  float inv[8];
+  unsigned bytes[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    unsigned byte = block_byte;
-    if constexpr (BLOCK_ROWS == 1) {
-      const int c = l16 * 8 + e;
-      byte = scale_byte(max(max(col_max[0][c], col_max[1][c]), max(col_max[2][c], col_max[3][c])));
-      if (g == 0 && cb * 128 + c < a.C) a.st[(cb * 128 + c) * a.ldst + rb] = (uint8_t)byte;
-    }
-    float v[8];
+    const int c = l16 * 8 + e;
+    bytes[e] = BLOCK_ROWS == 128 ? block_byte : scale_byte(max(max(col_max[0][c], col_max[1][c]), max(col_max[2][c], col_max[3][c])));
+    inv[e] = scale_inverse(bytes[e]);
+    if (BLOCK_ROWS == 1 && g == 0 && cb * 128 + c < a.C) a.st[(cb * 128 + c) * a.ldst + rb] = (uint8_t)bytes[e];
+  }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = f[i][e];
-    tile[l16 * 8 + e][g ^ l16] = to_e4m3x8(v, scale_inverse(byte), byte);
+  for (int h = 0; h < 2; ++h) {  // four rows of all eight columns, into half a word each
+    unsigned w[8];
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      float f0[8], f1[8];
+      x[4 * h + i].get(f0);
+      x[4 * h + i + 1].get(f1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (i == 0) w[e] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f0[e] * inv[e], f1[e] * inv[e], 0, false);
+        else w[e] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f0[e] * inv[e], f1[e] * inv[e], (int)w[e], true);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tile[l16 * 8 + e][g ^ l16][h] = bytes[e] == 255u ? 0x7F7F7F7Fu : w[e];
   }
   __syncthreads();
 #pragma unroll
   for (int it = 0; it < 4; ++it) {
-    const int c = it * 32 + (tid >> 3), at = tid & 7, x = c >> 3;
+    const int c = it * 32 + (tid >> 3), at = tid & 7, y = c >> 3;
     if (cb * 128 + c >= a.C) continue;
-    const u32x2 lo = tile[c][(2 * at) ^ x], hi = tile[c][(2 * at + 1) ^ x];
+    const u32x2 lo = tile[c][(2 * at) ^ y], hi = tile[c][(2 * at + 1) ^ y];
     *reinterpret_cast<u32x4*>(a.qt + (cb * 128 + c) * a.ldt + rb * 128 + at * 16) = u32x4{lo[0], lo[1], hi[0], hi[1]};
   }
 }
