@@ -393,10 +393,10 @@ Shape shape_of(int C) {
 // rows forward (8,192 channels: one row 5.8 TB/s, four 5.4; 2,048: four 5.8, sixteen 5.4), 36 with a quantised output, whose arithmetic needs
 // more waves (5,120: two 3.4, four 4.5), 32 of x and g backward (2,048: four 4.9, twelve 3.8; 5,120: two 5.2, four 4.4).
 int rows_per_cu(int64_t row_bytes, int64_t in_flight, int least) { return (int)((in_flight + row_bytes / 2) / row_bytes < least ? least : (in_flight + row_bytes / 2) / row_bytes); }
-// Workgroups of one group of so many rows, of all groups' `target`
+// Workgroups of one group of so many rows, of all groups' `target`, and no more than go through them in as many rounds
 int blocks_of(int64_t groups, int64_t rows, int64_t target) {
-  const int64_t n = (target + groups - 1) / groups;
-  return (int)(n < rows ? n : rows);
+  const int64_t n = (target + groups - 1) / groups, rounds = (rows + n - 1) / n;
+  return (int)((rows + rounds - 1) / rounds);
 }
 struct BwdShape {
   Shape s;

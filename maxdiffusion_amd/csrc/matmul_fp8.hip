@@ -47,12 +47,15 @@ __device__ __forceinline__ float bias_at(const void* p, int f32, int64_t i) {
   return f32 ? static_cast<const float*>(p)[i] : (float)static_cast<const __bf16*>(p)[i];
 }
 
-// What a workgroup keeps in LDS: two stages, two sets of scale words, each wave's bias values and a place to turn its outputs
-template <int BM, int BN>
+// What a workgroup keeps in LDS: S stages, sets of scale words (a set serves four stages, or a tile's last ones: as many sets as stages can be
+// under way, and the one that is read), each wave's bias values and a place to turn its outputs.  Stages and sets follow one another in rings
+// whose sizes are powers of two.
+template <int BM, int BN, int S>
 struct Layout {
-  static constexpr int kStage = (BM + BN) * 128, kScales = (BM + BN) * 4;
-  static constexpr int kScaleAt = 2 * kStage;  // (stages, and sets of scales, change places by an exclusive or)
-  static constexpr int kBiasAt = kScaleAt + 2 * kScales;
+  static constexpr int kStage = (BM + BN) * 128, kScales = (BM + BN) * 4, kSets = S == 2 ? 4 : 8;
+  static constexpr int kRing = S * kStage, kSetRing = kSets * kScales;
+  static constexpr int kScaleAt = kRing;
+  static constexpr int kBiasAt = kScaleAt + kSetRing;
   static constexpr int kCols = BN >= 256 ? 64 : 32;  // columns that are turned at a time
   static constexpr int kTurnAt = kBiasAt + 4 * (BN / 2) * 4;
   static constexpr int kBytes = kTurnAt + 4 * 32 * kCols * 2;
@@ -61,9 +64,9 @@ struct Layout {
 // A wave's sums to memory: of each 16 x 16, lane l holds row l % 16 and columns 4 (l / 16) to + 3.  By whole rows, through LDS: 32 rows x kCols
 // columns at a time, 16-byte chunk c of row r at c ^ ((r >> 1) & (chunks - 1)).  (Stored from the registers, 16 bytes of a row at a time, they
 // took as long as 20 steps.)
-template <int BM, int BN, int TM, int TN>
+template <int BM, int BN, int S, int TM, int TN>
 __device__ __forceinline__ void store_rows(const MatmulArgs& p, f32x4 (&acc)[TN][TM], char* smem, int64_t m0, int64_t n0, int lane, int wave) {
-  using L = Layout<BM, BN>;
+  using L = Layout<BM, BN, S>;
   constexpr int WM = BM / 2, WN = BN / 2;
   const int l16 = lane & 15, h = lane >> 4;
   m0 += (wave & 1) * WM;
@@ -146,15 +149,14 @@ __device__ __forceinline__ void store_piece(const MatmulArgs& p, f32x4 (&acc)[TN
 // c ^ ((r >> 1) & 7), which spreads 16 rows' reads of one chunk over all banks.  A step multiplies all of a wave's rows of a with the
 // first half of its rows of b, then with the second.  Under the products of the first half the stage's remaining fragments are read (the second
 // halves of a and b); then the one barrier of the step, by which the next stage has landed and this one has been read; under the products of
-// the second half the next stage's first fragments are read, each into the registers of one that has been used up, and the stage after it is
-// requested into the place of this one.  A matrix instruction keeps its pipe busy for 32 cycles, in which the wave issues the reads and
+// the second half the next stage's first fragments are read, each into the registers of one that has been used up, and the stage S further on
+// is requested into the place of this one.  A matrix instruction keeps its pipe busy for 32 cycles, in which the wave issues the reads and
 // requests that stand behind it: their order is the program's (sched_barrier).  The stages are one stream over a workgroup's tiles: while the
 // outputs of one tile are stored, the first stages of the next are on their way.
-template <int BM, int BN, bool PIECES>
+template <int BM, int BN, int S, bool PIECES>
 __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
-  using L = Layout<BM, BN>;
+  using L = Layout<BM, BN, S>;
   constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16, HM = TM / 2, HN = TN / 2, kProducts = TM * HN;
-  constexpr int kStage = L::kStage, kScales = L::kScales;
   constexpr int kLoads = (BM + BN) / 32;  // direct loads of a stage by one wave: 8 rows each; the first of them a's rows
   constexpr int kLoadsA = BM / 32;
   constexpr int kScaleLoads = (BM + BN) / 256;
@@ -211,25 +213,25 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     to_request = t.nk;
     requested_of_tile = 0;
   };
-  const unsigned lds = lds_addr_of(smem);
-  unsigned place = lds + wave * 1024;  // of the stage that is requested next
+  const unsigned lds = lds_addr_of(smem);  // (0: a kernel's only LDS)
+  unsigned place = lds + wave * 1024;      // of the stage that is requested next
   auto request = [&](int i) {  // its i-th load
     lds_dma16(i < kLoadsA ? a_at : b_at, from[i], (unsigned)__builtin_amdgcn_readfirstlane(place + i * 4096));
   };
-  unsigned scale_place = lds + L::kScaleAt + wave * 256;
+  unsigned scale_place = wave * 256;
   int aimed = index;  // the tile whose stages are being requested; past the die's last one, that one again
   auto requested = [&] {
     if ((requested_of_tile & 3) == 0) {  // the scales of four stages, with the first of them
 #pragma unroll
       for (int i = 0; i < kScaleLoads; ++i)
-        lds_dma4((wave + 4 * i) * 64 < BM ? sa_at : sb_at, from_s[i], (unsigned)__builtin_amdgcn_readfirstlane(scale_place + i * 1024));
+        lds_dma4((wave + 4 * i) * 64 < BM ? sa_at : sb_at, from_s[i], (unsigned)__builtin_amdgcn_readfirstlane(lds + L::kScaleAt + scale_place + i * 1024));
       sa_at = uniform(sa_at + 4);
       sb_at = uniform(sb_at + 4);
-      scale_place ^= kScales;
+      scale_place = (scale_place + L::kScales) & (L::kSetRing - 1);
     }
     a_at = uniform(a_at + 128);
     b_at = uniform(b_at + 128);
-    place ^= kStage;
+    place = (place + L::kStage) & (L::kRing - 1);
     ++requested_of_tile;
     if (--to_request == 0) {
       aimed += per_die;
@@ -241,7 +243,7 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   i32x8 fa[TM], fb[TN];
   int sa[TM], sb[TN];
   // where this lane's two 16-byte chunks of a fragment, and its scale, are in the stage that is read: the rest of an address is a constant of
-  // the instruction.  The two stages are kStage apart, a power of two.
+  // the instruction.
   typedef const char __attribute__((address_space(3))) * Lds;
   typedef const u32x4 __attribute__((address_space(3))) * Quad;
   typedef const uint8_t __attribute__((address_space(3))) * Byte;
@@ -252,8 +254,9 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     ra[q] = lds + (wm * WM + l16) * 128 + chunk;
     rb[q] = lds + (BM + wn * WN + l16) * 128 + chunk;
   }
-  unsigned rsa = lds + L::kScaleAt + (wm * WM + l16) * 4, rsb = lds + L::kScaleAt + (BM + wn * WN + l16) * 4;
-  auto read_a = [&](int m, unsigned k) {  // k: the step's place among the four of a scale word
+  const unsigned rsa = lds + L::kScaleAt + (wm * WM + l16) * 4, rsb = lds + L::kScaleAt + (BM + wn * WN + l16) * 4;
+  unsigned set = 0;  // of scales, the one that is read
+  auto read_a = [&](int m, unsigned k) {  // k: the byte of the step's scales
     const u32x4 lo = *(Quad)((Lds)(uintptr_t)ra[0] + m * 2048), hi = *(Quad)((Lds)(uintptr_t)ra[1] + m * 2048);
     fa[m] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
     sa[m] = *((Byte)(uintptr_t)(rsa + k) + m * 64);
@@ -263,17 +266,18 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     fb[n] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
     sb[n] = *((Byte)(uintptr_t)(rsb + k) + n * 64);
   };
-  auto everyone_has_it = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  // the next stage's loads have landed (behind them there are at least those of the stages beyond), in all waves
+  auto everyone_has_it = [](auto beyond) { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(decltype(beyond)::value * kLoads) : "memory"); };
 
   Tile t = tile_at(index);
   aim(t);
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) request(i);
-  requested();
-  everyone_has_it();
+  for (int s = 0; s < S; ++s) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) request(i);
-  requested();
+    for (int i = 0; i < kLoads; ++i) request(i);
+    requested();
+  }
+  everyone_has_it(std::integral_constant<int, S - 1>{});
 #pragma unroll
   for (int m = 0; m < HM; ++m) read_a(m, 0);
 #pragma unroll
@@ -293,23 +297,20 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
 #pragma unroll
         for (int r = 0; r < kReads; ++r)  // a's first: their products come in this half.  Done by three quarters: the barrier waits for them
           if (r * 3 * kProducts / 4 / kReads == i) {
-            if (r < HM) read_a(HM + r, k & 3);
-            else read_b(HN + r - HM, k & 3);
+            if (r < HM) read_a(HM + r, set + (k & 3));
+            else read_b(HN + r - HM, set + (k & 3));
           }
         __builtin_amdgcn_sched_barrier(0);
       }
-      everyone_has_it();
+      everyone_has_it(std::integral_constant<int, S - 2>{});
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        ra[q] ^= kStage;
-        rb[q] ^= kStage;
+        ra[q] = S == 2 ? ra[q] ^ L::kStage : (ra[q] + L::kStage) & (L::kRing - 1);
+        rb[q] = S == 2 ? rb[q] ^ L::kStage : (rb[q] + L::kStage) & (L::kRing - 1);
       }
       const bool next_four = k + 1 == t.nk || (k & 3) == 3;
-      if (next_four) {
-        rsa ^= kScales;
-        rsb ^= kScales;
-      }
-      const unsigned next = next_four ? 0 : (k + 1) & 3;
+      if (next_four) set = (set + L::kScales) & (L::kSetRing - 1);
+      const unsigned next = next_four ? set : set + ((k + 1) & 3);
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
         const int m = i / HN, n = HN + i % HN;
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     if constexpr (PIECES) {
       store_piece<BM, BN>(p, acc, t.tile, t.piece, lane, wave);
     } else {
-      store_rows<BM, BN>(p, acc, smem, t.m0, t.n0, lane, wave);
+      store_rows<BM, BN, S>(p, acc, smem, t.m0, t.n0, lane, wave);
     }
     index += per_die;
     if (index >= last) break;
@@ -446,9 +447,12 @@ struct Plan {
   int tile, pieces, kb_piece;
 };
 constexpr int kFewRows = 32;
-// The fastest by these measured times: a step of 128 of K takes 1.42 us in a tile of 256, 0.85 in one of 128 that has its CU to itself, and
-// 1.0 where two share it; a tile 8 and 3 us beside its steps; the pieces' sums pass through memory at 1.4 TB/s.  (4,096^3: one round of
-// 256 tiles 58 us, of 128 73; 1,000 x 1,000 x 16,384: 16 tiles of 256 187 us, 64 of 128 112, in eight pieces 33.)
+// Tiles of 128 by whose number each has its CU to itself, and four stages on it instead of two (257 x 5,120 x 1,280: 10.3 and 10.0 us;
+// 512 x 5,120 x 5,120 40 and 31; 4,680 x 4,608 x 1,536, 1,332 tiles, 51 with four stages and 41 with two).
+constexpr int kAlone = 256;
+// The fastest by these measured times: a step of 128 of K takes 1.42 us in a tile of 256, 0.57 in one of 128 that has its CU to itself, and
+// 1.0 where two share it; a tile 8 and 4 us beside its steps; the pieces' sums pass through memory at 1.4 TB/s.  (4,096^3: one round of
+// 256 tiles 58 us, of 128 79; 1,000 x 1,000 x 16,384: 16 tiles of 256 186 us, 64 of 128 73, in four pieces 31.)
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
   const int kb = (int)((K + 127) / 128);
   if (M <= kFewRows) return {0, 1, kb};
@@ -461,8 +465,8 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
       if (made != pieces) continue;
       if (pieces > 1 && tiles * pieces > 1024) break;
       const int64_t all = tiles * pieces, resident = tile == 256 ? 256 : 512;
-      const double step = tile == 256 ? 1.42 : all <= 256 ? 0.85 : 1.0;
-      double us = (double)((all + resident - 1) / resident) * ((tile == 256 ? 8.0 : 3.0) + step * (pieces == 1 ? kb : per));
+      const double step = tile == 256 ? 1.42 : all <= kAlone ? 0.57 : 1.0;
+      double us = (double)((all + resident - 1) / resident) * ((tile == 256 ? 8.0 : 4.0) + step * (pieces == 1 ? kb : per));
       if (pieces > 1) us += 2.0 + (double)all * tile * tile * 4 / 1.4e6;
       if (us < least) {
         least = us;
@@ -478,25 +482,25 @@ bool sizes_ok(int64_t M, int64_t N, int64_t K) {
   return M > 0 && N > 0 && K > 0 && M < ((int64_t)1 << 31) && N < ((int64_t)1 << 31) && K <= (1 << 23) && (M + 127) / 128 * ((N + 127) / 128) < (1 << 27);
 }
 
-template <int BM, int BN, bool PIECES>
+template <int BM, int BN, int S, bool PIECES>
 int launch(hipStream_t st, const MatmulArgs& a) {
-  constexpr int kBytes = Layout<BM, BN>::kBytes, kResident = 256 * (160 * 1024 / kBytes);
+  constexpr int kBytes = Layout<BM, BN, S>::kBytes, kResident = 256 * (160 * 1024 / kBytes);
   static LdsOptIn flag;
-  const int rc = lds_opt_in(flag, reinterpret_cast<const void*>(&matmul_fp8_kernel<BM, BN, PIECES>), kBytes);
+  const int rc = lds_opt_in(flag, reinterpret_cast<const void*>(&matmul_fp8_kernel<BM, BN, S, PIECES>), kBytes);
   if (rc != MDATTN_OK) return rc;
   const int grid = a.chunk * 8 < kResident ? a.chunk * 8 : kResident;
-  MDATTN_LAUNCH((matmul_fp8_kernel<BM, BN, PIECES>), dim3((unsigned)grid), dim3(256), kBytes, st, a);
+  MDATTN_LAUNCH((matmul_fp8_kernel<BM, BN, S, PIECES>), dim3((unsigned)grid), dim3(256), kBytes, st, a);
   return launch_status();
 }
-template <int BM, int BN>
+template <int BM, int BN, int S>
 int launch_tiles(hipStream_t st, MatmulArgs& a, int pieces) {
   a.mt = (int)((a.M + BM - 1) / BM);
   a.nt = (int)((a.N + BN - 1) / BN);
   a.total = a.mt * a.nt * pieces;
   a.chunk = (a.total + 7) / 8;
-  if (pieces == 1) return launch<BM, BN, false>(st, a);
+  if (pieces == 1) return launch<BM, BN, S, false>(st, a);
   if (a.mt * a.nt > 65535) return MDATTN_E_UNSUPPORTED;  // (only few tiles are split)
-  const int rc = launch<BM, BN, true>(st, a);
+  const int rc = launch<BM, BN, S, true>(st, a);
   if (rc != MDATTN_OK) return rc;
   MDATTN_LAUNCH((join_pieces_kernel<BM, BN>), dim3(BM * BN / 1024, (unsigned)(a.mt * a.nt)), dim3(256), 0, st, a, pieces);
   return launch_status();
@@ -537,5 +541,7 @@ extern "C" int mdattn_matmul_fp8_block(void* stream, const void* a, const void* 
     else MDATTN_LAUNCH((matmul_fp8_rows_kernel<2, 8>), grid, dim3(512), 0, st, p);
     return launch_status();
   }
-  return plan.tile == 256 ? launch_tiles<256, 256>(st, p, plan.pieces) : launch_tiles<128, 128>(st, p, plan.pieces);
+  if (plan.tile == 256) return launch_tiles<256, 256, 2>(st, p, plan.pieces);
+  const bool alone = (M + 127) / 128 * ((N + 127) / 128) * plan.pieces <= kAlone;
+  return alone ? launch_tiles<128, 128, 4>(st, p, plan.pieces) : launch_tiles<128, 128, 2>(st, p, plan.pieces);
 }
