@@ -412,3 +412,58 @@ def test_in_a_graph(dev):
       graph.replay()
       torch.cuda.synchronize()
       assert all(torch.equal(p, q) for p, q in zip(got, call()))
+
+
+# ------------------------------------------------------------------------------------------------ all of them in one block
+def plain_block(block, x, modulation, freqs, heads, held):
+  """The example's block in 64 bits.  held(t, block_rows): a matrix as the dense layers' products see it."""
+  shift1, scale1, gate1, shift2, scale2, gate2 = modulation.double()
+  b = {n: t.double() for n, t in block.items()}
+
+  def norm(h, scale, shift):
+    return norm64(h, None, None, 1e-6, 0.0)[0] * (1 + scale[:, None]) + shift[:, None]
+
+  def dense(h, name, bias=True):
+    y = held(h.reshape(-1, h.shape[-1]), 1) @ held(b[name], 128).t()
+    return y.reshape(*h.shape[:-1], -1) + (b[name + "_bias"] if bias else 0.0)
+
+  def prologue(t, w):
+    t = t * (t.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w
+    t = torch.view_as_complex(t.reshape(*t.shape[:-1], heads, -1, 2)) * freqs[0, 0][None, :, None].to(torch.complex128)
+    return torch.view_as_real(t).flatten(-2).transpose(1, 2)
+
+  q, k, v = dense(norm(x.double(), scale1, shift1), "qkv").chunk(3, dim=-1)
+  q, k = prologue(q, b["norm_q"]), prologue(k, b["norm_k"])
+  v = v.reshape(*v.shape[:-1], heads, -1).transpose(1, 2)
+  att = torch.softmax(q @ k.transpose(-1, -2).contiguous() * q.shape[-1] ** -0.5, dim=-1) @ v
+  x = x.double() + gate1[:, None] * dense(att.transpose(1, 2).flatten(2), "out")
+  h = torch.nn.functional.gelu(dense(norm(x, scale2, shift2), "up"), approximate="tanh")
+  return x + gate2[:, None] * dense(h, "down")
+
+
+def test_example_block(dev):
+  """The example's block on a small clip, ragged against every tile: inference and training give one output, as near to 64 bits as
+  operands that are rounded to bf16 between the layers and then to e4m3 can be (2^-4 of a value at most in the dense layers' inputs, which
+  a sum over many of them averages out: a few hundredths of a half's output), and every weight gets a gradient."""
+  import importlib.util
+  import os
+
+  path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "wan_block_fp8.py")
+  spec = importlib.util.spec_from_file_location("wan_block_fp8", path)
+  ex = importlib.util.module_from_spec(spec)
+  spec.loader.exec_module(ex)
+  heads, grid = 2, (3, 6, 7)
+  block = ex.make_block(heads, dev)
+  x = rand(dev, 2, 126, 256, seed=1, dtype=BF16)
+  modulation, freqs = rand(dev, 6, 2, 256, seed=2, std=0.1), ex.rotary_table(*grid, dev)
+  with torch.no_grad():
+    y = ex.run_block(ex.quantize(block), x, modulation, freqs, heads)
+  same = plain_block(block, x, modulation, freqs, heads, lambda t, br: ops.quant_block_e4m3(t.float().contiguous(), br).dequantize(torch.float64))
+  full = plain_block(block, x, modulation, freqs, heads, lambda t, br: t)
+  part = (full - x.double()).norm()  # what the block adds
+  assert (y.double() - same).norm() <= 0.05 * part and (same - full).norm() <= 0.1 * part
+  leaves = [t.requires_grad_(True) for t in block.values()]
+  z = ex.run_block(block, x, modulation, freqs, heads)
+  assert (z.double() - same).norm() <= 0.05 * part
+  for name, g, t in zip(block, torch.autograd.grad(z.float().square().mean(), leaves), leaves):
+    assert g.shape == t.shape and bool(g.isfinite().all()) and bool((g != 0).any()), name
