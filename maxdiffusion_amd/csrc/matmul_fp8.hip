@@ -1,6 +1,7 @@
 // c [M, N] = a b^T + bias over e4m3 operands with one power-of-two scale per block of 128 along K:
 //   c[m, n] = sum over k-blocks 2^(ea[m, kb] + eb[n, kb]) sum over k in kb qa[m, k] qb[n, k]
-// The scales are operands of the matrix cores' scaled product (32 x 32 x 64): a block costs no instruction but the read of its byte.
+// The scales are operands of the matrix cores' scaled product (16 x 16 x 128, a block of K): a block costs no instruction but the read of its
+// scales' word and a shift.
 #include <type_traits>
 
 #include "mdattn_common.h"
@@ -220,8 +221,8 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   };
   unsigned scale_place = wave * 256;
   int aimed = index;  // the tile whose stages are being requested; past the die's last one, that one again
-  auto requested = [&] {
-    if ((requested_of_tile & 3) == 0) {  // the scales of four stages, with the first of them
+  auto request_scales = [&] {  // of four stages, with the first of them
+    if ((requested_of_tile & 3) == 0) {
 #pragma unroll
       for (int i = 0; i < kScaleLoads; ++i)
         lds_dma4((wave + 4 * i) * 64 < BM ? sa_at : sb_at, from_s[i], (unsigned)__builtin_amdgcn_readfirstlane(lds + L::kScaleAt + scale_place + i * 1024));
@@ -229,9 +230,13 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
       sb_at = uniform(sb_at + 4);
       scale_place = (scale_place + L::kScales) & (L::kSetRing - 1);
     }
+  };
+  auto advance = [&] {
     a_at = uniform(a_at + 128);
     b_at = uniform(b_at + 128);
     place = (place + L::kStage) & (L::kRing - 1);
+  };
+  auto count = [&] {
     ++requested_of_tile;
     if (--to_request == 0) {
       aimed += per_die;
@@ -246,7 +251,7 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   // the instruction.
   typedef const char __attribute__((address_space(3))) * Lds;
   typedef const u32x4 __attribute__((address_space(3))) * Quad;
-  typedef const uint8_t __attribute__((address_space(3))) * Byte;
+  typedef const int __attribute__((address_space(3))) * Word;
   unsigned ra[2], rb[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
@@ -256,15 +261,17 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   }
   const unsigned rsa = lds + L::kScaleAt + (wm * WM + l16) * 4, rsb = lds + L::kScaleAt + (BM + wn * WN + l16) * 4;
   unsigned set = 0;  // of scales, the one that is read
-  auto read_a = [&](int m, unsigned k) {  // k: the byte of the step's scales
+  // (a scale is read with its word, the four steps', and shifted where it is used: read as a byte it was masked, and waited for, at the
+  // end of a step)
+  auto read_a = [&](int m, unsigned set) {
     const u32x4 lo = *(Quad)((Lds)(uintptr_t)ra[0] + m * 2048), hi = *(Quad)((Lds)(uintptr_t)ra[1] + m * 2048);
     fa[m] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-    sa[m] = *((Byte)(uintptr_t)(rsa + k) + m * 64);
+    sa[m] = *((Word)(uintptr_t)(rsa + set) + m * 16);
   };
-  auto read_b = [&](int n, unsigned k) {
+  auto read_b = [&](int n, unsigned set) {
     const u32x4 lo = *(Quad)((Lds)(uintptr_t)rb[0] + n * 2048), hi = *(Quad)((Lds)(uintptr_t)rb[1] + n * 2048);
     fb[n] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-    sb[n] = *((Byte)(uintptr_t)(rsb + k) + n * 64);
+    sb[n] = *((Word)(uintptr_t)(rsb + set) + n * 16);
   };
   // the next stage's loads have landed (behind them there are at least those of the stages beyond), in all waves
   auto everyone_has_it = [](auto beyond) { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(decltype(beyond)::value * kLoads) : "memory"); };
@@ -275,7 +282,11 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   for (int s = 0; s < S; ++s) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) request(i);
-    requested();
+    request_scales();
+    if (s + 1 < S) {
+      advance();
+      count();
+    }
   }
   everyone_has_it(std::integral_constant<int, S - 1>{});
 #pragma unroll
@@ -290,43 +301,49 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
       for (int m = 0; m < TM; ++m) mfma_zero(acc[n][m]);
 #pragma unroll 1
     for (int k = 0; k < t.nk; ++k) {
+      const int shift = 8 * (k & 3);
+      unsigned next_set = set;
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
         const int m = i / HN, n = i % HN;
-        mfma(acc[n][m], fb[n], fa[m], sb[n], sa[m]);
+        mfma(acc[n][m], fb[n], fa[m], sb[n] >> shift, sa[m] >> shift);
 #pragma unroll
         for (int r = 0; r < kReads; ++r)  // a's first: their products come in this half.  Done by three quarters: the barrier waits for them
           if (r * 3 * kProducts / 4 / kReads == i) {
-            if (r < HM) read_a(HM + r, set + (k & 3));
-            else read_b(HN + r - HM, set + (k & 3));
+            if (r < HM) read_a(HM + r, set);
+            else read_b(HN + r - HM, set);
           }
+        // what a step keeps count of, a few instructions behind a product each
+        if (i == kProducts - 6) advance();
+        if (i == kProducts - 4) count();
+        if (i == kProducts - 2 && (k + 1 == t.nk || (k & 3) == 3)) next_set = (set + L::kScales) & (L::kSetRing - 1);
         __builtin_amdgcn_sched_barrier(0);
       }
       everyone_has_it(std::integral_constant<int, S - 2>{});
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        ra[q] = S == 2 ? ra[q] ^ L::kStage : (ra[q] + L::kStage) & (L::kRing - 1);
-        rb[q] = S == 2 ? rb[q] ^ L::kStage : (rb[q] + L::kStage) & (L::kRing - 1);
-      }
-      const bool next_four = k + 1 == t.nk || (k & 3) == 3;
-      if (next_four) set = (set + L::kScales) & (L::kSetRing - 1);
-      const unsigned next = next_four ? set : set + ((k + 1) & 3);
+      set = next_set;
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
         const int m = i / HN, n = HN + i % HN;
-        mfma(acc[n][m], fb[n], fa[m], sb[n], sa[m]);
+        mfma(acc[n][m], fb[n], fa[m], sb[n] >> shift, sa[m] >> shift);
+        if (i == 0) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            ra[q] = S == 2 ? ra[q] ^ L::kStage : (ra[q] + L::kStage) & (L::kRing - 1);
+            rb[q] = S == 2 ? rb[q] ^ L::kStage : (rb[q] + L::kStage) & (L::kRing - 1);
+          }
+        }
 #pragma unroll
         for (int r = 0; r < kReads; ++r)  // b's and a's in turn, a's behind the products that use up what was there
           if (r * kProducts / kReads == i) {
-            if (r % 2 == 0) read_b(r / 2, next);
-            else read_a(r / 2, next);
+            if (r % 2 == 0) read_b(r / 2, set);
+            else read_a(r / 2, set);
           }
 #pragma unroll
         for (int l = 0; l < kLoads; ++l)
           if (l * kProducts / kLoads == i) request(l);
+        if (i == kProducts - 1) request_scales();
         __builtin_amdgcn_sched_barrier(0);
       }
-      requested();
     }
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // (the last product's result: 16 passes and a few)
     if constexpr (PIECES) {
