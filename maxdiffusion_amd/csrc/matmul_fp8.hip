@@ -34,7 +34,7 @@ struct MatmulArgs {
   int64_t ld, ls;    // bytes of an operand's row, and of a row of scales
   int b_shift, bias_f32;
   int kb, kb_piece;  // k-blocks, and those of a piece (a multiple of 4)
-  int mt, nt, total, chunk;
+  int mt, nt, total;  // tiles: down, across, and with the pieces
   int wide;          // 16-byte stores of c
 };
 
@@ -60,7 +60,22 @@ struct Layout {
   static constexpr int kCols = BN >= 256 ? 64 : 32;  // columns that are turned at a time
   static constexpr int kTurnAt = kBiasAt + 4 * (BN / 2) * 4;
   static constexpr int kBytes = kTurnAt + 4 * 32 * kCols * 2;
+  static constexpr int kResident = 256 * (160 * 1024 / kBytes), kDieTiles = kResident / 8;
 };
+
+// The order of a product's tiles: down, then across, in bands of kBand rows of them.  A round of the resident workgroups so covers 16 rows and 16
+// columns of tiles of 256, of which each die takes 8 and 4: the dies share what they read through the memory's own cache, and a round's part
+// of both operands (32 x 256 rows of K bytes) stays in it up to a K of 30,000.  (Each die on a stretch of the order of its own, which reads
+// the same through its L2, needs 8 such stretches' rows: 18,900 x 5,120 x 15,360 1,160 us against 1,067, 75,600 x 5,120 x 13,824 4,155
+// against 3,763, 18,900 x 5,120 x 10,240 692 and 693.)
+constexpr int kBand = 16, kDieRows = 8, kDiesDown = kBand / kDieRows;
+struct TileAt {
+  int m, n;
+};
+__device__ __forceinline__ TileAt tile_of(int id, int mt, int nt) {
+  const int band = id / (kBand * nt), rows = min(mt - band * kBand, kBand), in = id - band * kBand * nt;
+  return {band * kBand + in % rows, in / rows};
+}
 
 // A wave's sums to memory: of each 16 x 16, lane l holds row l % 16 and columns 4 (l / 16) to + 3.  By whole rows, through LDS: 32 rows x kCols
 // columns at a time, 16-byte chunk c of row r at c ^ ((r >> 1) & (chunks - 1)).  (Stored from the registers, 16 bytes of a row at a time, they
@@ -166,28 +181,33 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, h = lane >> 4, wm = wave & 1, wn = wave >> 1;
 
-  // Neighbouring workgroups sit on different dies: each die takes a contiguous piece of the tiles, in groups of 8 rows of them.
+  // Round by round, as many tiles as there are resident workgroups, in the order of tile_of; of a last, smaller round each die takes a
+  // contiguous eighth.
   struct Tile {
     int64_t m0, n0;
     int tile, piece, kb0, nk;
   };
-  const int per_die = gridDim.x >> 3, die = blockIdx.x & 7;
-  auto tile_at = [&](int i) {  // i-th of the die
-    int id = min(die * p.chunk + min(i, p.chunk - 1), p.total - 1);
+  constexpr int kResident = L::kResident, kWide = L::kDieTiles / kDieRows;
+  const int die = blockIdx.x & 7, slot = blockIdx.x >> 3;  // neighbouring workgroups sit on different dies
+  const int full = p.total / kResident, rest = p.total % kResident, rest_die = (rest + 7) / 8;
+  const int in_full = ((die / kDiesDown) * kWide + slot / kDieRows) * kBand + (die % kDiesDown) * kDieRows + slot % kDieRows;
+  const int in_rest = die * rest_die + slot;
+  const int last = full + (slot < rest_die && in_rest < rest);  // rounds of this workgroup
+  auto tile_at = [&](int round) {
+    int id = round * kResident + (round < full ? in_full : in_rest);
     Tile t;
     t.piece = id / (p.mt * p.nt);
     id -= t.piece * p.mt * p.nt;
     t.tile = id;
-    const int band = id / (8 * p.nt), rows = min(p.mt - band * 8, 8), in = id - band * 8 * p.nt;
-    t.m0 = (int64_t)(band * 8 + in % rows) * BM;
-    t.n0 = (int64_t)(in / rows) * BN;
+    const TileAt at = tile_of(id, p.mt, p.nt);
+    t.m0 = (int64_t)at.m * BM;
+    t.n0 = (int64_t)at.n * BN;
     t.kb0 = t.piece * p.kb_piece;
     t.nk = min(p.kb_piece, p.kb - t.kb0);
     return t;
   };
-  const int last = min(p.chunk, p.total - die * p.chunk);  // tiles of this die
-  int index = blockIdx.x >> 3;
-  if (index >= last) return;
+  int round = 0;
+  if (last == 0) return;
 
   // what this lane loads: byte offsets from the tile's first row (rows past the end read the last one; they are not stored)
   unsigned from[kLoads], from_s[kScaleLoads];
@@ -220,7 +240,7 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     lds_dma16(i < kLoadsA ? a_at : b_at, from[i], (unsigned)__builtin_amdgcn_readfirstlane(place + i * 4096));
   };
   unsigned scale_place = wave * 256;
-  int aimed = index;  // the tile whose stages are being requested; past the die's last one, that one again
+  int aimed = 0;  // the round whose tile's stages are being requested; past the last one, that one again
   auto request_scales = [&] {  // of four stages, with the first of them
     if ((requested_of_tile & 3) == 0) {
 #pragma unroll
@@ -239,7 +259,7 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   auto count = [&] {
     ++requested_of_tile;
     if (--to_request == 0) {
-      aimed += per_die;
+      ++aimed;
       aim(tile_at(min(aimed, last - 1)));
     }
   };
@@ -276,7 +296,7 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   // the next stage's loads have landed (behind them there are at least those of the stages beyond), in all waves
   auto everyone_has_it = [](auto beyond) { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(decltype(beyond)::value * kLoads) : "memory"); };
 
-  Tile t = tile_at(index);
+  Tile t = tile_at(0);
   aim(t);
 #pragma unroll
   for (int s = 0; s < S; ++s) {
@@ -351,9 +371,8 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     } else {
       store_rows<BM, BN, S>(p, acc, smem, t.m0, t.n0, lane, wave);
     }
-    index += per_die;
-    if (index >= last) break;
-    t = tile_at(index);
+    if (++round >= last) break;
+    t = tile_at(round);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was requested past the end
 }
@@ -365,9 +384,9 @@ __global__ __launch_bounds__(256) void join_pieces_kernel(MatmulArgs p, int piec
   constexpr int TM = BM / 32, TN = BN / 32;
   const int tile = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
   const int lane = i & 63, m = (i >> 6) % TM, n = (i >> 6) / TM % TN, wave = i / (BM * BN / 16);
-  const int band = tile / (8 * p.nt), rows = min(p.mt - band * 8, 8), in = tile - band * 8 * p.nt;
-  const int64_t row = (int64_t)(band * 8 + in % rows) * BM + (wave & 1) * (BM / 2) + m * 16 + (lane & 15);
-  const int64_t col = (int64_t)(in / rows) * BN + (wave >> 1) * (BN / 2) + n * 16 + 4 * (lane >> 4);
+  const TileAt t = tile_of(tile, p.mt, p.nt);
+  const int64_t row = (int64_t)t.m * BM + (wave & 1) * (BM / 2) + m * 16 + (lane & 15);
+  const int64_t col = (int64_t)t.n * BN + (wave >> 1) * (BN / 2) + n * 16 + 4 * (lane >> 4);
   if (row >= p.M || col >= p.N) return;
   const f32x4* at = reinterpret_cast<const f32x4*>(p.part) + (int64_t)tile * (BM * BN / 4) + i;
   const int64_t step = (int64_t)p.mt * p.nt * (BM * BN / 4);
@@ -509,11 +528,12 @@ bool sizes_ok(int64_t M, int64_t N, int64_t K) {
 
 template <int BM, int BN, int S, bool PIECES>
 int launch(hipStream_t st, const MatmulArgs& a) {
-  constexpr int kBytes = Layout<BM, BN, S>::kBytes, kResident = 256 * (160 * 1024 / kBytes);
+  using L = Layout<BM, BN, S>;
+  constexpr int kBytes = L::kBytes;
   static LdsOptIn flag;
   const int rc = lds_opt_in(flag, reinterpret_cast<const void*>(&matmul_fp8_kernel<BM, BN, S, PIECES>), kBytes);
   if (rc != MDATTN_OK) return rc;
-  const int grid = a.chunk * 8 < kResident ? a.chunk * 8 : kResident;
+  const int grid = a.total < L::kResident ? (a.total + 7) / 8 * 8 : L::kResident;
   MDATTN_LAUNCH((matmul_fp8_kernel<BM, BN, S, PIECES>), dim3((unsigned)grid), dim3(256), kBytes, st, a);
   return launch_status();
 }
@@ -522,7 +542,6 @@ int launch_tiles(hipStream_t st, MatmulArgs& a, int pieces) {
   a.mt = (int)((a.M + BM - 1) / BM);
   a.nt = (int)((a.N + BN - 1) / BN);
   a.total = a.mt * a.nt * pieces;
-  a.chunk = (a.total + 7) / 8;
   if (pieces == 1) return launch<BM, BN, S, false>(st, a);
   if (a.mt * a.nt > 65535) return MDATTN_E_UNSUPPORTED;  // (only few tiles are split)
   const int rc = launch<BM, BN, S, true>(st, a);

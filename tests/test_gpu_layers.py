@@ -467,3 +467,85 @@ def test_example_block(dev):
   assert (z.double() - same).norm() <= 0.05 * part
   for name, g, t in zip(block, torch.autograd.grad(z.float().square().mean(), leaves), leaves):
     assert g.shape == t.shape and bool(g.isfinite().all()) and bool((g != 0).any()), name
+
+
+# ------------------------------------------------------------------------------------------------ many tiles, long tensors, in place
+@pytest.mark.parametrize("m,n,k", [(4116, 4096, 4096), (4300, 4096, 8192), (8200, 4500, 384), (8000, 2600, 4096), (16500, 4100, 1300)])
+def test_product_of_several_rounds_of_tiles(dev, m, n, k):
+  """Whole rounds of tiles and what they leave: a few rows, a split over K, a last round with idle workgroups.  Sums of whole numbers below
+  256 are exact; as few nonzeros as that needs."""
+  gen = torch.Generator(device=dev).manual_seed(0)
+  pick = lambda r: torch.randint(-2, 3, (r, k), generator=gen, device=dev) * (torch.rand((r, k), generator=gen, device=dev) < 3.0 * k**-0.5)
+  a, b = pick(m).float(), pick(n).float()
+  want = a @ b.t()
+  assert want.abs().max() < 256
+  qa, qb = ops.quant_block_e4m3(a.to(BF16)), ops.quant_block_e4m3(b.to(BF16), 128)
+  got = ops.matmul_fp8_block(qa, qb)
+  assert torch.equal(got.float(), want)
+  bias = torch.randint(-2, 3, (n,), generator=gen, device=dev).float()
+  assert torch.equal(ops.matmul_fp8_block(qa, qb, bias).float(), (want + bias).to(BF16).float())
+
+
+LONG = 430_000  # rows of 5,120: 2.2e9 elements, past 2^31
+
+
+def test_norm_past_2_31_elements(dev):
+  x = rand(dev, 1, LONG, 5120, seed=1, dtype=BF16)
+  w, b = rand(dev, 5120, seed=2), rand(dev, 5120, seed=3)
+  at = [0, 1, LONG // 2, 2**31 // 5120 - 1, 2**31 // 5120, LONG - 1]
+  some = x[:, at].contiguous()
+  y = ops.layer_norm(x, w, b, 1e-6, 0.0)
+  want, _, _, _, size = norm64(some, w, b, 1e-6, 0.0)
+  close(y[:, at], want, half_ulp(want, BF16) + 16 * U * size, "norm")
+  dx, _, db = ops.layer_norm_backward(x, w, b, y, 1e-6, 0.0)
+  _, h, r, m, _ = norm64(some, w, b, 1e-6, 0.0)
+  a = y[:, at].double() * m
+  want = r * (a - a.mean(-1, keepdim=True) - h * (a * h).mean(-1, keepdim=True))
+  hx = h.abs() + r * some.double().abs().amax(-1, keepdim=True)
+  size = r * (a.abs() + a.abs().mean(-1, keepdim=True) + hx * (a * h).abs().mean(-1, keepdim=True) + h.abs() * (a.abs() * hx).mean(-1, keepdim=True))
+  close(dx[:, at], want, half_ulp(want, BF16) + 32 * U * size, "dx")
+  # db: the sum of g's columns (in pieces: a tensor of g in 64 bits has no place here)
+  total, size = torch.zeros(5120, device=dev, dtype=torch.float64), torch.zeros(5120, device=dev, dtype=torch.float64)
+  for part in y[0].split(43_000):
+    total += part.double().sum(0)
+    size += part.double().abs().sum(0)
+  close(db, total, half_ulp(total, F32) + (2 * math.sqrt(LONG) + 16) * U * size, "db")
+
+
+def test_blocks_and_products_past_2_31_elements(dev):
+  x = rand(dev, LONG, 5120, seed=1, dtype=BF16)
+  at = [0, 2**31 // 5120 - 1, 2**31 // 5120, LONG - 1]
+  q = ops.quant_block_e4m3(x)
+  some = ops.quant_block_e4m3(x[at].contiguous())
+  assert torch.equal(q.values[at], some.values) and torch.equal(q.scales[at], some.scales)
+  q128, t128 = ops.quant_block_e4m3(x, 1, transposed=True)
+  assert torch.equal(q128.values[at], some.values)
+  last = x[LONG // 128 * 128 - 256 :]  # whole blocks of the transposed rows
+  _, tail_t = ops.quant_block_e4m3(last, 1, transposed=True)
+  assert torch.equal(t128.values[:, LONG // 128 * 128 - 256 : LONG], tail_t.values[:, : last.shape[0]])
+  del t128, q128, x
+  # rows of a, rows of b and rows of c past 2^31 bytes and elements
+  b = ops.quant_block_e4m3(rand(dev, 5120, 5120, seed=2, std=5120**-0.5), 128)
+  want, size = some.dequantize(torch.float64) @ b.dequantize(torch.float64).t(), some.dequantize(torch.float64).abs() @ b.dequantize(torch.float64).abs().t()
+  tol = 2.0**-8 * want.abs() + (1 + 2.0**-8) * 2.0**-11 * size + 1e-38
+  close(ops.matmul_fp8_block(q, b)[at], want, tol, "rows of a and of c")
+  few = ops.quant_block_e4m3(rand(dev, 40, 5120, seed=4))
+  want = few.dequantize(torch.float64) @ some.dequantize(torch.float64).t()
+  size = few.dequantize(torch.float64).abs() @ some.dequantize(torch.float64).abs().t()
+  tol = 2.0**-8 * want.abs() + (1 + 2.0**-8) * 2.0**-11 * size + 1e-38
+  close(ops.matmul_fp8_block(few, q)[:, at], want, tol, "rows of b")
+  one = ops.quant_block_e4m3(rand(dev, 40, 5120, seed=4)[:1].contiguous())
+  close(ops.matmul_fp8_block(one, q)[:, at], want[:1], tol[:1], "rows of b, one row of a")
+
+
+@pytest.mark.parametrize("c", [7, 512, 5120])
+def test_norm_in_place_at_the_c_entry(dev, lib, c):
+  import ctypes
+
+  P = ctypes.c_void_p
+  x = rand(dev, 2, 33, c, seed=1, dtype=BF16)
+  want = ops.layer_norm(x, None, None, 1e-6)
+  rc = lib.mdattn_layer_norm(P(torch.cuda.current_stream().cuda_stream), P(x.data_ptr()), 0, P(x.data_ptr()), 0, None, None, 1, 2, 33, c, 33 * c, c,
+                             33 * c, c, 0, 1e-6, 0.0)
+  assert rc == _lib.E_OK
+  assert torch.equal(x, want)
