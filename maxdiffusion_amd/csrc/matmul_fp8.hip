@@ -163,12 +163,16 @@ __device__ __forceinline__ void store_piece(const MatmulArgs& p, f32x4 (&acc)[TN
 // A workgroup of four waves in 2 x 2 computes BM x BN at a time, and as many such tiles as it takes for the resident workgroups to get through
 // all of them.  A stage of LDS holds 128 bytes of each row of both operands, written by direct loads; 16-byte chunk c of row r sits at
 // c ^ ((r >> 1) & 7), which spreads 16 rows' reads of one chunk over all banks.  A step multiplies all of a wave's rows of a with the
-// first half of its rows of b, then with the second.  Under the products of the first half the stage's remaining fragments are read (the second
-// halves of a and b); then the one barrier of the step, by which the next stage has landed and this one has been read; under the products of
-// the second half the next stage's first fragments are read, each into the registers of one that has been used up, and the stage S further on
-// is requested into the place of this one.  A matrix instruction keeps its pipe busy for 32 cycles, in which the wave issues the reads and
-// requests that stand behind it: their order is the program's (sched_barrier).  The stages are one stream over a workgroup's tiles: while the
-// outputs of one tile are stored, the first stages of the next are on their way.
+// first half of its rows of b, then with the second.  Under the products of the first half the stage's second fragments are read (the lower half
+// of a wave's rows has the first ones), and the lower halves of the stage S further on are requested into the place of this one's, which
+// all waves have read; under the products of the second half the next stage's first fragments are read, each into the registers of one that
+// has been used up, and the upper halves are requested.  A barrier ends each half.  So the requests are spread evenly (a CU takes 64 bytes a
+// cycle, half of a step's cycles for its 64 KB: all of them under one half stood in each other's way and the products'), and each has a
+// whole step to land: 75,600 x 5,120 x 5,120 on zeros, where power is no limit, 1,320 us with one barrier a step and the requests in its
+// second half, 1,191 so; on normal numbers 1,525 and 1,481.
+// A matrix instruction keeps its pipe busy for 32 cycles, in which the wave issues the reads and requests that stand behind it: their order is
+// the program's (sched_barrier).  The stages are one stream over a workgroup's tiles: while the outputs of one tile are stored, the first
+// stages of the next are on their way.
 template <int BM, int BN, int S, bool PIECES>
 __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   using L = Layout<BM, BN, S>;
@@ -239,6 +243,12 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   auto request = [&](int i) {  // its i-th load
     lds_dma16(i < kLoadsA ? a_at : b_at, from[i], (unsigned)__builtin_amdgcn_readfirstlane(place + i * 4096));
   };
+  // the order of a stage's loads: first the rows that a wave's first fragments are in, the lower half of its rows of a and of b
+  auto load_of = [](int l) {
+    constexpr int kRun = BM / 128;  // loads of half a wave's rows
+    const int in = l % (kLoads / 2);
+    return in / kRun * 2 * kRun + l / (kLoads / 2) * kRun + in % kRun;
+  };
   unsigned scale_place = wave * 256;
   int aimed = 0;  // the round whose tile's stages are being requested; past the last one, that one again
   auto request_scales = [&] {  // of four stages, with the first of them
@@ -293,26 +303,26 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     fb[n] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
     sb[n] = *((Word)(uintptr_t)(rsb + set) + n * 16);
   };
-  // the next stage's loads have landed (behind them there are at least those of the stages beyond), in all waves
-  auto everyone_has_it = [](auto beyond) { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(decltype(beyond)::value * kLoads) : "memory"); };
+  // the half of the next stage that is read next has landed (behind its loads there are at least those of S - 1 stages), and this wave has
+  // what it read: in all waves
+  auto everyone_has_it = [] { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 1) * kLoads) : "memory"); };
 
   Tile t = tile_at(0);
   aim(t);
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) request(i);
     request_scales();
-    if (s + 1 < S) {
-      advance();
-      count();
-    }
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) request(load_of(l));
+    advance();
+    count();
   }
-  everyone_has_it(std::integral_constant<int, S - 1>{});
+  everyone_has_it();
 #pragma unroll
   for (int m = 0; m < HM; ++m) read_a(m, 0);
 #pragma unroll
   for (int n = 0; n < HN; ++n) read_b(n, 0);
+  everyone_has_it();
   for (;;) {
     // zeros, made where they stay: from the vector registers they would be copied in every pass of the loop
 #pragma unroll
@@ -333,13 +343,14 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
             if (r < HM) read_a(HM + r, set);
             else read_b(HN + r - HM, set);
           }
-        // what a step keeps count of, a few instructions behind a product each
-        if (i == kProducts - 6) advance();
-        if (i == kProducts - 4) count();
+        if (i == 0) request_scales();
+#pragma unroll
+        for (int l = 0; l < kLoads / 2; ++l)
+          if ((2 * l + 1) * kProducts / kLoads == i) request(load_of(l));
         if (i == kProducts - 2 && (k + 1 == t.nk || (k & 3) == 3)) next_set = (set + L::kScales) & (L::kSetRing - 1);
         __builtin_amdgcn_sched_barrier(0);
       }
-      everyone_has_it(std::integral_constant<int, S - 2>{});
+      everyone_has_it();
       set = next_set;
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
@@ -354,16 +365,18 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
         }
 #pragma unroll
         for (int r = 0; r < kReads; ++r)  // b's and a's in turn, a's behind the products that use up what was there
-          if (r * kProducts / kReads == i) {
+          if (r * 3 * kProducts / 4 / kReads == i) {
             if (r % 2 == 0) read_b(r / 2, set);
             else read_a(r / 2, set);
           }
 #pragma unroll
-        for (int l = 0; l < kLoads; ++l)
-          if (l * kProducts / kLoads == i) request(l);
-        if (i == kProducts - 1) request_scales();
+        for (int l = 0; l < kLoads / 2; ++l)
+          if (2 * l * kProducts / kLoads == i) request(load_of(kLoads / 2 + l));
+        if (i == kProducts - 2) advance();
+        if (i == kProducts - 1) count();
         __builtin_amdgcn_sched_barrier(0);
       }
+      everyone_has_it();
     }
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // (the last product's result: 16 passes and a few)
     if constexpr (PIECES) {
