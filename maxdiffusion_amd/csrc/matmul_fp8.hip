@@ -291,17 +291,20 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   }
   const unsigned rsa = lds + L::kScaleAt + (wm * WM + l16) * 4, rsb = lds + L::kScaleAt + (BM + wn * WN + l16) * 4;
   unsigned set = 0;  // of scales, the one that is read
-  // (a scale is read with its word, the four steps', and shifted where it is used: read as a byte it was masked, and waited for, at the
-  // end of a step)
-  auto read_a = [&](int m, unsigned set) {
+  auto read_a = [&](int m) {
     const u32x4 lo = *(Quad)((Lds)(uintptr_t)ra[0] + m * 2048), hi = *(Quad)((Lds)(uintptr_t)ra[1] + m * 2048);
     fa[m] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-    sa[m] = *((Word)(uintptr_t)(rsa + set) + m * 16);
   };
-  auto read_b = [&](int n, unsigned set) {
+  auto read_b = [&](int n) {
     const u32x4 lo = *(Quad)((Lds)(uintptr_t)rb[0] + n * 2048), hi = *(Quad)((Lds)(uintptr_t)rb[1] + n * 2048);
     fb[n] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-    sb[n] = *((Word)(uintptr_t)(rsb + set) + n * 16);
+  };
+  // the scales of the first fragments (half 0) or of the second: words of four steps, shifted where they are used
+  auto read_scales = [&](int half) {
+#pragma unroll
+    for (int m = 0; m < HM; ++m) sa[half * HM + m] = *((Word)(uintptr_t)(rsa + set) + (half * HM + m) * 16);
+#pragma unroll
+    for (int n = 0; n < HN; ++n) sb[half * HN + n] = *((Word)(uintptr_t)(rsb + set) + (half * HN + n) * 16);
   };
   // the half of the next stage that is read next has landed (behind its loads there are at least those of S - 1 stages), and this wave has
   // what it read: in all waves
@@ -319,9 +322,10 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   }
   everyone_has_it();
 #pragma unroll
-  for (int m = 0; m < HM; ++m) read_a(m, 0);
+  for (int m = 0; m < HM; ++m) read_a(m);
 #pragma unroll
-  for (int n = 0; n < HN; ++n) read_b(n, 0);
+  for (int n = 0; n < HN; ++n) read_b(n);
+  read_scales(0);
   everyone_has_it();
   for (;;) {
     // zeros, made where they stay: from the vector registers they would be copied in every pass of the loop
@@ -332,26 +336,26 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
 #pragma unroll 1
     for (int k = 0; k < t.nk; ++k) {
       const int shift = 8 * (k & 3);
-      unsigned next_set = set;
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
         const int m = i / HN, n = i % HN;
         mfma(acc[n][m], fb[n], fa[m], sb[n] >> shift, sa[m] >> shift);
+        if (i == 0) {
+          if (shift == 0) read_scales(1);
+          request_scales();
+        }
 #pragma unroll
         for (int r = 0; r < kReads; ++r)  // a's first: their products come in this half.  Done by three quarters: the barrier waits for them
           if (r * 3 * kProducts / 4 / kReads == i) {
-            if (r < HM) read_a(HM + r, set);
-            else read_b(HN + r - HM, set);
+            if (r < HM) read_a(HM + r);
+            else read_b(HN + r - HM);
           }
-        if (i == 0) request_scales();
 #pragma unroll
         for (int l = 0; l < kLoads / 2; ++l)
           if ((2 * l + 1) * kProducts / kLoads == i) request(load_of(l));
-        if (i == kProducts - 2 && (k + 1 == t.nk || (k & 3) == 3)) next_set = (set + L::kScales) & (L::kSetRing - 1);
         __builtin_amdgcn_sched_barrier(0);
       }
       everyone_has_it();
-      set = next_set;
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
         const int m = i / HN, n = HN + i % HN;
@@ -366,9 +370,13 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
 #pragma unroll
         for (int r = 0; r < kReads; ++r)  // b's and a's in turn, a's behind the products that use up what was there
           if (r * 3 * kProducts / 4 / kReads == i) {
-            if (r % 2 == 0) read_b(r / 2, set);
-            else read_a(r / 2, set);
+            if (r % 2 == 0) read_b(r / 2);
+            else read_a(r / 2);
           }
+        if (i == 3 * kProducts / 4 && (k + 1 == t.nk || shift == 24)) {
+          set = (set + L::kScales) & (L::kSetRing - 1);
+          read_scales(0);
+        }
 #pragma unroll
         for (int l = 0; l < kLoads / 2; ++l)
           if (2 * l * kProducts / kLoads == i) request(load_of(kLoads / 2 + l));
