@@ -337,7 +337,7 @@ __global__ __launch_bounds__(MAXT) void layer_norm_bwd_kernel(NormBwdArgs a) {
   }
 }
 
-// out[g][c] = sum over i < n of part[g * n + i][plane][c], plane 0 to dw, 1 to db.  64 columns per workgroup, 16 partial sums each.
+// out[g][c] = sum over i < n of part[g * n + i][plane][c], plane 0 to dw, 1 to db.  64 columns of a group per workgroup, 16 partial sums each.
 struct SumArgs {
   const float* part;
   void *out0, *out1;
@@ -348,10 +348,10 @@ struct SumArgs {
 __global__ __launch_bounds__(1024) void sum_rows_kernel(SumArgs a) {
   __shared__ float part[16][64];
   const int lane = threadIdx.x & 63, i0 = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  const int64_t cols = (a.C + 63) / 64, group = blockIdx.x / cols, c = (blockIdx.x - group * cols) * 64 + lane;
   void* out = blockIdx.y ? a.out1 : a.out0;
   if (out == nullptr) return;
-  const float* p = a.part + blockIdx.z * a.n * a.row_stride + blockIdx.y * a.plane_stride + (c < a.C ? c : a.C - 1);
+  const float* p = a.part + group * a.n * a.row_stride + blockIdx.y * a.plane_stride + (c < a.C ? c : a.C - 1);
   float s = 0.f;
   int64_t i = i0;
   for (; i + 112 < a.n; i += 128) {  // eight loads on their way
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(SumArgs a) {
     s = 0.f;
 #pragma unroll
     for (int j = 0; j < 16; ++j) s += part[j][lane];
-    const int64_t at = blockIdx.z * a.C + c;
+    const int64_t at = group * a.C + c;
     if (a.f32) static_cast<float*>(out)[at] = s;
     else static_cast<__bf16*>(out)[at] = (__bf16)s;
   }
@@ -411,6 +411,23 @@ BwdShape bwd_shape(int64_t groups, int64_t rows, int C, int x_is_f32) {
   return b;
 }
 
+// A tensor's strides of a group and of a row.  Groups that share w and b, and follow one another as rows do, are one group of all rows.
+struct Strides {
+  int64_t *group, *row;
+};
+template <int N>
+void merge_groups(int64_t& groups, int64_t& rows, int64_t wb_stride, const Strides (&all)[N]) {
+  if (groups == 1 || wb_stride != 0) return;
+  for (const Strides& s : all) {
+    if (rows > 1 && *s.group != rows * *s.row) return;
+  }
+  if (rows == 1) {
+    for (const Strides& s : all) *s.row = *s.group;
+  }
+  rows *= groups;
+  groups = 1;
+}
+
 bool sizes_ok(int64_t groups, int64_t rows, int C) {
   return groups > 0 && rows > 0 && C > 0 && rows < ((int64_t)1 << 40) / groups;
 }
@@ -429,6 +446,8 @@ int launch_norm(hipStream_t st, const NormArgs& a, const Shape& s, unsigned grid
 }
 
 int norm(hipStream_t st, NormArgs& a, int x_is_f32, int out, int64_t groups) {
+  if (out == kToE4m3) merge_groups(groups, a.rows, a.wb_stride, {{&a.x_sg, &a.x_sr}});
+  else merge_groups(groups, a.rows, a.wb_stride, {{&a.x_sg, &a.x_sr}, {&a.y_sg, &a.y_sr}});
   const Shape s = shape_of(a.C);
   const int64_t row_bytes = (int64_t)a.C * (x_is_f32 ? 4 : 2);
   a.blocks = blocks_of(groups, a.rows, 256 * (int64_t)(out == kToE4m3 ? rows_per_cu(row_bytes, 36864, 2) : rows_per_cu(row_bytes, 18432, 1)));
@@ -475,7 +494,9 @@ extern "C" int mdattn_layer_norm_e4m3(void* stream, const void* x, int x_is_f32,
 
 extern "C" int64_t mdattn_layer_norm_bwd_workspace_floats(int64_t groups, int64_t rows, int C) {
   if (!sizes_ok(groups, rows, C) || C > kMaxC) return 0;
-  return groups * bwd_shape(groups, rows, C, 0).blocks * 2 * C;  // (bf16 rows: as many workgroups as f32 ones, or more)
+  // (bf16 rows: as many workgroups as f32 ones, or more; and for groups that are merged, or not)
+  const int64_t apart = groups * bwd_shape(groups, rows, C, 0).blocks, merged = bwd_shape(1, groups * rows, C, 0).blocks;
+  return (apart > merged ? apart : merged) * 2 * C;
 }
 
 extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, const void* g, void* dx, const void* w, void* dw, void* db,
@@ -489,15 +510,16 @@ extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, 
   if (!elem_aligned(x, x_is_f32) || !elem_aligned(g, x_is_f32) || !elem_aligned(dx, x_is_f32) || !elem_aligned(w, wb_is_f32) ||
       !elem_aligned(dw, wb_is_f32) || !elem_aligned(db, wb_is_f32) || !elem_aligned(workspace, 1))
     return MDATTN_E_ALIGN;
-  const BwdShape b = bwd_shape(groups, rows, C, x_is_f32);
   NormBwdArgs a{};
   a.x = x; a.g = g; a.w = w; a.dx = dx; a.part = sums ? workspace : nullptr;
   a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w_offset;
   a.x_sg = x_stride_group; a.x_sr = x_stride_row; a.g_sg = g_stride_group; a.g_sr = g_stride_row; a.d_sg = dx_stride_group; a.d_sr = dx_stride_row;
+  merge_groups(groups, a.rows, wb_stride, {{&a.x_sg, &a.x_sr}, {&a.g_sg, &a.g_sr}, {&a.d_sg, &a.d_sr}});
+  const BwdShape b = bwd_shape(groups, a.rows, C, x_is_f32);
   a.blocks = b.blocks;
   a.team = b.s.threads;
-  const int64_t grid = groups * a.blocks;
-  if (grid > 0x7FFFFFFF || groups > 65535) return MDATTN_E_UNSUPPORTED;
+  const int64_t grid = groups * a.blocks, sum_grid = (C + 63) / 64 * (wb_stride ? groups : 1);
+  if (grid > 0x7FFFFFFF || sum_grid > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   const unsigned threads = (unsigned)(b.s.threads * b.teams), lds = b.teams > 1 ? 8u * C : 0u;
 #define MDATTN_NORM(T, NV, MAXT)                                                                                                      \
@@ -513,9 +535,8 @@ extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, 
   const int rc = launch_status();
   if (rc != MDATTN_OK || !sums) return rc;
   // shared w and b: one sum over the workgroups of all groups
-  const int64_t out_groups = wb_stride ? groups : 1;
   const SumArgs r{workspace, dw, db, wb_stride ? a.blocks : grid, 2 * (int64_t)C, C, C, wb_is_f32};
-  MDATTN_LAUNCH(sum_rows_kernel, dim3((C + 63) / 64, 2, (unsigned)out_groups), dim3(1024), 0, st, r);
+  MDATTN_LAUNCH(sum_rows_kernel, dim3((unsigned)sum_grid, 2), dim3(1024), 0, st, r);
   return launch_status();
 }
 
