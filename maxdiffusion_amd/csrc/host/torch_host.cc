@@ -701,19 +701,25 @@ bool float_on(const Tensor& t, const Tensor& ref) {
 }
 int is_f32(const Tensor& t) { return t.defined() && t.scalar_type() == at::kFloat; }
 
-// x [..., C] as the norm walks it: the first axis, and the ones between it and the last, which have to be dense
+// x [..., C] as the norm walks it: the first axis, and the ones between it and the last, which have to be dense (an axis of one element
+// may have any stride)
 struct Rows3 {
   int64_t groups = 0, rows = 0, c = 0, sg = 0, sr = 0;
   int64_t all() const { return groups * rows; }
 };
 std::optional<Rows3> as_rows(const Tensor& x) {
   const int64_t n = x.dim();
-  if (n < 2 || x.numel() == 0 || x.stride(n - 1) != 1) return std::nullopt;
-  for (int64_t i = 1; i < n - 2; ++i)
-    if (x.stride(i) != x.stride(i + 1) * x.size(i + 1)) return std::nullopt;
+  if (n < 2 || x.numel() == 0 || (x.stride(n - 1) != 1 && x.size(n - 1) > 1)) return std::nullopt;
   Rows3 r;
   r.c = x.size(n - 1);
-  r.sr = x.stride(n - 2);
+  r.sr = n == 2 ? x.stride(0) : r.c;
+  int64_t next = -1;  // the stride that the next axis outwards has to have
+  for (int64_t i = n - 2; i > 0 && n > 2; --i) {
+    if (x.size(i) == 1) continue;
+    if (next < 0) r.sr = x.stride(i);
+    else if (x.stride(i) != next) return std::nullopt;
+    next = x.stride(i) * x.size(i);
+  }
   r.groups = n == 2 ? 1 : x.size(0);
   r.sg = n == 2 ? 0 : x.stride(0);
   r.rows = x.numel() / r.c / r.groups;

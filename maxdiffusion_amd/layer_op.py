@@ -23,9 +23,7 @@ def _wants_grad(*ts) -> bool:
 
 def _rows(x):
   """x [..., C] as the norm walks it: its last axis contiguous and the axes between the first and the last dense."""
-  if x.stride(-1) == 1 and (x.dim() <= 3 or all(x.stride(i) == x.stride(i + 1) * x.shape[i + 1] for i in range(1, x.dim() - 2))):
-    return x
-  return x.contiguous()
+  return x if (x.stride(-1) == 1 or x.shape[-1] == 1) and ops.row_stride(x) is not None else x.contiguous()
 
 
 class _HipLayerNorm(torch.autograd.Function):

@@ -603,12 +603,25 @@ def _norm_rows(x, name="x"):
     raise ValueError(f"{name} must have shape [..., C] with a contiguous last axis, got {tuple(x.shape)} strides {x.stride()}")
   if x.dim() == 2:
     return 1, x.shape[0], x.shape[1], 0, x.stride(0)
-  if x.dim() == 3:
-    return x.shape[0], x.shape[1], x.shape[2], x.stride(0), x.stride(1)
-  for i in range(1, x.dim() - 2):
-    if x.stride(i) != x.stride(i + 1) * x.shape[i + 1]:
-      raise ValueError(f"the axes of {name} between the first and the last must be dense, got {tuple(x.shape)} strides {x.stride()}")
-  return x.shape[0], math.prod(x.shape[1:-1]), x.shape[-1], x.stride(0), x.stride(-2)
+  step = row_stride(x)
+  if step is None:
+    raise ValueError(f"the axes of {name} between the first and the last must be dense, got {tuple(x.shape)} strides {x.stride()}")
+  return x.shape[0], math.prod(x.shape[1:-1]), x.shape[-1], x.stride(0), step
+
+
+def row_stride(x):
+  """The stride that all axes of x between the first and the last have together, None if there is none.  (An axis of one element may
+  have any.)"""
+  step = following = None
+  for i in range(x.dim() - 2, 0, -1):
+    if x.shape[i] == 1:
+      continue
+    if step is None:
+      step = x.stride(i)
+    elif x.stride(i) != following:
+      return None
+    following = x.stride(i) * x.shape[i]
+  return x.shape[-1] if step is None else step
 
 
 def _norm_vectors(weight, bias, groups, c):

@@ -549,3 +549,54 @@ def test_norm_in_place_at_the_c_entry(dev, lib, c):
                              33 * c, c, 0, 1e-6, 0.0)
   assert rc == _lib.E_OK
   assert torch.equal(x, want)
+
+
+# ------------------------------------------------------------------------------------------------ axes of one element, many groups
+@pytest.mark.parametrize("shape,strides", [((1, 1, 1), (0, 0, 0)), ((1, 1, 5, 64), (9, 7, 64, 1)), ((2, 1, 3, 64), (192, 5, 64, 1)),
+                                           ((1, 4, 1, 72), (3, 72, 11, 1)), ((3, 1), (1, 9)), ((1, 2, 3, 1), (0, 3, 1, 0))])
+def test_norm_of_axes_of_one_element_with_any_stride(dev, shape, strides):
+  """Such strides mean nothing, and `contiguous` leaves them as they are."""
+  size = 1 + sum((n - 1) * s for n, s in zip(shape, strides))
+  x, g = (rand(dev, size, seed=i, dtype=BF16).as_strided(shape, strides) for i in (1, 2))
+  plain_x, plain_g = (t.clone().reshape(-1).view(shape) for t in (x, g))
+  w = rand(dev, shape[-1], seed=3)
+  results = []
+  for a, b in ((x, g), (plain_x, plain_g)):
+    a, v = a.detach().requires_grad_(), w.clone().requires_grad_()
+    y = L.hip_layer_norm(a, v, None, 1e-3)
+    results.append((y, *torch.autograd.grad(y, (a, v), b)))
+    ops_y = ops.layer_norm(a.detach(), w, None, 1e-3)
+    assert torch.equal(ops_y, y)
+  for p, q in zip(*results):
+    assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("per_group", [False, True])
+def test_norm_of_very_many_groups(dev, per_group):
+  b, s, c = 70_001, 2, 64
+  x, g = rand(dev, b, s, c, seed=1, dtype=BF16), rand(dev, b, s, c, seed=2, dtype=BF16)
+  w, v = (rand(dev, *((b, c) if per_group else (c,)), seed=i, std=0.5) for i in (3, 4))
+  want, h, r, m, size = norm64(x, w, v, 1e-6, 1.0)
+  close(ops.layer_norm(x, w, v, 1e-6, 1.0), want, half_ulp(want, BF16) + 16 * U * size, "y")
+  dx, dw, db = ops.layer_norm_backward(x, w, v, g, 1e-6, 1.0)
+  a = g.double() * m
+  want = r * (a - a.mean(-1, keepdim=True) - h * (a * h).mean(-1, keepdim=True))
+  hx = h.abs() + r * x.double().abs().amax(-1, keepdim=True)
+  size = r * (a.abs() + a.abs().mean(-1, keepdim=True) + hx * (a * h).abs().mean(-1, keepdim=True) + h.abs() * (a.abs() * hx).mean(-1, keepdim=True))
+  close(dx, want, half_ulp(want, BF16) + 32 * U * size, "dx")
+  over, n = (1, s) if per_group else ((0, 1), b * s)
+  want_w, want_b = (g.double() * h).sum(over), g.double().sum(over)
+  slack = (2 * math.sqrt(n) + 16) * U
+  close(dw, want_w, half_ulp(want_w, F32) + slack * (g.double().abs() * hx).sum(over), "dw")
+  close(db, want_b, half_ulp(want_b, F32) + slack * g.double().abs().sum(over), "db")
+
+
+def test_norm_of_strided_groups_that_share_vectors(dev):
+  """Groups that are not one after the other, next to the same rows dense."""
+  big = rand(dev, 5, 9, 200, seed=1, dtype=BF16)
+  w = rand(dev, 200, seed=2)
+  for x in (big[:, 2:7], big[:, :1], big[::2], big[1:2, 3:]):
+    assert torch.equal(ops.layer_norm(x, w), ops.layer_norm(x.contiguous(), w))
+    assert torch.equal(ops.layer_norm_quant(x, w).values, ops.layer_norm_quant(x.contiguous(), w).values)
+    for p, q in zip(ops.layer_norm_backward(x, w, None, x)[:1], ops.layer_norm_backward(x.contiguous(), w, None, x.contiguous())[:1]):
+      assert torch.equal(p, q)
