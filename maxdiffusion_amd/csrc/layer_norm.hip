@@ -9,6 +9,8 @@
 // its own part and the squares around that mean; the parts join as  M2 = sum M2_w + n_w (mean_w - mean)^2  (Chan et al., Updating
 // formulae and a pairwise algorithm for computing sample variances, 1979), which loses nothing where the mean is large against the
 // deviation, and takes one exchange through LDS, and one barrier, per row.
+// Bound by memory.  bf16 rows, read and written: 75,600 x 5,120 forward 284 us and backward 426 us, both 5.4 TB/s; 32,760 x 1,536 35 us, 5.7 TB/s;
+// with a quantised output 30 us, 5.0 TB/s (75,600 x 5,120 252 us, 4.6: the scale bytes are scattered stores).
 #include "mdattn_common.h"
 #include "mdlayers.h"
 #include "quant_block.h"

@@ -48,13 +48,14 @@ __device__ __forceinline__ float bias_at(const void* p, int f32, int64_t i) {
   return f32 ? static_cast<const float*>(p)[i] : (float)static_cast<const __bf16*>(p)[i];
 }
 
-// What a workgroup keeps in LDS: S stages, sets of scale words (a set serves four stages, or a tile's last ones: as many sets as stages can be
+// What a workgroup keeps in LDS: two stages, sets of scale words (a set serves four stages, or a tile's last ones: as many sets as stages can be
 // under way, and the one that is read), each wave's bias values and a place to turn its outputs.  Stages and sets follow one another in rings
 // whose sizes are powers of two.
-template <int BM, int BN, int S>
+constexpr int kStages = 2;
+template <int BM, int BN>
 struct Layout {
-  static constexpr int kStage = (BM + BN) * 128, kScales = (BM + BN) * 4, kSets = S == 2 ? 4 : 8;
-  static constexpr int kRing = S * kStage, kSetRing = kSets * kScales;
+  static constexpr int kStage = (BM + BN) * 128, kScales = (BM + BN) * 4, kSets = 4;
+  static constexpr int kRing = kStages * kStage, kSetRing = kSets * kScales;
   static constexpr int kScaleAt = kRing;
   static constexpr int kBiasAt = kScaleAt + kSetRing;
   static constexpr int kCols = BN >= 256 ? 64 : 32;  // columns that are turned at a time
@@ -80,9 +81,9 @@ __device__ __forceinline__ TileAt tile_of(int id, int mt, int nt) {
 // A wave's sums to memory: of each 16 x 16, lane l holds row l % 16 and columns 4 (l / 16) to + 3.  By whole rows, through LDS: 32 rows x kCols
 // columns at a time, 16-byte chunk c of row r at c ^ ((r >> 1) & (chunks - 1)).  (Stored from the registers, 16 bytes of a row at a time, they
 // took as long as 20 steps.)
-template <int BM, int BN, int S, int TM, int TN>
+template <int BM, int BN, int TM, int TN>
 __device__ __forceinline__ void store_rows(const MatmulArgs& p, f32x4 (&acc)[TN][TM], char* smem, int64_t m0, int64_t n0, int lane, int wave) {
-  using L = Layout<BM, BN, S>;
+  using L = Layout<BM, BN>;
   constexpr int WM = BM / 2, WN = BN / 2;
   const int l16 = lane & 15, h = lane >> 4;
   m0 += (wave & 1) * WM;
@@ -164,18 +165,21 @@ __device__ __forceinline__ void store_piece(const MatmulArgs& p, f32x4 (&acc)[TN
 // all of them.  A stage of LDS holds 128 bytes of each row of both operands, written by direct loads; 16-byte chunk c of row r sits at
 // c ^ ((r >> 1) & 7), which spreads 16 rows' reads of one chunk over all banks.  A step multiplies all of a wave's rows of a with the
 // first half of its rows of b, then with the second.  Under the products of the first half the stage's second fragments are read (the lower half
-// of a wave's rows has the first ones), and the lower halves of the stage S further on are requested into the place of this one's, which
+// of a wave's rows has the first ones), and the lower halves of the stage two further on are requested into the place of this one's, which
 // all waves have read; under the products of the second half the next stage's first fragments are read, each into the registers of one that
 // has been used up, and the upper halves are requested.  A barrier ends each half.  So the requests are spread evenly (a CU takes 64 bytes a
 // cycle, half of a step's cycles for its 64 KB: all of them under one half stood in each other's way and the products'), and each has a
 // whole step to land: 75,600 x 5,120 x 5,120 on zeros, where power is no limit, 1,320 us with one barrier a step and the requests in its
 // second half, 1,191 so; on normal numbers 1,525 and 1,481.
+// Bound by the matrix cores under the chip's power limit: 75,600 x 5,120 x 5,120 at 2.7 PFLOP/s, on zeros at 3.4.  Of what is left on zeros,
+// the barriers cost 4 %, the requests 2 to 11 % (the longer K, the more comes from beyond L2), the stores of the outputs 1 to 6 %, turning
+// them 2.5 us a tile; the waits for what was requested nothing.
 // A matrix instruction keeps its pipe busy for 32 cycles, in which the wave issues the reads and requests that stand behind it: their order is
 // the program's (sched_barrier).  The stages are one stream over a workgroup's tiles: while the outputs of one tile are stored, the first
 // stages of the next are on their way.
-template <int BM, int BN, int S, bool PIECES>
+template <int BM, int BN, bool PIECES>
 __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
-  using L = Layout<BM, BN, S>;
+  using L = Layout<BM, BN>;
   constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16, HM = TM / 2, HN = TN / 2, kProducts = TM * HN;
   constexpr int kLoads = (BM + BN) / 32;  // direct loads of a stage by one wave: 8 rows each; the first of them a's rows
   constexpr int kLoadsA = BM / 32;
@@ -306,14 +310,14 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
 #pragma unroll
     for (int n = 0; n < HN; ++n) sb[half * HN + n] = *((Word)(uintptr_t)(rsb + set) + (half * HN + n) * 16);
   };
-  // the half of the next stage that is read next has landed (behind its loads there are at least those of S - 1 stages), and this wave has
+  // the half of the next stage that is read next has landed (behind its loads there are at least those of a stage), and this wave has
   // what it read: in all waves
-  auto everyone_has_it = [] { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 1) * kLoads) : "memory"); };
+  auto everyone_has_it = [] { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((kStages - 1) * kLoads) : "memory"); };
 
   Tile t = tile_at(0);
   aim(t);
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
+  for (int s = 0; s < kStages; ++s) {
     request_scales();
 #pragma unroll
     for (int l = 0; l < kLoads; ++l) request(load_of(l));
@@ -363,8 +367,8 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
         if (i == 0) {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            ra[q] = S == 2 ? ra[q] ^ L::kStage : (ra[q] + L::kStage) & (L::kRing - 1);
-            rb[q] = S == 2 ? rb[q] ^ L::kStage : (rb[q] + L::kStage) & (L::kRing - 1);
+            ra[q] ^= L::kStage;
+            rb[q] ^= L::kStage;
           }
         }
 #pragma unroll
@@ -390,7 +394,7 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
     if constexpr (PIECES) {
       store_piece<BM, BN>(p, acc, t.tile, t.piece, lane, wave);
     } else {
-      store_rows<BM, BN, S>(p, acc, smem, t.m0, t.n0, lane, wave);
+      store_rows<BM, BN>(p, acc, smem, t.m0, t.n0, lane, wave);
     }
     if (++round >= last) break;
     t = tile_at(round);
@@ -427,7 +431,7 @@ __global__ __launch_bounds__(256) void join_pieces_kernel(MatmulArgs p, int piec
 }
 
 // Few rows of a: bound by b's bytes, which pass straight from memory to the registers of the one wave that multiplies them (16 x 16 x 128: a
-// load covers 64 bytes of each of 16 rows; of 32 rows, 32 bytes, it was 20 % slower).  A workgroup takes 16 rows of b and all of a's, 16 TM
+// load covers 64 bytes of each of 16 rows; of 32 rows, 32 bytes, it was 20 % slower): 1 x 5,120 by 30,720 rows, 157 MB, 27 us, 5.8 TB/s.  A workgroup takes 16 rows of b and all of a's, 16 TM
 // at most; its waves share K out in groups of four blocks, a scale word's, and their sums meet in LDS in a fixed order.
 template <int TM, int W>
 __global__ __launch_bounds__(64 * W) void matmul_fp8_rows_kernel(MatmulArgs p) {
@@ -505,12 +509,10 @@ struct Plan {
   double us;
 };
 constexpr int kFewRows = 32;
-// Tiles of 128 by whose number each has its CU to itself, and four stages on it instead of two (257 x 5,120 x 1,280: 10.3 and 10.0 us;
-// 512 x 5,120 x 5,120 40 and 31; 4,680 x 4,608 x 1,536, 1,332 tiles, 51 with four stages and 41 with two).
-constexpr int kAlone = 256;
+constexpr int kAlone = 256;  // tiles of 128 by whose number each has its CU to itself
 // The fastest by these measured times: a step of 128 of K takes 1.42 us in a tile of 256, 0.57 in one of 128 that has its CU to itself, and
-// 1.0 where two share it; a tile 8 and 4 us beside its steps; the pieces' sums pass through memory at 1.4 TB/s.  (4,096^3: one round of
-// 256 tiles 58 us, of 128 79; 1,000 x 1,000 x 16,384: 16 tiles of 256 186 us, 64 of 128 73, in four pieces 31.)
+// 1.0 where two share it; a tile 8 and 4 us beside its steps; the pieces' sums pass through memory at 1.4 TB/s.  (4,096^3:
+// tiles of 256 54 us, of 128 65; 4,680 x 4,608 x 1,536 43 and 40; 1,000 x 1,000 x 16,384: 64 tiles of 128 whole 56, in four pieces 27.)
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
   const int kb = (int)((K + 127) / 128);
   if (M <= kFewRows) return {0, 1, kb, 4.0 + (double)N * K / 3e6};
@@ -547,25 +549,25 @@ bool sizes_ok(int64_t M, int64_t N, int64_t K) {
   return M > 0 && N > 0 && K > 0 && M < ((int64_t)1 << 31) && N < ((int64_t)1 << 31) && K <= (1 << 23) && (M + 127) / 128 * ((N + 127) / 128) < (1 << 27);
 }
 
-template <int BM, int BN, int S, bool PIECES>
+template <int BM, int BN, bool PIECES>
 int launch(hipStream_t st, const MatmulArgs& a) {
-  using L = Layout<BM, BN, S>;
+  using L = Layout<BM, BN>;
   constexpr int kBytes = L::kBytes;
   static LdsOptIn flag;
-  const int rc = lds_opt_in(flag, reinterpret_cast<const void*>(&matmul_fp8_kernel<BM, BN, S, PIECES>), kBytes);
+  const int rc = lds_opt_in(flag, reinterpret_cast<const void*>(&matmul_fp8_kernel<BM, BN, PIECES>), kBytes);
   if (rc != MDATTN_OK) return rc;
   const int grid = a.total < L::kResident ? (a.total + 7) / 8 * 8 : L::kResident;
-  MDATTN_LAUNCH((matmul_fp8_kernel<BM, BN, S, PIECES>), dim3((unsigned)grid), dim3(256), kBytes, st, a);
+  MDATTN_LAUNCH((matmul_fp8_kernel<BM, BN, PIECES>), dim3((unsigned)grid), dim3(256), kBytes, st, a);
   return launch_status();
 }
-template <int BM, int BN, int S>
+template <int BM, int BN>
 int launch_tiles(hipStream_t st, MatmulArgs& a, int pieces) {
   a.mt = (int)((a.M + BM - 1) / BM);
   a.nt = (int)((a.N + BN - 1) / BN);
   a.total = a.mt * a.nt * pieces;
-  if (pieces == 1) return launch<BM, BN, S, false>(st, a);
+  if (pieces == 1) return launch<BM, BN, false>(st, a);
   if (a.mt * a.nt > 65535) return MDATTN_E_UNSUPPORTED;  // (only few tiles are split)
-  const int rc = launch<BM, BN, S, true>(st, a);
+  const int rc = launch<BM, BN, true>(st, a);
   if (rc != MDATTN_OK) return rc;
   MDATTN_LAUNCH((join_pieces_kernel<BM, BN>), dim3(BM * BN / 1024, (unsigned)(a.mt * a.nt)), dim3(256), 0, st, a, pieces);
   return launch_status();
@@ -581,9 +583,7 @@ int run(hipStream_t st, MatmulArgs p, Plan plan, int64_t workspace_floats, float
     else MDATTN_LAUNCH((matmul_fp8_rows_kernel<2, 8>), grid, dim3(512), 0, st, p);
     return launch_status();
   }
-  if (plan.tile == 256) return launch_tiles<256, 256, 2>(st, p, plan.pieces);
-  const bool alone = (p.M + 127) / 128 * ((p.N + 127) / 128) * plan.pieces <= kAlone;
-  return alone ? launch_tiles<128, 128, 4>(st, p, plan.pieces) : launch_tiles<128, 128, 2>(st, p, plan.pieces);
+  return plan.tile == 256 ? launch_tiles<256, 256>(st, p, plan.pieces) : launch_tiles<128, 128>(st, p, plan.pieces);
 }
 
 }  // namespace

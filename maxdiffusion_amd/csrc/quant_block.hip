@@ -30,7 +30,8 @@ struct QuantArgs {
   int64_t units;
 };
 
-// Rows alone, blocks of 1 x 128: 16 lanes to a block, four blocks per thread in flight.
+// Rows alone, blocks of 1 x 128: 16 lanes to a block, four blocks per thread in flight.  Bound by memory: 75,600 x 5,120 in bf16 203 us,
+// 5.7 TB/s read and written.
 constexpr int kUnits = 4;
 template <typename T>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
@@ -61,6 +62,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
 // A tile of 128 x 128 per workgroup.  A thread holds 8 rows x 8 columns: the 16 lanes of a row group cover a row's 128 columns, the 16
 // row groups the 128 rows.  The transposed bytes go through LDS, 8 rows of a column in one word, so that whole 128-byte rows of qt
 // are stored; word g of column c sits at g ^ (c / 8), without which the 16 lanes that write 8 columns apart would meet in one bank.
+// Bound by memory: both ways in blocks of 128 x 128, 15,360 x 5,120 in bf16, 55 us, 5.7 TB/s; of 1 x 128, 18,900 x 5,120, 77 to 83 us, 4.7 to
+// 5.0 TB/s, of which the transposed scales' bytes, each a store to a line of its own, cost a tenth.
 template <typename T, int BLOCK_ROWS>
 __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
   __shared__ u32x2 tile[128][16];
