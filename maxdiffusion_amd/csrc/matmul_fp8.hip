@@ -282,14 +282,15 @@ __global__ __launch_bounds__(256) void matmul_fp8_kernel(MatmulArgs p) {
   i32x8 fa[TM], fb[TN];
   int sa[TM], sb[TN];
   // where this lane's two 16-byte chunks of a fragment, and its scale, are in the stage that is read: the rest of an address is a constant of
-  // the instruction.
+  // the instruction.  (Chunks h and h + 4: which bytes of a block meet in which lane is free where it is the same for a and b.  The read
+  // serves lanes of different h together: with chunks 2 h and 2 h + 1 they met in their banks, 8.1 cycles a read against 4.3.)
   typedef const char __attribute__((address_space(3))) * Lds;
   typedef const u32x4 __attribute__((address_space(3))) * Quad;
   typedef const int __attribute__((address_space(3))) * Word;
   unsigned ra[2], rb[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
-    const int chunk = ((2 * h + q) ^ ((l16 >> 1) & 7)) * 16;
+    const int chunk = ((h + 4 * q) ^ ((l16 >> 1) & 7)) * 16;
     ra[q] = lds + (wm * WM + l16) * 128 + chunk;
     rb[q] = lds + (BM + wn * WN + l16) * 128 + chunk;
   }
