@@ -30,13 +30,13 @@ struct QuantArgs {
   int64_t units;
 };
 
-// Rows alone, blocks of 1 x 128: 16 lanes to a block, four blocks per thread in flight.  Bound by memory: 75,600 x 5,120 in bf16 203 us,
-// 5.7 TB/s read and written.
+// Rows alone, blocks of 1 x 128: 16 lanes to a block, four blocks per thread in flight.  Bound by memory: 75,600 x 5,120 in bf16 194 to 216 us,
+// 5.4 to 6.0 TB/s read and written.
 constexpr int kUnits = 4;
 template <typename T>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
   const int l16 = threadIdx.x & 15;
-  // one division of 64 bits, of the workgroup's first block, and small ones from there: 1 x 5,120, one workgroup, 2.6 and 2.0 us
+  // one division of 64 bits, of the workgroup's first block, and small ones from there: 1 x 5,120, one workgroup, 2.6 and 2.3 us
   const int64_t first = (int64_t)blockIdx.x * (16 * kUnits), row0 = first / a.blocks;
   const unsigned block0 = (unsigned)(first - row0 * a.blocks) + (threadIdx.x >> 4);
   const int64_t left = a.units - first - (threadIdx.x >> 4);
