@@ -213,7 +213,7 @@ struct NormBwdArgs {
 template <typename T, int NV, int MAXT, bool TAIL>
 __global__ __launch_bounds__(MAXT) void layer_norm_bwd_kernel(NormBwdArgs a) {
   __shared__ float4 part[2][kMaxWaves];
-  extern __shared__ float sums[];  // [2][C], of several teams
+  extern __shared__ __align__(16) float sums[];  // of several teams: [team][2][C rounded up to 8]
   const int group = blockIdx.x / a.blocks, block = blockIdx.x - group * a.blocks;
   const int teams = blockDim.x / a.team, waves = a.team >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave / waves, first_wave = mine * waves;
@@ -306,32 +306,35 @@ __global__ __launch_bounds__(MAXT) void layer_norm_bwd_kernel(NormBwdArgs a) {
     }
   }
   if (a.part == nullptr) return;
-  for (int i = 1; i < teams; ++i) {  // team 0 takes over the others', one after the other
-    __syncthreads();
-    if (mine == i) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (deal.has(j, e)) {
-            sums[deal.c[j] + e] = dw[j][e];
-            sums[a.C + deal.c[j] + e] = db[j][e];
-          }
-    }
-    __syncthreads();
-    if (mine == 0) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (deal.has(j, e)) {
-            dw[j][e] += sums[deal.c[j] + e];
-            db[j][e] += sums[a.C + deal.c[j] + e];
-          }
-    }
-  }
-  if (mine != 0) return;
   float* p = a.part + (int64_t)blockIdx.x * 2 * a.C;
+  if (teams > 1) {  // each team's row of sums to LDS, then every thread adds up a few columns of all teams, in their order
+    const int ld = (a.C + 7) / 8 * 8;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (deal.c[j] >= a.C) continue;
+      f32x4* at = reinterpret_cast<f32x4*>(sums + mine * 2 * ld + deal.c[j]);
+      at[0] = f32x4{dw[j][0], dw[j][1], dw[j][2], dw[j][3]};
+      at[1] = f32x4{dw[j][4], dw[j][5], dw[j][6], dw[j][7]};
+      at += ld / 4;
+      at[0] = f32x4{db[j][0], db[j][1], db[j][2], db[j][3]};
+      at[1] = f32x4{db[j][4], db[j][5], db[j][6], db[j][7]};
+    }
+    __syncthreads();
+    for (int i = threadIdx.x * 4; i < 2 * ld; i += blockDim.x * 4) {
+      f32x4 s = *reinterpret_cast<const f32x4*>(sums + i);
+      for (int t = 1; t < teams; ++t) s += *reinterpret_cast<const f32x4*>(sums + t * 2 * ld + i);
+      const int plane = i >= ld, c = i - plane * ld;
+      float* out = p + plane * a.C + c;
+      if (!TAIL || c + 4 <= a.C) {
+        *reinterpret_cast<f32x4_any*>(out) = s;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < a.C) out[e] = s[e];
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     deal.keep(j, p, dw[j]);
@@ -452,7 +455,9 @@ int norm(hipStream_t st, NormArgs& a, int x_is_f32, int out, int64_t groups) {
   else merge_groups(groups, a.rows, a.wb_stride, {{&a.x_sg, &a.x_sr}, {&a.y_sg, &a.y_sr}});
   const Shape s = shape_of(a.C);
   const int64_t row_bytes = (int64_t)a.C * (x_is_f32 ? 4 : 2);
-  a.blocks = blocks_of(groups, a.rows, 256 * (int64_t)(out == kToE4m3 ? rows_per_cu(row_bytes, 36864, 2) : rows_per_cu(row_bytes, 18432, 1)));
+  const int64_t target = 256 * (int64_t)(out == kToE4m3 ? rows_per_cu(row_bytes, 36864, 2) : rows_per_cu(row_bytes, 18432, 1));
+  // a few rows per workgroup: one each, whose latencies then overlap (2,674 x 1,001 in f32 8.1 and 6.7 us, 4,680 x 1,536 7.8 and 6.8)
+  a.blocks = groups * a.rows <= 4 * target ? (int)a.rows : blocks_of(groups, a.rows, target);
   const int64_t grid = groups * a.blocks;
   if (grid > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
   if (x_is_f32) {
@@ -523,7 +528,7 @@ extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, 
   const int64_t grid = groups * a.blocks, sum_grid = (C + 63) / 64 * (wb_stride ? groups : 1);
   if (grid > 0x7FFFFFFF || sum_grid > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
-  const unsigned threads = (unsigned)(b.s.threads * b.teams), lds = b.teams > 1 ? 8u * C : 0u;
+  const unsigned threads = (unsigned)(b.s.threads * b.teams), lds = b.teams > 1 ? b.teams * 8u * (unsigned)ceil_to(C, 8) : 0u;
 #define MDATTN_NORM(T, NV, MAXT)                                                                                                      \
   if (b.s.nv == NV && (threads <= 256 ? 256 : threads) == MAXT) {                                                                         \
     if (C % 8) MDATTN_LAUNCH((layer_norm_bwd_kernel<T, NV, MAXT, true>), dim3((unsigned)grid), dim3(threads), lds, st, a);          \
