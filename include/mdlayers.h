@@ -5,6 +5,9 @@
  * Part of libmdattn.so, with the conventions and the MDATTN_E_* codes of mdattn.h: a HIP stream first, work only enqueued,
  * nothing allocated or synchronised, arguments checked on the host before any launch, caller-owned device pointers,
  * re-entrant.
+ *
+ * A grid has fewer than 2^32 threads: MDATTN_E_UNSUPPORTED, before anything is launched, for norms of more than 2^32 / 1024 groups that
+ * are not walked as one and need more, for dw and db of more than 2^22 groups x 64 channels, and for quantising 2^38 elements.
  */
 #ifndef MDLAYERS_H_
 #define MDLAYERS_H_

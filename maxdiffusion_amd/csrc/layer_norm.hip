@@ -461,7 +461,7 @@ int norm(hipStream_t st, NormArgs& a, int x_is_f32, int out, int64_t groups) {
   // a few rows per workgroup: one each, whose latencies then overlap (2,674 x 1,001 in f32 8.1 and 6.7 us, 4,680 x 1,536 7.8 and 6.8)
   a.blocks = groups * a.rows <= 4 * target ? (int)a.rows : blocks_of(groups, a.rows, target);
   const int64_t grid = groups * a.blocks;
-  if (grid > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
+  if (!grid_fits(grid, s.threads)) return MDATTN_E_UNSUPPORTED;
   if (x_is_f32) {
     if (out == kToE4m3) return launch_norm<float, kToE4m3>(st, a, s, (unsigned)grid);
     return out == kToF32 ? launch_norm<float, kToF32>(st, a, s, (unsigned)grid) : launch_norm<float, kToBf16>(st, a, s, (unsigned)grid);
@@ -528,7 +528,7 @@ extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, 
   a.blocks = b.blocks;
   a.team = b.s.threads;
   const int64_t grid = groups * a.blocks, sum_grid = (C + 63) / 64 * (wb_stride ? groups : 1);
-  if (grid > 0x7FFFFFFF || sum_grid > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
+  if (!grid_fits(grid, b.s.threads * b.teams) || (sums && !grid_fits(sum_grid, 1024))) return MDATTN_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   const unsigned threads = (unsigned)(b.s.threads * b.teams), lds = b.teams > 1 ? b.teams * 8u * (unsigned)ceil_to(C, 8) : 0u;
 #define MDATTN_NORM(T, NV, MAXT)                                                                                                      \
@@ -551,7 +551,7 @@ extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, 
 
 extern "C" int mdattn_sum_rows(void* stream, const float* rows, int64_t n, int64_t C, void* out, int out_is_f32) {
   if (!rows || !out || n <= 0 || C <= 0) return MDATTN_E_BADARG;
-  if ((C + 63) / 64 > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
+  if (!grid_fits((C + 63) / 64, 1024)) return MDATTN_E_UNSUPPORTED;
   if (!elem_aligned(rows, 1) || !elem_aligned(out, out_is_f32)) return MDATTN_E_ALIGN;
   const SumArgs r{rows, out, nullptr, n, C, 0, C, out_is_f32};
   MDATTN_LAUNCH(sum_rows_kernel, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, (hipStream_t)stream, r);

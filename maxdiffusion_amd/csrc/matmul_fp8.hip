@@ -516,7 +516,7 @@ constexpr int kAlone = 256;  // tiles of 128 by whose number each has its CU to 
 // tiles of 256 54 us, of 128 65; 4,680 x 4,608 x 1,536 43 and 40; 1,000 x 1,000 x 16,384: 64 tiles of 128 whole 56, in four pieces 27.)
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
   const int kb = (int)((K + 127) / 128);
-  if (M <= kFewRows) return {0, 1, kb, 4.0 + (double)N * K / 3e6};
+  if (M <= kFewRows && grid_fits((N + 15) / 16, 512)) return {0, 1, kb, 4.0 + (double)N * K / 3e6};
   Plan best{128, 1, (kb + 3) / 4 * 4, 1e30};
   for (int tile = 128; tile <= 256; tile += 128) {
     const int64_t tiles = (M + tile - 1) / tile * ((N + tile - 1) / tile);

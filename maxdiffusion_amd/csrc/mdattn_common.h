@@ -209,12 +209,25 @@ inline bool strides_ok(const mdattn_strides* s, int64_t mult) {
 // code left pending would otherwise surface here as MDATTN_E_LAUNCH of a launch that went fine: MDATTN_LAUNCH reads
 // the pending error first.  That clears it: a caller who wants to see its own sticky error has to read it before
 // calling into the library.
-#define MDATTN_LAUNCH(...)         \
-  do {                             \
-    (void)hipGetLastError();       \
-    hipLaunchKernelGGL(__VA_ARGS__); \
+// A grid is counted in threads, in 32 bits, and the runtime takes a larger one without an error: it runs modulo 2^32 (67,200,000
+// workgroups of 64: 91,136 ran).  Such a launch is not made, and launch_status() says so; an entry of several launches asks
+// grid_fits() before its first.
+inline bool grid_fits(int64_t workgroups, int64_t threads) { return workgroups <= 0x7FFFFFFF && workgroups * threads <= 0xFFFFFFFFll; }
+inline bool& launch_left_out() {
+  static thread_local bool left_out = false;
+  return left_out;
+}
+#define MDATTN_LAUNCH(kernel, grid, block, ...)                                           \
+  do {                                                                                    \
+    const dim3 mdattn_grid = (grid), mdattn_block = (block);                              \
+    (void)hipGetLastError();                                                              \
+    mdattn::launch_left_out() = !mdattn::grid_fits(mdattn_grid.x, mdattn_block.x);        \
+    if (!mdattn::launch_left_out()) hipLaunchKernelGGL(kernel, mdattn_grid, mdattn_block, __VA_ARGS__); \
   } while (0)
-inline int launch_status() { return hipGetLastError() == hipSuccess ? MDATTN_OK : MDATTN_E_LAUNCH; }
+inline int launch_status() {
+  if (launch_left_out()) return MDATTN_E_UNSUPPORTED;
+  return hipGetLastError() == hipSuccess ? MDATTN_OK : MDATTN_E_LAUNCH;
+}
 
 // A kernel that needs more dynamic LDS than the default limit has to opt in with hipFuncSetAttribute, once per
 // kernel and device: one LdsOptIn per kernel instance remembers the devices that have been told.

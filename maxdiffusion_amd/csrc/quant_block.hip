@@ -201,16 +201,15 @@ extern "C" int mdattn_quant_block_e4m3(void* stream, const void* x, int x_is_f32
   a.ldq = ceil_to(C, 128); a.lds = scale_stride(C); a.ldt = ceil_to(R, 128); a.ldst = scale_stride(R);
   a.blocks = (int)((C + 127) / 128);
   hipStream_t st = (hipStream_t)stream;
-  if (block_rows == 1 && !qt && !colsum) {
-    a.units = R * a.blocks;
-    const int64_t grid = (a.units + 16 * kUnits - 1) / (16 * kUnits);
-    if (grid > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
-    if (x_is_f32) MDATTN_LAUNCH((quant_rows_kernel<float>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    else MDATTN_LAUNCH((quant_rows_kernel<__bf16>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  a.units = R * a.blocks;
+  const int64_t rows_grid = (a.units + 16 * kUnits - 1) / (16 * kUnits);
+  if (block_rows == 1 && !qt && !colsum && grid_fits(rows_grid, 256)) {  // (past 1.07e9 blocks by tiles, of which there are half as many)
+    if (x_is_f32) MDATTN_LAUNCH((quant_rows_kernel<float>), dim3((unsigned)rows_grid), dim3(256), 0, st, a);
+    else MDATTN_LAUNCH((quant_rows_kernel<__bf16>), dim3((unsigned)rows_grid), dim3(256), 0, st, a);
     return launch_status();
   }
   const int64_t grid = (R + 127) / 128 * a.blocks;
-  if (grid > 0x7FFFFFFF) return MDATTN_E_UNSUPPORTED;
+  if (!grid_fits(grid, 256)) return MDATTN_E_UNSUPPORTED;
 #define MDATTN_QUANT(T, BR) MDATTN_LAUNCH((quant_tile_kernel<T, BR>), dim3((unsigned)grid), dim3(256), 0, st, a)
   if (x_is_f32) { if (block_rows == 1) MDATTN_QUANT(float, 1); else MDATTN_QUANT(float, 128); }
   else { if (block_rows == 1) MDATTN_QUANT(__bf16, 1); else MDATTN_QUANT(__bf16, 128); }

@@ -1,0 +1,39 @@
+"""The layers beside attention as programs use them: calls past what a grid can count, outputs that are changed in place, hooks, autograd's
+other modes, arguments that the usual path leaves aside.  Tolerances as in the tests of the kernels: bit for bit where nothing is said."""
+import torch
+
+import pytest
+
+from maxdiffusion_amd import ops
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def rand(dev, *shape, seed=0, dtype=F32, std=1.0):
+  gen = torch.Generator(device=dev).manual_seed(seed)
+  return (torch.randn(shape, generator=gen, device=dev) * std).to(dtype)
+
+
+# ------------------------------------------------------------------------------------------------ grids past 2^32 threads
+def test_one_row_against_very_many_columns(dev):
+  """More rows of b than workgroups of 16 of them can be launched."""
+  n = 134_300_000  # 8,393,750 workgroups of 512 threads: 2^32 is 8,388,608
+  values = torch.zeros((n, 128), dtype=torch.uint8, device=dev)
+  values[:, 0] = torch.arange(n, device=dev, dtype=torch.int32).remainder_(64).add_(8).to(torch.uint8)
+  b = ops.BlockQuant(values, torch.full((n, 4), 127, dtype=torch.uint8, device=dev), n, 1, 1)
+  a = ops.quant_block_e4m3(torch.ones((1, 1), dtype=BF16, device=dev))
+  got = ops.matmul_fp8_block(a, b)
+  assert torch.equal(got[0], values[:, 0].contiguous().view(torch.float8_e4m3fn).to(BF16))
+
+
+def test_quantising_very_many_blocks(dev):
+  """More blocks than the kernel of rows alone can be launched for."""
+  n = 1_080_000_000  # 16,875,000 workgroups of 256 threads: 2^32 is 16,777,216
+  x = torch.arange(n, dtype=torch.int32, device=dev).remainder_(250).add_(1).to(BF16).view(n, 1)
+  q = ops.quant_block_e4m3(x)
+  some = ops.quant_block_e4m3(x[:250].contiguous())
+  for i in range(0, n, 60_000_000):  # (a whole number of periods)
+    assert torch.equal(q.values[i : i + 60_000_000, 0].view(-1, 250), some.values[:, 0].expand(240_000, 250))
+    assert torch.equal(q.scales[i : i + 60_000_000, 0].view(-1, 250), some.scales[:, 0].expand(240_000, 250))
+  assert not bool(q.values[-1000:, 1:].any())

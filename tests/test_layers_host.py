@@ -1,0 +1,31 @@
+"""The layers beside attention without a GPU: requests whose grids the card cannot count, and what the host side says of unusual arguments."""
+import ctypes
+
+from maxdiffusion_amd import _lib
+
+P = ctypes.c_void_p
+FAKE = P(0x1000)  # never dereferenced: every call below must be refused before it launches anything
+
+
+def test_grids_past_2_32_threads_are_refused_before_a_launch(lib):
+  """A launch of 2^32 threads or more is taken by the runtime and runs modulo 2^32."""
+  norm = lambda groups, c: lib.mdattn_layer_norm(None, FAKE, 1, FAKE, 1, FAKE, None, 1, groups, 1, c, c, c, c, c, c, 1e-6, 0.0)
+  assert norm(2**32 // 64, 1) == norm(2**32 // 1024, 16384) == _lib.E_UNSUPPORTED
+  blocks = lambda groups, c: lib.mdattn_layer_norm_e4m3(None, FAKE, 1, FAKE, FAKE, FAKE, None, 1, groups, 1, c, c, c, c, 1e-6, 0.0)
+  assert blocks(2**32 // 64, 1) == _lib.E_UNSUPPORTED
+
+  def backward(groups, c, vectors):
+    nws = lib.mdattn_layer_norm_bwd_workspace_floats(groups, 1, c)
+    d = FAKE if vectors else None
+    return lib.mdattn_layer_norm_bwd(None, FAKE, 1, FAKE, FAKE, FAKE, d, d, 1, groups, 1, c, c, c, c, c, c, c, c, 1e-6, 0.0, FAKE, nws)
+
+  assert backward(2**32 // 1024, 64, True) == backward(2**31 // 1024, 65, True) == _lib.E_UNSUPPORTED  # the sums' grid
+  assert backward(2**32 // 256, 1, False) == _lib.E_UNSUPPORTED
+  assert lib.mdattn_sum_rows(None, FAKE, 1, 2**28, FAKE, 1) == _lib.E_UNSUPPORTED
+  quant = lambda r: lib.mdattn_quant_block_e4m3(None, FAKE, 0, r, 1, 1, 1, FAKE, FAKE, None, None, None)
+  assert quant(2**31) == _lib.E_UNSUPPORTED
+
+
+def test_every_launch_asks_whether_its_grid_can_be_counted(lib):
+  """An older entry, whose own checks know nothing of it."""
+  assert lib.mdattn_host_copy(None, FAKE, FAKE, None, None, ctypes.c_int64(2**24 * 256 * 16)) == _lib.E_UNSUPPORTED
