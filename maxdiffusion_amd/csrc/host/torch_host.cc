@@ -834,8 +834,10 @@ int quant(const Tensor& x, int64_t block_rows, const Blocks* q, const Blocks* qt
   return mdattn_quant_block_e4m3(stream(), ptr(x), is_f32(x), x.size(0), x.size(1), x.stride(0), (int)block_rows, q ? q->values() : nullptr,
                                  q ? q->scales() : nullptr, qt ? qt->values() : nullptr, qt ? qt->scales() : nullptr, f32(sums));
 }
-int product(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t* sb, int64_t b_block_rows, const Tensor& bias, const Tensor& out, int64_t k) {
-  const int64_t m = out.size(0), n = out.size(1), nws = mdattn_matmul_fp8_block_workspace_floats(m, n, k);
+// into out, dense, of m x n elements in whatever shape the caller wants: a view of it would be one that autograd forbids to change in place
+int product(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t* sb, int64_t b_block_rows, const Tensor& bias, const Tensor& out, int64_t m,
+            int64_t n, int64_t k) {
+  const int64_t nws = mdattn_matmul_fp8_block_workspace_floats(m, n, k);
   const Tensor ws = nws ? at::empty({nws}, out.options().dtype(at::kFloat)) : Tensor();
   return mdattn_matmul_fp8_block(stream(), a, sa, b, sb, (int)b_block_rows, ptr(bias), is_f32(bias), mut(out), n, m, n, k, f32(ws), nws);
 }
@@ -871,10 +873,11 @@ OptTensor linear_quantized(const Tensor& x, const Tensor& values, const Tensor& 
                                                stride, (float)eps, (float)offset)
                       : quant(rows, 1, &q, nullptr, Tensor());
   if (rc != MDATTN_OK) return std::nullopt;
-  Tensor y = at::empty({m, n}, x.options().dtype(at::kBFloat16));
-  if (product(q.values(), q.scales(), static_cast<const uint8_t*>(ptr(values)), static_cast<const uint8_t*>(ptr(scales)), block_rows, bias, y, k) != MDATTN_OK)
+  Tensor y = at::empty(with_last(x, n), x.options().dtype(at::kBFloat16));
+  if (product(q.values(), q.scales(), static_cast<const uint8_t*>(ptr(values)), static_cast<const uint8_t*>(ptr(scales)), block_rows, bias, y, m, n, k) !=
+      MDATTN_OK)
     return std::nullopt;
-  return x.dim() == 2 ? y : y.view(with_last(x, n));
+  return y;
 }
 
 // y = x8 w8^T + b, dx = dy8 w8, dw = dy8'^T x8', ' quantised along the tokens.  Saved: x and w in e4m3, transposed, from one read of each.
@@ -888,12 +891,12 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     if (need_dw) xt.emplace(x, k, m, 1);
     if (need_dx) wt.emplace(x, k, n, 128);
     if (quant(rows, 1, &xq, xt ? &*xt : nullptr, Tensor()) != MDATTN_OK || quant(w, 128, &wq, wt ? &*wt : nullptr, Tensor()) != MDATTN_OK) throw Refused{};
-    Tensor y = at::empty({m, n}, x.options());
-    if (product(xq.values(), xq.scales(), wq.values(), wq.scales(), 128, bias, y, k) != MDATTN_OK) throw Refused{};
+    Tensor y = at::empty(with_last(x, n), x.options());
+    if (product(xq.values(), xq.scales(), wq.values(), wq.scales(), 128, bias, y, m, n, k) != MDATTN_OK) throw Refused{};
     ctx->save_for_backward({xt ? xt->buf : Tensor(), wt ? wt->buf : Tensor()});
     ctx->saved_data["i"] = c10::List<int64_t>({m, n, k, need_dx, need_dw, need_db, is_f32(bias)});
     ctx->saved_data["shape"] = x.sizes().vec();
-    return x.dim() == 2 ? y : y.view(with_last(x, n));
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
@@ -914,13 +917,12 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     must(quant(rows, 1, gq ? &*gq : nullptr, gt ? &*gt : nullptr, sums), "mdattn_quant_block_e4m3");
     Tensor dx, dw, db;
     if (i[3]) {
-      dx = at::empty({m, k}, rows.options());
-      must(product(gq->values(), gq->scales(), wt->values(), wt->scales(), 128, Tensor(), dx, n), "mdattn_matmul_fp8_block");
-      dx = dx.view(shape);
+      dx = at::empty(shape, rows.options());
+      must(product(gq->values(), gq->scales(), wt->values(), wt->scales(), 128, Tensor(), dx, m, k, n), "mdattn_matmul_fp8_block");
     }
     if (i[4]) {
       dw = at::empty({n, k}, rows.options());
-      must(product(gt->values(), gt->scales(), xt->values(), xt->scales(), 1, Tensor(), dw, m), "mdattn_matmul_fp8_block");
+      must(product(gt->values(), gt->scales(), xt->values(), xt->scales(), 1, Tensor(), dw, n, k, m), "mdattn_matmul_fp8_block");
     }
     if (i[5]) {
       db = at::empty({n}, rows.options().dtype(i[6] ? at::kFloat : at::kBFloat16));

@@ -75,7 +75,7 @@ class _HipLinearFp8(torch.autograd.Function):
     keep = [q for q in (xt, wt) if q is not None]
     ctx.save_for_backward(*(t for q in keep for t in (q.values, q.scales)))
     ctx.cfg = (x.shape, weight.shape, xt is not None, wt is not None, None if bias is None else bias.dtype)
-    return ops.matmul_fp8_block(xq, wq, bias).view(*x.shape[:-1], weight.shape[0])
+    return ops.matmul_fp8_block_as(xq, wq, bias, x.shape[:-1])
 
   @staticmethod
   def backward(ctx, dy):
@@ -92,7 +92,7 @@ class _HipLinearFp8(torch.autograd.Function):
       parts = list(_tuple(ops.quant_block_e4m3(g, plain=has_w or not has_x, transposed=has_x, sums=need_db)))
       gq = parts.pop(0) if has_w or not has_x else None
       if has_w:
-        dx = ops.matmul_fp8_block(gq, wt).view(shape)
+        dx = ops.matmul_fp8_block_as(gq, wt, None, shape[:-1])
       if has_x:
         dw = ops.matmul_fp8_block(parts.pop(0), xt)
       if need_db:
@@ -118,7 +118,7 @@ def hip_linear_fp8(x, weight, bias=None):
       raise NotImplementedError("hip_linear_fp8 has no gradient through a quantised weight: give the weight itself, or call it under torch.no_grad()")
     rows = x.reshape(-1, x.shape[-1])
     rows = rows if rows.stride(1) == 1 else rows.contiguous()
-    return ops.matmul_fp8_block(ops.quant_block_e4m3(rows), weight, bias).view(*x.shape[:-1], weight.rows)
+    return ops.matmul_fp8_block_as(ops.quant_block_e4m3(rows), weight, bias, x.shape[:-1])
   if x.is_cuda and _wants_grad(x, weight, bias):
     y = _lib.host().linear_autograd(x, weight, bias)
     if y is not None:
@@ -143,4 +143,4 @@ def hip_layer_norm_linear_fp8(x, weight, bias, w8: BlockQuant, out_bias=None, ep
   if _wants_grad(x, weight, bias, out_bias):
     raise NotImplementedError("hip_layer_norm_linear_fp8 has no backward pass: use hip_layer_norm and hip_linear_fp8 for training")
   weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
-  return ops.matmul_fp8_block(ops.layer_norm_quant(_rows(x), weight, bias, eps, weight_offset), w8, out_bias).view(*x.shape[:-1], w8.rows)
+  return ops.matmul_fp8_block_as(ops.layer_norm_quant(_rows(x), weight, bias, eps, weight_offset), w8, out_bias, x.shape[:-1])

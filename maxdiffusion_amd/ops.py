@@ -772,6 +772,12 @@ def sum_rows(rows, out_dtype=torch.float32):
 def matmul_fp8_block(a: BlockQuant, b: BlockQuant, bias=None):
   """a b^T + bias in bf16: a [M, K] in blocks of 1 x 128, b [N, K] in blocks of 1 x 128 or 128 x 128; bias bf16 or f32 [N] or None.
   Sums in f32 on the matrix cores, whose 8-bit products are added eight at a time with 14 bits below the largest of them; rounded once."""
+  return matmul_fp8_block_as(a, b, bias, (a.rows,))
+
+
+def matmul_fp8_block_as(a, b, bias, rows_shape):
+  """`matmul_fp8_block` with the rows in several axes, [*rows_shape, N].  (A view of [M, N] would be one that autograd forbids to change in
+  place where it is made without gradients or inside a node.)"""
   _check_dev(a.values, a.scales, b.values, b.scales, bias)
   if a.block_rows != 1:
     raise ValueError("the first operand's blocks must be 1 x 128")
@@ -781,11 +787,11 @@ def matmul_fp8_block(a: BlockQuant, b: BlockQuant, bias=None):
     raise ValueError(f"bias must be a contiguous tensor of shape [{b.rows}], got {tuple(bias.shape)}")
   bias_f32 = 0 if bias is None else _float_kind(bias, "bias")
   m, n, k = a.rows, b.rows, a.cols
-  out = torch.empty((m, n), dtype=torch.bfloat16, device=a.values.device)
+  out = torch.empty((*rows_shape, n), dtype=torch.bfloat16, device=a.values.device)
   if not out.numel():
     return out
   if not k:
-    return out.zero_() if bias is None else out.copy_(bias.expand(m, n))
+    return out.zero_() if bias is None else out.copy_(bias.expand(out.shape))
   lib = _lib.load()
   nws = lib.mdattn_matmul_fp8_block_workspace_floats(m, n, k)
   ws = torch.empty(nws, dtype=torch.float32, device=out.device) if nws else None

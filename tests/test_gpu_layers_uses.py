@@ -4,6 +4,7 @@ import torch
 
 import pytest
 
+from maxdiffusion_amd import layer_op as L
 from maxdiffusion_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -37,3 +38,33 @@ def test_quantising_very_many_blocks(dev):
     assert torch.equal(q.values[i : i + 60_000_000, 0].view(-1, 250), some.values[:, 0].expand(240_000, 250))
     assert torch.equal(q.scales[i : i + 60_000_000, 0].view(-1, 250), some.scales[:, 0].expand(240_000, 250))
   assert not bool(q.values[-1000:, 1:].any())
+
+
+# ------------------------------------------------------------------------------------------------ outputs that are changed in place
+LAYOUTS = {"dense": lambda x: x, "apart": lambda x: torch.cat((x, x), -1)[..., : x.shape[-1]]}  # (the second one goes through the Python node)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("shape", [(5, 256), (2, 5, 256), (2, 1, 5, 256)])
+def test_outputs_take_terms_in_place(dev, layout, shape):
+  """A residual added in place, to a layer in training and, as a term that wants a gradient, to a frozen one."""
+  x = LAYOUTS[layout](rand(dev, *shape, seed=1, dtype=BF16))
+  w, v, g = rand(dev, 130, 256, seed=2, dtype=BF16), rand(dev, 256, seed=3), rand(dev, *shape[:-1], 130, seed=4, dtype=BF16)
+  w8 = L.quantize_weight(w)
+  term = rand(dev, *shape[:-1], 130, seed=5, dtype=BF16).requires_grad_(True)
+  for frozen in (lambda: L.hip_linear_fp8(x, w8), lambda: L.hip_layer_norm_linear_fp8(x, v, None, w8)):
+    y, want = frozen(), frozen() + term
+    assert not y._is_view()
+    y += term
+    assert torch.equal(y, want) and torch.equal(torch.autograd.grad(y, term, g)[0], g)
+  xr, wr = x.detach().requires_grad_(True), w.clone().requires_grad_(True)
+  y = L.hip_linear_fp8(xr, wr)
+  want = torch.autograd.grad(y, (xr, wr), g)
+  y = L.hip_linear_fp8(xr, wr)
+  y += term
+  for a, b in zip(torch.autograd.grad(y, (xr, wr, term), g), (*want, g)):
+    assert torch.equal(a, b)
+  vr, g = v.clone().requires_grad_(True), rand(dev, *shape, seed=6, dtype=BF16)
+  y = L.hip_layer_norm(xr, vr)
+  y += 1.0
+  assert torch.equal(torch.autograd.grad(y, vr, g)[0], torch.autograd.grad(L.hip_layer_norm(xr, vr), vr, g)[0])
