@@ -762,7 +762,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     if (!y.defined()) throw Refused{};
     ctx->save_for_backward({x, w});
     ctx->saved_data["f"] = c10::List<double>({eps, offset});
-    ctx->saved_data["i"] = c10::List<int64_t>({stride, f32, w.defined(), b.defined(), (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())});
+    ctx->saved_data["i"] = c10::List<int64_t>({stride, f32, w.defined(), b.defined(), (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()), is_f32(x)});
     ctx->saved_data["wshape"] = w.defined() ? w.sizes().vec() : std::vector<int64_t>{};
     ctx->saved_data["bshape"] = b.defined() ? b.sizes().vec() : std::vector<int64_t>{};
     return y;
@@ -774,7 +774,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     const Tensor &x = saved[0], &w = saved[1];
     Tensor g = grads[0];
     const auto r = as_rows(x);
-    unpacked(r && float_on(x, x) && x.sizes() == g.sizes() && w.defined() == (bool)i[2] &&
+    unpacked(r && float_on(x, x) && is_f32(x) == (int)i[5] && x.sizes() == g.sizes() && w.defined() == (bool)i[2] &&
              (!w.defined() || (float_on(w, x) && is_f32(w) == (int)i[1] && w.is_contiguous() && w.sizes() == at::IntArrayRef(ctx->saved_data["wshape"].toIntVector()))));
     if (g.scalar_type() != x.scalar_type()) g = g.to(x.scalar_type());
     auto rg = as_rows(g);

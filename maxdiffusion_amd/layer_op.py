@@ -21,6 +21,11 @@ def _wants_grad(*ts) -> bool:
   return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+def _forms(*ts):
+  """What a saved-tensor hook has to hand back as it was (strides are read again)."""
+  return [None if t is None else (t.dtype, t.shape, t.device) for t in ts]
+
+
 def _rows(x):
   """x [..., C] as the norm walks it: its last axis contiguous and the axes between the first and the last dense."""
   return x if (x.stride(-1) == 1 or x.shape[-1] == 1) and ops.row_stride(x) is not None else x.contiguous()
@@ -32,12 +37,14 @@ class _HipLayerNorm(torch.autograd.Function):
   @staticmethod
   def forward(ctx, x, weight, bias, eps, weight_offset):
     ctx.save_for_backward(x, weight, bias)
-    ctx.cfg = (eps, weight_offset)
+    ctx.cfg, ctx.forms = (eps, weight_offset), _forms(x, weight, bias)
     return ops.layer_norm(x, weight, bias, eps, weight_offset)
 
   @staticmethod
   def backward(ctx, g):
     x, weight, bias = ctx.saved_tensors
+    if _forms(x, weight, bias) != ctx.forms:
+      raise ValueError("a tensor saved for the backward pass came back from its hook with another dtype, shape or device")
     dx, dw, db = ops.layer_norm_backward(x, weight, bias, _rows(g.to(x.dtype)), *ctx.cfg, needs_vectors=any(ctx.needs_input_grad[1:3]))
     return dx, dw, db, None, None
 

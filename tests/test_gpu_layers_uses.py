@@ -68,3 +68,32 @@ def test_outputs_take_terms_in_place(dev, layout, shape):
   y = L.hip_layer_norm(xr, vr)
   y += 1.0
   assert torch.equal(torch.autograd.grad(y, vr, g)[0], torch.autograd.grad(L.hip_layer_norm(xr, vr), vr, g)[0])
+
+
+# ------------------------------------------------------------------------------------------------ saved-tensor hooks
+@pytest.mark.parametrize("xt", [BF16, F32])
+def test_saved_tensor_hooks(dev, xt):
+  """What a hook hands back is used where it is what was saved (a copy, as an offloading hook returns it), and refused where its dtype
+  is another one."""
+  x, w, v = rand(dev, 2, 5, 256, seed=1, dtype=xt), rand(dev, 256, seed=2), rand(dev, 130, 256, seed=3, dtype=BF16)
+  x, w, v = (t.requires_grad_(True) for t in (x, w, v))
+  norm_python = lambda: L.hip_layer_norm(torch.cat((x, x), -1)[..., :256].transpose(0, 1)[:, :, None], torch.cat((w, w))[::2], None)
+  calls = {"norm": (lambda: L.hip_layer_norm(x, w), (x, w)), "norm, plain": (lambda: L.hip_layer_norm(x), (x,)), "norm, Python node": (norm_python, (x, w))}
+  if xt == BF16:
+    calls["linear"] = (lambda: L.hip_linear_fp8(x, v), (x, v))
+    calls["linear, Python node"] = (lambda: L.hip_linear_fp8(torch.cat((x, x), -1)[..., :256], v), (x, v))
+  swaps = {BF16: F32, F32: BF16, torch.uint8: F32}
+  for name, (call, leaves) in calls.items():
+    print(name, flush=True)
+    loss = lambda y: y.float().square().sum()
+    want = torch.autograd.grad(loss(call()), leaves)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(dev)):
+      out = call()
+    for a, b in zip(torch.autograd.grad(loss(out), leaves), want):
+      assert torch.equal(a, b), name
+    for which in {t.dtype for t in leaves}:  # x alone, the weight alone, or both where they are of one type
+      lossy = lambda t: t.to(swaps[t.dtype]) if t.dtype == (torch.uint8 if name.startswith("linear") else which) else t
+      with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lossy):
+        out = call()
+      with pytest.raises(ValueError):
+        torch.autograd.grad(out, leaves, torch.ones_like(out))
