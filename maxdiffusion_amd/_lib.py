@@ -142,3 +142,21 @@ def strerror(code: int) -> str:
 def check(code: int, where: str) -> None:
   if code != E_OK:
     raise MdattnError(code, where, strerror(code))
+
+
+def first_order(backward):
+  """Decorates an autograd node's backward: where autograd records it (create_graph), a second derivative through its results is refused, not
+  left out."""
+  import functools
+
+  import torch
+
+  @functools.wraps(backward)
+  def run(ctx, *grads):
+    if not torch.is_grad_enabled():
+      return backward(ctx, *grads)
+    with torch.no_grad():
+      results = backward(ctx, *grads)
+    return tuple(host().first_order(list(grads), list(results) if isinstance(results, tuple) else [results]))
+
+  return run

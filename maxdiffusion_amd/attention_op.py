@@ -131,6 +131,7 @@ class _HipFlashAttention(torch.autograd.Function):
     return out
 
   @staticmethod
+  @_lib.first_order
   def backward(ctx, dout):
     q, k, v, out, lse = ctx.saved_tensors
     dq, dk, dv = ops.flash_attention_backward(q, k, v, out, dout.to(torch.bfloat16), lse, scale=ctx.scale, key_bias=ctx.key_bias)
@@ -239,6 +240,7 @@ class _HipNormRopeFullrow(torch.autograd.Function):
     return q_out, k_out
 
   @staticmethod
+  @_lib.first_order
   def backward(ctx, gq, gk):
     q, k, wq, wk, cos, sin = ctx.saved_tensors
     heads, eps, q_mul, kind = ctx.cfg
@@ -261,6 +263,7 @@ class _HipNormRopeQkv(torch.autograd.Function):
     return q_out, k_out, v_out
 
   @staticmethod
+  @_lib.first_order
   def backward(ctx, gq, gk, gv):
     qkv, bias, wq, wk, cos, sin = ctx.saved_tensors
     heads, eps, q_mul, kind = ctx.cfg
@@ -289,6 +292,7 @@ class _HipNormRopePerhead(torch.autograd.Function):
     return q_out, k_out
 
   @staticmethod
+  @_lib.first_order
   def backward(ctx, gq, gk):
     q, k, wq, wk, wq_txt, wk_txt, cos, sin = ctx.saved_tensors
     eps, n_txt, q_mul, kind = ctx.cfg
@@ -309,6 +313,7 @@ class _HipNormRopeRows(torch.autograd.Function):
     return out
 
   @staticmethod
+  @_lib.first_order
   def backward(ctx, g):
     x, w, cos, sin = ctx.saved_tensors
     heads, mode, eps = ctx.cfg

@@ -74,6 +74,44 @@ auto unless_refused(F&& apply) -> std::optional<decltype(apply())> {
   }
 }
 
+// Gradients have none of their own.  Where autograd records a backward pass (create_graph), its results hang on a node that leads to what the
+// differentiated node led to, and to the gradients that came in, so that a second derivative reaches it and is refused, not left out.
+struct NoSecondDerivative : torch::autograd::Node {
+  using Node::Node;
+  variable_list apply(variable_list&&) override {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "the gradients of this package's operators cannot be differentiated again: second derivatives are not implemented");
+  }
+};
+variable_list first_order(const variable_list& grads, variable_list results) {
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return results;
+  torch::autograd::edge_list to;
+  for (const auto& e : node->next_edges())
+    if (e.is_valid()) to.push_back(e);
+  for (const Tensor& g : grads)
+    if (g.defined() && g.requires_grad()) to.push_back(torch::autograd::impl::gradient_edge(g));
+  const std::shared_ptr<torch::autograd::Node> refuses(new NoSecondDerivative(std::move(to)), torch::autograd::deleteNode);
+  for (Tensor& r : results) {
+    if (!r.defined()) continue;
+    r = r.detach();
+    torch::autograd::create_gradient_edge(r, refuses);
+  }
+  return results;
+}
+// A node that makes its gradients in F::gradients
+template <class F>
+struct FirstOrder : torch::autograd::Function<F> {
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!at::GradMode::is_enabled()) return F::gradients(ctx, std::move(grads));
+    variable_list results;
+    {
+      at::NoGradGuard guard;
+      results = F::gradients(ctx, grads);
+    }
+    return first_order(grads, std::move(results));
+  }
+};
+
 // [B,S,H,D] as the kernels walk it, over a rank-3 [B,S,H*D] or a rank-4 [B,H,S,D] tensor (attention_op._as_bshd)
 struct View {
   int64_t b = 0, s = 0, h = 0, d = 0;
@@ -171,7 +209,7 @@ bool operands(const Tensor& q, const Tensor& k, const Tensor& v, int64_t heads, 
 }
 
 // q, k, v in the caller's own rank; out [B,Sq,H*D]
-struct FlashFn : torch::autograd::Function<FlashFn> {
+struct FlashFn : FirstOrder<FlashFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask_, int64_t heads, double scale) {
     const Tensor mask = value(mask_);
     const View vq = *as_view(q, heads), vk = *as_view(k, heads), vv = *as_view(v, heads);
@@ -184,7 +222,7 @@ struct FlashFn : torch::autograd::Function<FlashFn> {
     ctx->saved_data["scale"] = scale;
     return out;
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  static variable_list gradients(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4];
     const Tensor mask = ctx->saved_data["mask"].toTensor();
@@ -388,7 +426,7 @@ variable_list fullrow_run(const Tensor& q, const Tensor& k, const Tensor& wq, co
   if (rc != MDATTN_OK) return {};
   return k.defined() ? variable_list{qo, ko} : variable_list{qo};
 }
-struct FullrowFn : torch::autograd::Function<FullrowFn> {
+struct FullrowFn : FirstOrder<FullrowFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k_, const Tensor& wq, const OptTensor& wk_,
                                const OptTensor& cos_, const OptTensor& sin_, const Prologue& p) {
     const Tensor k = value(k_), wk = value(wk_), cos = value(cos_), sin = value(sin_);
@@ -398,7 +436,7 @@ struct FullrowFn : torch::autograd::Function<FullrowFn> {
     p.save(ctx);
     return out;
   }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
+  static variable_list gradients(AutogradContext* ctx, variable_list g) {
     const auto sv = ctx->get_saved_variables();
     const Tensor &q = sv[0], &k = sv[1], &wq = sv[2], &wk = sv[3];
     const Prologue p = Prologue::saved(ctx);
@@ -453,7 +491,7 @@ variable_list perhead_run(const Tensor& q, const Tensor& k, const Tensor& wq, co
   if (rc != MDATTN_OK) return {};
   return k.defined() ? variable_list{qo, ko} : variable_list{qo};
 }
-struct PerheadFn : torch::autograd::Function<PerheadFn> {
+struct PerheadFn : FirstOrder<PerheadFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k_, const Tensor& wq, const OptTensor& wk_, const OptTensor& wqt_,
                                const OptTensor& wkt_, const OptTensor& cos_, const OptTensor& sin_, const Prologue& p) {
     const Tensor k = value(k_), wk = value(wk_), wqt = value(wqt_), wkt = value(wkt_), cos = value(cos_), sin = value(sin_);
@@ -463,7 +501,7 @@ struct PerheadFn : torch::autograd::Function<PerheadFn> {
     p.save(ctx);
     return out;
   }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
+  static variable_list gradients(AutogradContext* ctx, variable_list g) {
     const auto sv = ctx->get_saved_variables();
     const Tensor &q = sv[0], &k = sv[1], &wq = sv[2], &wk = sv[3], &wqt = sv[4], &wkt = sv[5];
     const Prologue p = Prologue::saved(ctx);
@@ -521,7 +559,7 @@ variable_list qkv_run(const Tensor& x, const Tensor& bias, const Tensor& wq, con
   if (rc != MDATTN_OK) return {};
   return {o[0], o[1], o[2]};
 }
-struct QkvFn : torch::autograd::Function<QkvFn> {
+struct QkvFn : FirstOrder<QkvFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& bias, const Tensor& wq, const Tensor& wk, const OptTensor& cos_,
                                const OptTensor& sin_, const Prologue& p) {
     const Tensor cos = value(cos_), sin = value(sin_);
@@ -531,7 +569,7 @@ struct QkvFn : torch::autograd::Function<QkvFn> {
     p.save(ctx);
     return out;
   }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
+  static variable_list gradients(AutogradContext* ctx, variable_list g) {
     const auto sv = ctx->get_saved_variables();
     const Tensor &x = sv[0], &bias = sv[1], &wq = sv[2], &wk = sv[3];
     const Prologue p = Prologue::saved(ctx);
@@ -589,7 +627,7 @@ variable_list rows_run(const Tensor& q, const Tensor& k, const Tensor& wq, const
   if (rc != MDATTN_OK) return {};
   return k.defined() ? variable_list{qo, ko} : variable_list{qo};
 }
-struct RowsFn : torch::autograd::Function<RowsFn> {
+struct RowsFn : FirstOrder<RowsFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k_, const Tensor& wq, const OptTensor& wk_, const OptTensor& cos_,
                                const OptTensor& sin_, const Rows& p) {
     const Tensor k = value(k_), wk = value(wk_), cos = value(cos_), sin = value(sin_);
@@ -631,7 +669,7 @@ struct RowsFn : torch::autograd::Function<RowsFn> {
       return left;
     }
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  static variable_list gradients(AutogradContext* ctx, variable_list grads) {
     const bool has[2] = {grads[0].defined(), grads.size() > 1 && grads[1].defined()};
     if (!has[0] && !has[1]) return variable_list(7);
     const bool pair = has[0] && has[1];
@@ -751,7 +789,7 @@ Tensor norm_run(const Tensor& x, const Rows3& r, const Tensor& w, const Tensor& 
   return rc == MDATTN_OK ? y : Tensor();
 }
 // Saved for the backward: x and w; of b only its shape and type.
-struct NormFn : torch::autograd::Function<NormFn> {
+struct NormFn : FirstOrder<NormFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w_, const OptTensor& b_, double eps, double offset) {
     const Tensor w = value(w_), b = value(b_);
     const Rows3 r = *as_rows(x);
@@ -767,7 +805,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     ctx->saved_data["bshape"] = b.defined() ? b.sizes().vec() : std::vector<int64_t>{};
     return y;
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  static variable_list gradients(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const auto f = ctx->saved_data["f"].toDoubleVector();
     const auto i = ctx->saved_data["i"].toIntVector();
@@ -881,7 +919,7 @@ OptTensor linear_quantized(const Tensor& x, const Tensor& values, const Tensor& 
 }
 
 // y = x8 w8^T + b, dx = dy8 w8, dw = dy8'^T x8', ' quantised along the tokens.  Saved: x and w in e4m3, transposed, from one read of each.
-struct LinearFn : torch::autograd::Function<LinearFn> {
+struct LinearFn : FirstOrder<LinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias_) {
     const Tensor bias = value(bias_), rows = as_matrix(x);
     const bool need_dx = x.requires_grad(), need_dw = w.requires_grad(), need_db = bias.defined() && bias.requires_grad();
@@ -898,7 +936,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     ctx->saved_data["shape"] = x.sizes().vec();
     return y;
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  static variable_list gradients(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const auto i = ctx->saved_data["i"].toIntVector();
     const auto shape = ctx->saved_data["shape"].toIntVector();
@@ -959,5 +997,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("norm_rope_rows", &norm_rope_rows, Unlocked());
   m.def("layer_norm", &layer_norm, Unlocked());
   m.def("linear_quantized", &linear_quantized, Unlocked());
+  m.def("first_order", [](const std::vector<OptTensor>& grads, const std::vector<OptTensor>& results) {
+    variable_list g, r;
+    for (const auto& t : grads) g.push_back(value(t));
+    for (const auto& t : results) r.push_back(value(t));
+    std::vector<OptTensor> out;
+    for (const Tensor& t : first_order(g, std::move(r))) out.push_back(opt(t));
+    return out;
+  });
   m.def("linear_autograd", &linear_autograd, Unlocked());
 }

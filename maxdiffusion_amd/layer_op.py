@@ -41,6 +41,7 @@ class _HipLayerNorm(torch.autograd.Function):
     return ops.layer_norm(x, weight, bias, eps, weight_offset)
 
   @staticmethod
+  @_lib.first_order
   def backward(ctx, g):
     x, weight, bias = ctx.saved_tensors
     if _forms(x, weight, bias) != ctx.forms:
@@ -85,6 +86,7 @@ class _HipLinearFp8(torch.autograd.Function):
     return ops.matmul_fp8_block_as(xq, wq, bias, x.shape[:-1])
 
   @staticmethod
+  @_lib.first_order
   def backward(ctx, dy):
     shape, (n, k), has_x, has_w, bias_dtype = ctx.cfg
     saved = list(ctx.saved_tensors)

@@ -4,6 +4,7 @@ import torch
 
 import pytest
 
+from maxdiffusion_amd import attention_op as A
 from maxdiffusion_amd import layer_op as L
 from maxdiffusion_amd import ops
 
@@ -97,3 +98,24 @@ def test_saved_tensor_hooks(dev, xt):
         out = call()
       with pytest.raises(ValueError):
         torch.autograd.grad(out, leaves, torch.ones_like(out))
+
+
+# ------------------------------------------------------------------------------------------------ autograd's other modes
+def test_second_derivatives_are_refused(dev):
+  """A penalty on gradients fails, and does not come out as a constant."""
+  x, w, v = rand(dev, 2, 5, 256, seed=1, dtype=BF16), rand(dev, 256, seed=2), rand(dev, 128, 256, seed=3, dtype=BF16)
+  x, w, v = (t.requires_grad_(True) for t in (x, w, v))
+  apart = lambda: torch.cat((x, x), -1)[..., :256]
+  op = A.AttentionOp(attention_kernel="hip_flash", scale=0.125, heads=4, dim_head=64, dtype=BF16)
+  hw = torch.ones(256, dtype=BF16, device=dev, requires_grad=True)
+  calls = {"norm": lambda: L.hip_layer_norm(x, w), "norm, Python node": lambda: L.hip_layer_norm(apart().transpose(0, 1)[:, :, None], torch.cat((w, w))[::2]),
+           "linear": lambda: L.hip_linear_fp8(x, v), "linear, Python node": lambda: L.hip_linear_fp8(apart(), v),
+           "attention": lambda: op.apply_attention(x, x, x), "prologue": lambda: A.hip_norm_rope(x, x, hw, hw, None, 4)[0]}
+  for name, call in calls.items():
+    print(name, flush=True)
+    loss = lambda: call().float().square().sum()
+    (plain,) = torch.autograd.grad(loss(), x)
+    (dx,) = torch.autograd.grad(loss(), x, create_graph=True)
+    assert torch.equal(dx, plain) and dx.requires_grad and not plain.requires_grad
+    with pytest.raises(NotImplementedError, match="second derivatives"):
+      torch.autograd.grad(dx.float().square().sum() + x.float().sum(), x)

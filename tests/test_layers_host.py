@@ -1,6 +1,9 @@
 """The layers beside attention without a GPU: requests whose grids the card cannot count, and what the host side says of unusual arguments."""
 import ctypes
 
+import pytest
+import torch
+
 from maxdiffusion_amd import _lib
 
 P = ctypes.c_void_p
@@ -29,3 +32,39 @@ def test_grids_past_2_32_threads_are_refused_before_a_launch(lib):
 def test_every_launch_asks_whether_its_grid_can_be_counted(lib):
   """An older entry, whose own checks know nothing of it."""
   assert lib.mdattn_host_copy(None, FAKE, FAKE, None, None, ctypes.c_int64(2**24 * 256 * 16)) == _lib.E_UNSUPPORTED
+
+
+# ------------------------------------------------------------------------------------------------ second derivatives
+class Square(torch.autograd.Function):
+  """A node as the package's: its gradient comes from code that autograd does not see."""
+
+  @staticmethod
+  def forward(ctx, x, y):
+    ctx.save_for_backward(x)
+    return x * x
+
+  @staticmethod
+  @_lib.first_order
+  def backward(ctx, g):
+    (x,) = ctx.saved_tensors
+    return torch.from_numpy((2 * x * g).detach().numpy()), None
+
+
+def test_second_derivatives_are_refused():
+  x = torch.arange(1.0, 4.0, requires_grad=True)
+  (dx,) = torch.autograd.grad(Square.apply(x, None).sum(), x)
+  assert torch.equal(dx, 2 * x) and not dx.requires_grad
+  (dx,) = torch.autograd.grad(Square.apply(x, None).sum(), x, create_graph=True)  # recorded, and as right
+  assert torch.equal(dx, 2 * x) and dx.requires_grad
+  for penalty in (dx.square().sum(), dx.square().sum() + x.sum()):  # also where x is reached beside it
+    with pytest.raises(NotImplementedError, match="second derivatives"):
+      torch.autograd.grad(penalty, x, retain_graph=True)
+  with pytest.raises(NotImplementedError, match="second derivatives"):
+    dx.sum().backward()
+  g = torch.ones(3, requires_grad=True)  # along the incoming gradient alone
+  (dx,) = torch.autograd.grad(Square.apply(x, None), x, g, create_graph=True)
+  with pytest.raises(NotImplementedError, match="second derivatives"):
+    torch.autograd.grad(dx.sum(), g)
+  y = torch.ones(3, requires_grad=True)  # a gradient that nothing differentiates is left alone
+  (dy,) = torch.autograd.grad((Square.apply(x, None) * y).sum(), y, create_graph=True)
+  assert torch.equal(torch.autograd.grad(dy.sum(), x)[0], 2 * x)
