@@ -160,3 +160,11 @@ def first_order(backward):
     return tuple(host().first_order(list(grads), list(results) if isinstance(results, tuple) else [results]))
 
   return run
+
+
+def no_tangents(*ts):
+  """Refuses tensors that carry a tangent (forward-mode differentiation): a kernel would drop it."""
+  from torch.autograd import forward_ad
+
+  if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+    raise NotImplementedError("this package's operators have no forward-mode derivative: their inputs may not carry tangents")

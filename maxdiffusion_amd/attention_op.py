@@ -168,6 +168,7 @@ def hip_flash_kernel(q, k, v, context):
     if out is not None:
       return out
   # what the native path leaves: other dtypes, head dims to be padded, views to be copied, and every error
+  _lib.no_tangents(q, k, v)
   qv, kv, vv = _as_bshd(q, heads), _as_bshd(k, heads), _as_bshd(v, heads)
   # LTX2 hands f32 q/k next to a v in the model dtype (norm dtype f32, attention_ltx2.py:415-432); the MFMA operands are
   # bf16.  Each such cast is one more pass over the tensor in HBM: `hip_norm_rope_ltx2` in front of this entry emits
@@ -207,6 +208,7 @@ def hip_flash_fp8_kernel(q, k, v, context):
     out = _lib.host().flash_fp8(q, k, v, heads, context["scale"], context.get("attention_mask"))
     if out is not None:
       return out
+  _lib.no_tangents(q, k, v)
   qv, kv, vv, d0 = _pad_head_dim(*(_as_bshd(t, heads).to(torch.bfloat16) for t in (q, k, v)))
   qv, kv, vv = qv.contiguous(), kv.contiguous(), vv.contiguous()
   # the softmax scale rides on q's quantisation (one rounding either way) and the q and k scales are powers of two:
@@ -329,6 +331,7 @@ def _norm_rope_rows(x, w, cos, sin, heads, mode, eps):
     out = _lib.host().norm_rope_rows(x, None, w, None, cos, sin, heads, _ROWS_MODES[mode], eps, 1.0)
     if out is not None:
       return out[0]
+  _lib.no_tangents(x, w)
   if _wants_grad(x, w):
     return _HipNormRopeRows.apply(x, w, cos, sin, heads, mode, eps)
   return ops.norm_rope_rows(x, w, cos, sin, heads=heads, mode=mode, eps=eps)
@@ -345,6 +348,7 @@ def hip_norm_rope_qkv(qkv, wq, wk, freqs_cis, heads: int, bias=None, eps: float 
     out = _lib.host().norm_rope_qkv(qkv, bias, wq, wk, *_table_pair(freqs_cis), heads, eps, q_mul, out_layout == "bhsd")
     if out is not None:
       return tuple(out)
+  _lib.no_tangents(qkv, bias, wq, wk)
   b, s, n3 = qkv.shape
   wq, wk = _dense_weight(wq), _dense_weight(wk)
   table = _rope_table(freqs_cis, s, n3 // 3 // heads)
@@ -624,6 +628,7 @@ def hip_norm_rope(q, k, wq, wk, freqs_cis, heads: int, eps: float = 1e-6, per_he
       out = host.norm_rope(q, k, wq, wk, *_table_pair(freqs_cis), heads, eps, q_mul, bhsd)
     if out is not None:
       return (out[0], out[1] if k is not None else None)
+  _lib.no_tangents(q, k, wq, wk, wq_txt, wk_txt)
   wq, wk, wq_txt, wk_txt = (_dense_weight(w) for w in (wq, wk, wq_txt, wk_txt))
   if per_head:
     b, s, h, d = q.shape

@@ -39,8 +39,10 @@ float* f32(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr
 Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 // autograd's apply() takes an argument that may be missing as an optional, never as an undefined tensor
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+// a tensor that carries a tangent (forward-mode differentiation): left to the Python path, which refuses it
+bool dual(const Tensor& t) { return t._fw_grad(0).defined(); }
 bool bf16_on(const Tensor& t, const Tensor& ref) {
-  return t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.get_device() == ref.get_device() && !t.is_neg();
+  return t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.get_device() == ref.get_device() && !t.is_neg() && !dual(t);
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
@@ -347,7 +349,7 @@ struct Table {
 };
 bool in_place(const Tensor& t, at::ScalarType dtype, int64_t numel, const Tensor& ref) {
   return t.is_cuda() && t.get_device() == ref.get_device() && t.scalar_type() == dtype && t.is_contiguous() && t.numel() == numel &&
-         !t.is_conj() && !t.is_neg() && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+         !t.is_conj() && !t.is_neg() && !dual(t) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
 }
 std::optional<Table> as_table(const OptTensor& a, const OptTensor& b, int64_t s, int64_t d, bool per_head, const Tensor& ref) {
   Table t;
@@ -704,12 +706,12 @@ struct RowsFn : FirstOrder<RowsFn> {
 std::optional<variable_list> norm_rope_rows(const Tensor& q, const OptTensor& k_, const Tensor& wq, const OptTensor& wk_, const OptTensor& cos_,
                                             const OptTensor& sin_, int64_t heads, int64_t mode, double eps, double w_mul) {
   const Tensor k = value(k_), wk = value(wk_), cos = value(cos_), sin = value(sin_);
-  if (!q.is_cuda() || (q.scalar_type() != at::kFloat && q.scalar_type() != at::kBFloat16) || q.is_neg() || q.dim() != 3 || q.numel() == 0 ||
+  if (!q.is_cuda() || (q.scalar_type() != at::kFloat && q.scalar_type() != at::kBFloat16) || q.is_neg() || dual(q) || q.dim() != 3 || q.numel() == 0 ||
       q.stride(2) != 1 || heads <= 0 || q.size(2) % heads)
     return std::nullopt;
   const int64_t b = q.size(0), s = q.size(1), n = q.size(2);
   if (!in_place(wq, at::kFloat, n, q)) return std::nullopt;
-  if (k.defined() && (n > 4096 || k.scalar_type() != q.scalar_type() || !k.is_cuda() || k.get_device() != q.get_device() || k.is_neg() ||
+  if (k.defined() && (n > 4096 || k.scalar_type() != q.scalar_type() || !k.is_cuda() || k.get_device() != q.get_device() || k.is_neg() || dual(k) ||
                       k.sizes() != q.sizes() || k.strides() != q.strides() || !wk.defined() || !in_place(wk, at::kFloat, n, q)))
     return std::nullopt;
   if (mode) {
@@ -735,7 +737,8 @@ std::optional<variable_list> norm_rope_rows(const Tensor& q, const OptTensor& k_
 // ------------------------------------------------------------------------------------------------ the layers beside attention
 // (layer_op.py, ops.py.)  An undefined tensor is a missing one.
 bool float_on(const Tensor& t, const Tensor& ref) {
-  return t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) && t.get_device() == ref.get_device() && !t.is_neg();
+  return t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) && t.get_device() == ref.get_device() && !t.is_neg() &&
+         !dual(t);
 }
 int is_f32(const Tensor& t) { return t.defined() && t.scalar_type() == at::kFloat; }
 

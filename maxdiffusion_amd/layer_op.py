@@ -59,6 +59,7 @@ def hip_layer_norm(x, weight=None, bias=None, eps: float = 1e-6, weight_offset: 
     if y is not None:
       return y
   # what the native path leaves: views to be copied, nothing to compute, and every error
+  _lib.no_tangents(x, weight, bias)
   weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
   if _wants_grad(x, weight, bias):
     return _HipLayerNorm.apply(_rows(x), weight, bias, eps, weight_offset)
@@ -123,6 +124,7 @@ def hip_linear_fp8(x, weight, bias=None):
       y = _lib.host().linear_quantized(x, weight.values, weight.scales, weight.rows, weight.cols, weight.block_rows, bias, False, None, None, 0.0, 0.0)
       if y is not None:
         return y
+    _lib.no_tangents(x, bias)
     if _wants_grad(x, bias):
       raise NotImplementedError("hip_linear_fp8 has no gradient through a quantised weight: give the weight itself, or call it under torch.no_grad()")
     rows = x.reshape(-1, x.shape[-1])
@@ -132,6 +134,7 @@ def hip_linear_fp8(x, weight, bias=None):
     y = _lib.host().linear_autograd(x, weight, bias)
     if y is not None:
       return y
+  _lib.no_tangents(x, weight, bias)
   if weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
     raise ValueError(f"weight must be a BlockQuant or a [N, {x.shape[-1]}] tensor, got {tuple(weight.shape)}")
   x, weight = (t if t.stride(-1) == 1 else t.contiguous() for t in (x, weight))
@@ -149,6 +152,7 @@ def hip_layer_norm_linear_fp8(x, weight, bias, w8: BlockQuant, out_bias=None, ep
     y = _lib.host().linear_quantized(x, w8.values, w8.scales, w8.rows, w8.cols, w8.block_rows, out_bias, True, weight, bias, eps, weight_offset)
     if y is not None:
       return y
+  _lib.no_tangents(x, weight, bias, out_bias)
   if _wants_grad(x, weight, bias, out_bias):
     raise NotImplementedError("hip_layer_norm_linear_fp8 has no backward pass: use hip_layer_norm and hip_linear_fp8 for training")
   weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))

@@ -1,8 +1,8 @@
 """The layers beside attention as programs use them: calls past what a grid can count, outputs that are changed in place, hooks, autograd's
 other modes, arguments that the usual path leaves aside.  Tolerances as in the tests of the kernels: bit for bit where nothing is said."""
-import torch
-
 import pytest
+import torch
+from torch.autograd import forward_ad
 
 from maxdiffusion_amd import attention_op as A
 from maxdiffusion_amd import layer_op as L
@@ -119,3 +119,19 @@ def test_second_derivatives_are_refused(dev):
     assert torch.equal(dx, plain) and dx.requires_grad and not plain.requires_grad
     with pytest.raises(NotImplementedError, match="second derivatives"):
       torch.autograd.grad(dx.float().square().sum() + x.float().sum(), x)
+
+
+@pytest.mark.parametrize("recording", [True, False])
+def test_tangents_are_refused(dev, recording):
+  """Forward-mode differentiation fails, and does not lose its tangent."""
+  x, w, v = rand(dev, 2, 5, 256, seed=1, dtype=BF16), rand(dev, 256, seed=2), rand(dev, 128, 256, seed=3, dtype=BF16)
+  w8, hw = L.quantize_weight(v), rand(dev, 256, seed=4, dtype=BF16)
+  op = A.AttentionOp(attention_kernel="hip_flash", scale=0.125, heads=4, dim_head=64, dtype=BF16)
+  with forward_ad.dual_level(), torch.set_grad_enabled(recording):
+    d, e, f = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w, v))
+    for call in (lambda: L.hip_layer_norm(d), lambda: L.hip_layer_norm(x, e), lambda: L.hip_linear_fp8(d, w8), lambda: L.hip_linear_fp8(x, f),
+                 lambda: L.hip_layer_norm_linear_fp8(d, w, None, w8), lambda: L.hip_layer_norm_linear_fp8(x, e, None, w8),
+                 lambda: op.apply_attention(d, x, x), lambda: op.apply_attention(x, x, d), lambda: A.hip_norm_rope(d, x, hw, hw, None, 4),
+                 lambda: A.hip_norm_rope_ltx2(d, x, w, w, 4), lambda: A.hip_norm_rope_ltx2(x, x, e, w, 4)):
+      with pytest.raises(NotImplementedError, match="tangents"):
+        call()

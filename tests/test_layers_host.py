@@ -3,8 +3,9 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from maxdiffusion_amd import _lib
+from maxdiffusion_amd import _lib, attention_op, layer_op, ops
 
 P = ctypes.c_void_p
 FAKE = P(0x1000)  # never dereferenced: every call below must be refused before it launches anything
@@ -68,3 +69,18 @@ def test_second_derivatives_are_refused():
   y = torch.ones(3, requires_grad=True)  # a gradient that nothing differentiates is left alone
   (dy,) = torch.autograd.grad((Square.apply(x, None) * y).sum(), y, create_graph=True)
   assert torch.equal(torch.autograd.grad(dy.sum(), x)[0], 2 * x)
+
+
+def test_tangents_are_refused():
+  x, w = torch.zeros(2, 100), ops.BlockQuant(torch.zeros((130, 128), dtype=torch.uint8), torch.zeros((2, 4), dtype=torch.uint8), 130, 100, 128)
+  context = dict(heads=1, scale=1.0)
+  with forward_ad.dual_level():
+    d = forward_ad.make_dual(x, torch.ones_like(x))
+    q, v = d.view(1, 2, 100), torch.zeros(100)
+    for call in (lambda: layer_op.hip_layer_norm(d), lambda: layer_op.hip_layer_norm(x, d[0]), lambda: layer_op.hip_linear_fp8(d, w),
+                 lambda: layer_op.hip_linear_fp8(x, d), lambda: layer_op.hip_layer_norm_linear_fp8(d, None, None, w), lambda: layer_op.hip_linear_fp8(x, x, d[:, 0]),
+                 lambda: attention_op.hip_flash_kernel(q, q, q, context), lambda: attention_op.hip_flash_fp8_kernel(q, q, q, context),
+                 lambda: attention_op.hip_norm_rope(q, q, v, v, None, 1), lambda: attention_op.hip_norm_rope_ltx2(q, q, v, v, 1),
+                 lambda: attention_op.hip_norm_rope_qkv(torch.cat((q, q, q), -1), v, v, None, 1)):
+      with pytest.raises(NotImplementedError, match="tangents"):
+        call()
