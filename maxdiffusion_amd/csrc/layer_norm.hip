@@ -77,7 +77,7 @@ struct Deal {
         if (c[j] + e < C) row[c[j] + e] = f[e];
     }
   }
-  // w or b of one group as f32; `none` where there is none or no channel
+  // w or b of one group as f32; `none` where there is none, zeros where there is no channel
   __device__ __forceinline__ void vector(float (&v)[NV][8], const void* p, int is_f32, int64_t at, float none) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -113,7 +113,7 @@ struct NormArgs {
   int64_t x_sg, x_sr, y_sg, y_sr;
   int64_t scale_stride;
   int C, wb_f32, blocks;                  // workgroups of a group
-  float eps, offset;
+  float eps, offset;                      // offset: 0 where there is no w
 };
 
 enum { kToBf16 = 0, kToF32 = 1, kToE4m3 = 2 };
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(MAXT) void layer_norm_kernel(NormArgs a) {
   Chunk<T> now[NV], next[NV];
   deal.load(next, x + block * a.x_sr);
   float w[NV][8], b[NV][8];
-  deal.vector(w, a.w, a.wb_f32, group * a.wb_stride, 1.f - a.offset);
+  deal.vector(w, a.w, a.wb_f32, group * a.wb_stride, 1.f);
   deal.vector(b, a.b, a.wb_f32, group * a.wb_stride, 0.f);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(MAXT) void layer_norm_bwd_kernel(NormBwdArgs a) {
     deal.load(gn, g + at * a.g_sr);
   }
   float w[NV][8], dw[NV][8], db[NV][8];
-  deal.vector(w, a.w, a.wb_f32, group * a.wb_stride, 1.f - a.offset);
+  deal.vector(w, a.w, a.wb_f32, group * a.wb_stride, 1.f);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -483,7 +483,7 @@ extern "C" int mdattn_layer_norm(void* stream, const void* x, int x_is_f32, void
   if (!elem_aligned(x, x_is_f32) || !elem_aligned(y, y_is_f32) || !elem_aligned(w, wb_is_f32) || !elem_aligned(b, wb_is_f32)) return MDATTN_E_ALIGN;
   NormArgs a{};
   a.x = x; a.y = y; a.w = w; a.b = b;
-  a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w_offset;
+  a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w ? w_offset : 0.f;
   a.x_sg = x_stride_group; a.x_sr = x_stride_row; a.y_sg = y_stride_group; a.y_sr = y_stride_row;
   return norm((hipStream_t)stream, a, x_is_f32, y_is_f32 ? kToF32 : kToBf16, groups);
 }
@@ -496,7 +496,7 @@ extern "C" int mdattn_layer_norm_e4m3(void* stream, const void* x, int x_is_f32,
   if (!elem_aligned(x, x_is_f32) || !aligned16(q) || !elem_aligned(w, wb_is_f32) || !elem_aligned(b, wb_is_f32)) return MDATTN_E_ALIGN;
   NormArgs a{};
   a.x = x; a.y = q; a.scales = static_cast<uint8_t*>(scales); a.w = w; a.b = b;
-  a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w_offset;
+  a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w ? w_offset : 0.f;
   a.x_sg = x_stride_group; a.x_sr = x_stride_row; a.scale_stride = scale_stride(C);
   return norm((hipStream_t)stream, a, x_is_f32, kToE4m3, groups);
 }
@@ -521,7 +521,7 @@ extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, 
     return MDATTN_E_ALIGN;
   NormBwdArgs a{};
   a.x = x; a.g = g; a.w = w; a.dx = dx; a.part = sums ? workspace : nullptr;
-  a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w_offset;
+  a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w ? w_offset : 0.f;
   a.x_sg = x_stride_group; a.x_sr = x_stride_row; a.g_sg = g_stride_group; a.g_sr = g_stride_row; a.d_sg = dx_stride_group; a.d_sr = dx_stride_row;
   merge_groups(groups, a.rows, wb_stride, {{&a.x_sg, &a.x_sr}, {&a.g_sg, &a.g_sr}, {&a.d_sg, &a.d_sr}});
   const BwdShape b = bwd_shape(groups, a.rows, C, x_is_f32);

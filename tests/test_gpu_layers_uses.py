@@ -135,3 +135,16 @@ def test_tangents_are_refused(dev, recording):
                  lambda: A.hip_norm_rope_ltx2(d, x, w, w, 4), lambda: A.hip_norm_rope_ltx2(x, x, e, w, 4)):
       with pytest.raises(NotImplementedError, match="tangents"):
         call()
+
+
+# ------------------------------------------------------------------------------------------------ arguments
+@pytest.mark.parametrize("offset", [1.0, -1.0, 1e8, 3e38, float("inf")])
+def test_the_weight_offset_is_the_weights(dev, offset):
+  """Without a weight the factor is 1, whatever the offset."""
+  x, b, g = rand(dev, 2, 5, 200, seed=1), rand(dev, 200, seed=2), rand(dev, 2, 5, 200, seed=3)
+  for bias in (None, b):
+    assert torch.equal(ops.layer_norm(x, None, bias, weight_offset=offset), ops.layer_norm(x, None, bias))
+    got, want = ops.layer_norm_quant(x, None, bias, weight_offset=offset), ops.layer_norm_quant(x, None, bias)
+    assert torch.equal(got.values, want.values) and torch.equal(got.scales[:, :2], want.scales[:, :2])
+    for p, q in zip(ops.layer_norm_backward(x, None, bias, g, 1e-6, offset), ops.layer_norm_backward(x, None, bias, g)):
+      assert (p is None and q is None) or torch.equal(p, q)
