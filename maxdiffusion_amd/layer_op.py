@@ -71,6 +71,10 @@ def quantize_weight(weight) -> BlockQuant:
   return ops.quant_block_e4m3(weight.contiguous(), block_rows=128)
 
 
+def _matrix(x):
+  return x.reshape(x.shape[:-1].numel(), x.shape[-1])  # (-1 stands for nothing where the last axis is empty)
+
+
 class _HipLinearFp8(torch.autograd.Function):
   """y = x8 w8^T + b, dx = dy8 w8, dw = dy8'^T x8', ' quantised along the tokens.  Saved for the backward: the weight and x in
   e4m3, transposed (half the bytes of x in bf16); the forms come from one read of each tensor."""
@@ -78,7 +82,7 @@ class _HipLinearFp8(torch.autograd.Function):
   @staticmethod
   def forward(ctx, x, weight, bias):
     need_dx, need_dw, _ = ctx.needs_input_grad
-    rows = x.reshape(-1, x.shape[-1])
+    rows = _matrix(x)
     xq, xt = ops.quant_block_e4m3(rows, transposed=True) if need_dw else (ops.quant_block_e4m3(rows), None)
     wq, wt = ops.quant_block_e4m3(weight, block_rows=128, transposed=True) if need_dx else (ops.quant_block_e4m3(weight, block_rows=128), None)
     keep = [q for q in (xt, wt) if q is not None]
@@ -127,7 +131,7 @@ def hip_linear_fp8(x, weight, bias=None):
     _lib.no_tangents(x, bias)
     if _wants_grad(x, bias):
       raise NotImplementedError("hip_linear_fp8 has no gradient through a quantised weight: give the weight itself, or call it under torch.no_grad()")
-    rows = x.reshape(-1, x.shape[-1])
+    rows = _matrix(x)
     rows = rows if rows.stride(1) == 1 else rows.contiguous()
     return ops.matmul_fp8_block_as(ops.quant_block_e4m3(rows), weight, bias, x.shape[:-1])
   if x.is_cuda and _wants_grad(x, weight, bias):

@@ -148,3 +148,21 @@ def test_the_weight_offset_is_the_weights(dev, offset):
     assert torch.equal(got.values, want.values) and torch.equal(got.scales[:, :2], want.scales[:, :2])
     for p, q in zip(ops.layer_norm_backward(x, None, bias, g, 1e-6, offset), ops.layer_norm_backward(x, None, bias, g)):
       assert (p is None and q is None) or torch.equal(p, q)
+
+
+@pytest.mark.parametrize("shape", [(3, 0), (2, 3, 0), (2, 0, 0), (0,)])
+def test_linear_over_an_empty_axis(dev, shape):
+  """A sum over nothing: the bias alone, and gradients of no elements."""
+  x, g = torch.empty(shape, dtype=BF16, device=dev), rand(dev, *shape[:-1], 4, seed=1, dtype=BF16)
+  w, b = torch.empty((4, 0), dtype=BF16, device=dev), rand(dev, 4, seed=2, dtype=BF16)
+  want = b.expand(*shape[:-1], 4)
+  assert torch.equal(L.hip_linear_fp8(x, w, b), want) and torch.equal(L.hip_linear_fp8(x, L.quantize_weight(w), b), want)
+  assert torch.equal(L.hip_linear_fp8(x, w), torch.zeros_like(want))
+  x, w, b = (t.requires_grad_(True) for t in (x, w, b))
+  y = L.hip_linear_fp8(x, w, b)
+  dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+  assert torch.equal(y, want) and dx.shape == x.shape and dw.shape == w.shape
+  if len(shape) > 1:
+    assert torch.equal(db, g.float().reshape(-1, 4).sum(0).to(BF16))
+    w8 = L.quantize_weight(w.detach())
+    assert torch.equal(L.hip_layer_norm_linear_fp8(x.detach(), None, None, w8, b.detach()), want)

@@ -84,3 +84,11 @@ def test_tangents_are_refused():
                  lambda: attention_op.hip_norm_rope_qkv(torch.cat((q, q, q), -1), v, v, None, 1)):
       with pytest.raises(NotImplementedError, match="tangents"):
         call()
+
+
+# ------------------------------------------------------------------------------------------------ arguments
+def test_an_empty_inner_axis_is_no_error_of_its_own():
+  w = ops.BlockQuant(torch.zeros((4, 0), dtype=torch.uint8), torch.zeros((1, 0), dtype=torch.uint8), 4, 0, 128)
+  for weight in (w, torch.zeros(4, 0, dtype=torch.bfloat16)):
+    with pytest.raises(ValueError, match="device memory"):
+      layer_op.hip_linear_fp8(torch.zeros(2, 3, 0, dtype=torch.bfloat16), weight)
