@@ -773,7 +773,7 @@ bool norm_vectors(const Tensor& x, const Rows3& r, const Tensor& w, const Tensor
   f32 = 0;
   for (const Tensor* t : {&w, &b}) {
     if (!t->defined()) continue;
-    if (!float_on(*t, x) || !t->is_contiguous() || t->numel() == 0 || t->size(t->dim() - 1) != r.c) return false;
+    if (!float_on(*t, x) || !t->is_contiguous() || t->numel() == 0 || t->dim() == 0 || t->size(t->dim() - 1) != r.c) return false;
     const bool per_group = (t->dim() == 2 && t->size(0) == r.groups) || (t->dim() == 3 && t->size(0) == r.groups && t->size(1) == 1);
     if (!per_group && t->dim() != 1) return false;
     const int64_t mine = per_group ? r.c : 0;

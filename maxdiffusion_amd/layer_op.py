@@ -28,6 +28,8 @@ def _forms(*ts):
 
 def _rows(x):
   """x [..., C] as the norm walks it: its last axis contiguous and the axes between the first and the last dense."""
+  if x.dim() < 2:
+    return x  # (refused by the call)
   return x if (x.stride(-1) == 1 or x.shape[-1] == 1) and ops.row_stride(x) is not None else x.contiguous()
 
 
@@ -72,6 +74,8 @@ def quantize_weight(weight) -> BlockQuant:
 
 
 def _matrix(x):
+  if x.dim() == 0:
+    raise ValueError("x must have shape [..., K], got a tensor without axes")
   return x.reshape(x.shape[:-1].numel(), x.shape[-1])  # (-1 stands for nothing where the last axis is empty)
 
 
@@ -139,8 +143,8 @@ def hip_linear_fp8(x, weight, bias=None):
     if y is not None:
       return y
   _lib.no_tangents(x, weight, bias)
-  if weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-    raise ValueError(f"weight must be a BlockQuant or a [N, {x.shape[-1]}] tensor, got {tuple(weight.shape)}")
+  if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
+    raise ValueError(f"weight must be a BlockQuant or a [N, K] tensor for an x [..., K], got {tuple(weight.shape)} for {tuple(x.shape)}")
   x, weight = (t if t.stride(-1) == 1 else t.contiguous() for t in (x, weight))
   if _wants_grad(x, weight, bias):
     if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:

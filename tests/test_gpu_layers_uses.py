@@ -166,3 +166,12 @@ def test_linear_over_an_empty_axis(dev, shape):
     assert torch.equal(db, g.float().reshape(-1, 4).sum(0).to(BF16))
     w8 = L.quantize_weight(w.detach())
     assert torch.equal(L.hip_layer_norm_linear_fp8(x.detach(), None, None, w8, b.detach()), want)
+
+
+def test_tensors_without_axes_are_refused(dev):
+  x, one = rand(dev, 2, 3, 64, seed=1), torch.ones((), device=dev)
+  w8 = L.quantize_weight(rand(dev, 8, 64, seed=2))
+  for call in (lambda: L.hip_layer_norm(one), lambda: L.hip_layer_norm(x, one), lambda: L.hip_layer_norm(x, None, one), lambda: L.hip_linear_fp8(one, w8),
+               lambda: L.hip_linear_fp8(x, w8, one), lambda: L.hip_linear_fp8(x, one), lambda: L.hip_layer_norm_linear_fp8(x, one, None, w8)):
+    with pytest.raises(ValueError):
+      call()

@@ -92,3 +92,13 @@ def test_an_empty_inner_axis_is_no_error_of_its_own():
   for weight in (w, torch.zeros(4, 0, dtype=torch.bfloat16)):
     with pytest.raises(ValueError, match="device memory"):
       layer_op.hip_linear_fp8(torch.zeros(2, 3, 0, dtype=torch.bfloat16), weight)
+
+
+def test_tensors_without_axes_are_refused():
+  x, one = torch.zeros(2, 0), torch.zeros(())
+  w = ops.BlockQuant(torch.zeros((4, 0), dtype=torch.uint8), torch.zeros((1, 0), dtype=torch.uint8), 4, 0, 128)
+  for call in (lambda: layer_op.hip_layer_norm(one), lambda: layer_op.hip_layer_norm(torch.zeros(3)), lambda: layer_op.hip_linear_fp8(one, w),
+               lambda: layer_op.hip_linear_fp8(one, x), lambda: layer_op.hip_linear_fp8(x, one), lambda: layer_op.hip_layer_norm_linear_fp8(one, None, None, w),
+               lambda: layer_op.quantize_weight(one)):
+    with pytest.raises(ValueError):
+      call()
