@@ -9,6 +9,7 @@
 // 16.5; a training step's backward runs in autograd's own thread without the interpreter: 255-465 us of host time per
 // step become 91-108.
 #include <ATen/ATen.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -41,8 +42,10 @@ Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 // a tensor that carries a tangent (forward-mode differentiation): left to the Python path, which refuses it
 bool dual(const Tensor& t) { return t._fw_grad(0).defined(); }
+// ref is the call's first tensor, on the device whose current stream the call takes
+bool beside(const Tensor& t, const Tensor& ref) { return t.get_device() == (&t == &ref ? c10::hip::current_device() : ref.get_device()); }
 bool bf16_on(const Tensor& t, const Tensor& ref) {
-  return t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.get_device() == ref.get_device() && !t.is_neg() && !dual(t);
+  return t.is_cuda() && t.scalar_type() == at::kBFloat16 && beside(t, ref) && !t.is_neg() && !dual(t);
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
@@ -333,6 +336,7 @@ bool flash_merge(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
     return false;
   if (q.stride(3) != 1 || k.stride(3) != 1 || v.stride(3) != 1 || o_run.stride(3) != 1 || k.sizes() != v.sizes() || k.size(0) != q.size(0) ||
       k.size(2) != q.size(2) || k.size(3) != q.size(3) || o_run.sizes() != q.sizes() || o_run.scalar_type() != at::kFloat || !o_run.is_cuda() ||
+      !beside(o_run, q) || !beside(lse_run, q) ||
       lse_run.scalar_type() != at::kFloat || !lse_run.is_cuda() || !lse_run.is_contiguous() || lse_run.dim() != 3 || lse_run.size(0) != q.size(0) ||
       lse_run.size(1) != q.size(2) || lse_run.size(2) != q.size(1))
     return false;
@@ -706,7 +710,7 @@ struct RowsFn : FirstOrder<RowsFn> {
 std::optional<variable_list> norm_rope_rows(const Tensor& q, const OptTensor& k_, const Tensor& wq, const OptTensor& wk_, const OptTensor& cos_,
                                             const OptTensor& sin_, int64_t heads, int64_t mode, double eps, double w_mul) {
   const Tensor k = value(k_), wk = value(wk_), cos = value(cos_), sin = value(sin_);
-  if (!q.is_cuda() || (q.scalar_type() != at::kFloat && q.scalar_type() != at::kBFloat16) || q.is_neg() || dual(q) || q.dim() != 3 || q.numel() == 0 ||
+  if (!q.is_cuda() || !beside(q, q) || (q.scalar_type() != at::kFloat && q.scalar_type() != at::kBFloat16) || q.is_neg() || dual(q) || q.dim() != 3 || q.numel() == 0 ||
       q.stride(2) != 1 || heads <= 0 || q.size(2) % heads)
     return std::nullopt;
   const int64_t b = q.size(0), s = q.size(1), n = q.size(2);
@@ -737,7 +741,7 @@ std::optional<variable_list> norm_rope_rows(const Tensor& q, const OptTensor& k_
 // ------------------------------------------------------------------------------------------------ the layers beside attention
 // (layer_op.py, ops.py.)  An undefined tensor is a missing one.
 bool float_on(const Tensor& t, const Tensor& ref) {
-  return t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) && t.get_device() == ref.get_device() && !t.is_neg() &&
+  return t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) && beside(t, ref) && !t.is_neg() &&
          !dual(t);
 }
 int is_f32(const Tensor& t) { return t.defined() && t.scalar_type() == at::kFloat; }

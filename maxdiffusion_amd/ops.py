@@ -55,9 +55,17 @@ def _stream():
 
 
 def _check_dev(*ts):
+  """All in the memory of the current device, whose stream the kernels run on: another one's may not be theirs to read."""
+  device = None
   for t in ts:
-    if t is not None and not t.is_cuda:
+    if t is None:
+      continue
+    if not t.is_cuda:
       raise ValueError("mdattn operators need tensors in device memory (cuda/HIP); there is no CPU path")
+    if device is None:
+      device = torch.cuda.current_device()
+    if t.get_device() != device:
+      raise ValueError(f"mdattn operators need their tensors on the current device, cuda:{device}: one is on cuda:{t.get_device()}")
 
 
 def _strides(t: torch.Tensor) -> Strides:

@@ -102,3 +102,17 @@ def test_tensors_without_axes_are_refused():
                lambda: layer_op.quantize_weight(one)):
     with pytest.raises(ValueError):
       call()
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+  class On:
+    is_cuda = True
+
+    def __init__(self, device):
+      self.get_device = lambda: device
+
+  monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+  ops._check_dev(On(1), None, On(1))
+  for ts in ((On(1), On(0)), (On(0),), (None, On(0), On(0))):
+    with pytest.raises(ValueError, match="current device"):
+      ops._check_dev(*ts)
