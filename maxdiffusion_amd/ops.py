@@ -726,8 +726,9 @@ class BlockQuant:
 
   def dequantize(self, dtype=torch.float32):
     """The numbers that it stands for, [rows, cols] (plain torch, for inspection)."""
-    v = self.values.view(torch.float8_e4m3fn).to(torch.float32)
-    s = torch.exp2(self.scales.to(torch.float32) - 127).masked_fill_(self.scales == 255, math.nan)
+    wide = torch.promote_types(dtype, torch.float32)  # (256 * 2^120, which f32's largest numbers round to, is no f32)
+    v = self.values.view(torch.float8_e4m3fn).to(wide)
+    s = torch.exp2(self.scales.to(wide) - 127).masked_fill_(self.scales == 255, math.nan)
     s = s.repeat_interleave(self.block_rows, 0)[:self.rows].repeat_interleave(128, 1)[:, :v.shape[1]]
     return (v * s)[:, :self.cols].to(dtype)
 

@@ -116,3 +116,12 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
   for ts in ((On(1), On(0)), (On(0),), (None, On(0), On(0))):
     with pytest.raises(ValueError, match="current device"):
       ops._check_dev(*ts)
+
+
+def test_dequantized_in_64_bits():
+  """f32's largest numbers round up to 2^128, the smallest block's last place is 2^-136."""
+  values = torch.zeros((3, 128), dtype=torch.uint8)
+  values[0, 0], values[1, 0], values[2, 0] = 0x78, 0x01, 0x7E  # 256, 2^-9, 448
+  q = ops.BlockQuant(values, torch.tensor([[247, 0, 0, 0], [0, 0, 0, 0], [127, 0, 0, 0]], dtype=torch.uint8), 3, 1, 1)
+  assert q.dequantize(torch.float64)[:, 0].tolist() == [2.0**128, 2.0**-136, 448.0]
+  assert q.dequantize()[:, 0].tolist() == [float("inf"), 2.0**-136, 448.0]
