@@ -4,6 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import layer_inputs
 from maxdiffusion_amd import attention_op as A
 from maxdiffusion_amd import layer_op as L
 from maxdiffusion_amd import ops
@@ -175,3 +176,36 @@ def test_tensors_without_axes_are_refused(dev):
                lambda: L.hip_linear_fp8(x, w8, one), lambda: L.hip_linear_fp8(x, one), lambda: L.hip_layer_norm_linear_fp8(x, one, None, w8)):
     with pytest.raises(ValueError):
       call()
+
+
+# ------------------------------------------------------------------------------------------------ every form of the product
+# (few rows; tiles of 128 and of 256; either with K split, which only its workspace says; whole rounds of tiles and what they leave)
+FORMS = [(7, 300, 4100, 0), (30, 1501, 1000, 0), (130, 300, 4096, 128), (700, 900, 4096, 128), (333, 520, 1000, None), (2900, 1507, 15759, 256), (2900, 1504, 15759, 256),
+         (4200, 3800, 900, None), (3900, 4051, 1100, None), (4300, 4096, 4100, 128)]
+
+
+def test_forms_are_the_ones_that_are_meant(lib):
+  for m, n, k, tile in FORMS:
+    floats = lib.mdattn_matmul_fp8_block_workspace_floats(m, n, k)
+    if not tile:
+      assert floats == 0
+      continue
+    rows = m if m < 4300 else m - 4096  # (whole rounds of 16 x 16 tiles of 256 go first)
+    area = -(-rows // tile) * tile * -(-n // tile) * tile
+    assert floats >= 2 * area and floats % area == 0
+    if tile == 256:  # and not of 128
+      assert floats % (-(-rows // 128) * 128 * -(-n // 128) * 128) != 0
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("m,n,k,tile", FORMS)
+def test_product_by_every_form(dev, m, n, k, tile, block_rows):
+  """Scale bytes that differ between rows and blocks, sums that need f32: exact, with a bias and without."""
+  for make in (layer_inputs.scaled, layer_inputs.cancelling):
+    a, b, want = make(m, n, k, dev, seed=m + block_rows)
+    qa, qb = ops.quant_block_e4m3(a), ops.quant_block_e4m3(b, block_rows)
+    assert torch.equal(qa.dequantize(), a) and torch.equal(qb.dequantize(), b)  # (blocks hold them as they are)
+    assert torch.equal(ops.matmul_fp8_block(qa, qb).float(), want)
+    bias = torch.randint(-4, 5, (n,), device=dev).float()
+    for t in (bias, bias.to(BF16)):
+      assert torch.equal(ops.matmul_fp8_block(qa, qb, t).float(), (want + bias).to(BF16).float())

@@ -5,6 +5,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import layer_inputs
 from maxdiffusion_amd import _lib, attention_op, layer_op, ops
 
 P = ctypes.c_void_p
@@ -125,3 +126,22 @@ def test_dequantized_in_64_bits():
   q = ops.BlockQuant(values, torch.tensor([[247, 0, 0, 0], [0, 0, 0, 0], [127, 0, 0, 0]], dtype=torch.uint8), 3, 1, 1)
   assert q.dequantize(torch.float64)[:, 0].tolist() == [2.0**128, 2.0**-136, 448.0]
   assert q.dequantize()[:, 0].tolist() == [float("inf"), 2.0**-136, 448.0]
+
+
+# ------------------------------------------------------------------------------------------------ what the tests of the product can see
+def test_exact_operands_show_a_wrong_scale_and_a_rounded_sum():
+  """Mistakes planted in a plain product of the operands that the GPU tests use."""
+  a, b, want = layer_inputs.cancelling(5, 7, 4096, "cpu")
+  for kept, steps in ((torch.float32, 0.0), (torch.bfloat16, 0.9), (torch.float16, 0.4)):  # (the share of results that come out wrong, at least)
+    s = torch.zeros(5, 7, dtype=kept)
+    for i in range(0, 4096, 128):
+      s = (s.double() + a[:, i : i + 128].double() @ b[:, i : i + 128].double().t()).to(kept)
+    wrong = (s.float() != want).float().mean()
+    assert wrong == 0 if kept == torch.float32 else wrong >= steps, kept
+  a, b, want = layer_inputs.scaled(300, 300, 900, "cpu")
+  assert torch.equal(a @ b.t(), want)
+  blocks = lambda t, by: torch.cat([t[:, i : i + 128] * (2.0 if i // 128 == by else 1.0) for i in range(0, 900, 128)], 1)
+  assert not torch.equal(blocks(a, 3) @ b.t(), want) and not torch.equal(blocks(a, 7) @ b.t(), want)
+  exps = lambda t: torch.frexp(t[:, :896].reshape(300, 7, 128).abs().amax(2))[1]
+  for t in (a, b):  # bytes that differ between a row's blocks and between a block's rows
+    assert len(exps(t)[0].unique()) > 3 and len(exps(t)[:, 0].unique()) > 2
