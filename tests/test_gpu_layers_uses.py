@@ -1,5 +1,8 @@
 """The layers beside attention as programs use them: calls past what a grid can count, outputs that are changed in place, hooks, autograd's
 other modes, arguments that the usual path leaves aside.  Tolerances as in the tests of the kernels: bit for bit where nothing is said."""
+import importlib.util
+import os
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -8,6 +11,8 @@ import layer_inputs
 from maxdiffusion_amd import attention_op as A
 from maxdiffusion_amd import layer_op as L
 from maxdiffusion_amd import ops
+
+from test_gpu_layers import assert_quant, blocks64, close, half_ulp, norm64, plain_block
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -209,3 +214,71 @@ def test_product_by_every_form(dev, m, n, k, tile, block_rows):
     bias = torch.randint(-4, 5, (n,), device=dev).float()
     for t in (bias, bias.to(BF16)):
       assert torch.equal(ops.matmul_fp8_block(qa, qb, t).float(), (want + bias).to(BF16).float())
+
+
+# ------------------------------------------------------------------------------------------------ the norm
+@pytest.mark.parametrize("xt", [BF16, F32])
+@pytest.mark.parametrize("c", [6145, 6200, 8191, 8192, 12288, 12289, 16383, 16384])
+def test_wide_norm_into_blocks(dev, c, xt):
+  """Teams of 512 and 1,024 threads, with a last block that the row ends in: values, scale bytes and the zeros behind the row."""
+  x = rand(dev, 2, 37, c, seed=c, dtype=xt) + 0.5
+  w, b = (rand(dev, 2, c, seed=i, std=0.3) for i in (2, 3))
+  got = ops.layer_norm_quant(x, w, b, weight_offset=1.0)
+  rows = ops.layer_norm(x, w, b, weight_offset=1.0, out_dtype=F32)
+  want, _, _, _, size = norm64(x, w, b, 1e-6, 1.0)
+  close(rows, want, half_ulp(want, F32) + 16 * 2.0**-24 * size, str(c))
+  assert_quant(got, rows.view(-1, c), 1, str(c))
+  assert not bool(got.values[:, c:].any())
+
+
+@pytest.mark.parametrize("xt", [BF16, F32])
+def test_norm_by_views_of_a_modulation(dev, xt):
+  """adaLN's scale and shift as a model has them, chunks of [B, 6, C]: the results of dense copies, and the gradient of the whole."""
+  x, g = rand(dev, 3, 50, 264, seed=1, dtype=xt), rand(dev, 3, 50, 264, seed=2, dtype=xt)
+  m = rand(dev, 3, 6, 264, seed=3).requires_grad_(True)
+  shift, scale = m.chunk(6, dim=1)[:2]
+  s, t = (v.detach().contiguous().requires_grad_(True) for v in (scale, shift))
+  w8 = L.quantize_weight(rand(dev, 130, 264, seed=4))
+  with torch.no_grad():
+    assert torch.equal(L.hip_layer_norm(x, scale, shift, weight_offset=1.0), L.hip_layer_norm(x, s, t, weight_offset=1.0))
+    assert torch.equal(L.hip_layer_norm_linear_fp8(x, scale, shift, w8, weight_offset=1.0), L.hip_layer_norm_linear_fp8(x, s, t, w8, weight_offset=1.0))
+  x = x.requires_grad_(True)
+  dx, dm = torch.autograd.grad(L.hip_layer_norm(x, scale, shift, weight_offset=1.0), (x, m), g)
+  wx, ws, wt = torch.autograd.grad(L.hip_layer_norm(x, s, t, weight_offset=1.0), (x, s, t), g)
+  assert torch.equal(dx, wx) and torch.equal(dm, torch.cat((wt, ws, torch.zeros(3, 4, 264, device=dev)), 1))
+
+
+# ------------------------------------------------------------------------------------------------ all of them in one block
+def test_gradients_of_the_example_block(dev):
+  """Each weight's gradient against that of the block in 64 bits on the CPU, its dense layers' operands as blocks of e4m3 hold them and rounding
+  passed through.  Left is what the kernels round beside: the output gradients, and x along the tokens, to e4m3 (2^-4 of a value at most, 2^-5
+  of a vector's length), in up to four products between the loss and a weight, a tenth in all if none cancels, and bf16 between the layers;
+  attention's backward subtracts, which is allowed to double it, and the sum of both to grow by a quarter."""
+  path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "wan_block_fp8.py")
+  spec = importlib.util.spec_from_file_location("wan_block_fp8", path)
+  ex = importlib.util.module_from_spec(spec)
+  spec.loader.exec_module(ex)
+  heads, grid = 2, (3, 6, 7)
+  block = ex.make_block(heads, dev)
+  x, modulation, freqs = rand(dev, 2, 126, 256, seed=1, dtype=BF16), rand(dev, 6, 2, 256, seed=2, std=0.1), ex.rotary_table(*grid, dev)
+
+  class Held(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, t, block_rows):
+      v, byte = blocks64(t, block_rows)
+      scale = torch.exp2(byte.double() - 127).repeat_interleave(block_rows, 0)[: t.shape[0]].repeat_interleave(128, 1)
+      return (v.view(torch.float8_e4m3fn).double() * scale)[:, : t.shape[1]]
+
+    @staticmethod
+    def backward(ctx, g):
+      return g, None
+
+  plain = {n: t.cpu().double().requires_grad_(True) for n, t in block.items()}
+  y = plain_block(plain, x.cpu(), modulation.cpu(), freqs.cpu(), heads, Held.apply)
+  want = torch.autograd.grad(y.square().mean(), list(plain.values()))
+  leaves = [t.requires_grad_(True) for t in block.values()]
+  z = ex.run_block(block, x, modulation, freqs, heads)
+  for name, g, w in zip(block, torch.autograd.grad(z.float().square().mean(), leaves), want):
+    off = (g.cpu().double() - w).norm() / w.norm()
+    print(f"{name}: {off.item():.4f}")
+    assert off <= 0.25, name
