@@ -25,7 +25,7 @@ extern "C" {
  *   x, y          bf16 or f32 (x_is_f32, y_is_f32), [groups, rows, C] by the strides of a group and of a row, in elements;
  *                 C contiguous.  A group is what shares w and b: a batch element.  y may be x where types and strides agree.
  *   w, b          bf16 or f32 (wb_is_f32), C channels each, dense; wb_stride elements between groups, 0: shared.  Either may be
- *                 NULL: y = h + b, y = h * (w_offset + w).
+ *                 NULL: y = h + b whatever w_offset is, y = h * (w_offset + w).
  * Statistics and arithmetic in f32, the variance from differences to the mean, one rounding.
  * 1 <= C <= 16384; pointers and strides need the alignment of an element only.
  */
@@ -63,7 +63,7 @@ int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, const void*
  * (0xFF, a NaN, and NaNs for the values, where the block holds an infinity or a NaN).
  *   x             bf16 or f32, rows x_stride elements apart, C contiguous
  *   q, scales     or NULL: e4m3 bytes [R, ceil128(C)], and [ceil(R / block_rows), ceil4(ceil(C / 128))] scale bytes; dense.  The
- *                 padding of q's rows is zero, that of the scales' rows unspecified.
+ *                 padding of q's rows is zero (NaN in a block that is not finite), that of the scales' rows unspecified.
  *   qt, scales_t  or NULL: the same of x transposed, [C, ceil128(R)], blocks of block_rows x 128 of the transposed matrix
  *   colsum        or NULL: f32 [ceil(R / 128), C], the sum of each column over each 128 rows
  * q, qt 16-byte aligned, scales 4-byte aligned; x the alignment of an element.

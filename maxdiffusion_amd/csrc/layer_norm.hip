@@ -10,8 +10,10 @@
 // formulae and a pairwise algorithm for computing sample variances, 1979), which loses nothing where the mean is large against the
 // deviation, and takes one exchange through LDS, and one barrier, per row.
 // Bound by memory.  bf16 rows, read and written: 75,600 x 5,120 forward 283 us and backward 426 us, both 5.4 TB/s; 32,760 x 1,536 32 to 35 us;
-// with a quantised output 30 us, 5.0 TB/s (75,600 x 5,120 252 us, 4.6: the scale bytes are scattered stores).  Short calls are bound by the
-// way of a row through memory and its reductions: 4,112 x 1,280 forward 7 us, backward 11 and 4 for the sums.
+// with a quantised output 30 us, 5.0 TB/s (75,600 x 5,120 252 us, 4.6: the scale bytes are scattered stores).  f32 rows of 600 MB: forward 4.1
+// to 5.6 TB/s, backward 4.4 to 5.2.  Backward above 12,288 channels, where 1,024 threads leave each 128 registers and 7 to 113 are spilled:
+// bf16 2.8 to 3.4 TB/s (5.3 at 12,288), f32 2.5 to 2.9.  Short calls are bound by the way of a row through memory and its reductions: 4,112 x
+// 1,280 forward 7 us, backward 11 and 4 for the sums.
 #include "mdattn_common.h"
 #include "mdlayers.h"
 #include "quant_block.h"
@@ -396,8 +398,9 @@ Shape shape_of(int C) {
       if (nv * t >= chunks && (best.nv == 0 || nv * t < best.nv * best.threads || (nv * t == best.nv * best.threads && nv > best.nv))) best = {nv, t};
   return best;
 }
-// Rows in flight on a CU, by their bytes: enough to keep the memory busy, and no more, which would make the rows' pages compete.  16 KB of
-// rows forward (8,192 channels: one row 5.8 TB/s, four 5.4; 2,048: four 5.8, sixteen 5.4), 36 with a quantised output, whose arithmetic needs
+// Rows in flight on a CU, by their bytes: enough to keep the memory busy, and no more, which would make the rows' pages compete.  18 KB of
+// rows forward, in bf16 the best number or near it at all but one of the widths measured (512 channels: eighteen rows 6.05 TB/s, six 3.7; 1,536: six
+// 5.9, three 4.9, twelve 5.5; 2,560: four 5.6, three 4.8; 5,120: two 5.5, four 5.2; 8,192: one 6.2, two 5.5; but 2,048: five 5.6, four 5.9), 36 with a quantised output, whose arithmetic needs
 // more waves (5,120: two 3.4, four 4.5), 32 of x and g backward (2,048: four 4.9, twelve 3.8; 5,120: two 5.2, four 4.4).
 int rows_per_cu(int64_t row_bytes, int64_t in_flight, int least) { return (int)((in_flight + row_bytes / 2) / row_bytes < least ? least : (in_flight + row_bytes / 2) / row_bytes); }
 // Workgroups of one group of so many rows, of all groups' `target`, and no more than go through them in as many rounds

@@ -80,7 +80,8 @@ __device__ __forceinline__ TileAt tile_of(int id, int mt, int nt) {
 
 // A wave's sums to memory: of each 16 x 16, lane l holds row l % 16 and columns 4 (l / 16) to + 3.  By whole rows, through LDS: 32 rows x kCols
 // columns at a time, 16-byte chunk c of row r at c ^ ((r >> 1) & (chunks - 1)).  (Stored from the registers, 16 bytes of a row at a time, they
-// took as long as 20 steps.)
+// took as long as 20 steps.)  Rows whose 16-byte chunks are not aligned (N or c_stride no multiple of 8) go two bytes at a time: 2,674 x 5,121 x
+// 2,048 53 us, 5,120 columns 31; 18,900 x 5,121 x 5,120 477 and 353.
 template <int BM, int BN, int TM, int TN>
 __device__ __forceinline__ void store_rows(const MatmulArgs& p, f32x4 (&acc)[TN][TM], char* smem, int64_t m0, int64_t n0, int lane, int wave) {
   using L = Layout<BM, BN>;
@@ -511,9 +512,13 @@ struct Plan {
 };
 constexpr int kFewRows = 32;
 constexpr int kAlone = 256;  // tiles of 128 by whose number each has its CU to itself
-// The fastest by these measured times: a step of 128 of K takes 1.42 us in a tile of 256, 0.57 in one of 128 that has its CU to itself, and
-// 1.0 where two share it; a tile 8 and 4 us beside its steps; the pieces' sums pass through memory at 1.4 TB/s.  (4,096^3:
-// tiles of 256 54 us, of 128 65; 4,680 x 4,608 x 1,536 43 and 40; 1,000 x 1,000 x 16,384: 64 tiles of 128 whole 56, in four pieces 27.)
+// The fastest by a model of steps of 128 of K, of a tile's time beside them, and of the pieces' sums.  Its constants (a step 1.42 us in a tile of
+// 256, 0.57 in one of 128 that has its CU to itself, 1.0 where two share it; 8 and 4 us beside the steps; the sums at 1.4 TB/s) compare the
+// forms; as times they are upper bounds, by up to 45 %.  Measured now: a step 1.35 us in a tile of 256 (1.0 while most CUs are idle, and the
+// clock is higher), 0.42 and 0.85 in one of 128; beside the steps 5 us and 3 more for the first tile of 256, 4.4 and 3.6; the sums 3.2 TB/s.  Each of 26
+// products from 64 x 5,120 x 5,120 to 32,760 x 4,608 x 1,536 was forced through both tiles in 1 to 8 pieces: what is chosen here was the fastest or within
+// 5 % of it.  (4,096^3: tiles of 256 52 us, of 128 61; 4,680 x 4,608 x 1,536 40 and 38; 1,000 x 1,000 x 16,384: 64 tiles of 128 whole 56, in
+// four pieces 25.)
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
   const int kb = (int)((K + 127) / 128);
   if (M <= kFewRows && grid_fits((N + 15) / 16, 512)) return {0, 1, kb, 4.0 + (double)N * K / 3e6};
@@ -534,8 +539,8 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 // Rows of c that go first, in tiles of 256 and whole rounds of them, where what remains is faster by a plan of its own than as one more round
-// that leaves most of the chip idle; 0: all go together.  (75,600 x 5,120 x 5,120, 23.1 rounds: 1,559 us and 1,547;
-// 4,200 x 5,120 x 13,824, 1.3 rounds: 271 and 239.)
+// that leaves most of the chip idle; 0: all go together.  (75,600 x 5,120 x 5,120, 23.1 rounds: 1,395 us and 1,386;
+// 4,200 x 5,120 x 13,824, 1.3 rounds: 262 and 236; 4,160 x 4,160 x 5,120 104 and 79.)
 int64_t rows_first(const Plan& all, int64_t M, int64_t N, int64_t K) {
   const int64_t nt = (N + 255) / 256, tiles = (M + 255) / 256 * nt;
   if (all.tile != 256 || all.pieces != 1 || tiles <= 256) return 0;

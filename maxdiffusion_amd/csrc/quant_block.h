@@ -8,7 +8,6 @@ namespace mdattn {
 // 16 bytes wide all the same: this card takes them at any address).
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
-typedef u32x2 u32x2_any __attribute__((aligned(4)));
 
 __device__ __forceinline__ unsigned row16_umax(unsigned x) {
   x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0u, x, 0xB1, 0xF, 0xF, true));

@@ -1,6 +1,7 @@
 """The layers beside attention in a DiT block, as a model calls them: layer norm and dense layers in blocks of e4m3.
 
-Differentiable where an input requires a gradient while autograd is recording (paths relative to ``src/maxdiffusion/``):
+Differentiable where an input requires a gradient while autograd is recording; once, and not in forward mode: second derivatives and
+tensors with a tangent raise NotImplementedError (paths relative to ``src/maxdiffusion/``):
 
   hip_layer_norm                FP32LayerNorm with adaLN's scale and shift, or affine   models/wan/transformers/transformer_wan.py:487
   hip_linear_fp8                a dense layer on e4m3 operands (the reference's qwix quantisation of dense layers, per tensor or
@@ -55,7 +56,8 @@ class _HipLayerNorm(torch.autograd.Function):
 def hip_layer_norm(x, weight=None, bias=None, eps: float = 1e-6, weight_offset: float = 0.0):
   """x [..., C], bf16 or f32 -> the same: h * (weight_offset + weight) + bias, h the row less its mean, over its deviation.
 
-  weight and bias [C], or per element of x's first axis [B, C] or [B, 1, C]: adaLN is (scale, shift, weight_offset=1)."""
+  weight and bias [C], or, where x has three axes or more, per element of its first one [B, C] or [B, 1, C]: adaLN is (scale, shift,
+  weight_offset=1).  Views that are not contiguous (chunks of a [B, 6, C]) are copied."""
   if x.is_cuda:
     y = _lib.host().layer_norm(x, weight, bias, eps, weight_offset)
     if y is not None:

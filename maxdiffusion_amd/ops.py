@@ -654,8 +654,8 @@ def _norm_vectors(weight, bias, groups, c):
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-6, weight_offset: float = 0.0, out_dtype=None):
   """h * (weight_offset + weight) + bias with h = (x - mean) / sqrt(var + eps) over the last axis of x [..., C], bf16 or f32.
 
-  weight, bias: bf16 or f32, [C], or one per element of x's first axis, [B, C] or [B, 1, C] (adaLN's scale and shift, with
-  weight_offset 1); None: h (+ bias), h * (weight_offset + weight).  Statistics and arithmetic in f32, rounded once to out_dtype (x's)."""
+  weight, bias: bf16 or f32, [C], or, for an x of three axes or more, one per element of its first axis, [B, C] or [B, 1, C] (adaLN's
+  scale and shift, with weight_offset 1); None: h (+ bias), whatever weight_offset is, and h * (weight_offset + weight).  Statistics and arithmetic in f32, rounded once to out_dtype (x's)."""
   _check_dev(x, weight, bias)
   x_f32 = _float_kind(x, "x")
   groups, rows, c, sg, sr = _norm_rows(x)
@@ -712,7 +712,7 @@ def layer_norm_backward(x, weight, bias, g, eps: float = 1e-6, weight_offset: fl
 class BlockQuant:
   """A matrix [rows, cols] held as e4m3 with one power-of-two scale per block of block_rows x 128.
 
-  values: uint8 [rows, cols rounded up to 128], the padding zero.  scales: uint8 [ceil(rows / block_rows), blocks of a row
+  values: uint8 [rows, cols rounded up to 128], the padding zero (NaN in a block that is not finite).  scales: uint8 [ceil(rows / block_rows), blocks of a row
   rounded up to 4], the exponents with a bias of 127 (0xFF: a block that is not finite).  Both dense."""
   __slots__ = ("values", "scales", "rows", "cols", "block_rows")
 
