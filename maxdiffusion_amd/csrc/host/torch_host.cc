@@ -32,7 +32,8 @@ using OptTensor = std::optional<Tensor>;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-void* stream() { return c10::hip::getCurrentHIPStream().stream(); }
+// the current stream of the device of a tensor that the call has checked (`beside`)
+void* stream(const Tensor& on) { return c10::hip::getCurrentHIPStream(on.get_device()).stream(); }
 const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* mut(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* f32(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
@@ -201,7 +202,7 @@ int fwd(const Tensor& q, const Tensor& k, const Tensor& v, const View& vq, const
   const mdattn_strides so{out.stride(0), out.stride(1), vq.d};
   const int64_t nws = m.bias ? 0 : mdattn_host_fwd_workspace_floats((int)vq.b, (int)vq.h, (int)vq.s, (int)vk.s, (int)vq.d);
   const Tensor ws = nws ? at::empty({nws}, q.options().dtype(at::kFloat)) : Tensor();
-  return mdattn_host_fwd_bf16(stream(), ptr(q), ptr(k), ptr(v), mut(out), f32(lse), (int)vq.b, (int)vq.h, (int)vq.s, (int)vk.s, (int)vq.d, &vq.st, &vk.st,
+  return mdattn_host_fwd_bf16(stream(q), ptr(q), ptr(k), ptr(v), mut(out), f32(lse), (int)vq.b, (int)vq.h, (int)vq.s, (int)vk.s, (int)vq.d, &vq.st, &vk.st,
                               &vv.st, &so, (float)scale, m.bias, m.stride, m.tiles, f32(ws), nws);
 }
 
@@ -247,7 +248,7 @@ struct FlashFn : FirstOrder<FlashFn> {
     const int64_t nws = mdattn_host_bwd_plan_floats(B, H, Sq, Skv, D, m.bias != nullptr, -1, &plan);
     Tensor ws = at::empty({nws}, lse.options());
     const mdattn_strides so{out.stride(0), out.stride(1), vq.d};
-    const int rc = mdattn_host_bwd_bf16(stream(), ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), f32(lse), mut(dq), mut(dk), mut(dv), f32(ws), nws, B, H, Sq,
+    const int rc = mdattn_host_bwd_bf16(stream(q), ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), f32(lse), mut(dq), mut(dk), mut(dv), f32(ws), nws, B, H, Sq,
                                         Skv, D, &vq.st, &vk.st, &vv.st, &so, (float)scale, m.bias, m.stride, m.tiles, &plan);
     must(rc, "mdattn_bwd_bf16");
     return {dq, dk, dv, Tensor(), Tensor(), Tensor()};
@@ -262,7 +263,7 @@ Tensor make_mask(const Tensor& keep, const View& vk, const Tensor& ref) {
   const int B = (int)vk.b, S = (int)vk.s;
   Tensor m = at::empty({Mask::floats(vk)}, keep.options().dtype(at::kFloat));
   const Mask v(m, vk);
-  return mdattn_host_key_tiles(stream(), ptr(keep), v.bias, v.tiles, B, S, v.stride) == MDATTN_OK ? m : Tensor();
+  return mdattn_host_key_tiles(stream(keep), ptr(keep), v.bias, v.tiles, B, S, v.stride) == MDATTN_OK ? m : Tensor();
 }
 
 // The registry entry's operands, checked: false when the Python path has to take over
@@ -313,7 +314,7 @@ OptTensor flash_fp8(const Tensor& q, const Tensor& k, const Tensor& v, int64_t h
   const auto bytes = q.options().dtype(at::kByte);
   Tensor q8 = at::empty({q.numel()}, bytes), k8 = at::empty({k.numel()}, bytes), v8 = at::empty({v.numel()}, bytes);
   Tensor ws = at::empty({mdattn_host_quant3_floats()}, q.options().dtype(at::kFloat));
-  if (mdattn_host_quant3_e4m3(stream(), ptr(q), ptr(k), ptr(v), mut(q8), mut(k8), mut(v8), f32(ws), q.numel(), k.numel(),
+  if (mdattn_host_quant3_e4m3(stream(q), ptr(q), ptr(k), ptr(v), mut(q8), mut(k8), mut(v8), f32(ws), q.numel(), k.numel(),
                               (float)(scale * 1.4426950408889634)) != MDATTN_OK)
     return std::nullopt;
   Tensor out = at::empty({vq.b, vq.s, vq.h * vq.d}, q.options());
@@ -322,9 +323,9 @@ OptTensor flash_fp8(const Tensor& q, const Tensor& k, const Tensor& v, int64_t h
   const float *s = f32(ws), scale8 = (float)0.6931471805599453;  // q's quantisation carries scale * log2(e)
   const int B = (int)vq.b, H = (int)vq.h, Sq = (int)vq.s, Skv = (int)vk.s, D = (int)vq.d;
   const Mask m(mask, vk);
-  const int rc = m.bias ? mdattn_fwd_fp8_bias(stream(), ptr(q8), ptr(k8), ptr(v8), mut(out), nullptr, B, H, Sq, Skv, D, &sq, &skv, &skv, &sq, scale8, s,
+  const int rc = m.bias ? mdattn_fwd_fp8_bias(stream(q8), ptr(q8), ptr(k8), ptr(v8), mut(out), nullptr, B, H, Sq, Skv, D, &sq, &skv, &skv, &sq, scale8, s,
                                               s + 2, s + 4, m.bias, m.stride)
-                        : mdattn_fwd_fp8(stream(), ptr(q8), ptr(k8), ptr(v8), mut(out), nullptr, B, H, Sq, Skv, D, &sq, &skv, &skv, &sq, scale8, s, s + 2,
+                        : mdattn_fwd_fp8(stream(q8), ptr(q8), ptr(k8), ptr(v8), mut(out), nullptr, B, H, Sq, Skv, D, &sq, &skv, &skv, &sq, scale8, s, s + 2,
                                          s + 4, MDATTN_FP8_SOFTMAX_BYTE_GRID);
   if (rc != MDATTN_OK) return std::nullopt;
   return out;
@@ -341,7 +342,7 @@ bool flash_merge(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
       lse_run.size(1) != q.size(2) || lse_run.size(2) != q.size(1))
     return false;
   const mdattn_strides sq = strides4(q), sk = strides4(k), sv = strides4(v), so = strides4(o_run);
-  return mdattn_fwd_bf16_merge(stream(), ptr(q), ptr(k), ptr(v), f32(o_run), f32(lse_run), (int)q.size(0), (int)q.size(2), (int)q.size(1),
+  return mdattn_fwd_bf16_merge(stream(q), ptr(q), ptr(k), ptr(v), f32(o_run), f32(lse_run), (int)q.size(0), (int)q.size(2), (int)q.size(1),
                                (int)k.size(1), (int)q.size(3), &sq, &sk, &sv, &so, (float)scale) == MDATTN_OK;
 }
 
@@ -377,7 +378,7 @@ std::optional<Table> as_table(const OptTensor& a, const OptTensor& b, int64_t s,
 // replaced, for a size that is no multiple of 16 bytes: no kernel takes such rows either.
 bool own(Tensor& a, Tensor& b) {
   const Tensor x = at::empty(a.sizes(), a.options()), y = b.defined() ? at::empty(b.sizes(), b.options()) : Tensor();
-  if (mdattn_host_copy(stream(), ptr(a), mut(x), ptr(b), mut(y), (int64_t)a.nbytes()) != MDATTN_OK) return false;
+  if (mdattn_host_copy(stream(a), ptr(a), mut(x), ptr(b), mut(y), (int64_t)a.nbytes()) != MDATTN_OK) return false;
   a = x;
   b = y;
   return true;
@@ -427,7 +428,7 @@ variable_list fullrow_run(const Tensor& q, const Tensor& k, const Tensor& wq, co
   const int64_t b = q.size(0), s = q.size(1), d = q.size(2) / p.heads;
   Tensor qo = alloc_bshd(q, b, s, p.heads, d, p.bhsd), ko = k.defined() ? alloc_bshd(q, b, s, p.heads, d, p.bhsd) : Tensor();
   const mdattn_strides so = strides4(qo);
-  const int rc = mdattn_host_norm_rope_fullrow(stream(), ptr(q), ptr(k), mut(qo), mut(ko), ptr(wq), ptr(wk), table_ptr(cos), table_ptr(sin), (int)p.kind,
+  const int rc = mdattn_host_norm_rope_fullrow(stream(q), ptr(q), ptr(k), mut(qo), mut(ko), ptr(wq), ptr(wk), table_ptr(cos), table_ptr(sin), (int)p.kind,
                                                (int)b, (int)s, (int)p.heads, (int)d, (float)p.eps, (float)p.q_mul, q.stride(0), q.stride(1), &so);
   if (rc != MDATTN_OK) return {};
   return k.defined() ? variable_list{qo, ko} : variable_list{qo};
@@ -457,7 +458,7 @@ struct FullrowFn : FirstOrder<FullrowFn> {
     const int64_t nws = mdattn_norm_rope_bwd_workspace_floats(b * s, (has_k ? 2 : 1) * n);
     Tensor ws = at::empty({nws}, q.options().dtype(at::kFloat));
     const mdattn_strides sg = strides4(gq);
-    must(mdattn_host_norm_rope_fullrow_bwd(stream(), ptr(q), ptr(k), nullptr, ptr(gq), ptr(gk), mut(dq), mut(dk), ptr(wq), ptr(wk), mut(dwq), mut(dwk),
+    must(mdattn_host_norm_rope_fullrow_bwd(stream(q), ptr(q), ptr(k), nullptr, ptr(gq), ptr(gk), mut(dq), mut(dk), ptr(wq), ptr(wk), mut(dwq), mut(dwk),
                                            nullptr, 1, nullptr, nullptr, table_ptr(sv[4]), table_ptr(sv[5]), (int)p.kind, (int)b, (int)s, (int)p.heads, (int)d, (float)p.eps,
                                            (float)p.q_mul, q.stride(0), q.stride(1), dq.stride(0), dq.stride(1), &sg, f32(ws), nws),
          "mdattn_norm_rope_fullrow_bwd");
@@ -491,7 +492,7 @@ variable_list perhead_run(const Tensor& q, const Tensor& k, const Tensor& wq, co
   const int64_t b = q.size(0), s = q.size(1), h = q.size(2), d = q.size(3);
   Tensor qo = alloc_bshd(q, b, s, h, d, p.bhsd), ko = k.defined() ? alloc_bshd(q, b, s, h, d, p.bhsd) : Tensor();
   const mdattn_strides si = strides4(q), so = strides4(qo);
-  const int rc = mdattn_host_norm_rope_perhead(stream(), ptr(q), ptr(k), mut(qo), mut(ko), ptr(wq), ptr(wk), ptr(wqt), ptr(wkt), (int)p.n_txt,
+  const int rc = mdattn_host_norm_rope_perhead(stream(q), ptr(q), ptr(k), mut(qo), mut(ko), ptr(wq), ptr(wk), ptr(wqt), ptr(wkt), (int)p.n_txt,
                                                table_ptr(cos), table_ptr(sin), (int)p.kind, (int)b, (int)s, (int)h, (int)d, (float)p.eps, (float)p.q_mul,
                                                &si, &so);
   if (rc != MDATTN_OK) return {};
@@ -523,7 +524,7 @@ struct PerheadFn : FirstOrder<PerheadFn> {
     const int64_t nws = mdattn_norm_rope_bwd_workspace_floats(b * s * h, 4 * d);
     Tensor ws = at::empty({nws}, q.options().dtype(at::kFloat));
     const mdattn_strides si = strides4(q), sd = strides4(dq), sg = strides4(gq);
-    must(mdattn_host_norm_rope_perhead_bwd(stream(), ptr(q), ptr(k), ptr(gq), ptr(gk), mut(dq), mut(dk), ptr(wq), ptr(wk), ptr(wqt),
+    must(mdattn_host_norm_rope_perhead_bwd(stream(q), ptr(q), ptr(k), ptr(gq), ptr(gk), mut(dq), mut(dk), ptr(wq), ptr(wk), ptr(wqt),
                                            has_k ? ptr(wkt) : nullptr, (int)p.n_txt, mut(dwq), mut(dwk), mut(dwqt), mut(dwkt), 1, table_ptr(sv[6]),
                                            table_ptr(sv[7]), (int)p.kind, (int)b, (int)s, (int)h, (int)d, (float)p.eps, (float)p.q_mul, &si, &sd, &sg,
                                            f32(ws), nws),
@@ -560,7 +561,7 @@ variable_list qkv_run(const Tensor& x, const Tensor& bias, const Tensor& wq, con
   Tensor o[3];
   for (Tensor& t : o) t = alloc_bshd(x, b, s, p.heads, d, p.bhsd);
   const mdattn_strides so = strides4(o[0]);
-  const int rc = mdattn_host_norm_rope_qkv(stream(), ptr(x), ptr(bias), mut(o[0]), mut(o[1]), mut(o[2]), ptr(wq), ptr(wk), table_ptr(cos), table_ptr(sin),
+  const int rc = mdattn_host_norm_rope_qkv(stream(x), ptr(x), ptr(bias), mut(o[0]), mut(o[1]), mut(o[2]), ptr(wq), ptr(wk), table_ptr(cos), table_ptr(sin),
                                            (int)p.kind, (int)b, (int)s, (int)p.heads, (int)d, (float)p.eps, (float)p.q_mul, x.stride(0), x.stride(1), &so);
   if (rc != MDATTN_OK) return {};
   return {o[0], o[1], o[2]};
@@ -594,7 +595,7 @@ struct QkvFn : FirstOrder<QkvFn> {
     const mdattn_strides sg = strides4(gq);
     const char* xp = static_cast<const char*>(ptr(x));
     char* dp = static_cast<char*>(mut(dx));
-    must(mdattn_host_norm_rope_fullrow_bwd(stream(), xp, xp + 2 * n, ptr(bias), ptr(gq), ptr(gk), dp, dp + 2 * n, ptr(wq), ptr(wk), mut(dwq), mut(dwk),
+    must(mdattn_host_norm_rope_fullrow_bwd(stream(x), xp, xp + 2 * n, ptr(bias), ptr(gq), ptr(gk), dp, dp + 2 * n, ptr(wq), ptr(wk), mut(dwq), mut(dwk),
                                            mut(db), 1, ptr(gv), dp + 4 * n, table_ptr(sv[4]), table_ptr(sv[5]), (int)p.kind, (int)b, (int)s, (int)p.heads, (int)d, (float)p.eps,
                                            (float)p.q_mul, x.stride(0), x.stride(1), dx.stride(0), dx.stride(1), &sg, f32(ws), nws),
          "mdattn_norm_rope_fullrow_bwd");
@@ -628,7 +629,7 @@ variable_list rows_run(const Tensor& q, const Tensor& k, const Tensor& wq, const
   const int64_t b = q.size(0), s = q.size(1), d = q.size(2) / p.heads;
   Tensor qo = alloc_bshd(q, b, s, p.heads, d, false), ko = k.defined() ? alloc_bshd(q, b, s, p.heads, d, false) : Tensor();
   const mdattn_strides so = strides4(qo);
-  const int rc = mdattn_host_norm_rope_rows(stream(), ptr(q), ptr(k), q.scalar_type() == at::kFloat, mut(qo), mut(ko), f32(wq), f32(wk), f32(cos), f32(sin),
+  const int rc = mdattn_host_norm_rope_rows(stream(q), ptr(q), ptr(k), q.scalar_type() == at::kFloat, mut(qo), mut(ko), f32(wq), f32(wk), f32(cos), f32(sin),
                                             (int)p.mode, (int)b, (int)s, (int)p.heads, (int)d, (float)p.eps, (float)p.w_mul, q.stride(0), q.stride(1), &so);
   if (rc != MDATTN_OK) return {};
   return k.defined() ? variable_list{qo, ko} : variable_list{qo};
@@ -698,7 +699,7 @@ struct RowsFn : FirstOrder<RowsFn> {
     const int64_t nws = mdattn_norm_rope_bwd_workspace_floats(b * s, (pair ? 2 : 1) * n);
     Tensor ws = at::empty({nws}, wq.options());
     const mdattn_strides sg = strides4(gq);
-    must(mdattn_host_norm_rope_rows_bwd(stream(), ptr(q), ptr(k), q.scalar_type() == at::kFloat, ptr(gq), ptr(gk), mut(dq), mut(dk), f32(wq), f32(wk),
+    must(mdattn_host_norm_rope_rows_bwd(stream(q), ptr(q), ptr(k), q.scalar_type() == at::kFloat, ptr(gq), ptr(gk), mut(dq), mut(dk), f32(wq), f32(wk),
                                         f32(dwq), f32(dwk), f32(sv[4]), f32(sv[5]), (int)mode, (int)b, (int)s, (int)heads, (int)(n / heads), (float)fv[0],
                                         one ? 1.0f : (float)fv[1], q.stride(0), q.stride(1), dq.stride(0), dq.stride(1), &sg, f32(ws), nws),
          "mdattn_norm_rope_rows_bwd");
@@ -791,7 +792,7 @@ bool norm_vectors(const Tensor& x, const Rows3& r, const Tensor& w, const Tensor
 
 Tensor norm_run(const Tensor& x, const Rows3& r, const Tensor& w, const Tensor& b, int64_t stride, int f32, double eps, double offset) {
   Tensor y = at::empty(x.sizes(), x.options());
-  const int rc = mdattn_layer_norm(stream(), ptr(x), is_f32(x), mut(y), is_f32(x), ptr(w), ptr(b), f32, r.groups, r.rows, (int)r.c, r.sg, r.sr, r.rows * r.c,
+  const int rc = mdattn_layer_norm(stream(x), ptr(x), is_f32(x), mut(y), is_f32(x), ptr(w), ptr(b), f32, r.groups, r.rows, (int)r.c, r.sg, r.sr, r.rows * r.c,
                                    r.c, stride, (float)eps, (float)offset);
   return rc == MDATTN_OK ? y : Tensor();
 }
@@ -834,7 +835,7 @@ struct NormFn : FirstOrder<NormFn> {
     Tensor db = vectors && i[3] ? at::empty(ctx->saved_data["bshape"].toIntVector(), vec) : Tensor();
     const int64_t nws = dw.defined() || db.defined() ? mdattn_layer_norm_bwd_workspace_floats(r->groups, r->rows, (int)r->c) : 0;
     const Tensor ws = nws ? at::empty({nws}, x.options().dtype(at::kFloat)) : Tensor();
-    must(mdattn_layer_norm_bwd(stream(), ptr(x), is_f32(x), ptr(g), mut(dx), ptr(w), mut(dw), mut(db), (int)i[1], r->groups, r->rows, (int)r->c, r->sg, r->sr,
+    must(mdattn_layer_norm_bwd(stream(x), ptr(x), is_f32(x), ptr(g), mut(dx), ptr(w), mut(dw), mut(db), (int)i[1], r->groups, r->rows, (int)r->c, r->sg, r->sr,
                                rg->sg, rg->sr, r->rows * r->c, r->c, i[0], (float)f[0], (float)f[1], f32(ws), nws),
          "mdattn_layer_norm_bwd");
     return {dx, dw, db, Tensor(), Tensor()};
@@ -876,7 +877,7 @@ Tensor as_matrix(const Tensor& x) {
   return Tensor();
 }
 int quant(const Tensor& x, int64_t block_rows, const Blocks* q, const Blocks* qt, const Tensor& sums) {
-  return mdattn_quant_block_e4m3(stream(), ptr(x), is_f32(x), x.size(0), x.size(1), x.stride(0), (int)block_rows, q ? q->values() : nullptr,
+  return mdattn_quant_block_e4m3(stream(x), ptr(x), is_f32(x), x.size(0), x.size(1), x.stride(0), (int)block_rows, q ? q->values() : nullptr,
                                  q ? q->scales() : nullptr, qt ? qt->values() : nullptr, qt ? qt->scales() : nullptr, f32(sums));
 }
 // into out, dense, of m x n elements in whatever shape the caller wants: a view of it would be one that autograd forbids to change in place
@@ -884,7 +885,7 @@ int product(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t
             int64_t n, int64_t k) {
   const int64_t nws = mdattn_matmul_fp8_block_workspace_floats(m, n, k);
   const Tensor ws = nws ? at::empty({nws}, out.options().dtype(at::kFloat)) : Tensor();
-  return mdattn_matmul_fp8_block(stream(), a, sa, b, sb, (int)b_block_rows, ptr(bias), is_f32(bias), mut(out), n, m, n, k, f32(ws), nws);
+  return mdattn_matmul_fp8_block(stream(out), a, sa, b, sb, (int)b_block_rows, ptr(bias), is_f32(bias), mut(out), n, m, n, k, f32(ws), nws);
 }
 std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
   auto v = x.sizes().vec();
@@ -914,7 +915,7 @@ OptTensor linear_quantized(const Tensor& x, const Tensor& values, const Tensor& 
   }
   const int64_t m = norm ? r->all() : rows.size(0);
   const Blocks q(x, m, k, 1);
-  const int rc = norm ? mdattn_layer_norm_e4m3(stream(), ptr(x), is_f32(x), q.values(), q.scales(), ptr(w), ptr(b), f32, r->groups, r->rows, (int)r->c, r->sg, r->sr,
+  const int rc = norm ? mdattn_layer_norm_e4m3(stream(x), ptr(x), is_f32(x), q.values(), q.scales(), ptr(w), ptr(b), f32, r->groups, r->rows, (int)r->c, r->sg, r->sr,
                                                stride, (float)eps, (float)offset)
                       : quant(rows, 1, &q, nullptr, Tensor());
   if (rc != MDATTN_OK) return std::nullopt;
@@ -971,7 +972,7 @@ struct LinearFn : FirstOrder<LinearFn> {
     }
     if (i[5]) {
       db = at::empty({n}, rows.options().dtype(i[6] ? at::kFloat : at::kBFloat16));
-      must(mdattn_sum_rows(stream(), f32(sums), sums.size(0), n, mut(db), (int)i[6]), "mdattn_sum_rows");
+      must(mdattn_sum_rows(stream(sums), f32(sums), sums.size(0), n, mut(db), (int)i[6]), "mdattn_sum_rows");
     }
     return {dx, dw, db};
   }

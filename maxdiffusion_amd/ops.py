@@ -51,7 +51,11 @@ def _ptr(t):
 
 def _stream():
   # the raw handle of the current stream of the current device (building a torch.cuda.Stream object around it costs 10 us)
-  return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+  return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(_current_device()))
+
+
+def _current_device() -> int:
+  return torch._C._cuda_getDevice()  # (once there is a tensor on a device; half the time of torch.cuda.current_device)
 
 
 def _check_dev(*ts):
@@ -63,7 +67,7 @@ def _check_dev(*ts):
     if not t.is_cuda:
       raise ValueError("mdattn operators need tensors in device memory (cuda/HIP); there is no CPU path")
     if device is None:
-      device = torch.cuda.current_device()
+      device = _current_device()
     if t.get_device() != device:
       raise ValueError(f"mdattn operators need their tensors on the current device, cuda:{device}: one is on cuda:{t.get_device()}")
 

@@ -112,7 +112,7 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
     def __init__(self, device):
       self.get_device = lambda: device
 
-  monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+  monkeypatch.setattr(ops, "_current_device", lambda: 1)
   ops._check_dev(On(1), None, On(1))
   for ts in ((On(1), On(0)), (On(0),), (None, On(0), On(0))):
     with pytest.raises(ValueError, match="current device"):
