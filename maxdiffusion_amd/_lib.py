@@ -1,4 +1,4 @@
-"""ctypes binding of libmdattn.so (the C ABI declared in include/mdattn.h and include/mdlayers.h).
+"""ctypes binding of libmdattn.so (the C ABI declared in include/mdattn.h, include/mdlayers.h and include/mdpacked.h).
 
 There is no fallback: when the library is missing or a call fails this module raises.
 """
@@ -16,6 +16,13 @@ class Strides(ctypes.Structure):
   _fields_ = [("batch", ctypes.c_int64), ("seq", ctypes.c_int64), ("head", ctypes.c_int64)]
 
 
+class Packed(ctypes.Structure):
+  """mdattn_packed"""
+  _fields_ = [("q_offsets", ctypes.c_void_p), ("k_offsets", ctypes.c_void_p), ("k_lengths", ctypes.c_void_p), ("sequences", ctypes.c_int),
+              ("q_rows", ctypes.c_int), ("k_rows", ctypes.c_int), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+              ("causal", ctypes.c_int), ("max_q", ctypes.c_int), ("max_k", ctypes.c_int)]
+
+
 class MdattnError(RuntimeError):
 
   def __init__(self, code: int, where: str, text: str):
@@ -28,6 +35,7 @@ _I = ctypes.c_int
 _L = ctypes.c_int64
 _F = ctypes.c_float
 _S = ctypes.POINTER(Strides)
+_K = ctypes.POINTER(Packed)
 
 # symbol -> argtypes; every symbol include/mdattn.h declares
 SIGNATURES = {
@@ -71,6 +79,14 @@ LAYER_SIGNATURES = {
     "mdattn_matmul_fp8_block": ([_P, _P, _P, _P, _P, _I, _P, _I, _P, _L, _L, _L, _L, _P, _L], _I),
 }
 
+# symbol -> argtypes; every symbol include/mdpacked.h declares
+PACKED_SIGNATURES = {
+    "mdattn_fwd_bf16_packed_workspace_floats": ([_K], _L),
+    "mdattn_fwd_bf16_packed": ([_P, _K, _P, _P, _P, _P, _P, _S, _S, _S, _S, _F, _P, _L], _I),
+    "mdattn_bwd_bf16_packed_workspace_floats": ([_K], _L),
+    "mdattn_bwd_bf16_packed": ([_P, _K, _P, _P, _P, _P, _P, _P, _P, _P, _P, _S, _S, _S, _S, _S, _S, _S, _F, _P, _L], _I),
+}
+
 # what csrc/mdattn_host.h declares: entry points for this package's own host side
 HOST_SIGNATURES = {
     "mdattn_bwd_split_workspace_floats": ([_I, _I, _I, _I, _I], _L),
@@ -96,7 +112,7 @@ def load() -> ctypes.CDLL:
           f"{LIB_PATH} is missing: build it with `python -m maxdiffusion_amd.build` "
           "(there is no non-HIP fallback for this path)")
     lib = ctypes.CDLL(LIB_PATH)
-    for name, (argtypes, restype) in {**SIGNATURES, **LAYER_SIGNATURES, **HOST_SIGNATURES}.items():
+    for name, (argtypes, restype) in {**SIGNATURES, **LAYER_SIGNATURES, **PACKED_SIGNATURES, **HOST_SIGNATURES}.items():
       fn = getattr(lib, name)
       fn.argtypes = argtypes
       fn.restype = restype

@@ -23,7 +23,7 @@ from . import _lib, ops
 
 __all__ = [
     "KERNEL_REGISTRY", "register_kernel", "AttentionOp", "hip_flash_kernel", "hip_flash_fp8_kernel",
-    "hip_norm_rope", "hip_norm_rope_qkv", "hip_norm_rope_ltx2", "hip_flash_attention_autograd", "HIP_KERNEL_NAMES",
+    "hip_norm_rope", "hip_norm_rope_qkv", "hip_norm_rope_ltx2", "hip_flash_attention_autograd", "hip_flash_packed", "HIP_KERNEL_NAMES",
 ]
 
 KERNEL_REGISTRY = {}
@@ -227,6 +227,49 @@ def hip_flash_fp8_kernel(q, k, v, context):
 
 def _wants_grad(*ts) -> bool:
   return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+class _HipFlashPacked(torch.autograd.Function):
+  """Saved for the backward: q, k, v, the offsets, out, lse."""
+
+  @staticmethod
+  def forward(ctx, q, k, v, q_offsets, k_offsets, causal, scale, max_q, max_k):
+    out, lse = ops.flash_attention_packed(q, k, v, q_offsets, k_offsets, causal=causal, scale=scale, max_q=max_q, max_k=max_k, return_lse=True)
+    ctx.save_for_backward(q, k, v, q_offsets, k_offsets, out, lse)
+    ctx.cfg = dict(causal=causal, scale=scale, max_q=max_q, max_k=max_k)
+    ctx.shapes = (q.shape, k.shape, q_offsets.shape)
+    return out
+
+  @staticmethod
+  @_lib.first_order
+  def backward(ctx, dout):
+    q, k, v, q_offsets, k_offsets, out, lse = ctx.saved_tensors
+    if (q.shape, k.shape, q_offsets.shape) != ctx.shapes:
+      raise ValueError("a tensor saved for the backward pass came back from its hook with another dtype, shape or layout")
+    dq, dk, dv = ops.flash_attention_packed_backward(q, k, v, out, dout.to(torch.bfloat16), lse, q_offsets, k_offsets, **ctx.cfg)
+    return dq, dk, dv, None, None, None, None, None, None
+
+
+def hip_flash_packed(q, k, v, q_offsets, k_offsets=None, *, k_lengths=None, causal: bool = True, scale: float | None = None, max_q: int | None = None,
+                     max_k: int | None = None):
+  """Attention over packed sequences: a prompt encoder's, causal, with grouped heads, its prompts one behind the other without padding (the
+  reference's masked form: models/qwen3_flax.py:285), or images of several sizes.  q [Tq, H, D], k, v [Tk, Hkv, D] -> [Tq, H, D], bf16.
+
+  The arguments are those of `ops.flash_attention_packed`.  Differentiable in q, k and v (not with k_lengths): where autograd is recording and one
+  of them requires a gradient, all three products' gradients come from the HIP backward pass."""
+  scale = float(q.shape[-1]**-0.5 if scale is None else scale) if q.dim() else 1.0
+  grad = _wants_grad(q, k, v)
+  if q.is_cuda and not (grad and k_lengths is not None):
+    out = _lib.host().flash_packed(q, k, v, q_offsets, k_offsets, k_lengths, bool(causal), scale, int(max_q or 0), int(max_k or 0))
+    if out is not None:
+      return out
+  # what the native path leaves: views to be copied, and every error
+  _lib.no_tangents(q, k, v)
+  if grad:
+    if k_lengths is not None:
+      raise NotImplementedError("hip_flash_packed has no gradient with k_lengths: call it under torch.no_grad()")
+    return _HipFlashPacked.apply(q, k, v, q_offsets, q_offsets if k_offsets is None else k_offsets, bool(causal), scale, max_q, max_k)
+  return ops.flash_attention_packed(q, k, v, q_offsets, k_offsets, k_lengths=k_lengths, causal=causal, scale=scale, max_q=max_q, max_k=max_k)
 
 
 class _HipNormRopeFullrow(torch.autograd.Function):

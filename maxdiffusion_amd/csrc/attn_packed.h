@@ -1,0 +1,143 @@
+// What the kernels of attention over packed sequences share: which sequence a workgroup works on, the tiles in LDS, rows of q by group.
+#pragma once
+#include "mdattn_common.h"
+#include "mdpacked.h"
+
+namespace mdattn {
+
+// Division of a row number (below 2^31) by the heads of a group: n / d = n * (2^(31 + l) / d rounded up) >> (31 + l) with 2^l >= d.
+struct Divisor {
+  unsigned d, mul, shift;
+};
+inline Divisor divisor(unsigned d) {
+  unsigned l = 0;
+  while ((1u << l) < d) ++l;
+  return {d, (unsigned)((1ull << (31 + l)) / d + 1), l};
+}
+__device__ __forceinline__ unsigned div_by(unsigned n, const Divisor& d) { return d.d == 1 ? n : __umulhi(n, d.mul) >> (d.shift - 1); }
+
+struct PackedSeqs {
+  const int *q_off, *k_off, *k_len;
+  int count, q_rows, k_rows;
+};
+
+// A workgroup's tile of a sequence: rows q0 .. q0 + m of q, k0 .. k0 + n of k and v.  Gap: rows of no sequence (m of q, or n of k), to be
+// filled with zeros.
+struct SeqTile {
+  int q0, m, k0, n, tile, tiles;
+  bool gap, none;
+};
+
+__device__ __forceinline__ int wave_prefix_sum(int x) {  // inclusive, over the 64 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);   // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);   // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);   // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
+// Tile `rank` of all sequences' tiles of BM rows (KEYS: of k; else of q, `group` rows for each of its tokens), in the order of the
+// sequences; the rows in front of the first sequence and behind the last follow as two more.  Offsets that decrease, or that point outside, are
+// brought into the tensors.  Every wave looks for itself, 64 sequences at a time.
+template <int BM, bool KEYS>
+__device__ __forceinline__ SeqTile find_tile(const PackedSeqs& s, int group, int rank, int lane) {
+  int before = 0;
+  for (int i0 = 0; i0 < s.count + 2; i0 += 64) {
+    const int i = i0 + lane, at = i < s.count ? i : s.count, next = i < s.count ? i + 1 : i == s.count ? 0 : s.count;
+    int qa = s.q_off[at], qb = s.q_off[next], ka = s.k_off[at], kb = s.k_off[next];
+    const int len = s.k_len && i < s.count ? s.k_len[i] : 0x7FFFFFFF;
+    if (i == s.count) qa = ka = 0;                       // in front of the first
+    if (i == s.count + 1) { qb = s.q_rows; kb = s.k_rows; }  // behind the last
+    qa = min(max(qa, 0), s.q_rows);
+    ka = min(max(ka, 0), s.k_rows);
+    const int m = min(max(qb, qa), s.q_rows) - qa, n = min(min(max(kb, ka), s.k_rows) - ka, max(len, 0));
+    const int rows = KEYS ? n : m * group;
+    const int tiles = i < s.count + 2 ? (int)(((unsigned)rows + (BM - 1)) / BM) : 0;
+    const int upto = wave_prefix_sum(tiles);
+    const uint64_t behind = __builtin_amdgcn_ballot_w64(before + upto > rank);
+    if (behind) {
+      const int j = __builtin_ctzll(behind);
+      SeqTile t;
+      t.q0 = __builtin_amdgcn_readlane(qa, j);
+      t.m = __builtin_amdgcn_readlane(m, j);
+      t.k0 = __builtin_amdgcn_readlane(ka, j);
+      t.n = __builtin_amdgcn_readlane(n, j);
+      t.tiles = __builtin_amdgcn_readlane(tiles, j);
+      t.tile = rank - before - (__builtin_amdgcn_readlane(upto, j) - t.tiles);
+      t.gap = i0 + j >= s.count;
+      t.none = false;
+      return t;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  SeqTile t{};
+  t.none = true;
+  return t;
+}
+
+// A block of 32 rows of HD elements in LDS, filled by loads of 1 KB: chunk c (16 bytes) of row r sits at position c ^ swizzle(r).  The
+// upper part of the swizzle, distinct within 4 rows that follow each other, moves the 64-byte segment, so that the transposing reads
+// (4 rows x 64 bytes) cover every bank once; the lower part makes all positions of 16 rows distinct, for the row reads.
+template <int HD>
+struct PackedBlock {
+  static constexpr int RPI = HD == 128 ? 4 : 8;  // rows that one load instruction fills
+  static constexpr int Row = HD * 2, Bytes = 32 * Row;
+  static __device__ __forceinline__ int swizzle(int r) { return HD == 128 ? 4 * (r & 3) + ((r >> 2) & 3) : 4 * ((r >> 1) & 1) + ((r >> 2) & 3); }
+  // the row of its group, and the chunk, that a lane of group g's load brings
+  static __device__ __forceinline__ int row(int lane) { return HD == 128 ? lane >> 4 : lane >> 3; }
+  static __device__ __forceinline__ int chunk(int lane, int g) { return (lane & (HD / 8 - 1)) ^ swizzle(RPI * g + row(lane)); }
+  // where a lane's part of a fragment sits: row read j (chunk 2 j + hh of row l32) at row_at ^ 32 j; transposing read of the 32-column slab sg
+  // at trans_at ^ 64 sg for the rows 4 hh + 0..3 and, eight rows on, at that ^ 32
+  static __device__ __forceinline__ unsigned row_at(int lane) {
+    const int l32 = lane & 31, hh = lane >> 5;
+    return (unsigned)(l32 * Row + ((hh ^ swizzle(l32)) * 16));
+  }
+  static __device__ __forceinline__ unsigned trans_at(int lane) {
+    const int r = 4 * (lane >> 5) + ((lane & 15) >> 2);
+    return (unsigned)(r * Row + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swizzle(r)) * 16 + (lane & 1) * 8);
+  }
+};
+
+typedef s16x4 __attribute__((address_space(3))) * lds_s16x4_at;
+typedef __attribute__((ext_vector_type(8))) short s16x8_p;
+typedef const bf16x8 __attribute__((address_space(3))) * lds_bf16x8_at;
+typedef const f32x4 __attribute__((address_space(3))) * lds_f32x4_at;
+__device__ __forceinline__ bf16x8 read_row_frag(unsigned at) { return *(lds_bf16x8_at)at; }
+__device__ __forceinline__ bf16x8 read_trans_frag(unsigned at0, unsigned at1) {
+  const s16x4 r0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_at)at0);
+  const s16x4 r1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_at)at1);
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(r0, r1, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Strides of a tensor [rows, heads, head_dim] in elements.
+struct RowStrides {
+  int64_t row, head;
+};
+
+// A few rows' strides are added up in 32 bits; heads' are not, but for q and dout in the dk / dv pass (`group` heads of them).
+inline bool packed_strides_ok(const mdattn_strides* s, int64_t group = 0) {
+  return s && s->seq % 8 == 0 && s->head % 8 == 0 && s->seq >= 0 && s->head >= 0 && s->seq < (1 << 23) && s->head < (1ll << 40) &&
+         group * s->head < (1 << 29);
+}
+// MDATTN_OK for sizes that the kernels take
+inline int packed_sizes(const mdattn_packed* p) {
+  if (!p || !p->q_offsets || !p->k_offsets || p->sequences < 0 || p->q_rows < 0 || p->k_rows < 0 || p->heads <= 0 || p->kv_heads <= 0 ||
+      p->heads % p->kv_heads || p->head_dim <= 0)
+    return MDATTN_E_BADARG;
+  if (p->head_dim % 8 || p->head_dim > 128) return MDATTN_E_UNSUPPORTED;
+  const int64_t group = p->heads / p->kv_heads;
+  // row numbers of a head's group, and the rows of all heads, are counted in 31 bits
+  if (group > 1024 || p->sequences > (1 << 24) || (int64_t)p->q_rows * p->heads >= (1ll << 31) - 4096 ||
+      (int64_t)p->k_rows * p->kv_heads >= (1ll << 31) - 4096)
+    return MDATTN_E_UNSUPPORTED;
+  return MDATTN_OK;
+}
+inline bool packed_aligned(const mdattn_packed* p) {
+  return ((reinterpret_cast<uintptr_t>(p->q_offsets) | reinterpret_cast<uintptr_t>(p->k_offsets) | reinterpret_cast<uintptr_t>(p->k_lengths)) & 3) == 0;
+}
+// tiles of BM rows that all sequences of `rows` rows have together at most, and the two gaps
+inline int64_t packed_tiles(int64_t rows, int64_t sequences, int BM) { return rows / BM + sequences + 2; }
+
+}  // namespace mdattn

@@ -23,6 +23,7 @@
 #include "mdattn.h"
 #include "mdattn_host.h"
 #include "mdlayers.h"
+#include "mdpacked.h"
 
 namespace {
 
@@ -344,6 +345,87 @@ bool flash_merge(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   const mdattn_strides sq = strides4(q), sk = strides4(k), sv = strides4(v), so = strides4(o_run);
   return mdattn_fwd_bf16_merge(stream(q), ptr(q), ptr(k), ptr(v), f32(o_run), f32(lse_run), (int)q.size(0), (int)q.size(2), (int)q.size(1),
                                (int)k.size(1), (int)q.size(3), &sq, &sk, &sv, &so, (float)scale) == MDATTN_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ attention over packed sequences
+// q [Tq,H,D], k, v [Tk,Hkv,D] as the kernels walk them (ops._packed_rows); an axis of one element may have any stride
+mdattn_strides row_strides(const Tensor& t) { return {0, t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0}; }
+bool packed_rows(const Tensor& t, const Tensor& ref, int64_t group) {
+  if (!bf16_on(t, ref) || t.dim() != 3 || t.numel() == 0 || t.stride(2) != 1 || !aligned(t)) return false;
+  const mdattn_strides s = row_strides(t);
+  return (s.seq | s.head) % 8 == 0 && s.seq < (1 << 23) && group * s.head < (1 << 29);
+}
+bool index_ok(const Tensor& t, int64_t n, const Tensor& ref) {
+  return t.is_cuda() && t.get_device() == ref.get_device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+// false: the Python path takes the call (and says what is wrong with it)
+bool packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qo, const Tensor& ko, const Tensor& kl, bool causal, int64_t max_q,
+                 int64_t max_k, mdattn_packed& p) {
+  if (!q.is_cuda() || q.dim() != 3 || k.dim() != 3 || k.sizes() != v.sizes() || k.numel() == 0 || q.size(1) % k.size(1) || q.size(2) != k.size(2) ||
+      std::max(q.size(0), k.size(0)) >= (int64_t)1 << 31 || !packed_rows(q, q, q.size(1) / k.size(1)) || !packed_rows(k, q, 0) || !packed_rows(v, q, 0))
+    return false;
+  const int64_t n = qo.numel();
+  if (n < 1 || n >= (int64_t)1 << 31 || !index_ok(qo, n, q) || !index_ok(ko, n, q) || (kl.defined() && !index_ok(kl, n - 1, q))) return false;
+  auto hint = [](int64_t x) { return (int)std::min<int64_t>(std::max<int64_t>(x, 0), INT32_MAX); };
+  p = {static_cast<const int*>(ptr(qo)), static_cast<const int*>(ptr(ko)), static_cast<const int*>(ptr(kl)), (int)(n - 1), (int)q.size(0),
+       (int)k.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), causal, hint(max_q), hint(max_k)};
+  return true;
+}
+int packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const mdattn_packed& p, double scale, const Tensor& out, const Tensor& lse) {
+  const int64_t nws = mdattn_fwd_bf16_packed_workspace_floats(&p);
+  const Tensor ws = nws ? at::empty({nws}, q.options().dtype(at::kFloat)) : Tensor();
+  const mdattn_strides sq = row_strides(q), sk = row_strides(k), sv = row_strides(v), so = row_strides(out);
+  return mdattn_fwd_bf16_packed(stream(q), &p, ptr(q), ptr(k), ptr(v), mut(out), f32(lse), &sq, &sk, &sv, &so, (float)scale, f32(ws), nws);
+}
+struct PackedFn : FirstOrder<PackedFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qo, const Tensor& ko, bool causal,
+                        double scale, int64_t max_q, int64_t max_k) {
+    mdattn_packed p;
+    packed_args(q, k, v, qo, ko, Tensor(), causal, max_q, max_k, p);
+    Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+    if (packed_fwd(q, k, v, p, scale, out, lse) != MDATTN_OK) throw Refused{};
+    ctx->save_for_backward({q, k, v, qo, ko, out, lse});
+    ctx->saved_data["i"] = c10::List<int64_t>({causal, max_q, max_k, q.size(0), q.size(1), q.size(2), k.size(0), k.size(1), qo.size(0)});
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list gradients(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto i = ctx->saved_data["i"].toIntVector();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &qo = saved[3], &ko = saved[4], &out = saved[5], &lse = saved[6];
+    mdattn_packed p;
+    unpacked(packed_args(q, k, v, qo, ko, Tensor(), i[0], i[1], i[2], p) && q.sizes() == at::IntArrayRef({i[3], i[4], i[5]}) &&
+             k.sizes() == at::IntArrayRef({i[6], i[7], i[5]}) && qo.size(0) == i[8] && bf16_on(out, q) && out.is_contiguous() && out.sizes() == q.sizes() &&
+             aligned(out) && lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+             lse.numel() == q.size(0) * q.size(1));
+    Tensor dout = grads[0];
+    if (dout.scalar_type() != at::kBFloat16) dout = dout.to(at::kBFloat16);
+    if (dout.is_neg()) dout = dout.resolve_neg();
+    dout = dout.contiguous();
+    if (!aligned(dout)) dout = dout.clone();
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(k.sizes(), k.options());
+    const int64_t nws = mdattn_bwd_bf16_packed_workspace_floats(&p);
+    const Tensor ws = at::empty({nws}, lse.options());
+    const mdattn_strides sq = row_strides(q), sk = row_strides(k), sv = row_strides(v), so = row_strides(out), dqs = row_strides(dq), dks = row_strides(dk);
+    must(mdattn_bwd_bf16_packed(stream(q), &p, ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), f32(lse), mut(dq), mut(dk), mut(dv), &sq, &sk, &sv, &so, &dqs, &dks,
+                                &dks, (float)ctx->saved_data["scale"].toDouble(), f32(ws), nws),
+         "mdattn_bwd_bf16_packed");
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+OptTensor flash_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qo, const OptTensor& ko_, const OptTensor& kl_, bool causal,
+                       double scale, int64_t max_q, int64_t max_k) {
+  const Tensor ko = ko_.has_value() ? *ko_ : qo, kl = value(kl_);
+  mdattn_packed p;
+  if (!packed_args(q, k, v, qo, ko, kl, causal, max_q, max_k, p)) return std::nullopt;
+  if (wants_grad({&q, &k, &v})) {
+    if (kl.defined()) return std::nullopt;
+    return unless_refused([&] { return PackedFn::apply(q, k, v, qo, ko, causal, scale, max_q, max_k); });
+  }
+  at::NoGradGuard guard;
+  Tensor out = at::empty(q.sizes(), q.options());
+  if (packed_fwd(q, k, v, p, scale, out, Tensor()) != MDATTN_OK) return std::nullopt;
+  return out;
 }
 
 // ------------------------------------------------------------------------------------------------ prologues
@@ -999,6 +1081,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("flash_autograd", &flash_autograd, Unlocked());
   m.def("flash_fp8", &flash_fp8, Unlocked());
   m.def("flash_merge", &flash_merge, Unlocked());
+  m.def("flash_packed", &flash_packed, Unlocked());
   m.def("norm_rope", &norm_rope, Unlocked());
   m.def("norm_rope_perhead", &norm_rope_perhead, Unlocked());
   m.def("norm_rope_qkv", &norm_rope_qkv, Unlocked());

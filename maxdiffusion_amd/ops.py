@@ -18,6 +18,7 @@ from ._lib import Strides
 __all__ = [
     "norm_rope_fullrow", "norm_rope_qkv", "norm_rope_perhead", "norm_rope_rows",
     "norm_rope_fullrow_backward", "norm_rope_perhead_backward", "norm_rope_rows_backward", "flash_attention", "flash_attention_backward", "flash_attention_backward_static", "flash_attention_fp8", "quant_e4m3", "key_mask_bias",
+    "flash_attention_packed", "flash_attention_packed_backward",
     "layer_norm", "layer_norm_quant", "layer_norm_backward", "BlockQuant", "quant_block_e4m3", "sum_rows", "matmul_fp8_block",
     "merge_partial", "flash_attention_merge", "finalize", "new_merge_state", "LSE_INIT", "FOLDED_SCALE", "folded_q_mul", "set_fwd_schedule", "FWD_SCHEDULES", "FP8_SOFTMAX_MODES",
 ]
@@ -599,6 +600,98 @@ def finalize(o_run: torch.Tensor) -> torch.Tensor:
   rc = _lib.load().mdattn_finalize(_stream(), _ptr(o_run), _ptr(out), o_run.numel())
   _lib.check(rc, "mdattn_finalize")
   return out
+
+
+# ------------------------------------------------------------------------------------------------ attention over packed sequences
+def _packed_rows(t: torch.Tensor, group: int = 0) -> torch.Tensor:
+  """t [rows, heads, D] as the kernels walk it (whole 16-byte pieces; strides below 2^23 between rows), copied if it is not.  group: heads of q
+  or dout whose strides the backward pass adds up in 32 bits."""
+  row, head = _packed_strides(t)
+  ok = (t.stride(2) == 1 or t.shape[2] == 1) and row % 8 == 0 and head % 8 == 0 and row < 1 << 23 and group * head < 1 << 29 and t.data_ptr() % 16 == 0
+  return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _packed_strides(t):
+  """Strides of rows and heads (an axis of one element may have any: 0)."""
+  return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def _row_strides(t) -> Strides:
+  return Strides(0, *_packed_strides(t))
+
+
+def _packed(q, k, v, q_offsets, k_offsets, k_lengths, causal, max_q, max_k) -> _lib.Packed:
+  """The checked mdattn_packed of a call."""
+  _check_dev(q, k, v, q_offsets, k_offsets, k_lengths)
+  for name, t in (("q", q), ("k", k), ("v", v)):
+    if t.dim() != 3 or t.dtype != torch.bfloat16:
+      raise ValueError(f"{name} must be a bf16 tensor of shape [rows, heads, head_dim], got {tuple(t.shape)} {t.dtype}")
+  if k.shape != v.shape or q.shape[2] != k.shape[2] or k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
+    raise ValueError(f"k and v must have one shape, q their head dim and a multiple of their heads, got q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
+  if not 0 < q.shape[2] <= 128 or q.shape[2] % 8:
+    raise ValueError(f"head_dim={q.shape[2]} not supported: a multiple of 8 up to 128.")
+  n = q_offsets.numel() - 1
+  for name, t, size in (("q_offsets", q_offsets, n + 1), ("k_offsets", k_offsets, n + 1), ("k_lengths", k_lengths, n)):
+    if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != size or n < 0 or not t.is_contiguous()):
+      raise ValueError(f"{name} must be a contiguous int32 tensor of {size} elements, got {tuple(t.shape)} {t.dtype}")
+  hint = lambda x: min(max(int(x or 0), 0), 2**31 - 1)
+  p = lambda t: None if t is None else t.data_ptr()
+  return _lib.Packed(p(q_offsets), p(k_offsets), p(k_lengths), n, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], int(bool(causal)),
+                     hint(max_q), hint(max_k))
+
+
+def flash_attention_packed(q, k, v, q_offsets, k_offsets=None, *, k_lengths=None, causal: bool = True, scale: float | None = None,
+                           max_q: int | None = None, max_k: int | None = None, return_lse: bool = False):
+  """softmax(scale * q k^T) v over sequences that lie one behind the other.  q [Tq, H, D], k, v [Tk, Hkv, D], bf16, any strides of rows and heads;
+  H a multiple of Hkv (head h of q meets head h // (H // Hkv)), D a multiple of 8 up to 128.
+
+  q_offsets, k_offsets: int32 [B + 1] on the device, not decreasing: sequence i is the rows q_offsets[i] .. q_offsets[i + 1] of q and those of
+  k_offsets (None: the same) of k and v.  k_lengths int32 [B]: only the first k_lengths[i] of them are keys (a cache with room).  causal: of a
+  sequence with m queries and n keys, query i sees the keys up to i + n - m.  max_q, max_k: the longest sequence's queries and keys, if the
+  caller knows them; they choose how the work is cut and no result depends on them but for its roundings.
+
+  Returns out [Tq, H, D] and, if asked, lse f32 [H, Tq] (natural log).  Rows that see no key and rows of no sequence: 0 and -inf."""
+  k_offsets = q_offsets if k_offsets is None else k_offsets
+  p = _packed(q, k, v, q_offsets, k_offsets, k_lengths, causal, max_q, max_k)
+  q, k, v = (_packed_rows(t) for t in (q, k, v))
+  out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+  lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if return_lse else None
+  lib = _lib.load()
+  nws = lib.mdattn_fwd_bf16_packed_workspace_floats(ctypes.byref(p))
+  ws = torch.empty(nws, dtype=torch.float32, device=q.device) if nws else None
+  st = [ctypes.byref(_row_strides(t)) for t in (q, k, v, out)]
+  rc = lib.mdattn_fwd_bf16_packed(_stream(), ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), *st,
+                                  float(q.shape[2]**-0.5 if scale is None else scale), _ptr(ws), nws)
+  _lib.check(rc, "mdattn_fwd_bf16_packed")
+  return (out, lse) if return_lse else out
+
+
+def flash_attention_packed_backward(q, k, v, out, dout, lse, q_offsets, k_offsets=None, *, causal: bool = True, scale: float | None = None,
+                                    max_q: int | None = None, max_k: int | None = None):
+  """Backward of `flash_attention_packed`: its inputs, its out and lse, and the gradient of out (bf16).  Returns (dq, dk, dv), bf16, dense; rows
+  of no sequence get zeros."""
+  k_offsets = q_offsets if k_offsets is None else k_offsets
+  p = _packed(q, k, v, q_offsets, k_offsets, None, causal, max_q, max_k)
+  _check_dev(q, out, dout, lse)
+  for name, t in (("out", out), ("dout", dout)):
+    if t.shape != q.shape or t.dtype != torch.bfloat16:
+      raise ValueError(f"{name} must be bf16 and shaped like q, {tuple(q.shape)}, got {tuple(t.shape)} {t.dtype}")
+  if lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[1], q.shape[0]) or not lse.is_contiguous():
+    raise ValueError(f"lse must be a contiguous f32 tensor of shape {(q.shape[1], q.shape[0])}, got {tuple(lse.shape)} {lse.dtype}")
+  group = q.shape[1] // k.shape[1]
+  q, k, v = _packed_rows(q, group), _packed_rows(k), _packed_rows(v)
+  out, dout = _packed_rows(out, group), _packed_rows(dout, group)
+  if _packed_strides(out) != _packed_strides(dout):
+    out, dout = out.contiguous(), dout.contiguous()
+  dq, dk, dv = (torch.empty(t.shape, dtype=torch.bfloat16, device=q.device) for t in (q, k, v))
+  lib = _lib.load()
+  nws = lib.mdattn_bwd_bf16_packed_workspace_floats(ctypes.byref(p))
+  ws = torch.empty(max(nws, 4), dtype=torch.float32, device=q.device)
+  st = [ctypes.byref(_row_strides(t)) for t in (q, k, v, out, dq, dk, dv)]
+  rc = lib.mdattn_bwd_bf16_packed(_stream(), ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), _ptr(lse), _ptr(dq), _ptr(dk),
+                                  _ptr(dv), *st, float(q.shape[2]**-0.5 if scale is None else scale), _ptr(ws), nws)
+  _lib.check(rc, "mdattn_bwd_bf16_packed")
+  return dq, dk, dv
 
 
 # ------------------------------------------------------------------------------------------------ the layers beside attention
