@@ -1,5 +1,5 @@
 /*
- * mdlayers.h -- C ABI of the layers beside attention in a DiT block: layer norm with its backward pass, quantisation to
+ * mdlayers.h -- C ABI of the layers beside attention in a DiT block: layer norm and RMS norm with their backward passes, quantisation to
  * e4m3 in blocks of 128, and the product of such operands.
  *
  * Part of libmdattn.so, with the conventions and the MDATTN_E_* codes of mdattn.h: a HIP stream first, work only enqueued,
@@ -56,6 +56,43 @@ int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, const void*
                           int64_t groups, int64_t rows, int C, int64_t x_stride_group, int64_t x_stride_row, int64_t g_stride_group,
                           int64_t g_stride_row, int64_t dx_stride_group, int64_t dx_stride_row, int64_t wb_stride, float eps,
                           float w_offset, float* workspace, int64_t workspace_floats);
+
+/*
+ * RMS norm of the sum of x and a residual:  s = x + residual,  y = s * r * (w_offset + w) + b,  r = (mean of s^2 over the row + eps)^-1/2.
+ * A prompt encoder's norms (models/qwen3_flax.py), LTX-2's with scale and shift (w_offset 1, w and b per batch element;
+ * models/ltx2/transformer_ltx2.py), the addition in front of them done on the way.
+ *   x, y          bf16 or f32 (x_is_f32), as mdattn_layer_norm's x
+ *   residual      or NULL: s = x; of x's type, or f32 beside a bf16 x (r_is_f32); its own strides.  s, of the residual's type, gets the sum;
+ *                 both or neither.  s may be residual, and y x, where the strides agree.
+ *   w, b          as mdattn_layer_norm's
+ * The norm is that of the unrounded f32 sum.  Arithmetic in f32, one rounding of y and one of s.  1 <= C <= 16384.
+ */
+int mdattn_rms_norm(void* stream, const void* x, int x_is_f32, const void* residual, int r_is_f32, void* y, void* s, const void* w, const void* b,
+                    int wb_is_f32, int64_t groups, int64_t rows, int C, int64_t x_stride_group, int64_t x_stride_row, int64_t r_stride_group,
+                    int64_t r_stride_row, int64_t y_stride_group, int64_t y_stride_row, int64_t s_stride_group, int64_t s_stride_row,
+                    int64_t wb_stride, float eps, float w_offset);
+/* The same, y quantised without being stored: q and scales as mdattn_layer_norm_e4m3 has them. */
+int mdattn_rms_norm_e4m3(void* stream, const void* x, int x_is_f32, const void* residual, int r_is_f32, void* q, void* scales, void* s, const void* w,
+                         const void* b, int wb_is_f32, int64_t groups, int64_t rows, int C, int64_t x_stride_group, int64_t x_stride_row,
+                         int64_t r_stride_group, int64_t r_stride_row, int64_t s_stride_group, int64_t s_stride_row, int64_t wb_stride, float eps,
+                         float w_offset);
+
+/*
+ * Backward of mdattn_rms_norm.  With a = g * (w_offset + w) and h = s r:
+ *   ds = r (a - h mean(a h)) + gs,  dw = sum of g h,  db = sum of g, over the rows that share w and b; x's gradient and the residual's are ds.
+ *   s             the forward's sum (x, where it had no residual), bf16 or f32; r is computed again
+ *   g             gradient of y, bf16 or f32; of s's type, or bf16 beside an f32 s
+ *   gs            gradient of s, of its type, or NULL
+ *   ds            of s's type;  dx: the same rounded to bf16, where g is bf16 and s f32, or NULL
+ *   dw, db        of w's type (wb_is_f32; db has it without w too), as mdattn_layer_norm_bwd's; either may be NULL
+ *   workspace     mdattn_rms_norm_bwd_workspace_floats floats; unused, and may be NULL, without dw and db
+ * ds and dx are dense [groups, rows, C].  Deterministic.
+ */
+int64_t mdattn_rms_norm_bwd_workspace_floats(int64_t groups, int64_t rows, int C);
+int mdattn_rms_norm_bwd(void* stream, const void* s, int s_is_f32, const void* g, int g_is_f32, const void* gs, void* ds, void* dx, const void* w,
+                        void* dw, void* db, int wb_is_f32, int64_t groups, int64_t rows, int C, int64_t s_stride_group, int64_t s_stride_row,
+                        int64_t g_stride_group, int64_t g_stride_row, int64_t gs_stride_group, int64_t gs_stride_row, int64_t wb_stride, float eps,
+                        float w_offset, float* workspace, int64_t workspace_floats);
 
 /*
  * Quantisation of x [R, C] to e4m3 with one power-of-two scale per block of block_rows x 128 (block_rows 1 or 128).  Over a block,

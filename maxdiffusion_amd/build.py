@@ -18,7 +18,7 @@ FFI_LIB_PATH = os.path.join(PKG_DIR, "libmdattn_ffi.so")
 HOST_EXT_NAME = "_mdattn_torch"
 HOST_EXT_PATH = os.path.join(PKG_DIR, HOST_EXT_NAME + ".so")  # the torch-side host path in C++ (csrc/host/torch_host.cc)
 
-SOURCES = ["mdattn_api.hip", "norm_rope.hip", "norm_rope_bwd.hip", "attn_fwd_bf16.hip", "attn_fwd_fp8.hip", "attn_bwd_bf16.hip", "merge_quant.hip", "layer_norm.hip", "quant_block.hip",
+SOURCES = ["mdattn_api.hip", "norm_rope.hip", "norm_rope_bwd.hip", "attn_fwd_bf16.hip", "attn_fwd_fp8.hip", "attn_bwd_bf16.hip", "merge_quant.hip", "layer_norm.hip", "rms_norm.hip", "quant_block.hip",
            "matmul_fp8.hip", "attn_packed.hip", "attn_packed_bwd.hip", "probes.hip",
            # the bodies of the XLA custom-call handlers on plain structs (no XLA header): part of the library
            os.path.join("ffi", "mdattn_marshal.cc")]

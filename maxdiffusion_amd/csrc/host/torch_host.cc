@@ -936,6 +936,96 @@ OptTensor layer_norm(const Tensor& x, const OptTensor& w_, const OptTensor& b_, 
   return opt(y);
 }
 
+// The residual beside x: its rows, or none; false: the Python path says what is wrong
+bool residual_rows(const Tensor& x, const Tensor& res, Rows3& r) {
+  if (!res.defined()) return true;
+  if (!float_on(res, x) || res.sizes() != x.sizes() || is_f32(res) < is_f32(x)) return false;
+  const auto rows = as_rows(res);
+  if (!rows) return false;
+  r = *rows;
+  return true;
+}
+// {y} or {y, s}, or empty where a kernel refuses the request
+variable_list rms_run(const Tensor& x, const Rows3& r, const Tensor& w, const Tensor& b, const Tensor& res, const Rows3& rr, int64_t stride, int f32, double eps,
+                      double offset) {
+  Tensor y = at::empty(x.sizes(), x.options()), s = res.defined() ? at::empty(x.sizes(), res.options()) : Tensor();
+  const int64_t sg = r.rows * r.c;
+  if (mdattn_rms_norm(stream(x), ptr(x), is_f32(x), ptr(res), is_f32(res), mut(y), mut(s), ptr(w), ptr(b), f32, r.groups, r.rows, (int)r.c, r.sg, r.sr, rr.sg,
+                      rr.sr, sg, r.c, sg, r.c, stride, (float)eps, (float)offset) != MDATTN_OK)
+    return {};
+  return s.defined() ? variable_list{y, s} : variable_list{y};
+}
+// Saved for the backward: s (x, without a residual) and w; of b only its shape and type.
+struct RmsFn : FirstOrder<RmsFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w_, const OptTensor& b_, const OptTensor& res_, double eps, double offset) {
+    const Tensor w = value(w_), b = value(b_), res = value(res_);
+    const Rows3 r = *as_rows(x);
+    Rows3 rr;
+    int64_t stride;
+    int f32;
+    residual_rows(x, res, rr);
+    norm_vectors(x, r, w, b, stride, f32);
+    variable_list out = rms_run(x, r, w, b, res, rr, stride, f32, eps, offset);
+    if (out.empty()) throw Refused{};
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({res.defined() ? out[1] : x, w});
+    ctx->saved_data["f"] = c10::List<double>({eps, offset});
+    ctx->saved_data["i"] = c10::List<int64_t>({stride, f32, w.defined(), b.defined(), (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()),
+                                               is_f32(res.defined() ? res : x), is_f32(x), res.defined()});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["wshape"] = w.defined() ? w.sizes().vec() : std::vector<int64_t>{};
+    ctx->saved_data["bshape"] = b.defined() ? b.sizes().vec() : std::vector<int64_t>{};
+    return out;
+  }
+  // a gradient as rows of the wanted type
+  static Rows3 as_gradient(Tensor& g, at::ScalarType type) {
+    if (g.scalar_type() != type) g = g.to(type);
+    auto r = as_rows(g);
+    if (!r || g.is_neg()) {
+      g = g.resolve_neg().contiguous();
+      r = as_rows(g);
+    }
+    return *r;
+  }
+  static variable_list gradients(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto f = ctx->saved_data["f"].toDoubleVector();
+    const auto i = ctx->saved_data["i"].toIntVector();
+    const Tensor &s = saved[0], &w = saved[1];
+    const auto r = as_rows(s);
+    unpacked(r && float_on(s, s) && is_f32(s) == (int)i[5] && s.sizes() == at::IntArrayRef(ctx->saved_data["shape"].toIntVector()) && w.defined() == (bool)i[2] &&
+             (!w.defined() || (float_on(w, s) && is_f32(w) == (int)i[1] && w.is_contiguous() && w.sizes() == at::IntArrayRef(ctx->saved_data["wshape"].toIntVector()))));
+    const auto g_type = i[6] ? at::kFloat : at::kBFloat16;
+    Tensor g = grads[0].defined() ? grads[0] : at::zeros(s.sizes(), s.options().dtype(g_type)), gs = i[7] ? grads[1] : Tensor();
+    const Rows3 rg = as_gradient(g, g_type), rs = gs.defined() ? as_gradient(gs, s.scalar_type()) : Rows3{};
+    const bool vectors = i[4], narrow = i[5] != i[6];
+    const auto vec = s.options().dtype(i[1] ? at::kFloat : at::kBFloat16);
+    Tensor ds = at::empty(s.sizes(), s.options()), dx = narrow ? at::empty(s.sizes(), s.options().dtype(at::kBFloat16)) : Tensor();
+    Tensor dw = vectors && i[2] ? at::empty(ctx->saved_data["wshape"].toIntVector(), vec) : Tensor();
+    Tensor db = vectors && i[3] ? at::empty(ctx->saved_data["bshape"].toIntVector(), vec) : Tensor();
+    const int64_t nws = dw.defined() || db.defined() ? mdattn_rms_norm_bwd_workspace_floats(r->groups, r->rows, (int)r->c) : 0;
+    const Tensor ws = nws ? at::empty({nws}, s.options().dtype(at::kFloat)) : Tensor();
+    must(mdattn_rms_norm_bwd(stream(s), ptr(s), is_f32(s), ptr(g), is_f32(g), ptr(gs), mut(ds), mut(dx), ptr(w), mut(dw), mut(db), (int)i[1], r->groups, r->rows,
+                             (int)r->c, r->sg, r->sr, rg.sg, rg.sr, rs.sg, rs.sr, i[0], (float)f[0], (float)f[1], f32(ws), nws),
+         "mdattn_rms_norm_bwd");
+    return {narrow ? dx : ds, dw, db, i[7] ? ds : Tensor(), Tensor(), Tensor()};
+  }
+};
+std::optional<variable_list> rms_norm(const Tensor& x, const OptTensor& w_, const OptTensor& b_, const OptTensor& res_, double eps, double offset) {
+  const Tensor w = value(w_), b = value(b_), res = value(res_);
+  int64_t stride;
+  int f32;
+  Rows3 rr;
+  if (!x.is_cuda() || !float_on(x, x)) return std::nullopt;
+  const auto r = as_rows(x);
+  if (!r || !norm_vectors(x, *r, w, b, stride, f32) || !residual_rows(x, res, rr)) return std::nullopt;
+  if (wants_grad({&x, &w, &b, &res})) return unless_refused([&] { return RmsFn::apply(x, w_, b_, res_, eps, offset); });
+  at::NoGradGuard guard;
+  variable_list out = rms_run(x, *r, w, b, res, rr, stride, f32, eps, offset);
+  if (out.empty()) return std::nullopt;
+  return out;
+}
+
 // [rows, cols] in blocks of e4m3 (ops.BlockQuant), in one buffer: the values, then the scales
 struct Blocks {
   Tensor buf;
@@ -1006,6 +1096,32 @@ OptTensor linear_quantized(const Tensor& x, const Tensor& values, const Tensor& 
       MDATTN_OK)
     return std::nullopt;
   return y;
+}
+
+// RMS norm, with the residual's addition, and the product with a weight that the program keeps quantised: {product} or {product, s}
+std::optional<variable_list> rms_norm_linear(const Tensor& x, const Tensor& values, const Tensor& scales, int64_t n, int64_t k, int64_t block_rows,
+                                             const OptTensor& bias_, const OptTensor& w_, const OptTensor& b_, const OptTensor& res_, double eps, double offset) {
+  const Tensor bias = value(bias_), w = value(w_), b = value(b_), res = value(res_);
+  if (!x.is_cuda() || !float_on(x, x) || x.dim() < 1 || x.size(-1) != k || x.numel() == 0 || k <= 0 || n <= 0 || !values.is_cuda() ||
+      values.get_device() != x.get_device() || scales.get_device() != x.get_device() || !bias_ok(bias, n, x) || wants_grad({&x, &bias, &w, &b, &res}))
+    return std::nullopt;
+  at::NoGradGuard guard;
+  int64_t stride;
+  int f32;
+  Rows3 rr;
+  const auto r = as_rows(x);
+  if (!r || !norm_vectors(x, *r, w, b, stride, f32) || !residual_rows(x, res, rr)) return std::nullopt;
+  const int64_t m = r->all(), sg = r->rows * r->c;
+  const Blocks q(x, m, k, 1);
+  Tensor s = res.defined() ? at::empty(x.sizes(), res.options()) : Tensor();
+  if (mdattn_rms_norm_e4m3(stream(x), ptr(x), is_f32(x), ptr(res), is_f32(res), q.values(), q.scales(), mut(s), ptr(w), ptr(b), f32, r->groups, r->rows, (int)r->c,
+                           r->sg, r->sr, rr.sg, rr.sr, sg, r->c, stride, (float)eps, (float)offset) != MDATTN_OK)
+    return std::nullopt;
+  Tensor y = at::empty(with_last(x, n), x.options().dtype(at::kBFloat16));
+  if (product(q.values(), q.scales(), static_cast<const uint8_t*>(ptr(values)), static_cast<const uint8_t*>(ptr(scales)), block_rows, bias, y, m, n, k) !=
+      MDATTN_OK)
+    return std::nullopt;
+  return s.defined() ? variable_list{y, s} : variable_list{y};
 }
 
 // y = x8 w8^T + b, dx = dy8 w8, dw = dy8'^T x8', ' quantised along the tokens.  Saved: x and w in e4m3, transposed, from one read of each.
@@ -1088,6 +1204,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("norm_rope_rows", &norm_rope_rows, Unlocked());
   m.def("layer_norm", &layer_norm, Unlocked());
   m.def("linear_quantized", &linear_quantized, Unlocked());
+  m.def("rms_norm", &rms_norm, Unlocked());
+  m.def("rms_norm_linear", &rms_norm_linear, Unlocked());
   m.def("first_order", [](const std::vector<OptTensor>& grads, const std::vector<OptTensor>& results) {
     variable_list g, r;
     for (const auto& t : grads) g.push_back(value(t));

@@ -14,97 +14,10 @@
 // to 5.6 TB/s, backward 4.4 to 5.2.  Backward above 12,288 channels, where 1,024 threads leave each 128 registers and 7 to 113 are spilled:
 // bf16 2.8 to 3.4 TB/s (5.3 at 12,288), f32 2.5 to 2.9.  Short calls are bound by the way of a row through memory and its reductions: 4,112 x
 // 1,280 forward 7 us, backward 11 and 4 for the sums.
-#include "mdattn_common.h"
-#include "mdlayers.h"
-#include "quant_block.h"
+#include "norm_rows.h"
 
 namespace mdattn {
 namespace {
-
-constexpr int kMaxWaves = 16;
-
-__device__ __forceinline__ float wave_sum(float x) {
-  x = row16_sum(x);
-  const u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return xhalf_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-}
-
-__device__ __forceinline__ void store8(__bf16* p, const float* f) {
-  const uint4 u = pack8(f);
-  __builtin_nontemporal_store(u32x4{u.x, u.y, u.z, u.w}, reinterpret_cast<u32x4_any*>(p));
-}
-__device__ __forceinline__ void store8(float* p, const float* f) {
-  __builtin_nontemporal_store(f32x4{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32x4_any*>(p));
-  __builtin_nontemporal_store(f32x4{f[4], f[5], f[6], f[7]}, reinterpret_cast<f32x4_any*>(p + 4));
-}
-
-// A row of C channels dealt to a team of threads: slot j of a thread is chunk j * team + tid.  TAIL: C is not a multiple of 8, and the
-// last chunk is walked by elements.
-template <int NV, bool TAIL>
-struct Deal {
-  int c[NV];  // first channel of each slot
-  int C, team;
-  __device__ __forceinline__ Deal(int C_, int tid, int team_) : C(C_), team(team_) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) c[j] = (j * team + tid) * 8;
-  }
-  __device__ __forceinline__ bool has(int j, int e) const { return TAIL ? c[j] + e < C : c[j] < C; }
-  template <typename T>
-  __device__ __forceinline__ void load(Chunk<T> (&x)[NV], const T* row) const {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (TAIL ? c[j] + 8 <= C : c[j] < C) x[j].load(row + c[j]);
-      else if (TAIL && c[j] < C) x[j].load_some(row + c[j], C - c[j]);
-      else x[j].zero();
-    }
-  }
-  template <typename T>
-  __device__ __forceinline__ void store(int j, T* row, const float* f) const {
-    if (TAIL ? c[j] + 8 <= C : c[j] < C) {
-      store8(row + c[j], f);
-    } else if (TAIL && c[j] < C) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c[j] + e < C) row[c[j] + e] = (T)f[e];
-    }
-  }
-  // f32 that is read again soon
-  __device__ __forceinline__ void keep(int j, float* row, const float* f) const {
-    if (TAIL ? c[j] + 8 <= C : c[j] < C) {
-      *reinterpret_cast<f32x4_any*>(row + c[j]) = f32x4{f[0], f[1], f[2], f[3]};
-      *reinterpret_cast<f32x4_any*>(row + c[j] + 4) = f32x4{f[4], f[5], f[6], f[7]};
-    } else if (TAIL && c[j] < C) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c[j] + e < C) row[c[j] + e] = f[e];
-    }
-  }
-  // w or b of one group as f32; `none` where there is none, zeros where there is no channel
-  __device__ __forceinline__ void vector(float (&v)[NV][8], const void* p, int is_f32, int64_t at, float none) const {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] = none;
-      if (p == nullptr) continue;
-      if (is_f32) {
-        Chunk<float> x[NV];
-        load(x, static_cast<const float*>(p) + at);
-        x[j].get(v[j]);
-      } else {
-        Chunk<__bf16> x[NV];
-        load(x, static_cast<const __bf16*>(p) + at);
-        x[j].get(v[j]);
-      }
-    }
-  }
-  // channels that the slots of the team's wave `w` hold
-  __device__ __forceinline__ float count(int w) const {
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) n += min(max(C - (j * team + w * 64) * 8, 0), 512);
-    return (float)n;
-  }
-};
 
 struct NormArgs {
   const void* x;
@@ -346,14 +259,7 @@ __global__ __launch_bounds__(MAXT) void layer_norm_bwd_kernel(NormBwdArgs a) {
   }
 }
 
-// out[g][c] = sum over i < n of part[g * n + i][plane][c], plane 0 to dw, 1 to db.  64 columns of a group per workgroup, 16 partial sums each.
-struct SumArgs {
-  const float* part;
-  void *out0, *out1;
-  int64_t n, row_stride, plane_stride;
-  int64_t C;
-  int f32;
-};
+// 64 columns of a group per workgroup, 16 partial sums each.
 __global__ __launch_bounds__(1024) void sum_rows_kernel(SumArgs a) {
   __shared__ float part[16][64];
   const int lane = threadIdx.x & 63, i0 = threadIdx.x >> 6;
@@ -383,31 +289,10 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(SumArgs a) {
   }
 }
 
-constexpr int kMaxC = 16384;
-// How a row is dealt: chunks per thread and threads of a team.  The fewest places that hold a row, with a power of two of threads: teams of
-// five or six waves sit unevenly on the four SIMDs of a CU (quantised rows of 5,120: 320 threads 2.6 TB/s, 256 with a sixth of the places
-// empty 4.5).
-struct Shape {
-  int nv, threads;
-};
-Shape shape_of(int C) {
-  const int chunks = (C + 7) / 8;
-  Shape best{0, 0};
-  for (int t = 64; t <= 1024; t *= 2)
-    for (int nv = 1; nv <= 3; ++nv)
-      if (nv * t >= chunks && (best.nv == 0 || nv * t < best.nv * best.threads || (nv * t == best.nv * best.threads && nv > best.nv))) best = {nv, t};
-  return best;
-}
 // Rows in flight on a CU, by their bytes: enough to keep the memory busy, and no more, which would make the rows' pages compete.  18 KB of
 // rows forward, in bf16 the best number or near it at all but one of the widths measured (512 channels: eighteen rows 6.05 TB/s, six 3.7; 1,536: six
 // 5.9, three 4.9, twelve 5.5; 2,560: four 5.6, three 4.8; 5,120: two 5.5, four 5.2; 8,192: one 6.2, two 5.5; but 2,048: five 5.6, four 5.9), 36 with a quantised output, whose arithmetic needs
 // more waves (5,120: two 3.4, four 4.5), 32 of x and g backward (2,048: four 4.9, twelve 3.8; 5,120: two 5.2, four 4.4).
-int rows_per_cu(int64_t row_bytes, int64_t in_flight, int least) { return (int)((in_flight + row_bytes / 2) / row_bytes < least ? least : (in_flight + row_bytes / 2) / row_bytes); }
-// Workgroups of one group of so many rows, of all groups' `target`, and no more than go through them in as many rounds
-int blocks_of(int64_t groups, int64_t rows, int64_t target) {
-  const int64_t n = (target + groups - 1) / groups, rounds = (rows + n - 1) / n;
-  return (int)((rows + rounds - 1) / rounds);
-}
 struct BwdShape {
   Shape s;
   int teams, blocks;
@@ -420,28 +305,6 @@ BwdShape bwd_shape(int64_t groups, int64_t rows, int C, int x_is_f32) {
   b.blocks = blocks_of(groups, (rows + b.teams - 1) / b.teams, 256 * (int64_t)((per_cu + b.teams - 1) / b.teams));
   return b;
 }
-
-// A tensor's strides of a group and of a row.  Groups that share w and b, and follow one another as rows do, are one group of all rows.
-struct Strides {
-  int64_t *group, *row;
-};
-template <int N>
-void merge_groups(int64_t& groups, int64_t& rows, int64_t wb_stride, const Strides (&all)[N]) {
-  if (groups == 1 || wb_stride != 0) return;
-  for (const Strides& s : all) {
-    if (rows > 1 && *s.group != rows * *s.row) return;
-  }
-  if (rows == 1) {
-    for (const Strides& s : all) *s.row = *s.group;
-  }
-  rows *= groups;
-  groups = 1;
-}
-
-bool sizes_ok(int64_t groups, int64_t rows, int C) {
-  return groups > 0 && rows > 0 && C > 0 && rows < ((int64_t)1 << 40) / groups;
-}
-bool elem_aligned(const void* p, int is_f32) { return (reinterpret_cast<uintptr_t>(p) & (is_f32 ? 3u : 1u)) == 0; }
 
 template <typename T, int OUT>
 int launch_norm(hipStream_t st, const NormArgs& a, const Shape& s, unsigned grid) {
@@ -474,6 +337,11 @@ int norm(hipStream_t st, NormArgs& a, int x_is_f32, int out, int64_t groups) {
 }
 
 }  // namespace
+
+int sum_rows_launch(hipStream_t st, const SumArgs& a, int64_t groups, int planes) {
+  MDATTN_LAUNCH(sum_rows_kernel, dim3((unsigned)sum_rows_grid(groups, a.C), (unsigned)planes), dim3(1024), 0, st, a);
+  return launch_status();
+}
 }  // namespace mdattn
 
 using namespace mdattn;
@@ -530,7 +398,7 @@ extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, 
   const BwdShape b = bwd_shape(groups, a.rows, C, x_is_f32);
   a.blocks = b.blocks;
   a.team = b.s.threads;
-  const int64_t grid = groups * a.blocks, sum_grid = (C + 63) / 64 * (wb_stride ? groups : 1);
+  const int64_t grid = groups * a.blocks, sum_grid = sum_rows_grid(wb_stride ? groups : 1, C);
   if (!grid_fits(grid, b.s.threads * b.teams) || (sums && !grid_fits(sum_grid, 1024))) return MDATTN_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   const unsigned threads = (unsigned)(b.s.threads * b.teams), lds = b.teams > 1 ? b.teams * 8u * (unsigned)ceil_to(C, 8) : 0u;
@@ -548,8 +416,7 @@ extern "C" int mdattn_layer_norm_bwd(void* stream, const void* x, int x_is_f32, 
   if (rc != MDATTN_OK || !sums) return rc;
   // shared w and b: one sum over the workgroups of all groups
   const SumArgs r{workspace, dw, db, wb_stride ? a.blocks : grid, 2 * (int64_t)C, C, C, wb_is_f32};
-  MDATTN_LAUNCH(sum_rows_kernel, dim3((unsigned)sum_grid, 2), dim3(1024), 0, st, r);
-  return launch_status();
+  return sum_rows_launch(st, r, wb_stride ? groups : 1, 2);
 }
 
 extern "C" int mdattn_sum_rows(void* stream, const float* rows, int64_t n, int64_t C, void* out, int out_is_f32) {
@@ -557,6 +424,5 @@ extern "C" int mdattn_sum_rows(void* stream, const float* rows, int64_t n, int64
   if (!grid_fits((C + 63) / 64, 1024)) return MDATTN_E_UNSUPPORTED;
   if (!elem_aligned(rows, 1) || !elem_aligned(out, out_is_f32)) return MDATTN_E_ALIGN;
   const SumArgs r{rows, out, nullptr, n, C, 0, C, out_is_f32};
-  MDATTN_LAUNCH(sum_rows_kernel, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, (hipStream_t)stream, r);
-  return launch_status();
+  return sum_rows_launch((hipStream_t)stream, r, 1, 1);
 }

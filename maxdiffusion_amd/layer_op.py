@@ -1,4 +1,4 @@
-"""The layers beside attention in a DiT block, as a model calls them: layer norm and dense layers in blocks of e4m3.
+"""The layers beside attention in a DiT block, as a model calls them: layer norm, RMS norm and dense layers in blocks of e4m3.
 
 Differentiable where an input requires a gradient while autograd is recording; once, and not in forward mode: second derivatives and
 tensors with a tangent raise NotImplementedError (paths relative to ``src/maxdiffusion/``):
@@ -7,6 +7,9 @@ tensors with a tangent raise NotImplementedError (paths relative to ``src/maxdif
   hip_linear_fp8                a dense layer on e4m3 operands (the reference's qwix quantisation of dense layers, per tensor or
                                 channel there, pipelines/wan/wan_pipeline.py:581-626)
   hip_layer_norm_linear_fp8     the norm and the dense layer behind it, the normalised rows never stored
+  hip_rms_norm                  the norms of a prompt encoder (models/qwen3_flax.py) and of LTX-2's blocks (models/ltx2/transformer_ltx2.py), with
+                                the residual's addition in front of them
+  hip_rms_norm_linear_fp8       that norm and the dense layer behind it
 """
 from __future__ import annotations
 
@@ -15,7 +18,7 @@ import torch
 from . import _lib, ops
 from .ops import BlockQuant
 
-__all__ = ["hip_layer_norm", "hip_linear_fp8", "hip_layer_norm_linear_fp8", "quantize_weight", "BlockQuant"]
+__all__ = ["hip_layer_norm", "hip_rms_norm", "hip_linear_fp8", "hip_layer_norm_linear_fp8", "hip_rms_norm_linear_fp8", "quantize_weight", "BlockQuant"]
 
 
 def _wants_grad(*ts) -> bool:
@@ -68,6 +71,49 @@ def hip_layer_norm(x, weight=None, bias=None, eps: float = 1e-6, weight_offset: 
   if _wants_grad(x, weight, bias):
     return _HipLayerNorm.apply(_rows(x), weight, bias, eps, weight_offset)
   return ops.layer_norm(_rows(x), weight, bias, eps, weight_offset)
+
+
+class _HipRmsNorm(torch.autograd.Function):
+  """Saved for the backward: s (x, without a residual) and the vectors; the rows' statistics are computed again."""
+
+  @staticmethod
+  def forward(ctx, x, weight, bias, residual, eps, weight_offset):
+    ctx.set_materialize_grads(False)
+    out = ops.rms_norm(x, weight, bias, residual, eps, weight_offset)
+    s = x if residual is None else out[1]
+    ctx.save_for_backward(s, weight, bias)
+    ctx.cfg, ctx.forms = (eps, weight_offset), _forms(s, weight, bias)
+    ctx.narrow, ctx.g_dtype, ctx.has_residual = s.dtype != x.dtype, x.dtype, residual is not None
+    return out
+
+  @staticmethod
+  @_lib.first_order
+  def backward(ctx, g, gs=None):
+    s, weight, bias = ctx.saved_tensors
+    if _forms(s, weight, bias) != ctx.forms:
+      raise ValueError("a tensor saved for the backward pass came back from its hook with another dtype, shape or device")
+    g = torch.zeros(s.shape, dtype=ctx.g_dtype, device=s.device) if g is None else _rows(g.to(ctx.g_dtype))
+    gs = None if gs is None else _rows(gs.to(s.dtype))
+    ds, dx, dw, db = ops.rms_norm_backward(_rows(s), weight, bias, g, gs, *ctx.cfg, needs_vectors=any(ctx.needs_input_grad[1:3]), narrow=ctx.narrow)
+    return ds if dx is None else dx, dw, db, ds if ctx.has_residual else None, None, None
+
+
+def hip_rms_norm(x, weight=None, bias=None, residual=None, eps: float = 1e-6, weight_offset: float = 0.0):
+  """x [..., C], bf16 or f32 -> y = s * (mean s^2 + eps)^-1/2 * (weight_offset + weight) + bias, with s = x + residual; (y, s) where there is one.
+
+  residual: of x's shape and dtype, or f32 beside a bf16 x; s has its dtype and is the next residual.  weight, bias and weight_offset as
+  `hip_layer_norm`'s: a prompt encoder has (weight), LTX-2 (scale, shift, weight_offset=1)."""
+  if x.is_cuda:
+    out = _lib.host().rms_norm(x, weight, bias, residual, eps, weight_offset)
+    if out is not None:
+      return out[0] if residual is None else tuple(out)
+  # what the native path leaves: views to be copied, nothing to compute, and every error
+  _lib.no_tangents(x, weight, bias, residual)
+  weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
+  residual = residual if residual is None else _rows(residual)
+  if _wants_grad(x, weight, bias, residual):
+    return _HipRmsNorm.apply(_rows(x), weight, bias, residual, eps, weight_offset)
+  return ops.rms_norm(_rows(x), weight, bias, residual, eps, weight_offset)
 
 
 def quantize_weight(weight) -> BlockQuant:
@@ -167,3 +213,20 @@ def hip_layer_norm_linear_fp8(x, weight, bias, w8: BlockQuant, out_bias=None, ep
     raise NotImplementedError("hip_layer_norm_linear_fp8 has no backward pass: use hip_layer_norm and hip_linear_fp8 for training")
   weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
   return ops.matmul_fp8_block_as(ops.layer_norm_quant(_rows(x), weight, bias, eps, weight_offset), w8, out_bias, x.shape[:-1])
+
+
+def hip_rms_norm_linear_fp8(x, weight, bias, w8: BlockQuant, out_bias=None, residual=None, eps: float = 1e-6, weight_offset: float = 0.0):
+  """`hip_linear_fp8` of `hip_rms_norm`'s y with w8 and out_bias, the norm's f32 rows quantised where they are made: (the product, s), or the product alone
+  without a residual.  Inference only."""
+  if x.is_cuda:
+    out = _lib.host().rms_norm_linear(x, w8.values, w8.scales, w8.rows, w8.cols, w8.block_rows, out_bias, weight, bias, residual, eps, weight_offset)
+    if out is not None:
+      return out[0] if residual is None else tuple(out)
+  _lib.no_tangents(x, weight, bias, out_bias, residual)
+  if _wants_grad(x, weight, bias, out_bias, residual):
+    raise NotImplementedError("hip_rms_norm_linear_fp8 has no backward pass: use hip_rms_norm and hip_linear_fp8 for training")
+  weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
+  out = ops.rms_norm_quant(_rows(x), weight, bias, residual if residual is None else _rows(residual), eps, weight_offset)
+  q, s = (out, None) if residual is None else out
+  y = ops.matmul_fp8_block_as(q, w8, out_bias, x.shape[:-1])
+  return y if residual is None else (y, s)

@@ -19,7 +19,7 @@ __all__ = [
     "norm_rope_fullrow", "norm_rope_qkv", "norm_rope_perhead", "norm_rope_rows",
     "norm_rope_fullrow_backward", "norm_rope_perhead_backward", "norm_rope_rows_backward", "flash_attention", "flash_attention_backward", "flash_attention_backward_static", "flash_attention_fp8", "quant_e4m3", "key_mask_bias",
     "flash_attention_packed", "flash_attention_packed_backward",
-    "layer_norm", "layer_norm_quant", "layer_norm_backward", "BlockQuant", "quant_block_e4m3", "sum_rows", "matmul_fp8_block",
+    "layer_norm", "layer_norm_quant", "layer_norm_backward", "rms_norm", "rms_norm_quant", "rms_norm_backward", "BlockQuant", "quant_block_e4m3", "sum_rows", "matmul_fp8_block",
     "merge_partial", "flash_attention_merge", "finalize", "new_merge_state", "LSE_INIT", "FOLDED_SCALE", "folded_q_mul", "set_fwd_schedule", "FWD_SCHEDULES", "FP8_SOFTMAX_MODES",
 ]
 
@@ -804,6 +804,84 @@ def layer_norm_backward(x, weight, bias, g, eps: float = 1e-6, weight_offset: fl
                                  gg, gr, rows * c, c, stride, float(eps), float(weight_offset), _ptr(ws), nws)
   _lib.check(rc, "mdattn_layer_norm_bwd")
   return dx, dw, db
+
+
+def _residual(x, residual):
+  """(is f32, stride of a group, stride of a row) of a residual beside x."""
+  if residual is None:
+    return 0, 0, 0
+  r_f32 = _float_kind(residual, "residual")
+  if residual.shape != x.shape or residual.device != x.device or r_f32 < (x.dtype == torch.float32):
+    raise ValueError(f"residual must be shaped like x, {tuple(x.shape)}, and of its dtype, or f32 beside a bf16 x, got {tuple(residual.shape)} "
+                     f"{residual.dtype} for {x.dtype}")
+  return r_f32, *_norm_rows(residual, "residual")[3:]
+
+
+def rms_norm(x, weight=None, bias=None, residual=None, eps: float = 1e-6, weight_offset: float = 0.0):
+  """s = x + residual, y = s * (mean of s^2 over the last axis + eps)^-1/2 * (weight_offset + weight) + bias, for x [..., C], bf16 or f32.
+
+  residual: of x's dtype, or f32 beside a bf16 x; None: s = x.  weight and bias as `layer_norm`'s.  Arithmetic in f32, the norm that of the unrounded
+  sum.  Returns (y in x's dtype, s in the residual's), or y alone without a residual."""
+  _check_dev(x, weight, bias, residual)
+  x_f32 = _float_kind(x, "x")
+  groups, rows, c, sg, sr = _norm_rows(x)
+  r_f32, rg, rr = _residual(x, residual)
+  stride, wb_f32 = _norm_vectors(weight, bias, groups, c)
+  y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+  s = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+  if x.numel():
+    rc = _lib.load().mdattn_rms_norm(_stream(), _ptr(x), x_f32, _ptr(residual), r_f32, _ptr(y), _ptr(s), _ptr(weight), _ptr(bias), wb_f32, groups, rows, c,
+                                     sg, sr, rg, rr, rows * c, c, rows * c, c, stride, float(eps), float(weight_offset))
+    _lib.check(rc, "mdattn_rms_norm")
+  return y if residual is None else (y, s)
+
+
+def rms_norm_quant(x, weight=None, bias=None, residual=None, eps: float = 1e-6, weight_offset: float = 0.0):
+  """`rms_norm` with y's unrounded rows quantised (`quant_block_e4m3`, blocks of 1 x 128) instead of stored: (BlockQuant of as many rows as x
+  has, s), or the BlockQuant alone without a residual."""
+  _check_dev(x, weight, bias, residual)
+  x_f32 = _float_kind(x, "x")
+  groups, rows, c, sg, sr = _norm_rows(x)
+  r_f32, rg, rr = _residual(x, residual)
+  stride, wb_f32 = _norm_vectors(weight, bias, groups, c)
+  q = _new_quant(groups * rows, c, 1, x.device)
+  s = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+  if x.numel():
+    rc = _lib.load().mdattn_rms_norm_e4m3(_stream(), _ptr(x), x_f32, _ptr(residual), r_f32, _ptr(q.values), _ptr(q.scales), _ptr(s), _ptr(weight), _ptr(bias),
+                                          wb_f32, groups, rows, c, sg, sr, rg, rr, rows * c, c, stride, float(eps), float(weight_offset))
+    _lib.check(rc, "mdattn_rms_norm_e4m3")
+  return q if residual is None else (q, s)
+
+
+def rms_norm_backward(s, weight, bias, g, gs=None, eps: float = 1e-6, weight_offset: float = 0.0, needs_vectors: bool = True, narrow: bool = False):
+  """Backward of `rms_norm`: s as the forward returned it (x, where there was no residual), weight and bias as it had them (of bias only
+  whether there is one, its shape and dtype), g and gs the gradients of y and s (gs None: none), g in s's dtype or bf16 beside an f32 s.  Returns (ds, dx,
+  dweight, dbias): the gradient of the residual, and of x, in s's dtype; the same in bf16 where `narrow` (x was bf16 beside an f32
+  residual), else None; None for what there is not, or for the last two with needs_vectors False."""
+  _check_dev(s, weight, bias, g, gs)
+  s_f32, g_f32 = _float_kind(s, "s"), _float_kind(g, "g")
+  groups, rows, c, sg, sr = _norm_rows(s)
+  stride, wb_f32 = _norm_vectors(weight, bias, groups, c)
+  if g.shape != s.shape or g_f32 > s_f32 or (narrow and (g_f32 or not s_f32)):
+    raise ValueError(f"g must be shaped like s, {tuple(s.shape)}, and of its dtype, or bf16 beside an f32 s (and there alone `narrow`), got {tuple(g.shape)} "
+                     f"{g.dtype} for {s.dtype}")
+  if gs is not None and (gs.shape != s.shape or gs.dtype != s.dtype):
+    raise ValueError(f"gs must be shaped and typed like s, {tuple(s.shape)} {s.dtype}, got {tuple(gs.shape)} {gs.dtype}")
+  gg, gr = _norm_rows(g, "g")[3:]
+  ug, ur = (0, 0) if gs is None else _norm_rows(gs, "gs")[3:]
+  ds = torch.empty(s.shape, dtype=s.dtype, device=s.device)
+  dx = torch.empty(s.shape, dtype=torch.bfloat16, device=s.device) if narrow else None
+  dw = torch.empty_like(weight) if weight is not None and needs_vectors else None
+  db = torch.empty_like(bias) if bias is not None and needs_vectors else None
+  if not s.numel():
+    return ds, dx, *(None if t is None else t.zero_() for t in (dw, db))
+  lib = _lib.load()
+  nws = lib.mdattn_rms_norm_bwd_workspace_floats(groups, rows, c) if dw is not None or db is not None else 0
+  ws = torch.empty(nws, dtype=torch.float32, device=s.device) if nws else None
+  rc = lib.mdattn_rms_norm_bwd(_stream(), _ptr(s), s_f32, _ptr(g), g_f32, _ptr(gs), _ptr(ds), _ptr(dx), _ptr(weight), _ptr(dw), _ptr(db), wb_f32, groups, rows,
+                               c, sg, sr, gg, gr, ug, ur, stride, float(eps), float(weight_offset), _ptr(ws), nws)
+  _lib.check(rc, "mdattn_rms_norm_bwd")
+  return ds, dx, dw, db
 
 
 class BlockQuant:
