@@ -19,6 +19,7 @@ __device__ __forceinline__ unsigned div_by(unsigned n, const Divisor& d) { retur
 struct PackedSeqs {
   const int *q_off, *k_off, *k_len;
   int count, q_rows, k_rows;
+  int levels;  // see find_tile
 };
 
 // A workgroup's tile of a sequence: rows q0 .. q0 + m of q, k0 .. k0 + n of k and v.  Gap: rows of no sequence (m of q, or n of k), to be
@@ -38,41 +39,94 @@ __device__ __forceinline__ int wave_prefix_sum(int x) {  // inclusive, over the 
   return x;
 }
 
-// Tile `rank` of all sequences' tiles of BM rows (KEYS: of k; else of q, `group` rows for each of its tokens), in the order of the
-// sequences; the rows in front of the first sequence and behind the last follow as two more.  Offsets that decrease, or that point outside, are
-// brought into the tensors.  Every wave looks for itself, 64 sequences at a time.
+// Lane i's sequence, of those from i0 on: its rows (of q, and of k) and its tiles of BM rows (KEYS: of k; else of q, `group` rows for each of its
+// tokens).  The rows in front of the first sequence and behind the last follow as two more.  Offsets that decrease, or that point outside, are
+// brought into the tensors.
 template <int BM, bool KEYS>
-__device__ __forceinline__ SeqTile find_tile(const PackedSeqs& s, int group, int rank, int lane) {
+__device__ __forceinline__ int lane_sequence(const PackedSeqs& s, int group, int i0, int lane, int& qa, int& m, int& ka, int& n) {
+  const int i = i0 + lane, at = i < s.count ? i : s.count, next = i < s.count ? i + 1 : i == s.count ? 0 : s.count;
+  qa = s.q_off[at];
+  ka = s.k_off[at];
+  int qb = s.q_off[next], kb = s.k_off[next];
+  const int len = s.k_len && i < s.count ? s.k_len[i] : 0x7FFFFFFF;
+  if (i == s.count) qa = ka = 0;                           // in front of the first
+  if (i == s.count + 1) { qb = s.q_rows; kb = s.k_rows; }  // behind the last
+  qa = min(max(qa, 0), s.q_rows);
+  ka = min(max(ka, 0), s.k_rows);
+  m = min(max(qb, qa), s.q_rows) - qa;
+  n = min(min(max(kb, ka), s.k_rows) - ka, max(len, 0));
+  return i < s.count + 2 ? (int)(((unsigned)(KEYS ? n : m * group) + (BM - 1)) / BM) : 0;
+}
+
+// Tile `rank` of all sequences' tiles.  Every wave looks for itself, 64 sequences at a time, in their order, each one's last tile first.  levels (for
+// up to 62 sequences): all sequences' tiles by their number instead, the highest first.
+template <int BM, bool KEYS>
+__device__ __forceinline__ SeqTile find_tile(const PackedSeqs& s, int group, int rank, int lane, bool levels) {
+  SeqTile t{};
   int before = 0;
   for (int i0 = 0; i0 < s.count + 2; i0 += 64) {
-    const int i = i0 + lane, at = i < s.count ? i : s.count, next = i < s.count ? i + 1 : i == s.count ? 0 : s.count;
-    int qa = s.q_off[at], qb = s.q_off[next], ka = s.k_off[at], kb = s.k_off[next];
-    const int len = s.k_len && i < s.count ? s.k_len[i] : 0x7FFFFFFF;
-    if (i == s.count) qa = ka = 0;                       // in front of the first
-    if (i == s.count + 1) { qb = s.q_rows; kb = s.k_rows; }  // behind the last
-    qa = min(max(qa, 0), s.q_rows);
-    ka = min(max(ka, 0), s.k_rows);
-    const int m = min(max(qb, qa), s.q_rows) - qa, n = min(min(max(kb, ka), s.k_rows) - ka, max(len, 0));
-    const int rows = KEYS ? n : m * group;
-    const int tiles = i < s.count + 2 ? (int)(((unsigned)rows + (BM - 1)) / BM) : 0;
-    const int upto = wave_prefix_sum(tiles);
-    const uint64_t behind = __builtin_amdgcn_ballot_w64(before + upto > rank);
-    if (behind) {
-      const int j = __builtin_ctzll(behind);
-      SeqTile t;
-      t.q0 = __builtin_amdgcn_readlane(qa, j);
-      t.m = __builtin_amdgcn_readlane(m, j);
-      t.k0 = __builtin_amdgcn_readlane(ka, j);
-      t.n = __builtin_amdgcn_readlane(n, j);
-      t.tiles = __builtin_amdgcn_readlane(tiles, j);
-      t.tile = rank - before - (__builtin_amdgcn_readlane(upto, j) - t.tiles);
-      t.gap = i0 + j >= s.count;
-      t.none = false;
-      return t;
+    int qa, m, ka, n;
+    const int tiles = lane_sequence<BM, KEYS>(s, group, i0, lane, qa, m, ka, n);
+    const int upto = wave_prefix_sum(tiles), total = __builtin_amdgcn_readlane(upto, 63);
+    if (rank - before >= total) {
+      before += total;
+      continue;
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    int j;
+    if (levels) {  // the highest number with more than `rank` tiles of it and above
+      auto above = [&](int level) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(wave_prefix_sum(max(tiles - level, 0)), 63); };
+      int lo = 0, hi = (int)(((unsigned)(KEYS ? s.k_rows : s.q_rows * group)) / BM) + 1;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (above(mid) > rank) lo = mid;
+        else hi = mid;
+      }
+      uint64_t here = __builtin_amdgcn_ballot_w64(tiles > lo);
+      for (int skip = rank - above(hi); skip > 0; --skip) here &= here - 1;
+      j = __builtin_ctzll(here);
+      t.tile = lo;
+    } else {
+      j = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + upto > rank));
+      t.tile = before + __builtin_amdgcn_readlane(upto, j) - 1 - rank;
+    }
+    t.q0 = __builtin_amdgcn_readlane(qa, j);
+    t.m = __builtin_amdgcn_readlane(m, j);
+    t.k0 = __builtin_amdgcn_readlane(ka, j);
+    t.n = __builtin_amdgcn_readlane(n, j);
+    t.gap = i0 + j >= s.count;
+    t.tiles = __builtin_amdgcn_readlane(tiles, j);
+    return t;
   }
+  t.none = true;
+  return t;
+}
+
+// Item `rank` of all sequences' tiles of 32 rows with each of its pieces of piece_keys keys (up to `pieces`, the last of which takes the rest; one,
+// where there are no keys).
+__device__ __forceinline__ SeqTile find_piece(const PackedSeqs& s, int group, int rank, int lane, int piece_keys, int pieces, int& piece) {
   SeqTile t{};
+  int before = 0;
+  for (int i0 = 0; i0 < s.count + 2; i0 += 64) {
+    int qa, m, ka, n;
+    const int tiles = lane_sequence<32, false>(s, group, i0, lane, qa, m, ka, n);
+    const int each = i0 + lane < s.count ? max(min((int)(((unsigned)n + (unsigned)(piece_keys - 1)) / (unsigned)piece_keys), pieces), 1) : 1;
+    const int upto = wave_prefix_sum(tiles * each), total = __builtin_amdgcn_readlane(upto, 63);
+    if (rank - before >= total) {
+      before += total;
+      continue;
+    }
+    const int j = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + upto > rank)), per = __builtin_amdgcn_readlane(each, j);
+    t.tiles = __builtin_amdgcn_readlane(tiles, j);
+    const int at = rank - before - (__builtin_amdgcn_readlane(upto, j) - t.tiles * per);
+    t.tile = at / per;
+    piece = at - t.tile * per;
+    t.q0 = __builtin_amdgcn_readlane(qa, j);
+    t.m = __builtin_amdgcn_readlane(m, j);
+    t.k0 = __builtin_amdgcn_readlane(ka, j);
+    t.n = __builtin_amdgcn_readlane(n, j);
+    t.gap = i0 + j >= s.count;
+    return t;
+  }
   t.none = true;
   return t;
 }
@@ -137,6 +191,9 @@ inline int packed_sizes(const mdattn_packed* p) {
 inline bool packed_aligned(const mdattn_packed* p) {
   return ((reinterpret_cast<uintptr_t>(p->q_offsets) | reinterpret_cast<uintptr_t>(p->k_offsets) | reinterpret_cast<uintptr_t>(p->k_lengths)) & 3) == 0;
 }
+// Whether the tiles of a call go by their number, over all sequences: of a causal batch the high ones meet the most keys, and what starts last
+// should be short.  Only where they do not all start at once: the search for one costs some 0.5 us.
+inline bool packed_levels(const mdattn_packed* p, int64_t tiles, int64_t places) { return p->causal && p->sequences > 1 && p->sequences <= 62 && tiles > places; }
 // tiles of BM rows that all sequences of `rows` rows have together at most, and the two gaps
 inline int64_t packed_tiles(int64_t rows, int64_t sequences, int BM) { return rows / BM + sequences + 2; }
 

@@ -9,9 +9,8 @@
 // a lane holds 16 keys of one row and the accumulators are, packed to bf16, the B operand of O^T += V^T P^T.  The softmax keeps no running
 // maximum but a reference point per row, moved (in a rarely taken branch) when a sum of P leaves its range.  Keys that a row does not see get
 // s = -inf, in the blocks that hold such keys; blocks that no row of a wave sees are not computed.
-// NK: 1: four waves with 32 rows each.  4: four waves that share 32 rows and deal the keys among them, joined through LDS: for one or a few
-// tokens, where the time is that of the keys' way from memory.
-// With few rows the keys are cut into pieces besides; each leaves un-normalised f32 rows, joined by a second kernel in a fixed order.
+// Few rows (one or a few tokens) have a kernel of their own, bound by the keys' way from memory.
+// With few tiles the keys are cut into pieces besides; each leaves un-normalised f32 rows, joined by a third kernel in a fixed order.
 #include "attn_packed.h"
 
 namespace mdattn {
@@ -33,20 +32,76 @@ struct PackedArgs {
   float2* ml;   // [piece][kv_heads][q_rows * group]: reference point (log2 units) and sum of P
 };
 
-template <int HD, int NK>
+template <int HD>
 struct FwdShape {
-  static constexpr int NB = HD == 64 && NK == 1 ? 2 : 1;        // blocks of 32 keys that a wave computes per slot
-  static constexpr int SLOTS = HD == 128 ? (NK == 1 ? 3 : 2) : (NK == 1 ? 2 : 3);
-  static constexpr int Blocks = NB * NK, Keys = 32 * Blocks;    // of a slot
-  static constexpr int Half = Blocks * PackedBlock<HD>::Bytes, Slot = 2 * Half;
-  static constexpr int BM = NK == 1 ? 128 : 32;
+  static constexpr int NB = HD == 64 ? 2 : 1;      // blocks of 32 keys of a slot
+  static constexpr int SLOTS = HD == 64 ? 2 : 3;
+  static constexpr int Keys = 32 * NB, Half = NB * PackedBlock<HD>::Bytes, Slot = 2 * Half;
+  static constexpr int BM = 128;
 };
 
-template <int HD, int DC, bool PADDED, int NK>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NK == 4 ? 1 : HD == 64 ? 4 : 3, NK == 4 ? 2 : HD == 64 ? 4 : 3)))
-void packed_fwd_kernel(PackedArgs a) {
+// rows of no sequence: tile `tile` of them
+template <int BM, int HD>
+__device__ __forceinline__ void fill_gap(const PackedArgs& a, const SeqTile& s, int head, int tid) {
+  const int G = a.group.d, rows = s.m * G;
+  for (int i = tid; i < BM * (HD / 8); i += 256) {
+    const int r = s.tile * BM + i / (HD / 8), col = i % (HD / 8) * 8;
+    if (r >= rows) continue;
+    const int t = (int)div_by((unsigned)r, a.group), h = head * G + r - t * G;
+    if (col < a.D) *reinterpret_cast<uint4*>(a.out + (int64_t)(s.q0 + t) * a.os.row + (int64_t)h * a.os.head + col) = make_uint4(0u, 0u, 0u, 0u);
+    if (col == 0 && a.lse) a.lse[(int64_t)h * a.seqs.q_rows + s.q0 + t] = -INFINITY;
+  }
+}
+
+// The softmax of a row's running sums: P = exp2(c s - mc) of 16 keys per lane and their sum against the row's reference point m (mc = m c), which
+// moves, with O and l, when a sum leaves its range.  Rows that have seen no key yet have m = -1e30, from which any logit is out of range.
+struct RowState {
+  float m, mc, l;
+};
+template <int ND>
+__device__ __forceinline__ void soft_block(const f32x16& S, float c, RowState& st, f32x16 (&O)[ND], bf16x8 (&P)[2]) {
+  auto soft = [&]() __attribute__((always_inline)) {
+    float sum = 0.f;
+#pragma unroll
+    for (int hb = 0; hb < 2; ++hb) {
+      unsigned pk[4];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * hb + e], c, -st.mc));
+        const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * hb + e + 1], c, -st.mc));
+        sum = (hb == 0 && e == 0) ? x0 : sum + x0;
+        sum += x1;
+        pk[e >> 1] = pack2(x0, x1);
+        asm volatile("" : "+v"(pk[e >> 1]), "+v"(sum));  // packed as soon as they exist
+      }
+      P[hb] = __builtin_bit_cast(bf16x8, u32x4{pk[0], pk[1], pk[2], pk[3]});
+    }
+    return sum;
+  };
+  float sum = soft();
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum <= kRange)) != 0, 0)) {
+    float top = S[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, S[i]);
+    const float mnew = fmaxf(st.m, xhalf_max(top));
+    float alpha = __builtin_amdgcn_exp2f((st.m - mnew) * c);
+    st.m = mnew;
+    st.mc = st.m * c;
+    asm volatile("" : "+v"(alpha));  // keeps the rescale inside this rarely taken branch
+    st.l *= alpha;
+#pragma unroll
+    for (int db = 0; db < ND; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) O[db][i] *= alpha;
+    sum = soft();
+  }
+  st.l += sum;
+}
+
+template <int HD, int DC, bool PADDED>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 4 : 3, HD == 64 ? 4 : 3))) void packed_fwd_kernel(PackedArgs a) {
   using T = PackedBlock<HD>;
-  using F = FwdShape<HD, NK>;
+  using F = FwdShape<HD>;
   constexpr int NJ = DC / 16, ND = (DC + 31) / 32, NB = F::NB, SLOTS = F::SLOTS;
   constexpr int GPW = F::Keys / T::RPI / 4;  // row groups per wave, slot and tensor
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // (fragment addresses are formed by xor)
@@ -55,23 +110,14 @@ void packed_fwd_kernel(PackedArgs a) {
 
   // neighbouring workgroups, which go to different dies, take different heads: with eight heads of k and v each die's L2 holds one of them
   const int rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
-  const SeqTile s = find_tile<F::BM, false>(a.seqs, G, rank, lane);
+  const SeqTile s = find_tile<F::BM, false>(a.seqs, G, rank, lane, a.seqs.levels);
   if (s.none) return;
   const int64_t group_rows = (int64_t)a.seqs.q_rows * G;
-  const int tile = s.tiles - 1 - s.tile;  // (causal: the longest first)
-  const int rows = s.m * G, r0 = tile * F::BM + (NK == 1 ? wave * 32 : 0);
+  const int tile = s.tile, rows = s.m * G, r0 = tile * F::BM + wave * 32;
   const bool split = a.part != nullptr;
   auto token_of = [&](int r) __attribute__((always_inline)) { return (int)div_by((unsigned)r, a.group); };
-
-  if (s.gap) {  // rows of no sequence
-    if (blockIdx.y) return;
-    for (int i = tid; i < F::BM * (HD / 8); i += 256) {
-      const int r = tile * F::BM + i / (HD / 8), col = i % (HD / 8) * 8;
-      if (r >= rows) continue;
-      const int t = token_of(r), h = head * G + r - t * G;
-      if (col < a.D) *reinterpret_cast<uint4*>(a.out + (s.q0 + t) * a.os.row + h * a.os.head + col) = make_uint4(0u, 0u, 0u, 0u);
-      if (col == 0 && a.lse) a.lse[(int64_t)h * a.seqs.q_rows + s.q0 + t] = -INFINITY;
-    }
+  if (s.gap) {
+    if (blockIdx.y == 0) fill_gap<F::BM, HD>(a, s, head, tid);
     return;
   }
 
@@ -137,7 +183,7 @@ void packed_fwd_kernel(PackedArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) O[db][i] = 0.f;
   const float c = a.c;
-  float m = -1e30f, mc = -1e30f * c, l = 0.f;
+  RowState st{-1e30f, -1e30f * c, 0.f};
   const unsigned row_at = T::row_at(lane), trans_at = T::trans_at(lane);
 
   // a block of 32 keys, the first of them key `k0` of the piece, at `at` (its V a half slot on)
@@ -178,42 +224,7 @@ void packed_fwd_kernel(PackedArgs a) {
     }
     __builtin_amdgcn_s_setprio(0);
     bf16x8 P[2];
-    auto soft = [&](float rf) __attribute__((always_inline)) {
-      float sum = 0.f;
-#pragma unroll
-      for (int hb = 0; hb < 2; ++hb) {
-        unsigned pk[4];
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * hb + e], c, -rf));
-          const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * hb + e + 1], c, -rf));
-          sum = (hb == 0 && e == 0) ? x0 : sum + x0;
-          sum += x1;
-          pk[e >> 1] = pack2(x0, x1);
-          asm volatile("" : "+v"(pk[e >> 1]), "+v"(sum));  // packed as soon as they exist
-        }
-        P[hb] = __builtin_bit_cast(bf16x8, u32x4{pk[0], pk[1], pk[2], pk[3]});
-      }
-      return sum;
-    };
-    float sum = soft(mc);
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum <= kRange)) != 0, 0)) {
-      float top = S[0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, S[i]);
-      const float mnew = fmaxf(m, xhalf_max(top));
-      float alpha = __builtin_amdgcn_exp2f((m - mnew) * c);
-      m = mnew;
-      mc = m * c;
-      asm volatile("" : "+v"(alpha));  // keeps the rescale inside this rarely taken branch
-      l *= alpha;
-#pragma unroll
-      for (int db = 0; db < ND; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) O[db][i] *= alpha;
-      sum = soft(mc);
-    }
-    l += sum;
+    soft_block<ND>(S, c, st, O, P);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int jv = 0; jv < 2 * ND; ++jv) {
@@ -243,77 +254,193 @@ void packed_fwd_kernel(PackedArgs a) {
     const unsigned at = smem_addr + (unsigned)(slot * F::Slot);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int i = NK == 1 ? b : wave * NB + b, k0 = t * F::Keys + 32 * i;
-      if (k0 < some) block(at + (unsigned)(i * T::Bytes), k0);
+      const int k0 = t * F::Keys + 32 * b;
+      if (k0 < some) block(at + (unsigned)(b * T::Bytes), k0);
     }
     slot = slot == SLOTS - 1 ? 0 : slot + 1;
     fill = fill == SLOTS - 1 ? 0 : fill + 1;
   }
   __syncthreads();  // every wave has finished reading the ring, and no load into it is in flight: it now stages the output
-  l = xhalf_sum(l);
+  const float l = xhalf_sum(st.l), mc = st.mc;
 
-  const int64_t part_row = ((int64_t)piece * a.kv_heads + head) * group_rows + (int64_t)s.q0 * G;  // of the sequence's first row
-  if constexpr (NK == 1) {
-    if (split) {
-      if (r0 + l32 < rows) {
-        if (hh == 0) a.ml[part_row + r0 + l32] = make_float2(mc, l);
-        if (nt > 0) {
-          float* p = a.part + (part_row + r0 + l32) * a.D + 4 * hh;
-#pragma unroll
-          for (int db = 0; db < ND; ++db)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-              if (!PADDED || db * 32 + 8 * g < a.D)
-                *reinterpret_cast<f32x4*>(p + db * 32 + 8 * g) = f32x4{O[db][4 * g], O[db][4 * g + 1], O[db][4 * g + 2], O[db][4 * g + 3]};
-        }
-      }
-      return;
-    }
-    // rows that see no key give 0 and -inf; a sum that is not a number stays one
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    if (a.lse && hh == 0 && r0 + l32 < rows)
-      a.lse[(int64_t)(head * G + r - token * G) * a.seqs.q_rows + s.q0 + token] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * kLn2;
-    constexpr int RowB = ND * 64 + 16, LPR = ND == 3 ? 16 : ND * 4, RPI = 64 / LPR;  // a staged row; lanes per row, rows per store
-    static_assert(4 * 32 * RowB <= SLOTS * F::Slot, "the staged rows fit the ring");
-    char* stage = smem + wave * 32 * RowB;
-#pragma unroll
-    for (int db = 0; db < ND; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint2 u;
-        u.x = pack2(O[db][4 * g] * inv, O[db][4 * g + 1] * inv);
-        u.y = pack2(O[db][4 * g + 2] * inv, O[db][4 * g + 3] * inv);
-        *reinterpret_cast<uint2*>(stage + l32 * RowB + hh * 8 + (db * 32 + g * 8) * 2) = u;
-      }
-    // LDS accesses of one wave execute in order: the reads below see the writes above
-    const int rr = lane / LPR, cc = lane % LPR;
-    if (cc * 8 >= (PADDED ? a.D : DC)) return;
-#pragma unroll
-    for (int j = 0; j < 32 / RPI; ++j) {
-      const int row = r0 + j * RPI + rr;
-      if (row >= rows) break;
-      const int t = token_of(row);
-      st_nt(reinterpret_cast<uint4*>(a.out + (int64_t)(s.q0 + t) * a.os.row + (int64_t)(head * G + row - t * G) * a.os.head + cc * 8),
-            *reinterpret_cast<const uint4*>(stage + (j * RPI + rr) * RowB + cc * 16));
-    }
-  } else {
-    // the four waves' shares brought to one reference point
-    constexpr int Ld = ND * 32 + 4;  // floats of a staged row
-    static_assert((4 * 32 * Ld + 4 * 32 * 2) * 4 <= SLOTS * F::Slot, "the staged rows fit the ring");
-    float* stage = reinterpret_cast<float*>(smem);
-    float2* ml = reinterpret_cast<float2*>(stage + 4 * 32 * Ld);
+  if (split) {
+    if (r0 + l32 >= rows) return;
+    const int64_t at = ((int64_t)piece * a.kv_heads + head) * group_rows + (int64_t)s.q0 * G + r0 + l32;
+    if (hh == 0) a.ml[at] = make_float2(mc, l);
+    if (nt <= 0) return;
+    float* p = a.part + at * a.D + 4 * hh;
 #pragma unroll
     for (int db = 0; db < ND; ++db)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(stage + (wave * 32 + l32) * Ld + db * 32 + 8 * g + 4 * hh) =
-            f32x4{O[db][4 * g], O[db][4 * g + 1], O[db][4 * g + 2], O[db][4 * g + 3]};
-    if (hh == 0) ml[wave * 32 + l32] = make_float2(mc, l);
-    __syncthreads();
-    constexpr int CPR = ND * 4;  // chunks of 8 columns of a row
-    for (int i = tid; i < 32 * CPR; i += 256) {
-      const int lr = i / CPR, cc = i % CPR * 8, row = r0 + lr;
-      if (row >= rows || cc >= (PADDED ? a.D : DC)) continue;
+        if (!PADDED || db * 32 + 8 * g < a.D)
+          *reinterpret_cast<f32x4*>(p + db * 32 + 8 * g) = f32x4{O[db][4 * g], O[db][4 * g + 1], O[db][4 * g + 2], O[db][4 * g + 3]};
+    return;
+  }
+  // rows that see no key give 0 and -inf; a sum that is not a number stays one
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  if (a.lse && hh == 0 && r0 + l32 < rows)
+    a.lse[(int64_t)(head * G + r - token * G) * a.seqs.q_rows + s.q0 + token] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * kLn2;
+  constexpr int RowB = ND * 64 + 16, LPR = ND == 3 ? 16 : ND * 4, RPI = 64 / LPR;  // a staged row; lanes per row, rows per store
+  static_assert(4 * 32 * RowB <= SLOTS * F::Slot, "the staged rows fit the ring");
+  char* stage = smem + wave * 32 * RowB;
+#pragma unroll
+  for (int db = 0; db < ND; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uint2 u;
+      u.x = pack2(O[db][4 * g] * inv, O[db][4 * g + 1] * inv);
+      u.y = pack2(O[db][4 * g + 2] * inv, O[db][4 * g + 3] * inv);
+      *reinterpret_cast<uint2*>(stage + l32 * RowB + hh * 8 + (db * 32 + g * 8) * 2) = u;
+    }
+  // LDS accesses of one wave execute in order: the reads below see the writes above
+  const int rr = lane / LPR, cc = lane % LPR;
+  if (cc * 8 >= (PADDED ? a.D : DC)) return;
+#pragma unroll
+  for (int j = 0; j < 32 / RPI; ++j) {
+    const int row = r0 + j * RPI + rr;
+    if (row >= rows) break;
+    const int t = token_of(row);
+    st_nt(reinterpret_cast<uint4*>(a.out + (int64_t)(s.q0 + t) * a.os.row + (int64_t)(head * G + row - t * G) * a.os.head + cc * 8),
+          *reinterpret_cast<const uint4*>(stage + (j * RPI + rr) * RowB + cc * 16));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------- few rows
+// 32 rows of a group (four tokens of eight heads, say) per workgroup, all four waves the same ones.  The keys go by pieces of piece_keys, one to a
+// workgroup at a time; in a piece the waves take blocks of 32 keys in turn, each through buffers of its own in LDS, one for K and one for V, so that no
+// wave waits for another: the next K is requested once the scores of this one are formed, the next V once its product is.  Four waves and
+// two workgroups per CU keep some 64 to 128 KB of keys on their way, what 256 CUs need at 8 TB/s.  The waves' sums are joined through LDS,
+// the pieces' by packed_combine_kernel.  The workgroups walk the list of pieces, whose length is known on the device only.
+template <int HD>
+constexpr int few_bytes() {
+  constexpr int ring = 8 * PackedBlock<HD>::Bytes, stage = (4 * 32 * 68 + 4 * 32 * 2) * 4;
+  return ring > stage ? ring : stage;
+}
+template <int HD, int DC, bool PADDED>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : 2, HD == 64 ? 3 : 2))) void packed_few_kernel(PackedArgs a) {
+  using T = PackedBlock<HD>;
+  constexpr int NJ = DC / 16, ND = (DC + 31) / 32, LPB = 32 / T::RPI;  // loads per block and tensor
+  constexpr int NV = HD == 128 ? 4 : 2;                                 // row groups that the swizzle tells apart
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.group.d;
+  const int64_t group_rows = (int64_t)a.seqs.q_rows * G;
+  auto token_of = [&](int r) __attribute__((always_inline)) { return (int)div_by((unsigned)r, a.group); };
+  const unsigned mine = lds_addr_of(smem) + (unsigned)(wave * 2 * T::Bytes), row_at = T::row_at(lane), trans_at = T::trans_at(lane);
+  const int grow = T::row(lane);
+  int col[NV];
+  [[maybe_unused]] uint64_t mask[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    col[i] = T::chunk(lane, i) * 8;
+    mask[i] = __builtin_amdgcn_ballot_w64(col[i] < a.D);
+    if (PADDED && col[i] >= a.D) col[i] = 0;
+  }
+  const float c = a.c;
+
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    const int rank = item / a.kv_heads, head = item - rank * a.kv_heads;
+    int piece;
+    const SeqTile s = find_piece(a.seqs, G, rank, lane, a.piece_keys, a.pieces, piece);
+    if (s.none) return;
+    if (s.gap) {
+      fill_gap<32, HD>(a, s, head, tid);
+      continue;
+    }
+    const int rows = s.m * G, r0 = s.tile * 32, kb = piece * a.piece_keys;
+    const int ke = piece == a.pieces - 1 ? s.n : min(s.n, kb + a.piece_keys);
+    const int r = min(r0 + l32, rows - 1), token = token_of(r);  // (rows past the end repeat the last one and are not stored)
+    auto sees = [&](int t) __attribute__((always_inline)) { return min(ke, a.causal ? max(t + 1 + s.n - s.m, 0) : s.n) - kb; };
+    const int lim = sees(token), all = __builtin_amdgcn_readlane(lim, 0), some = __builtin_amdgcn_readlane(lim, 31);
+    const int nt = (some - 32 * wave + 127) / 128;  // this wave's blocks: 128 t + 32 wave; zero or less: none
+
+    const __bf16* kp = a.k + (int64_t)(s.k0 + kb) * a.ks.row + head * a.ks.head;
+    const __bf16* vp = a.v + (int64_t)(s.k0 + kb) * a.vs.row + head * a.vs.head;
+    auto request = [&](const __bf16* p, const RowStrides& st, unsigned to, int t) __attribute__((always_inline)) {
+      const int k0 = t * 128 + 32 * wave;
+#pragma unroll
+      for (int i = 0; i < LPB; ++i) {
+        // rows past the sequence's end repeat its last one
+        const __bf16* at = p + (int64_t)min(k0 + T::RPI * i + grow, s.n - kb - 1) * st.row + col[i % NV];
+        if constexpr (PADDED) lds_dma16(at, to + (unsigned)i * 1024u, mask[i % NV]);
+        else lds_dma16(at, to + (unsigned)i * 1024u);
+      }
+    };
+    bf16x8 qf[NJ];
+    {
+      const __bf16* p = a.q + (int64_t)(s.q0 + token) * a.qs.row + (int64_t)(head * G + r - token * G) * a.qs.head + hh * 8;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        qf[j] = !PADDED || j * 16 + hh * 8 < a.D ? *reinterpret_cast<const bf16x8*>(p + j * 16) : __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+    }
+    if constexpr (PADDED) {  // chunks past the head dim: zeros that no load touches
+      for (int i = lane * 16; i < 2 * T::Bytes; i += 1024) *reinterpret_cast<uint4*>(smem + wave * 2 * T::Bytes + i) = make_uint4(0u, 0u, 0u, 0u);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    if (nt > 0) {
+      request(kp, a.ks, mine, 0);
+      request(vp, a.vs, mine + T::Bytes, 0);
+    }
+    f32x16 O[ND];
+#pragma unroll
+    for (int db = 0; db < ND; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) O[db][i] = 0.f;
+    RowState st{-1e30f, -1e30f * c, 0.f};
+    for (int t = 0; t < nt; ++t) {
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LPB) : "memory");  // K has landed, V may be on its way
+      f32x16 S;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_row_frag((mine + row_at) ^ (unsigned)(32 * j)), qf[j], S, 0, 0, 0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K's buffer has been read
+      if (t + 1 < nt) request(kp, a.ks, mine, t + 1);
+      const int k0 = t * 128 + 32 * wave;
+      if (k0 + 32 > all) {
+        asm volatile("" ::: "memory");  // keeps the branch
+        const int at0 = k0 + 4 * hh;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (at0 + 8 * (i >> 2) + (i & 3) >= lim) S[i] = -INFINITY;
+      }
+      bf16x8 P[2];
+      soft_block<ND>(S, c, st, O, P);
+      if (t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LPB) : "memory");  // V has landed, the next K may be on its way
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int jv = 0; jv < 2 * ND; ++jv) {
+        const unsigned v = (mine + T::Bytes + trans_at) ^ (unsigned)(64 * (jv % ND));
+        constexpr int Up = T::Row;
+        O[jv % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            read_trans_frag(v + (unsigned)(jv / ND * 16 * Up), (v ^ 32u) + (unsigned)((8 + jv / ND * 16) * Up)), P[jv / ND], O[jv % ND], 0, 0, 0);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V's buffer has been read
+      if (t + 1 < nt) request(vp, a.vs, mine + T::Bytes, t + 1);
+    }
+    st.l = xhalf_sum(st.l);
+
+    // the four waves' shares brought to one reference point, 64 columns of a head at a time
+    constexpr int Ld = 64 + 4;  // floats of a staged row
+    static_assert((4 * 32 * Ld + 4 * 32 * 2) * 4 <= few_bytes<HD>(), "the staged rows fit");
+    float* stage = reinterpret_cast<float*>(smem);
+    float2* ml = reinterpret_cast<float2*>(stage + 4 * 32 * Ld);
+    const int64_t part_row = ((int64_t)piece * a.kv_heads + head) * group_rows + (int64_t)s.q0 * G;  // of the sequence's first row
+#pragma unroll
+    for (int d0 = 0; d0 < ND; d0 += 2) {
+      __syncthreads();  // the buffers, or the columns before, have been read
+#pragma unroll
+      for (int db = d0; db < (d0 + 2 < ND ? d0 + 2 : ND); ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(stage + (wave * 32 + l32) * Ld + (db - d0) * 32 + 8 * g + 4 * hh) =
+              f32x4{O[db][4 * g], O[db][4 * g + 1], O[db][4 * g + 2], O[db][4 * g + 3]};
+      if (hh == 0) ml[wave * 32 + l32] = make_float2(st.mc, st.l);
+      __syncthreads();
+      const int lr = tid >> 3, cc = (tid & 7) * 8, row = r0 + lr, at = d0 * 32 + cc;
+      if (row >= rows || at >= (PADDED ? a.D : DC)) continue;
       float top = -INFINITY, sum = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w)
@@ -327,100 +454,119 @@ void packed_fwd_kernel(PackedArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] += x * o[e];
       }
-      if (split) {
-        if (cc == 0) a.ml[part_row + row] = make_float2(top, sum);
-        if (nt > 0) {
-          f32x4* p = reinterpret_cast<f32x4*>(a.part + (part_row + row) * a.D + cc);
-          p[0] = f32x4{f[0], f[1], f[2], f[3]};
-          p[1] = f32x4{f[4], f[5], f[6], f[7]};
+      if (a.part) {
+        if (at == 0) {
+          a.ml[part_row + row] = make_float2(top, sum);
+          // the first piece says of the pieces that the sequence does not have that they have no weight
+          if (piece == 0)
+            for (int p = max(1, (s.n + a.piece_keys - 1) / a.piece_keys); p < a.pieces; ++p) a.ml[p * group_rows * a.kv_heads + part_row + row] = make_float2(0.f, 0.f);
         }
+        f32x4* p = reinterpret_cast<f32x4*>(a.part + (part_row + row) * a.D + at);
+        p[0] = f32x4{f[0], f[1], f[2], f[3]};
+        p[1] = f32x4{f[4], f[5], f[6], f[7]};
         continue;
       }
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] *= inv;
       const int t = token_of(row), h = head * G + row - t * G;
-      *reinterpret_cast<uint4*>(a.out + (int64_t)(s.q0 + t) * a.os.row + h * a.os.head + cc) = pack8(f);
-      if (cc == 0 && a.lse) a.lse[(int64_t)h * a.seqs.q_rows + s.q0 + t] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
+      *reinterpret_cast<uint4*>(a.out + (int64_t)(s.q0 + t) * a.os.row + (int64_t)h * a.os.head + at) = pack8(f);
+      if (at == 0 && a.lse) a.lse[(int64_t)h * a.seqs.q_rows + s.q0 + t] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
     }
+    __syncthreads();  // the next piece's keys go where the rows were staged
   }
 }
 
-// The pieces of the keys joined, in their order: one 16-byte store per lane.
-__global__ __launch_bounds__(256) void packed_combine_kernel(PackedArgs a, int cpr, int64_t chunks) {  // cpr: chunks of 8 columns per row
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= chunks) return;
-  const int64_t row = i / cpr, group_rows = (int64_t)a.seqs.q_rows * a.group.d, rows = group_rows * a.kv_heads;
-  const int cc = (int)(i - row * cpr) * 8;
+// The pieces of the keys joined, in their order: a workgroup per row, lane p of each wave with the weight of piece p, each wave the sums of every
+// fourth piece.
+constexpr int kMaxPieces = 64;
+__global__ __launch_bounds__(256) void packed_combine_kernel(PackedArgs a) {
+  __shared__ float part[3][128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = blockIdx.x, group_rows = (int64_t)a.seqs.q_rows * a.group.d, rows = group_rows * a.kv_heads;
   const int head = (int)(row / group_rows);
   const unsigned rg = (unsigned)(row - head * group_rows), t = div_by(rg, a.group), h = head * a.group.d + rg - t * a.group.d;
   if ((int)t < a.seqs.q_off[0] || (int)t >= a.seqs.q_off[a.seqs.count]) return;  // rows of no sequence: zeros already
-  float top = -INFINITY, sum = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < a.pieces; ++p) {
-    const float2 u = a.ml[p * rows + row];
-    if (u.y != 0.f) top = fmaxf(top, u.x);
-  }
-  for (int p = 0; p < a.pieces; ++p) {
-    const float2 u = a.ml[p * rows + row];
-    if (u.y == 0.f) continue;
-    const float x = __builtin_amdgcn_exp2f(u.x - top);
-    const f32x4* o = reinterpret_cast<const f32x4*>(a.part + (p * rows + row) * a.D + cc);
-    const f32x4 o0 = o[0], o1 = o[1];
-    sum += x * u.y;
+  const float2 u = lane < a.pieces ? a.ml[lane * rows + row] : make_float2(0.f, 0.f);
+  float top = u.y != 0.f ? u.x : -INFINITY;  // (a piece without weight carries no reference point)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { f[e] += x * o0[e]; f[4 + e] += x * o1[e]; }
+  for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+  const float x = u.y != 0.f ? __builtin_amdgcn_exp2f(u.x - top) : 0.f;
+  float sum = x * u.y;
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) sum += __shfl_xor(sum, i);
+  const int c = 2 * lane;
+  float f0 = 0.f, f1 = 0.f;
+  const float* p = a.part + row * a.D + (c < a.D ? c : 0);
+#pragma unroll 8
+  for (int i = wave; i < a.pieces; i += 4) {
+    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), i));
+    if (w == 0.f) continue;  // (nothing may stand there; a weight that is not a number stays one)
+    const float2 o = *reinterpret_cast<const float2*>(p + i * rows * a.D);
+    f0 += w * o.x;
+    f1 += w * o.y;
+  }
+  if (wave) {
+    part[wave - 1][c] = f0;
+    part[wave - 1][c + 1] = f1;
+  }
+  __syncthreads();
+  if (wave || c >= a.D) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w) {
+    f0 += part[w][c];
+    f1 += part[w][c + 1];
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] *= inv;
-  *reinterpret_cast<uint4*>(a.out + (int64_t)t * a.os.row + (int64_t)h * a.os.head + cc) = pack8(f);
-  if (cc == 0 && a.lse) a.lse[(int64_t)h * a.seqs.q_rows + t] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
+  *reinterpret_cast<unsigned*>(a.out + (int64_t)t * a.os.row + (int64_t)h * a.os.head + c) = pack2(f0 * inv, f1 * inv);
+  if (c == 0 && a.lse) a.lse[(int64_t)h * a.seqs.q_rows + t] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
 }
 
 // How a call is launched.
 struct FwdPlan {
-  int nk, pieces, piece_keys;
-  int64_t floats;
+  bool few;
+  int pieces, piece_keys;
+  int64_t floats, tiles;  // tiles: of rows, of all heads
 };
 FwdPlan fwd_plan(const mdattn_packed* p) {
   const int64_t group = p->heads / p->kv_heads;
   const int64_t max_q = p->max_q > 0 && p->max_q < p->q_rows ? p->max_q : p->q_rows, max_k = p->max_k > 0 && p->max_k < p->k_rows ? p->max_k : p->k_rows;
-  FwdPlan f{max_q * group <= 32 ? 4 : 1, 1, 1 << 30, 0};
-  const int bm = f.nk == 4 ? 32 : 128;
+  // (the list of all tiles' pieces is counted in 31 bits)
+  FwdPlan f{max_q * group <= 32 && packed_tiles(p->q_rows * group, p->sequences, 32) * kMaxPieces * p->kv_heads < (1ll << 31), 1, 1 << 30, 0, 0};
+  const int bm = f.few ? 32 : 128;
   // tiles that there are: of the tokens, or of so many sequences of the longest one's
   int64_t tiles = (max_q * group + bm - 1) / bm * p->sequences;
   const int64_t most = p->q_rows * group / bm + p->sequences;
-  tiles = (tiles < most ? tiles : most) * p->kv_heads;
-  const int64_t want = f.nk == 4 ? 1024 : 512, least = f.nk == 4 ? 256 : 512;
-  if (tiles <= 0 || tiles >= want / 2 || max_k < 2 * least) return f;
-  int64_t pieces = want / tiles;
-  if (pieces > max_k / least) pieces = max_k / least;
-  if (pieces > 64) pieces = 64;
+  f.tiles = tiles = (tiles < most ? tiles : most) * p->kv_heads;
+  const int64_t least = f.few ? 256 : 512;
+  if (tiles <= 0 || max_k < 2 * least) return f;
+  int64_t keys;
+  if (f.few) {
+    const int64_t all = max_k * p->sequences < p->k_rows ? max_k * p->sequences : p->k_rows;
+    keys = all * p->kv_heads / 2048;
+  } else {
+    if (tiles >= 256) return f;
+    keys = max_k * tiles / 512;
+  }
+  if (keys < least) keys = least;
+  if (keys * kMaxPieces < max_k) keys = (max_k + kMaxPieces - 1) / kMaxPieces;
+  keys = (keys + 127) / 128 * 128;
+  const int64_t pieces = (max_k + keys - 1) / keys;
   if (pieces < 2) return f;
-  f.piece_keys = (int)(((max_k + pieces - 1) / pieces + 127) / 128 * 128);
-  f.pieces = (int)((max_k + f.piece_keys - 1) / f.piece_keys);
-  f.floats = f.pieces * (int64_t)p->q_rows * p->heads * (p->head_dim + 2);
+  f.piece_keys = (int)keys;
+  f.pieces = (int)pieces;
+  f.floats = pieces * p->q_rows * p->heads * (p->head_dim + 2);
   return f;
 }
 
-template <int HD, int DC, bool PADDED, int NK>
-int launch(hipStream_t st, const PackedArgs& a, int64_t grid) {
-  constexpr int bytes = FwdShape<HD, NK>::SLOTS * FwdShape<HD, NK>::Slot;
-  const auto kernel = packed_fwd_kernel<HD, DC, PADDED, NK>;
-  if constexpr (bytes > 65536) {
-    static LdsOptIn opted;
-    if (lds_opt_in(opted, reinterpret_cast<const void*>(kernel), bytes) != MDATTN_OK) return MDATTN_E_LAUNCH;
+template <int HD, int DC, bool PADDED>
+int launch(hipStream_t st, const PackedArgs& a, bool few, int64_t grid) {
+  if (few) {
+    MDATTN_LAUNCH((packed_few_kernel<HD, DC, PADDED>), dim3((unsigned)grid), dim3(256), few_bytes<HD>(), st, a);
+  } else {
+    MDATTN_LAUNCH((packed_fwd_kernel<HD, DC, PADDED>), dim3((unsigned)grid, (unsigned)a.pieces), dim3(256), FwdShape<HD>::SLOTS * FwdShape<HD>::Slot, st, a);
   }
-  MDATTN_LAUNCH(kernel, dim3((unsigned)grid, (unsigned)a.pieces), dim3(256), bytes, st, a);
   return launch_status();
-}
-template <int NK>
-int launch_nk(hipStream_t st, const PackedArgs& a, int64_t grid) {
-  if (a.D == 64) return launch<64, 64, false, NK>(st, a, grid);
-  if (a.D < 64) return launch<64, 64, true, NK>(st, a, grid);
-  if (a.D <= 96) return launch<128, 96, true, NK>(st, a, grid);
-  if (a.D < 128) return launch<128, 128, true, NK>(st, a, grid);
-  return launch<128, 128, false, NK>(st, a, grid);
 }
 
 }  // namespace
@@ -453,7 +599,7 @@ extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   PackedArgs a{};
   a.q = static_cast<const __bf16*>(q); a.k = static_cast<const __bf16*>(k); a.v = static_cast<const __bf16*>(v);
   a.out = static_cast<__bf16*>(out); a.lse = lse;
-  a.seqs = {p->q_offsets, p->k_offsets, p->k_lengths, p->sequences, p->q_rows, p->k_rows};
+  a.seqs = {p->q_offsets, p->k_offsets, p->k_lengths, p->sequences, p->q_rows, p->k_rows, !f.few && packed_levels(p, f.tiles, 768)};
   a.group = divisor((unsigned)(p->heads / p->kv_heads));
   a.kv_heads = p->kv_heads; a.D = p->head_dim; a.causal = p->causal;
   a.qs = {q_strides->seq, q_strides->head}; a.ks = {k_strides->seq, k_strides->head};
@@ -465,11 +611,19 @@ extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, cons
     a.part = workspace;
     a.ml = reinterpret_cast<float2*>(workspace + f.pieces * rows * a.D);
   }
-  const int64_t grid = packed_tiles(group_rows, p->sequences, f.nk == 4 ? 32 : 128) * p->kv_heads, chunks = rows * (a.D / 8);
-  if (!grid_fits(grid, 256) || (f.pieces > 1 && !grid_fits((chunks + 255) / 256, 256))) return MDATTN_E_UNSUPPORTED;
+  int64_t grid = packed_tiles(group_rows, p->sequences, f.few ? 32 : 128) * p->kv_heads;
+  if (f.few) {  // two per CU, in whole rounds of the heads, walk what there is
+    const int64_t most = (512 + a.kv_heads - 1) / a.kv_heads * a.kv_heads;
+    grid = grid * f.pieces < most ? grid * f.pieces : most;
+  }
+  if (!grid_fits(grid, 256) || (f.pieces > 1 && !grid_fits(rows, 256))) return MDATTN_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
-  const int status = f.nk == 4 ? launch_nk<4>(st, a, grid) : launch_nk<1>(st, a, grid);
+  const int status = a.D == 64   ? launch<64, 64, false>(st, a, f.few, grid)
+                     : a.D < 64  ? launch<64, 64, true>(st, a, f.few, grid)
+                     : a.D <= 96 ? launch<128, 96, true>(st, a, f.few, grid)
+                     : a.D < 128 ? launch<128, 128, true>(st, a, f.few, grid)
+                                 : launch<128, 128, false>(st, a, f.few, grid);
   if (status != MDATTN_OK || f.pieces == 1) return status;
-  MDATTN_LAUNCH(packed_combine_kernel, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, st, a, a.D / 8, chunks);
+  MDATTN_LAUNCH(packed_combine_kernel, dim3((unsigned)rows), dim3(256), 0, st, a);
   return launch_status();
 }

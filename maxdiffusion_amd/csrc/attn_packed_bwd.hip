@@ -97,9 +97,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
-  const SeqTile s = find_tile<BM, false>(a.seqs, G, rank, lane);
+  const SeqTile s = find_tile<BM, false>(a.seqs, G, rank, lane, a.seqs.levels);
   if (s.none) return;
-  const int tile = s.tiles - 1 - s.tile, rows = s.m * G, r0 = tile * BM + wave * 32;
+  const int tile = s.tile, rows = s.m * G, r0 = tile * BM + wave * 32;
   auto token_of = [&](int r) __attribute__((always_inline)) { return (int)div_by((unsigned)r, a.group); };
   auto row_of = [&](__bf16* p, const RowStrides& st, int r) __attribute__((always_inline)) {
     const int t = token_of(r);
@@ -259,10 +259,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
-  const SeqTile s = find_tile<BM, true>(a.seqs, G, rank, lane);
+  const SeqTile s = find_tile<BM, true>(a.seqs, G, rank, lane, a.seqs.levels);
   if (s.none) return;
-  const int rows = s.m * G, key0 = s.tile * BM, w0 = key0 + wave * 32;  // (causal: the first keys meet the most rows)
-  const int piece = blockIdx.y;
+  const int rows = s.m * G, key0 = (s.tiles - 1 - s.tile) * BM, w0 = key0 + wave * 32;  // (causal: the first keys meet the most rows)
+  const int piece = a.pieces - 1 - blockIdx.y;                                            // (and the last rows the most keys)
   if (s.gap) {
     if (piece) return;
     for (int i = tid; i < BM * (HD / 8); i += 256) {
@@ -445,7 +445,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 // The pieces' sums of dk (blockIdx.y 0) and dv (1), added in their order, for the tiles of 128 keys whose rows were cut.
 __global__ __launch_bounds__(256) void packed_reduce_kernel(PackedBwdArgs a) {
   const int lane = threadIdx.x & 63, rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
-  const SeqTile s = find_tile<128, true>(a.seqs, G, rank, lane);
+  const SeqTile s = find_tile<128, true>(a.seqs, G, rank, lane, false);
   if (s.none || s.gap) return;
   const int key0 = s.tile * 128, cpr = a.D / 8;
   const KeyRows kr = key_rows(s, key0, G, a.causal, a.piece_rows, a.pieces);
@@ -472,18 +472,19 @@ __global__ __launch_bounds__(256) void packed_reduce_kernel(PackedBwdArgs a) {
 // How the dk / dv pass is cut, and the workspace: the rows' two numbers, then the pieces' sums.
 struct BwdPlan {
   int pieces, piece_rows;
-  int64_t aux_floats, floats;
+  int64_t aux_floats, floats, tiles;  // tiles of the dk / dv pass
 };
 BwdPlan bwd_plan(const mdattn_packed* p) {
   const int64_t group = p->heads / p->kv_heads;
   const int64_t max_q = p->max_q > 0 && p->max_q < p->q_rows ? p->max_q : p->q_rows, max_k = p->max_k > 0 && p->max_k < p->k_rows ? p->max_k : p->k_rows;
-  BwdPlan b{1, 1 << 30, 0, 0};
+  BwdPlan b{1, 1 << 30, 0, 0, 0};
   b.aux_floats = ((int64_t)p->q_rows * p->heads * 2 + 3) & ~(int64_t)3;
   int64_t tiles = (max_k + 127) / 128 * p->sequences;
   const int64_t most = p->k_rows / 128 + p->sequences, rows = max_q * group;
   tiles = (tiles < most ? tiles : most) * p->kv_heads;
   const int64_t whole = tiles * rows / (p->causal ? 2 : 1) / 512;  // rows per place on the chip
-  int64_t piece = (whole / 2 + 31) / 32 * 32;
+  b.tiles = tiles;
+  int64_t piece = (whole / 4 + 31) / 32 * 32;
   if (piece < 512) piece = 512;
   if (piece < rows) {
     b.piece_rows = (int)piece;
@@ -543,7 +544,7 @@ extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   a.dq = static_cast<__bf16*>(dq); a.dk = static_cast<__bf16*>(dk); a.dv = static_cast<__bf16*>(dv);
   a.aux = reinterpret_cast<float2*>(workspace);
   a.part = workspace + b.aux_floats;
-  a.seqs = {p->q_offsets, p->k_offsets, nullptr, p->sequences, p->q_rows, p->k_rows};
+  a.seqs = {p->q_offsets, p->k_offsets, nullptr, p->sequences, p->q_rows, p->k_rows, packed_levels(p, b.tiles, 512)};
   a.group = divisor((unsigned)(p->heads / p->kv_heads));
   a.kv_heads = p->kv_heads; a.D = p->head_dim; a.causal = p->causal;
   auto strides = [](const mdattn_strides* s) { return RowStrides{s->seq, s->head}; };
