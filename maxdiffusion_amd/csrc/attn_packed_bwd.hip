@@ -4,14 +4,17 @@
 //
 // Two passes, no atomics: every gradient is accumulated by the waves that own its rows.
 //   dq pass       a wave owns 32 rows of a group (head r % G of token r / G), their q and dout in registers, and walks the keys they see.
-//                 It leaves -lse (log2 units) and -delta of its rows, which start the MFMA chains that they are subtracted from.
-//   dk / dv pass  a wave owns 32 keys, their k and v in registers, and walks the rows that see them, of all heads of the group: the sum over
+//                 It leaves -lse / scale and -delta of its rows, which start the MFMA chains that they are subtracted from.
+//   dk / dv pass  a wave owns 32 keys, their k and v in registers, and walks the tokens that see them, head after head of the group: the sum over
 //                 the heads is the same accumulator.  S and dP are formed in both passes: seven matrix products where five are necessary.
 // Tiles of 32 rows pass through a ring of two slots in LDS, filled by direct global -> LDS loads.  Per tile, with the forward's fragments:
 // S^T or S and dP by row reads, then the accumulation by transposing reads; W = P or dS is packed to bf16 as the B operand it already is.
 // Blocks that no row of a wave sees, or no key of it is seen by, are not computed.
-// The dk / dv pass has a workgroup per 128 keys and head of k and v, of which the first ones of a causal sequence walk all of its rows: the rows
-// are cut into pieces, whose f32 sums a third kernel adds up in their order.
+// The dk / dv pass has a workgroup per 128 keys and head of k and v, of which the first ones of a causal sequence walk all of its tokens in every
+// head: these walks are cut into pieces, whose f32 sums a third kernel adds up in their order.
+#include <algorithm>
+#include <cmath>
+
 #include "attn_packed.h"
 
 namespace mdattn {
@@ -21,13 +24,13 @@ struct PackedBwdArgs {
   const __bf16 *q, *k, *v, *out, *dout;
   const float* lse;
   __bf16 *dq, *dk, *dv;
-  float2* aux;  // [kv_heads][q_rows * group]: -lse in log2 units and -delta
+  float* aux;  // [2][heads][q_rows]: -lse / scale, -delta
   PackedSeqs seqs;
   Divisor group;
   int kv_heads, D, causal;
   RowStrides qs, ks, vs, os, dqs, dks, dvs;
   float c, scale;
-  int pieces, piece_rows;  // of the dk / dv pass; piece_rows a multiple of 32
+  int pieces, piece_tiles;  // of the dk / dv pass, tiles of 32 tokens
   float* part;             // [piece][2][kv_heads][k_rows][D]
 };
 
@@ -166,8 +169,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   }
   ndelta = xhalf_sum(ndelta);
   const float lse = a.lse[(int64_t)(head * G + r - token * G) * a.seqs.q_rows + s.q0 + token];
-  const float nlse = lse == -INFINITY ? -INFINITY : -lse * kLog2e;  // rows that see no key: p = 0
-  if (hh == 0 && r0 + l32 < rows) a.aux[(int64_t)head * a.seqs.q_rows * G + (int64_t)s.q0 * G + r] = make_float2(nlse, ndelta);
+  // in front of the factor of the logits; rows that see no key: p = 0
+  const float nlse = lse == -INFINITY ? -INFINITY : -lse / a.scale;
+  if (hh == 0 && r0 + l32 < rows) {
+    float* to = a.aux + (int64_t)(head * G + r - token * G) * a.seqs.q_rows + s.q0 + token;
+    to[0] = nlse;
+    to[(int64_t)a.kv_heads * G * a.seqs.q_rows] = ndelta;
+  }
 
   f32x16 acc[ND];
 #pragma unroll
@@ -186,7 +194,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     };
     f32x16 S, dP;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) { S[i] = 0.f; dP[i] = ndelta; }
+    for (int i = 0; i < 16; ++i) { S[i] = nlse; dP[i] = ndelta; }
     bf16x8 win[LA];
 #pragma unroll
     for (int n = 0; n < LA; ++n) win[n] = frag(n);
@@ -210,8 +218,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
       unsigned pk[4];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * hb + e], c, nlse));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * hb + e + 1], c, nlse));
+        const float p0 = __builtin_amdgcn_exp2f(S[8 * hb + e] * c), p1 = __builtin_amdgcn_exp2f(S[8 * hb + e + 1] * c);
         pk[e >> 1] = pack2(p0 * dP[8 * hb + e], p1 * dP[8 * hb + e + 1]);  // (the factor `scale` is applied once, to the accumulators)
       }
       W[hb] = __builtin_bit_cast(bf16x8, u32x4{pk[0], pk[1], pk[2], pk[3]});
@@ -236,17 +243,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- dk, dv
-// The pieces of the rows that a tile of keys meets: the first row that sees one of its keys, of a tile of 32, and the first and the last piece
-// that hold any.
-struct KeyRows {
-  int first, begin, end;
+// What a tile of 128 keys meets: the tokens from `first` on, `tiles` tiles of 32 of them in each head; the walk over all heads in `pieces` pieces of
+// `each` tiles.
+struct KeyWalk {
+  int first, tiles, pieces, each;
 };
-__device__ __forceinline__ KeyRows key_rows(const SeqTile& s, int key0, int G, int causal, int piece_rows, int pieces) {
-  KeyRows k;
-  const int rows = s.m * G;
-  k.first = causal ? max(key0 - s.n + s.m, 0) * G & ~31 : 0;
-  k.begin = min(k.first / piece_rows, pieces - 1);
-  k.end = rows > 0 ? min((rows - 1) / piece_rows, pieces - 1) : k.begin;
+__device__ __forceinline__ KeyWalk key_walk(const SeqTile& s, int key0, int G, int causal, int piece_tiles, int pieces) {
+  KeyWalk k;
+  k.first = causal ? max(key0 - s.n + s.m, 0) & ~31 : 0;
+  k.tiles = (s.m - k.first + 31) >> 5;  // (none: no token)
+  const int walk = k.tiles * G;
+  k.pieces = min(max((walk + piece_tiles - 1) / piece_tiles, 1), pieces);
+  k.each = (walk + k.pieces - 1) / k.pieces;
   return k;
 }
 
@@ -261,8 +269,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   const int rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
   const SeqTile s = find_tile<BM, true>(a.seqs, G, rank, lane, a.seqs.levels);
   if (s.none) return;
-  const int rows = s.m * G, key0 = (s.tiles - 1 - s.tile) * BM, w0 = key0 + wave * 32;  // (causal: the first keys meet the most rows)
-  const int piece = a.pieces - 1 - blockIdx.y;                                            // (and the last rows the most keys)
+  const int key0 = (s.tiles - 1 - s.tile) * BM, w0 = key0 + wave * 32;  // (causal: the first keys meet the most tokens)
+  const int piece = blockIdx.y;
   if (s.gap) {
     if (piece) return;
     for (int i = tid; i < BM * (HD / 8); i += 256) {
@@ -274,46 +282,68 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     }
     return;
   }
-  const KeyRows kr = key_rows(s, key0, G, a.causal, a.piece_rows, a.pieces);
-  if (piece < kr.begin || piece > kr.end) return;
-  const int pb = max(kr.first, piece * a.piece_rows), pe = piece == a.pieces - 1 ? rows : min(rows, (piece + 1) * a.piece_rows);
-  const int nt = (pe - pb + 31) / 32;  // (no rows: none)
-  // the first row that sees a lane's key
-  const int from = a.causal ? max(min(w0 + l32, s.n - 1) - s.n + s.m, 0) * G : 0;
+  const KeyWalk kw = key_walk(s, key0, G, a.causal, a.piece_tiles, a.pieces);
+  if (piece >= kw.pieces) return;
+  const int begin = piece * kw.each, nt = min(kw.each, kw.tiles * G - begin);  // (no token: none; the last piece may be empty)
+  // the first token that sees a lane's key
+  const int from = a.causal ? max(min(w0 + l32, s.n - 1) - s.n + s.m, 0) : 0;
   const int none_below = __builtin_amdgcn_readlane(from, 0), all_from = __builtin_amdgcn_readlane(from, 31);
   const bool idle = w0 >= s.n;  // a wave without keys brings its share of the tiles
 
   const unsigned smem_addr = lds_addr_of(smem);
-  const __bf16* qp = a.q + (int64_t)s.q0 * a.qs.row + (int64_t)head * G * a.qs.head;
-  const __bf16* gp = a.dout + (int64_t)s.q0 * a.os.row + (int64_t)head * G * a.os.head;
-  const float* ap = reinterpret_cast<const float*>(a.aux + (int64_t)head * a.seqs.q_rows * G + (int64_t)s.q0 * G);
+  const int64_t aux_delta = (int64_t)a.kv_heads * G * a.seqs.q_rows;
   [[maybe_unused]] const uint64_t mask = __builtin_amdgcn_ballot_w64(!PADDED || T::chunk(lane, wave) * 8 < a.D);
   auto load = [&](auto... at) __attribute__((always_inline)) {
     if constexpr (PADDED) lds_dma16(at..., mask);
     else lds_dma16(at...);
   };
-  auto request = [&](int slot, int t) __attribute__((always_inline)) {
+  // the walk: head g of the group, tokens from token0 on
+  struct At {
+    int g, token0;
+  };
+  auto next = [&](At& at) __attribute__((always_inline)) {
+    at.token0 += 32;
+    if (at.token0 >= s.m) {
+      at.token0 = kw.first;
+      ++at.g;
+    }
+  };
+  auto request = [&](int slot, const At& at) __attribute__((always_inline)) {
     const unsigned Qs = smem_addr + (unsigned)(slot * kSlot), Gs = Qs + T::Bytes;
     int ln = lane;
     asm volatile("" : "+v"(ln));  // opaque: what follows from the lane is formed again for every tile, the accumulators need the registers
-    const int row0 = pb + t * 32, first = (int)div_by((unsigned)row0, a.group);
-    // wave 0: -lse and -delta of the 32 rows, interleaved, 64 floats behind the tiles (rows past the end repeat the last one)
-    if (wave == 0) lds_dma4(ap + 2 * (int64_t)row0, (unsigned)min(ln, 2 * (rows - row0 - 1) + (ln & 1)) * 4u, Qs + kAux);
-    const __bf16 *qt = qp + (int64_t)first * a.qs.row, *gt = gp + (int64_t)first * a.os.row;
+    const int64_t h = head * G + at.g, t0 = s.q0 + at.token0;
+    const int left = s.m - at.token0;  // tokens; those past the end repeat the last one
+    // wave 0: -lse / scale of the 32 tokens, then their -delta, 64 floats behind the tiles
+    if (wave == 0) {
+      const float* p = a.aux + h * a.seqs.q_rows + t0 + min(ln & 31, left - 1);
+      lds_dma4(ln < 32 ? p : p + aux_delta, Qs + kAux);
+    }
     const int c0 = T::chunk(ln, wave) * 8, col = !PADDED || c0 < a.D ? c0 : 0;
+    const __bf16 *qt = a.q + t0 * a.qs.row + h * a.qs.head, *gt = a.dout + t0 * a.os.row + h * a.os.head;
 #pragma unroll
     for (int i = 0; i < GPW; ++i) {
-      const int g = wave + 4 * i, r = min(row0 + T::RPI * g + T::row(ln), rows - 1), tk = (int)div_by((unsigned)r, a.group);
-      const int dt = tk - first, h = r - tk * G;
-      load(qt, (unsigned)(dt * (int)a.qs.row + h * (int)a.qs.head + col) * 2u, Qs + (unsigned)g * 1024u);
-      load(gt, (unsigned)(dt * (int)a.os.row + h * (int)a.os.head + col) * 2u, Gs + (unsigned)g * 1024u);
+      const int g = wave + 4 * i;
+      if (left >= 32) {
+        load(qt + (int64_t)(T::RPI * g) * a.qs.row, (unsigned)(T::row(ln) * (int)a.qs.row + col) * 2u, Qs + (unsigned)g * 1024u);
+        load(gt + (int64_t)(T::RPI * g) * a.os.row, (unsigned)(T::row(ln) * (int)a.os.row + col) * 2u, Gs + (unsigned)g * 1024u);
+      } else {
+        const int r = min(T::RPI * g + T::row(ln), left - 1);
+        load(qt, (unsigned)(r * (int)a.qs.row + col) * 2u, Qs + (unsigned)g * 1024u);
+        load(gt, (unsigned)(r * (int)a.os.row + col) * 2u, Gs + (unsigned)g * 1024u);
+      }
     }
   };
   if constexpr (PADDED) {  // chunks past the head dim: zeros that no load touches
     for (int i = tid * 16; i < 2 * kSlot; i += 4096) *reinterpret_cast<uint4*>(smem + i) = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
   }
-  if (nt > 0) request(0, 0);
+  At ahead{0, kw.first};
+  if (nt > 0) {
+    ahead.g = begin / kw.tiles;
+    ahead.token0 = kw.first + (begin - ahead.g * kw.tiles) * 32;
+    request(0, ahead);
+  }
   bf16x8 kf[NJ], vf[NJ];
   {
     const int64_t row = s.k0 + min(w0 + l32, s.n - 1);
@@ -332,7 +362,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   const float c = a.c;
   const unsigned row_at = T::row_at(lane), trans_at = T::trans_at(lane);
 
-  auto block = [&](unsigned at, int row0) __attribute__((always_inline)) {
+  auto block = [&](unsigned at, int token0) __attribute__((always_inline)) {
     auto aux4 = [&](int i) __attribute__((always_inline)) { return *(lds_f32x4_at)(at + (unsigned)(kAux + 4 * i)); };
     auto frag = [&](int n) __attribute__((always_inline)) {
       return n < NJ ? read_row_frag((at + row_at) ^ (unsigned)(32 * n)) : read_row_frag(((at + row_at) ^ (unsigned)(32 * (n - NJ))) + T::Bytes);
@@ -345,10 +375,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     f32x16 S, dP;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const f32x4 u0 = aux4(2 * (8 * g + 4 * hh)), u1 = aux4(2 * (8 * g + 4 * hh) + 4);
-      dP[4 * g] = u0[1]; dP[4 * g + 1] = u0[3]; dP[4 * g + 2] = u1[1]; dP[4 * g + 3] = u1[3];
+      const f32x4 u0 = aux4(8 * g + 4 * hh), u1 = aux4(32 + 8 * g + 4 * hh);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) S[4 * g + e] = 0.f;
+      for (int e = 0; e < 4; ++e) {
+        S[4 * g + e] = u0[e];
+        dP[4 * g + e] = u1[e];
+      }
     }
     if constexpr (LA1 > 0) {
       bf16x8 win[LA1];
@@ -367,29 +399,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 #pragma unroll
       for (int j = 0; j < NJ; ++j) dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(NJ + j), vf[j], dP, 0, 0, 0);
     }
-    if (row0 < all_from || row0 + 32 > pe) {  // rows that do not see the key, and rows past the end
+    if (token0 < all_from || token0 + 32 > s.m) {  // tokens that do not see the key, and what is behind the last
       asm volatile("" ::: "memory");  // keeps the branch
-      const int at0 = row0 + 4 * hh;
+      const int at0 = token0 + 4 * hh;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int row = at0 + 8 * (i >> 2) + (i & 3);
-        if (row < from || row >= pe) { S[i] = -INFINITY; dP[i] = 0.f; }
+        const int tk = at0 + 8 * (i >> 2) + (i & 3);
+        if (tk < from || tk >= s.m) { S[i] = -INFINITY; dP[i] = 0.f; }
       }
     }
     bf16x8 W[2], P[2];
 #pragma unroll
     for (int hb = 0; hb < 2; ++hb) {
-      float nl[8];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const f32x4 u0 = aux4(2 * (8 * (2 * hb + g) + 4 * hh)), u1 = aux4(2 * (8 * (2 * hb + g) + 4 * hh) + 4);
-        nl[4 * g] = u0[0]; nl[4 * g + 1] = u0[2]; nl[4 * g + 2] = u1[0]; nl[4 * g + 3] = u1[2];
-      }
       unsigned wpk[4], ppk[4];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * hb + e], c, nl[e]));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * hb + e + 1], c, nl[e + 1]));
+        const float p0 = __builtin_amdgcn_exp2f(S[8 * hb + e] * c), p1 = __builtin_amdgcn_exp2f(S[8 * hb + e + 1] * c);
         wpk[e >> 1] = pack2(p0 * dP[8 * hb + e], p1 * dP[8 * hb + e + 1]);
         ppk[e >> 1] = pack2(p0, p1);
       }
@@ -419,16 +444,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   for (int t = 0; t < nt; ++t) {
     __builtin_amdgcn_s_waitcnt(0x0F70);
     __syncthreads();
-    if (t + 1 < nt) request((t + 1) & 1, t + 1);
-    const int row0 = pb + t * 32;
-    const unsigned at = smem_addr + (unsigned)((t & 1) * kSlot);
-    if (!idle && row0 + 32 > none_below) block(at, row0);
+    const int token0 = ahead.token0;
+    if (t + 1 < nt) {
+      next(ahead);
+      request((t + 1) & 1, ahead);
+    }
+    if (!idle && token0 + 32 > none_below) block(smem_addr + (unsigned)((t & 1) * kSlot), token0);
   }
   __syncthreads();
   // the lane number once more: the loop has no register for it
   const int ln = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
   char* stage = smem + wave * kStageRows;
-  if (kr.begin != kr.end) {
+  if (kw.pieces > 1) {
     const int64_t tensor = (int64_t)a.kv_heads * a.seqs.k_rows * a.D, at = (int64_t)piece * 2 * tensor + ((int64_t)head * a.seqs.k_rows + s.k0) * a.D;
     store_partial<ND, PADDED>(dk, a.scale, a.part + at, w0, s.n, a.D, ln, stage);
     store_partial<ND, PADDED>(dv, 1.0f, a.part + at + tensor, w0, s.n, a.D, ln, stage);
@@ -448,8 +475,8 @@ __global__ __launch_bounds__(256) void packed_reduce_kernel(PackedBwdArgs a) {
   const SeqTile s = find_tile<128, true>(a.seqs, G, rank, lane, false);
   if (s.none || s.gap) return;
   const int key0 = s.tile * 128, cpr = a.D / 8;
-  const KeyRows kr = key_rows(s, key0, G, a.causal, a.piece_rows, a.pieces);
-  if (kr.begin == kr.end) return;
+  const KeyWalk kw = key_walk(s, key0, G, a.causal, a.piece_tiles, a.pieces);
+  if (kw.pieces == 1) return;
   const int64_t tensor = (int64_t)a.kv_heads * a.seqs.k_rows * a.D;
   const float* part = a.part + blockIdx.y * tensor + ((int64_t)head * a.seqs.k_rows + s.k0 + key0) * a.D;
   const RowStrides st = blockIdx.y ? a.dvs : a.dks;
@@ -457,9 +484,9 @@ __global__ __launch_bounds__(256) void packed_reduce_kernel(PackedBwdArgs a) {
   const int n = min(128, s.n - key0) * cpr;
   for (int i = threadIdx.x; i < n; i += 256) {
     float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const f32x4* p = reinterpret_cast<const f32x4*>(part + kr.begin * 2 * tensor) + 2 * i;
+    const f32x4* p = reinterpret_cast<const f32x4*>(part) + 2 * i;
 #pragma unroll 4
-    for (int k = kr.begin; k <= kr.end; ++k, p += tensor / 2) {
+    for (int k = 0; k < kw.pieces; ++k, p += tensor / 2) {
       const f32x4 u = p[0], v = p[1];
 #pragma unroll
       for (int e = 0; e < 4; ++e) { f[e] += u[e]; f[4 + e] += v[e]; }
@@ -471,24 +498,24 @@ __global__ __launch_bounds__(256) void packed_reduce_kernel(PackedBwdArgs a) {
 
 // How the dk / dv pass is cut, and the workspace: the rows' two numbers, then the pieces' sums.
 struct BwdPlan {
-  int pieces, piece_rows;
-  int64_t aux_floats, floats, tiles;  // tiles of the dk / dv pass
+  int pieces, piece_tiles;
+  int64_t aux_floats, floats, tiles;  // tiles: of 128 keys, of all heads
 };
 BwdPlan bwd_plan(const mdattn_packed* p) {
   const int64_t group = p->heads / p->kv_heads;
   const int64_t max_q = p->max_q > 0 && p->max_q < p->q_rows ? p->max_q : p->q_rows, max_k = p->max_k > 0 && p->max_k < p->k_rows ? p->max_k : p->k_rows;
   BwdPlan b{1, 1 << 30, 0, 0, 0};
   b.aux_floats = ((int64_t)p->q_rows * p->heads * 2 + 3) & ~(int64_t)3;
-  int64_t tiles = (max_k + 127) / 128 * p->sequences;
-  const int64_t most = p->k_rows / 128 + p->sequences, rows = max_q * group;
-  tiles = (tiles < most ? tiles : most) * p->kv_heads;
-  const int64_t whole = tiles * rows / (p->causal ? 2 : 1) / 512;  // rows per place on the chip
-  b.tiles = tiles;
-  int64_t piece = (whole / 4 + 31) / 32 * 32;
-  if (piece < 512) piece = 512;
-  if (piece < rows) {
-    b.piece_rows = (int)piece;
-    b.pieces = (int)((rows + piece - 1) / piece);
+  const int64_t tiles = (max_k + 127) / 128 * p->sequences, most = p->k_rows / 128 + p->sequences, walk = (max_q + 31) / 32 * group;
+  b.tiles = (tiles < most ? tiles : most) * p->kv_heads;
+  // Of what a place on the chip (512: two workgroups per CU) has to walk, a part: with n parts the last places end some 0.3 / n of the time
+  // late, and each part costs its sums' way to memory and back, 130 KB in each of the 512 places, as much as 15 tiles.
+  const double place = (double)b.tiles * walk / (p->causal ? 2 : 1) / 512;
+  int64_t piece = (int64_t)(place / std::max(1.0, std::sqrt(0.02 * place)));
+  if (piece < 16) piece = 16;
+  if (piece < walk) {
+    b.piece_tiles = (int)piece;
+    b.pieces = (int)((walk + piece - 1) / piece);
   }
   b.floats = b.aux_floats + (b.pieces > 1 ? (int64_t)b.pieces * 2 * p->k_rows * p->kv_heads * p->head_dim : 0);
   return b;
@@ -527,6 +554,7 @@ extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   const int rc = packed_sizes(p);
   if (rc != MDATTN_OK) return rc;
   if (!(scale > 0.f) || !(scale < INFINITY) || p->k_lengths) return MDATTN_E_BADARG;
+  if (scale < 1e-30f) return MDATTN_E_UNSUPPORTED;  // (lse / scale has to be a number)
   for (const mdattn_strides* s : {q_strides, k_strides, v_strides, o_strides, dq_strides, dk_strides, dv_strides}) {
     if (!s) return MDATTN_E_BADARG;
     if (!packed_strides_ok(s, s == q_strides || s == o_strides ? p->heads / p->kv_heads : 0)) return MDATTN_E_ALIGN;
@@ -542,7 +570,7 @@ extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   a.q = static_cast<const __bf16*>(q); a.k = static_cast<const __bf16*>(k); a.v = static_cast<const __bf16*>(v);
   a.out = static_cast<const __bf16*>(out); a.dout = static_cast<const __bf16*>(dout); a.lse = lse;
   a.dq = static_cast<__bf16*>(dq); a.dk = static_cast<__bf16*>(dk); a.dv = static_cast<__bf16*>(dv);
-  a.aux = reinterpret_cast<float2*>(workspace);
+  a.aux = workspace;
   a.part = workspace + b.aux_floats;
   a.seqs = {p->q_offsets, p->k_offsets, nullptr, p->sequences, p->q_rows, p->k_rows, packed_levels(p, b.tiles, 512)};
   a.group = divisor((unsigned)(p->heads / p->kv_heads));
@@ -551,7 +579,7 @@ extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   a.qs = strides(q_strides); a.ks = strides(k_strides); a.vs = strides(v_strides); a.os = strides(o_strides);
   a.dqs = strides(dq_strides); a.dks = strides(dk_strides); a.dvs = strides(dv_strides);
   a.c = scale * kLog2e; a.scale = scale;
-  a.pieces = b.pieces; a.piece_rows = b.piece_rows;
+  a.pieces = b.pieces; a.piece_tiles = b.piece_tiles;
   const int64_t dq_grid = p->q_rows ? packed_tiles((int64_t)p->q_rows * a.group.d, p->sequences, 128) * p->kv_heads : 0;
   const int64_t dkv_grid = p->k_rows ? packed_tiles(p->k_rows, p->sequences, 128) * p->kv_heads : 0;
   if (!grid_fits(dq_grid, 256) || !grid_fits(dkv_grid, 256) || b.pieces > 65535) return MDATTN_E_UNSUPPORTED;
