@@ -19,8 +19,9 @@ __device__ __forceinline__ unsigned div_by(unsigned n, const Divisor& d) { retur
 struct PackedSeqs {
   const int *q_off, *k_off, *k_len;
   int count, q_rows, k_rows;
-  int levels;  // see find_tile
+  int order, half;  // see find_tile
 };
+enum { kAsTheyCome, kCausal, kByLength };
 
 // A workgroup's tile of a sequence: rows q0 .. q0 + m of q, k0 .. k0 + n of k and v.  Gap: rows of no sequence (m of q, or n of k), to be
 // filled with zeros.
@@ -58,10 +59,12 @@ __device__ __forceinline__ int lane_sequence(const PackedSeqs& s, int group, int
   return i < s.count + 2 ? (int)(((unsigned)(KEYS ? n : m * group) + (BM - 1)) / BM) : 0;
 }
 
-// Tile `rank` of all sequences' tiles.  Every wave looks for itself, 64 sequences at a time, in their order, each one's last tile first.  levels (for
-// up to 62 sequences): all sequences' tiles by their number instead, the highest first.
+// Tile `rank` of all sequences' tiles.  Every wave looks for itself, 64 sequences at a time, in their order, each one's last tile first.  With an
+// order (of up to 62 sequences; see packed_order) the tiles go by what they meet, the most first: of a causal batch by their number, over all
+// sequences, of others by their sequence's length on the other side.  The second `half` of them, which share their CUs with the first, from
+// the other end.
 template <int BM, bool KEYS>
-__device__ __forceinline__ SeqTile find_tile(const PackedSeqs& s, int group, int rank, int lane, bool levels) {
+__device__ __forceinline__ SeqTile find_tile(const PackedSeqs& s, int group, int rank, int lane) {
   SeqTile t{};
   int before = 0;
   for (int i0 = 0; i0 < s.count + 2; i0 += 64) {
@@ -73,21 +76,27 @@ __device__ __forceinline__ SeqTile find_tile(const PackedSeqs& s, int group, int
       continue;
     }
     int j;
-    if (levels) {  // the highest number with more than `rank` tiles of it and above
-      auto above = [&](int level) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(wave_prefix_sum(max(tiles - level, 0)), 63); };
-      int lo = 0, hi = (int)(((unsigned)(KEYS ? s.k_rows : s.q_rows * group)) / BM) + 1;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (above(mid) > rank) lo = mid;
-        else hi = mid;
-      }
-      uint64_t here = __builtin_amdgcn_ballot_w64(tiles > lo);
-      for (int skip = rank - above(hi); skip > 0; --skip) here &= here - 1;
-      j = __builtin_ctzll(here);
-      t.tile = lo;
-    } else {
+    if (s.order == kAsTheyCome) {
       j = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + upto > rank));
       t.tile = before + __builtin_amdgcn_readlane(upto, j) - 1 - rank;
+    } else {
+      if (rank >= s.half && total <= 2 * s.half) rank = total - 1 - (rank - s.half);
+      // the tiles above a level: of each sequence those with a higher number, or all of them where its other side is longer
+      const bool causal = s.order == kCausal;
+      const int other = KEYS ? m : n;
+      auto above = [&](int level) __attribute__((always_inline)) { return causal ? max(tiles - level, 0) : other > level ? tiles : 0; };
+      // the highest level that, with what is above it, has more than `rank` tiles
+      int lo = -1, hi = causal ? (int)(((unsigned)(KEYS ? s.k_rows : s.q_rows * group)) / BM) + 1 : KEYS ? s.q_rows : s.k_rows;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__builtin_amdgcn_readlane(wave_prefix_sum(above(mid)), 63) > rank) lo = mid;
+        else hi = mid;
+      }
+      // of level lo, the tiles between those above it and those above hi
+      const int here = above(lo) - above(hi), sum = wave_prefix_sum(here);
+      const int at = rank - __builtin_amdgcn_readlane(wave_prefix_sum(above(hi)), 63);
+      j = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > at));
+      t.tile = causal ? lo : __builtin_amdgcn_readlane(sum, j) - 1 - at;
     }
     t.q0 = __builtin_amdgcn_readlane(qa, j);
     t.m = __builtin_amdgcn_readlane(m, j);
@@ -191,9 +200,11 @@ inline int packed_sizes(const mdattn_packed* p) {
 inline bool packed_aligned(const mdattn_packed* p) {
   return ((reinterpret_cast<uintptr_t>(p->q_offsets) | reinterpret_cast<uintptr_t>(p->k_offsets) | reinterpret_cast<uintptr_t>(p->k_lengths)) & 3) == 0;
 }
-// Whether the tiles of a call go by their number, over all sequences: of a causal batch the high ones meet the most keys, and what starts last
-// should be short.  Only where they do not all start at once: the search for one costs some 0.5 us.
-inline bool packed_levels(const mdattn_packed* p, int64_t tiles, int64_t places) { return p->causal && p->sequences > 1 && p->sequences <= 62 && tiles > places; }
+// Whether the tiles of a call go by what they meet: where they do not all have a CU of their own, what starts last should be short, and what shares a CU
+// with a long one too.  The search for a tile costs some 0.5 us.
+inline int packed_order(const mdattn_packed* p, int64_t tiles) {
+  return p->sequences == 0 || p->sequences > 62 || tiles <= 256 || (p->sequences == 1 && !p->causal) ? kAsTheyCome : p->causal ? kCausal : kByLength;
+}
 // tiles of BM rows that all sequences of `rows` rows have together at most, and the two gaps
 inline int64_t packed_tiles(int64_t rows, int64_t sequences, int BM) { return rows / BM + sequences + 2; }
 

@@ -11,6 +11,9 @@
 // s = -inf, in the blocks that hold such keys; blocks that no row of a wave sees are not computed.
 // Few rows (one or a few tokens) have a kernel of their own, bound by the keys' way from memory.
 // With few tiles the keys are cut into pieces besides; each leaves un-normalised f32 rows, joined by a third kernel in a fixed order.
+#include <algorithm>
+#include <type_traits>
+
 #include "attn_packed.h"
 
 namespace mdattn {
@@ -98,6 +101,43 @@ __device__ __forceinline__ void soft_block(const f32x16& S, float c, RowState& s
   st.l += sum;
 }
 
+// A wave's 32 rows from row r0 of the sequence on, normalised, rounded and stored as whole rows through `stage` (32 rows of kOutRow bytes that
+// nobody else touches any more): as the accumulators lie, a store would touch 16 bytes of each of 32 rows.
+template <int ND>
+constexpr int kOutRow = ND * 64 + 16;
+template <int ND, int DC, bool PADDED>
+__device__ __forceinline__ void store_out(const PackedArgs& a, const SeqTile& s, const f32x16 (&O)[ND], float l, float mc, int head, int r0, int lane,
+                                          char* stage) {
+  constexpr int RowB = kOutRow<ND>, LPR = ND == 3 ? 16 : ND * 4, RPI = 64 / LPR;  // lanes per row, rows per store
+  const int l32 = lane & 31, hh = lane >> 5, G = a.group.d, rows = s.m * G;
+  // rows that see no key give 0 and -inf; a sum that is not a number stays one
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  if (a.lse && hh == 0 && r0 + l32 < rows) {
+    const int t = (int)div_by((unsigned)(r0 + l32), a.group);
+    a.lse[(int64_t)(head * G + r0 + l32 - t * G) * a.seqs.q_rows + s.q0 + t] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * kLn2;
+  }
+#pragma unroll
+  for (int db = 0; db < ND; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uint2 u;
+      u.x = pack2(O[db][4 * g] * inv, O[db][4 * g + 1] * inv);
+      u.y = pack2(O[db][4 * g + 2] * inv, O[db][4 * g + 3] * inv);
+      *reinterpret_cast<uint2*>(stage + l32 * RowB + hh * 8 + (db * 32 + g * 8) * 2) = u;
+    }
+  // LDS accesses of one wave execute in order: the reads below see the writes above
+  const int rr = lane / LPR, cc = lane % LPR;
+  if (cc * 8 >= (PADDED ? a.D : DC)) return;
+#pragma unroll
+  for (int j = 0; j < 32 / RPI; ++j) {
+    const int row = r0 + j * RPI + rr;
+    if (row >= rows) break;
+    const int t = (int)div_by((unsigned)row, a.group);
+    st_nt(reinterpret_cast<uint4*>(a.out + (int64_t)(s.q0 + t) * a.os.row + (int64_t)(head * G + row - t * G) * a.os.head + cc * 8),
+          *reinterpret_cast<const uint4*>(stage + (j * RPI + rr) * RowB + cc * 16));
+  }
+}
+
 template <int HD, int DC, bool PADDED>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 4 : 3, HD == 64 ? 4 : 3))) void packed_fwd_kernel(PackedArgs a) {
   using T = PackedBlock<HD>;
@@ -110,7 +150,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 
   // neighbouring workgroups, which go to different dies, take different heads: with eight heads of k and v each die's L2 holds one of them
   const int rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
-  const SeqTile s = find_tile<F::BM, false>(a.seqs, G, rank, lane, a.seqs.levels);
+  const SeqTile s = find_tile<F::BM, false>(a.seqs, G, rank, lane);
   if (s.none) return;
   const int64_t group_rows = (int64_t)a.seqs.q_rows * G;
   const int tile = s.tile, rows = s.m * G, r0 = tile * F::BM + wave * 32;
@@ -277,33 +317,183 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
           *reinterpret_cast<f32x4*>(p + db * 32 + 8 * g) = f32x4{O[db][4 * g], O[db][4 * g + 1], O[db][4 * g + 2], O[db][4 * g + 3]};
     return;
   }
-  // rows that see no key give 0 and -inf; a sum that is not a number stays one
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  if (a.lse && hh == 0 && r0 + l32 < rows)
-    a.lse[(int64_t)(head * G + r - token * G) * a.seqs.q_rows + s.q0 + token] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * kLn2;
-  constexpr int RowB = ND * 64 + 16, LPR = ND == 3 ? 16 : ND * 4, RPI = 64 / LPR;  // a staged row; lanes per row, rows per store
-  static_assert(4 * 32 * RowB <= SLOTS * F::Slot, "the staged rows fit the ring");
-  char* stage = smem + wave * 32 * RowB;
-#pragma unroll
-  for (int db = 0; db < ND; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      uint2 u;
-      u.x = pack2(O[db][4 * g] * inv, O[db][4 * g + 1] * inv);
-      u.y = pack2(O[db][4 * g + 2] * inv, O[db][4 * g + 3] * inv);
-      *reinterpret_cast<uint2*>(stage + l32 * RowB + hh * 8 + (db * 32 + g * 8) * 2) = u;
-    }
-  // LDS accesses of one wave execute in order: the reads below see the writes above
-  const int rr = lane / LPR, cc = lane % LPR;
-  if (cc * 8 >= (PADDED ? a.D : DC)) return;
-#pragma unroll
-  for (int j = 0; j < 32 / RPI; ++j) {
-    const int row = r0 + j * RPI + rr;
-    if (row >= rows) break;
-    const int t = token_of(row);
-    st_nt(reinterpret_cast<uint4*>(a.out + (int64_t)(s.q0 + t) * a.os.row + (int64_t)(head * G + row - t * G) * a.os.head + cc * 8),
-          *reinterpret_cast<const uint4*>(stage + (j * RPI + rr) * RowB + cc * 16));
+  static_assert(4 * 32 * kOutRow<ND> <= SLOTS * F::Slot, "the staged rows fit the ring");
+  store_out<ND, DC, PADDED>(a, s, O, l, mc, head, r0, lane, smem + wave * 32 * kOutRow<ND>);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------- pipelined
+// The same for head dim 128, software-pipelined inside the wave: one instruction stream holds the eight PV products of key block b - 1, the eight
+// score products of block b + 1 and the softmax of block b, with a share of the softmax behind each product and the LDS read of a
+// fragment one product of its kind ahead of its use.  64 keys per slot, K(t) beside V(t - 1), in a ring of four slots (128 KB, a
+// workgroup per CU), whose loads are two slots ahead of their use; one barrier per 64 keys.  Blocks in front of the first and behind the last are
+// masked whole (P = 0) and walked like the others.
+constexpr int kPipeSlot = 4 * PackedBlock<128>::Bytes, kPipeHalf = 2 * PackedBlock<128>::Bytes, kPipeBytes = 4 * kPipeSlot;
+
+__device__ const u32x4 kZeros = {0u, 0u, 0u, 0u};
+
+template <int NW>
+__global__ __launch_bounds__(NW * 64) void packed_pipe_kernel(PackedArgs a) {
+  using T = PackedBlock<128>;
+  constexpr int BM = NW * 32, GPW = 16 / NW;  // row groups per wave, slot and tensor
+  constexpr int kFirst = 2;                   // the product behind which the softmax starts: the scores' last one has left the pipe
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
+  const SeqTile s = find_tile<BM, false>(a.seqs, G, rank, lane);
+  if (s.none) return;
+  if (s.gap) {
+    if (tid < 256) fill_gap<BM, 128>(a, s, head, tid);
+    return;
   }
+  const int rows = s.m * G, r0 = s.tile * BM + wave * 32;
+  auto token_of = [&](int r) __attribute__((always_inline)) { return (int)div_by((unsigned)r, a.group); };
+  const int r = min(r0 + l32, rows - 1), token = token_of(r);  // (rows past the end repeat the last one and are not stored)
+  auto sees = [&](int t) __attribute__((always_inline)) { return a.causal ? min(max(t + 1 + s.n - s.m, 0), s.n) : s.n; };
+  const int lim = sees(token), all = __builtin_amdgcn_readlane(lim, 0), some = __builtin_amdgcn_readlane(lim, 31);
+  const int nt = (sees(token_of(min(s.tile * BM + BM, rows) - 1)) + 63) / 64;  // slots that hold a key that some row of the workgroup sees
+
+  bf16x8 qf[8];
+  {
+    const __bf16* p = a.q + (int64_t)(s.q0 + token) * a.qs.row + (int64_t)(head * G + r - token * G) * a.qs.head + hh * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) qf[j] = *reinterpret_cast<const bf16x8*>(p + j * 16);
+  }
+  const __bf16* kp = a.k + (int64_t)s.k0 * a.ks.row + head * a.ks.head;
+  const __bf16* vp = a.v + (int64_t)s.k0 * a.vs.row + head * a.vs.head;
+  const unsigned smem_addr = lds_addr_of(smem);
+  const int grow = T::row(lane), col = T::chunk(lane, wave) * 8;  // (groups wave, wave + 4, ...: the swizzle sees the same)
+  const unsigned kofs = (unsigned)(grow * (int)a.ks.row + col) * 2u, vofs = (unsigned)(grow * (int)a.vs.row + col) * 2u;
+  auto request = [&](int slot, int t) __attribute__((always_inline)) {
+    const unsigned Ks = smem_addr + (unsigned)(slot * kPipeSlot), Vs = Ks + kPipeHalf;
+    if (t >= 1 && t * 64 + 64 <= s.n) {
+#pragma unroll
+      for (int i = 0; i < GPW; ++i) {
+        const int g = wave + NW * i;
+        lds_dma16(kp + (int64_t)(t * 64 + 4 * g) * a.ks.row, kofs, Ks + (unsigned)g * 1024u);
+        lds_dma16(vp + (int64_t)(t * 64 - 64 + 4 * g) * a.vs.row, vofs, Vs + (unsigned)g * 1024u);
+      }
+    } else {  // keys past the sequence's end repeat its last one and meet masked logits; V's rows outside it are zeros, which P = 0 meets
+#pragma unroll
+      for (int i = 0; i < GPW; ++i) {
+        const int g = wave + NW * i, row = t * 64 + 4 * g + grow;
+        const __bf16* v = (unsigned)(row - 64) < (unsigned)s.n ? vp + (int64_t)(row - 64) * a.vs.row + col : reinterpret_cast<const __bf16*>(&kZeros);
+        lds_dma16(kp + (int64_t)min(row, s.n - 1) * a.ks.row + col, Ks + (unsigned)g * 1024u);
+        lds_dma16(v, Vs + (unsigned)g * 1024u);
+      }
+    }
+  };
+  if (nt > 0) {
+    request(0, 0);
+    request(1, 1);
+    request(2, 2);
+  }
+  f32x16 O[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) O[db][i] = 0.f;
+  const float c = a.c;
+  RowState st{-1e30f, -1e30f * c, 0.f};
+  f32x16 Sa, Sb;        // logits of odd, even blocks
+  u32x4 Pa[2], Pb[2];   // probabilities of odd, even blocks as the PV product's operand
+  bf16x8 kf[2], vf[2];  // fragments read ahead
+#pragma unroll
+  for (int i = 0; i < 16; ++i) { Sa[i] = -INFINITY; Sb[i] = 0.f; }  // block -1
+#pragma unroll
+  for (int i = 0; i < 2; ++i) Pa[i] = Pb[i] = u32x4{0u, 0u, 0u, 0u};
+
+  const unsigned row_at = smem_addr + T::row_at(lane), trans_at = smem_addr + T::trans_at(lane);
+  // fragment j of K's block at byte `at` of the ring, jv of V's
+  auto k_frag = [&](int at, int j) __attribute__((always_inline)) { return read_row_frag((row_at ^ (unsigned)(32 * j)) + (unsigned)at); };
+  auto v_frag = [&](int at, int jv) __attribute__((always_inline)) {
+    const unsigned x = trans_at ^ (unsigned)(64 * (jv & 3));
+    return read_trans_frag(x + (unsigned)(at + (jv >> 2) * 16 * T::Row), (x ^ 32u) + (unsigned)(at + (8 + (jv >> 2) * 16) * T::Row));
+  };
+  // One block: the softmax of SC (block blk) into PC, the product of PP (blk - 1) with V at vc, the scores SN (blk + 1) from K at kc; kn, vn: the
+  // places of the next ones.
+  auto iter = [&](f32x16& SC, f32x16& SN, u32x4 (&PC)[2], u32x4 (&PP)[2], int kc, int kn, int vc, int vn, int blk) __attribute__((always_inline)) {
+    if (blk * 32 + 32 > all) {
+      asm volatile("" ::: "memory");  // keeps the branch
+      const int at0 = blk * 32 + 4 * hh;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (at0 + 8 * (i >> 2) + (i & 3) >= lim) SC[i] = -INFINITY;
+    }
+    float sum = 0.f, even = 0.f;
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+      const int j = n >> 1;
+      if ((n & 1) == 0) {
+        O[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j & 1], __builtin_bit_cast(bf16x8, PP[j >> 2]), O[j & 3], 0, 0, 0);
+        vf[(j + 1) & 1] = j < 7 ? v_frag(vc, j + 1) : v_frag(vn, 0);
+      } else {
+        if (j == 0) {
+          f32x16 z;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) z[i] = 0.f;
+          SN = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[0], qf[0], z, 0, 0, 0);
+        } else {
+          SN = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j & 1], qf[j], SN, 0, 0, 0);
+        }
+        kf[(j + 1) & 1] = j < 7 ? k_frag(kc, j + 1) : k_frag(kn, 0);
+      }
+      const int e0 = n < kFirst ? 0 : (n - kFirst) * 16 / (16 - kFirst), e1 = n < kFirst ? 0 : (n + 1 - kFirst) * 16 / (16 - kFirst);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (e < e0 || e >= e1) continue;
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(SC[e], c, -st.mc));
+        if ((e & 1) == 0) {
+          even = x;
+          asm volatile("" : "+v"(even));  // pins the work behind its product
+        } else {
+          unsigned pk = pack2(even, x);
+          sum = e == 1 ? even + x : sum + (even + x);
+          asm volatile("" : "+v"(pk), "+v"(sum));
+          PC[e >> 3][(e >> 1) & 3] = pk;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum <= kRange)) != 0, 0)) {  // (no product with V is on its way here)
+      bf16x8 P[2];
+      soft_block<4>(SC, c, st, O, P);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) PC[i] = __builtin_bit_cast(u32x4, P[i]);
+      sum = 0.f;
+    }
+    st.l += sum;
+  };
+
+  const int last = (some + 31) / 32;  // the block behind this wave's last: its iteration holds that one's product with V
+  auto period = [&](int t, auto slot) __attribute__((always_inline)) {
+    constexpr int cur = decltype(slot)::value * kPipeSlot, nxt = ((decltype(slot)::value + 1) & 3) * kPipeSlot, B = T::Bytes, H = kPipeHalf;
+    // slot t + 1 has landed, this wave's share and everyone's (the one requested after it may be on its way); slot t - 1 has been read
+    if (t + 2 <= nt) __builtin_amdgcn_s_waitcnt(0x0F70 | (2 * GPW));
+    else __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    if (2 * t - 1 <= last) iter(Sa, Sb, Pa, Pb, cur, cur + B, cur + H, cur + H + B, 2 * t - 1);
+    // in the middle of the period, where not all waves queue for it
+    if (t + 3 <= nt) request((decltype(slot)::value + 3) & 3, t + 3);
+    if (2 * t <= last) iter(Sb, Sa, Pb, Pa, cur + B, nxt, cur + H + B, nxt + H, 2 * t);
+  };
+  if (nt > 0) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    kf[0] = k_frag(0, 0);
+    vf[0] = v_frag(kPipeHalf, 0);
+    for (int t = 0; t <= nt; t += 4) {
+      period(t, std::integral_constant<int, 0>{});
+      if (t + 1 > nt) break;
+      period(t + 1, std::integral_constant<int, 1>{});
+      if (t + 2 > nt) break;
+      period(t + 2, std::integral_constant<int, 2>{});
+      if (t + 3 > nt) break;
+      period(t + 3, std::integral_constant<int, 3>{});
+    }
+  }
+  __syncthreads();  // every wave has finished reading the ring, and no load into it is in flight: it now stages the output
+  store_out<4, 128, false>(a, s, O, xhalf_sum(st.l), st.mc, head, r0, lane, smem + wave * 32 * kOutRow<4>);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- few rows
@@ -524,47 +714,73 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(PackedArgs a) {
 
 // How a call is launched.
 struct FwdPlan {
-  bool few;
-  int pieces, piece_keys;
-  int64_t floats, tiles;  // tiles: of rows, of all heads
+  int kind, pieces, piece_keys;
+  int64_t floats, tiles;  // tiles: of 128 rows (few rows: 32), of all heads
+  void cut(const mdattn_packed* p, int64_t max_k, int64_t keys) {
+    keys = (std::max(keys, (max_k + kMaxPieces - 1) / kMaxPieces) + 127) / 128 * 128;
+    const int64_t n = (max_k + keys - 1) / keys;
+    if (n < 2) return;
+    pieces = (int)n;
+    piece_keys = (int)keys;
+    floats = n * p->q_rows * p->heads * (p->head_dim + 2);
+  }
 };
+enum { kFew, kFlat, kPipe4, kPipe8 };
 FwdPlan fwd_plan(const mdattn_packed* p) {
   const int64_t group = p->heads / p->kv_heads;
   const int64_t max_q = p->max_q > 0 && p->max_q < p->q_rows ? p->max_q : p->q_rows, max_k = p->max_k > 0 && p->max_k < p->k_rows ? p->max_k : p->k_rows;
+  FwdPlan f{kFlat, 1, 1 << 30, 0, 0};
   // (the list of all tiles' pieces is counted in 31 bits)
-  FwdPlan f{max_q * group <= 32 && packed_tiles(p->q_rows * group, p->sequences, 32) * kMaxPieces * p->kv_heads < (1ll << 31), 1, 1 << 30, 0, 0};
-  const int bm = f.few ? 32 : 128;
+  if (max_q * group <= 32 && packed_tiles(p->q_rows * group, p->sequences, 32) * kMaxPieces * p->kv_heads < (1ll << 31)) f.kind = kFew;
+  const int bm = f.kind == kFew ? 32 : 128;
   // tiles that there are: of the tokens, or of so many sequences of the longest one's
-  int64_t tiles = (max_q * group + bm - 1) / bm * p->sequences;
-  const int64_t most = p->q_rows * group / bm + p->sequences;
-  f.tiles = tiles = (tiles < most ? tiles : most) * p->kv_heads;
-  const int64_t least = f.few ? 256 : 512;
-  if (tiles <= 0 || max_k < 2 * least) return f;
-  int64_t keys;
-  if (f.few) {
-    const int64_t all = max_k * p->sequences < p->k_rows ? max_k * p->sequences : p->k_rows;
-    keys = all * p->kv_heads / 2048;
-  } else {
-    if (tiles >= 256) return f;
-    keys = max_k * tiles / 512;
+  f.tiles = std::min((max_q * group + bm - 1) / bm * p->sequences, p->q_rows * group / bm + p->sequences) * p->kv_heads;
+  if (f.kind == kFew) {
+    const int64_t all = std::min(max_k * p->sequences, (int64_t)p->k_rows) * p->kv_heads;
+    if (max_k >= 512) f.cut(p, max_k, std::max<int64_t>(all / 2048, 256));
+    return f;
   }
-  if (keys < least) keys = least;
-  if (keys * kMaxPieces < max_k) keys = (max_k + kMaxPieces - 1) / kMaxPieces;
-  keys = (keys + 127) / 128 * 128;
-  const int64_t pieces = (max_k + keys - 1) / keys;
-  if (pieces < 2) return f;
-  f.piece_keys = (int)keys;
-  f.pieces = (int)pieces;
-  f.floats = pieces * p->q_rows * p->heads * (p->head_dim + 2);
+  const int64_t blocks = (max_k + 31) / 32;
+  if (f.tiles > 256) {
+    // (tiles of 256 rows that fill their last round)
+    const int64_t rounds = (f.tiles + 511) / 512;
+    if (p->head_dim == 128 && !p->causal && blocks >= 128 && f.tiles >= rounds * 480) f.kind = kPipe8;
+    return f;
+  }
+  const bool pipe = p->head_dim == 128;
+  if (pipe) f.kind = kPipe4;
+  // Alone on its CU a workgroup takes so many us per block of 32 keys; in n pieces, of the flat schedule, one n-th of them, and their rows go to
+  // memory and back, at some 4 TB/s, through a launch of 5 us.
+  const double row_us = (double)p->q_rows * p->heads * p->head_dim * 4 * 2 / 4e6 * (p->causal ? 0.6 : 1.0);
+  double best = 0.95 * blocks * (pipe ? 0.56 : 0.75);
+  int64_t pieces = 1;
+  for (int64_t n = 2; n <= 16 && blocks / n >= 16 && f.tiles * n <= 512; ++n) {
+    const double us = (double)blocks / n * (f.tiles * n <= 256 ? 0.75 : 1.06) + n * row_us + 5;
+    if (us < best) { best = us; pieces = n; }
+  }
+  if (pieces > 1) {
+    f.kind = kFlat;
+    f.cut(p, max_k, (max_k + pieces - 1) / pieces);
+  }
   return f;
 }
 
+template <int NW>
+int launch_pipe(hipStream_t st, const PackedArgs& a, int64_t grid) {
+  static LdsOptIn opted;
+  if (lds_opt_in(opted, reinterpret_cast<const void*>(packed_pipe_kernel<NW>), kPipeBytes) != MDATTN_OK) return MDATTN_E_LAUNCH;
+  MDATTN_LAUNCH(packed_pipe_kernel<NW>, dim3((unsigned)grid), dim3(NW * 64), kPipeBytes, st, a);
+  return launch_status();
+}
+
 template <int HD, int DC, bool PADDED>
-int launch(hipStream_t st, const PackedArgs& a, bool few, int64_t grid) {
-  if (few) {
+int launch(hipStream_t st, const PackedArgs& a, int kind, int64_t grid) {
+  if (kind == kFew) {
     MDATTN_LAUNCH((packed_few_kernel<HD, DC, PADDED>), dim3((unsigned)grid), dim3(256), few_bytes<HD>(), st, a);
-  } else {
+  } else if (kind == kFlat || HD != 128 || PADDED) {
     MDATTN_LAUNCH((packed_fwd_kernel<HD, DC, PADDED>), dim3((unsigned)grid, (unsigned)a.pieces), dim3(256), FwdShape<HD>::SLOTS * FwdShape<HD>::Slot, st, a);
+  } else {
+    return kind == kPipe4 ? launch_pipe<4>(st, a, grid) : launch_pipe<8>(st, a, grid);
   }
   return launch_status();
 }
@@ -590,7 +806,7 @@ extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, cons
       !packed_strides_ok(q_strides) || !packed_strides_ok(k_strides) || !packed_strides_ok(v_strides) || !packed_strides_ok(o_strides))
     return MDATTN_E_ALIGN;
   FwdPlan f = fwd_plan(p);
-  if (f.pieces > 1 && (!workspace || workspace_floats < f.floats)) {
+  if (f.pieces > 1 && (!workspace || workspace_floats < f.floats)) {  // (flat or few rows)
     f.pieces = 1;
     f.piece_keys = 1 << 30;
   } else if (f.pieces > 1 && !aligned16(workspace)) {
@@ -599,7 +815,7 @@ extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   PackedArgs a{};
   a.q = static_cast<const __bf16*>(q); a.k = static_cast<const __bf16*>(k); a.v = static_cast<const __bf16*>(v);
   a.out = static_cast<__bf16*>(out); a.lse = lse;
-  a.seqs = {p->q_offsets, p->k_offsets, p->k_lengths, p->sequences, p->q_rows, p->k_rows, !f.few && packed_levels(p, f.tiles, 768)};
+  a.seqs = {p->q_offsets, p->k_offsets, p->k_lengths, p->sequences, p->q_rows, p->k_rows, f.kind == kFew ? kAsTheyCome : packed_order(p, f.tiles), 256 / p->kv_heads};
   a.group = divisor((unsigned)(p->heads / p->kv_heads));
   a.kv_heads = p->kv_heads; a.D = p->head_dim; a.causal = p->causal;
   a.qs = {q_strides->seq, q_strides->head}; a.ks = {k_strides->seq, k_strides->head};
@@ -611,18 +827,18 @@ extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, cons
     a.part = workspace;
     a.ml = reinterpret_cast<float2*>(workspace + f.pieces * rows * a.D);
   }
-  int64_t grid = packed_tiles(group_rows, p->sequences, f.few ? 32 : 128) * p->kv_heads;
-  if (f.few) {  // two per CU, in whole rounds of the heads, walk what there is
+  int64_t grid = packed_tiles(group_rows, p->sequences, f.kind == kFew ? 32 : f.kind == kPipe8 ? 256 : 128) * p->kv_heads;
+  if (f.kind == kFew) {  // two per CU, in whole rounds of the heads, walk what there is
     const int64_t most = (512 + a.kv_heads - 1) / a.kv_heads * a.kv_heads;
     grid = grid * f.pieces < most ? grid * f.pieces : most;
   }
-  if (!grid_fits(grid, 256) || (f.pieces > 1 && !grid_fits(rows, 256))) return MDATTN_E_UNSUPPORTED;
+  if (!grid_fits(grid, f.kind == kPipe8 ? 512 : 256) || (f.pieces > 1 && !grid_fits(rows, 256))) return MDATTN_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
-  const int status = a.D == 64   ? launch<64, 64, false>(st, a, f.few, grid)
-                     : a.D < 64  ? launch<64, 64, true>(st, a, f.few, grid)
-                     : a.D <= 96 ? launch<128, 96, true>(st, a, f.few, grid)
-                     : a.D < 128 ? launch<128, 128, true>(st, a, f.few, grid)
-                                 : launch<128, 128, false>(st, a, f.few, grid);
+  const int status = a.D == 64   ? launch<64, 64, false>(st, a, f.kind, grid)
+                     : a.D < 64  ? launch<64, 64, true>(st, a, f.kind, grid)
+                     : a.D <= 96 ? launch<128, 96, true>(st, a, f.kind, grid)
+                     : a.D < 128 ? launch<128, 128, true>(st, a, f.kind, grid)
+                                 : launch<128, 128, false>(st, a, f.kind, grid);
   if (status != MDATTN_OK || f.pieces == 1) return status;
   MDATTN_LAUNCH(packed_combine_kernel, dim3((unsigned)rows), dim3(256), 0, st, a);
   return launch_status();

@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
-  const SeqTile s = find_tile<BM, false>(a.seqs, G, rank, lane, a.seqs.levels);
+  const SeqTile s = find_tile<BM, false>(a.seqs, G, rank, lane);
   if (s.none) return;
   const int tile = s.tile, rows = s.m * G, r0 = tile * BM + wave * 32;
   auto token_of = [&](int r) __attribute__((always_inline)) { return (int)div_by((unsigned)r, a.group); };
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
-  const SeqTile s = find_tile<BM, true>(a.seqs, G, rank, lane, a.seqs.levels);
+  const SeqTile s = find_tile<BM, true>(a.seqs, G, rank, lane);
   if (s.none) return;
   const int key0 = (s.tiles - 1 - s.tile) * BM, w0 = key0 + wave * 32;  // (causal: the first keys meet the most tokens)
   const int piece = blockIdx.y;
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 // The pieces' sums of dk (blockIdx.y 0) and dv (1), added in their order, for the tiles of 128 keys whose rows were cut.
 __global__ __launch_bounds__(256) void packed_reduce_kernel(PackedBwdArgs a) {
   const int lane = threadIdx.x & 63, rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
-  const SeqTile s = find_tile<128, true>(a.seqs, G, rank, lane, false);
+  const SeqTile s = find_tile<128, true>(a.seqs, G, rank, lane);
   if (s.none || s.gap) return;
   const int key0 = s.tile * 128, cpr = a.D / 8;
   const KeyWalk kw = key_walk(s, key0, G, a.causal, a.piece_tiles, a.pieces);
@@ -572,7 +572,7 @@ extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   a.dq = static_cast<__bf16*>(dq); a.dk = static_cast<__bf16*>(dk); a.dv = static_cast<__bf16*>(dv);
   a.aux = workspace;
   a.part = workspace + b.aux_floats;
-  a.seqs = {p->q_offsets, p->k_offsets, nullptr, p->sequences, p->q_rows, p->k_rows, packed_levels(p, b.tiles, 512)};
+  a.seqs = {p->q_offsets, p->k_offsets, nullptr, p->sequences, p->q_rows, p->k_rows, packed_order(p, b.tiles), 256 / p->kv_heads};
   a.group = divisor((unsigned)(p->heads / p->kv_heads));
   a.kv_heads = p->kv_heads; a.D = p->head_dim; a.causal = p->causal;
   auto strides = [](const mdattn_strides* s) { return RowStrides{s->seq, s->head}; };

@@ -18,6 +18,7 @@
 
 #include <array>
 #include <cmath>
+#include <cstring>
 #include <optional>
 
 #include "mdattn.h"
@@ -55,6 +56,31 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// A node's plain values as one entry of its saved_data (an entry each, boxed, cost a small backward call a few us)
+template <class T>
+void keep(AutogradContext* ctx, const T& values) {
+  static_assert(std::is_trivially_copyable_v<T>);
+  ctx->saved_data["values"] = std::string(reinterpret_cast<const char*>(&values), sizeof values);
+}
+template <class T>
+T kept(AutogradContext* ctx) {
+  T values;
+  const std::string& s = ctx->saved_data["values"].toStringRef();
+  TORCH_INTERNAL_ASSERT(s.size() == sizeof values);
+  std::memcpy(&values, s.data(), sizeof values);
+  return values;
+}
+// a tensor's shape of up to eight axes
+struct Shape8 {
+  int64_t dim = 0, size[8];
+  explicit Shape8(const Tensor& t = Tensor()) {
+    if (!t.defined()) return;
+    dim = t.dim();
+    for (int64_t i = 0; i < dim && i < 8; ++i) size[i] = t.size(i);
+  }
+  at::IntArrayRef get() const { return {size, (size_t)dim}; }
+};
+
 // what a saved-tensor hook hands back is read with the form that the forward checked, or refused
 void unpacked(bool ok) { TORCH_CHECK_VALUE(ok, "a tensor saved for the backward pass came back from its hook with another dtype, shape or layout"); }
 // a backward call: _lib.check(rc, where), whose MdattnError autograd's engine carries back to the thread that waits for it
@@ -378,6 +404,13 @@ int packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const mdattn_p
   return mdattn_fwd_bf16_packed(stream(q), &p, ptr(q), ptr(k), ptr(v), mut(out), f32(lse), &sq, &sk, &sv, &so, (float)scale, f32(ws), nws);
 }
 struct PackedFn : FirstOrder<PackedFn> {
+  struct Values {
+    double scale;
+    bool causal;
+    int64_t max_q, max_k;
+    Shape8 q, k;
+    int64_t offsets;
+  };
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qo, const Tensor& ko, bool causal,
                         double scale, int64_t max_q, int64_t max_k) {
     mdattn_packed p;
@@ -385,17 +418,15 @@ struct PackedFn : FirstOrder<PackedFn> {
     Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
     if (packed_fwd(q, k, v, p, scale, out, lse) != MDATTN_OK) throw Refused{};
     ctx->save_for_backward({q, k, v, qo, ko, out, lse});
-    ctx->saved_data["i"] = c10::List<int64_t>({causal, max_q, max_k, q.size(0), q.size(1), q.size(2), k.size(0), k.size(1), qo.size(0)});
-    ctx->saved_data["scale"] = scale;
+    keep(ctx, Values{scale, causal, max_q, max_k, Shape8(q), Shape8(k), qo.size(0)});
     return out;
   }
   static variable_list gradients(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const auto i = ctx->saved_data["i"].toIntVector();
+    const Values c = kept<Values>(ctx);
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &qo = saved[3], &ko = saved[4], &out = saved[5], &lse = saved[6];
     mdattn_packed p;
-    unpacked(packed_args(q, k, v, qo, ko, Tensor(), i[0], i[1], i[2], p) && q.sizes() == at::IntArrayRef({i[3], i[4], i[5]}) &&
-             k.sizes() == at::IntArrayRef({i[6], i[7], i[5]}) && qo.size(0) == i[8] && bf16_on(out, q) && out.is_contiguous() && out.sizes() == q.sizes() &&
+    unpacked(packed_args(q, k, v, qo, ko, Tensor(), c.causal, c.max_q, c.max_k, p) && q.sizes() == c.q.get() && k.sizes() == c.k.get() && qo.size(0) == c.offsets && bf16_on(out, q) && out.is_contiguous() && out.sizes() == q.sizes() &&
              aligned(out) && lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
              lse.numel() == q.size(0) * q.size(1));
     Tensor dout = grads[0];
@@ -408,7 +439,7 @@ struct PackedFn : FirstOrder<PackedFn> {
     const Tensor ws = at::empty({nws}, lse.options());
     const mdattn_strides sq = row_strides(q), sk = row_strides(k), sv = row_strides(v), so = row_strides(out), dqs = row_strides(dq), dks = row_strides(dk);
     must(mdattn_bwd_bf16_packed(stream(q), &p, ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), f32(lse), mut(dq), mut(dk), mut(dv), &sq, &sk, &sv, &so, &dqs, &dks,
-                                &dks, (float)ctx->saved_data["scale"].toDouble(), f32(ws), nws),
+                                &dks, (float)c.scale, f32(ws), nws),
          "mdattn_bwd_bf16_packed");
     return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -957,6 +988,13 @@ variable_list rms_run(const Tensor& x, const Rows3& r, const Tensor& w, const Te
 }
 // Saved for the backward: s (x, without a residual) and w; of b only its shape and type.
 struct RmsFn : FirstOrder<RmsFn> {
+  struct Values {
+    double eps, offset;
+    int64_t stride;
+    int vectors_f32, s_f32, x_f32;
+    bool w, b, vectors, residual;  // which there are; whether the vectors' gradients are wanted
+    Shape8 x, w_shape, b_shape;
+  };
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w_, const OptTensor& b_, const OptTensor& res_, double eps, double offset) {
     const Tensor w = value(w_), b = value(b_), res = value(res_);
     const Rows3 r = *as_rows(x);
@@ -969,12 +1007,8 @@ struct RmsFn : FirstOrder<RmsFn> {
     if (out.empty()) throw Refused{};
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({res.defined() ? out[1] : x, w});
-    ctx->saved_data["f"] = c10::List<double>({eps, offset});
-    ctx->saved_data["i"] = c10::List<int64_t>({stride, f32, w.defined(), b.defined(), (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()),
-                                               is_f32(res.defined() ? res : x), is_f32(x), res.defined()});
-    ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["wshape"] = w.defined() ? w.sizes().vec() : std::vector<int64_t>{};
-    ctx->saved_data["bshape"] = b.defined() ? b.sizes().vec() : std::vector<int64_t>{};
+    keep(ctx, Values{eps, offset, stride, f32, is_f32(res.defined() ? res : x), is_f32(x), w.defined(), b.defined(),
+                     (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()), res.defined(), Shape8(x), Shape8(w), Shape8(b)});
     return out;
   }
   // a gradient as rows of the wanted type
@@ -989,26 +1023,24 @@ struct RmsFn : FirstOrder<RmsFn> {
   }
   static variable_list gradients(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const auto f = ctx->saved_data["f"].toDoubleVector();
-    const auto i = ctx->saved_data["i"].toIntVector();
+    const Values c = kept<Values>(ctx);
     const Tensor &s = saved[0], &w = saved[1];
     const auto r = as_rows(s);
-    unpacked(r && float_on(s, s) && is_f32(s) == (int)i[5] && s.sizes() == at::IntArrayRef(ctx->saved_data["shape"].toIntVector()) && w.defined() == (bool)i[2] &&
-             (!w.defined() || (float_on(w, s) && is_f32(w) == (int)i[1] && w.is_contiguous() && w.sizes() == at::IntArrayRef(ctx->saved_data["wshape"].toIntVector()))));
-    const auto g_type = i[6] ? at::kFloat : at::kBFloat16;
-    Tensor g = grads[0].defined() ? grads[0] : at::zeros(s.sizes(), s.options().dtype(g_type)), gs = i[7] ? grads[1] : Tensor();
+    unpacked(r && float_on(s, s) && is_f32(s) == c.s_f32 && s.sizes() == c.x.get() && w.defined() == c.w &&
+             (!c.w || (float_on(w, s) && is_f32(w) == c.vectors_f32 && w.is_contiguous() && w.sizes() == c.w_shape.get())));
+    const auto g_type = c.x_f32 ? at::kFloat : at::kBFloat16;
+    Tensor g = grads[0].defined() ? grads[0] : at::zeros(s.sizes(), s.options().dtype(g_type)), gs = c.residual ? grads[1] : Tensor();
     const Rows3 rg = as_gradient(g, g_type), rs = gs.defined() ? as_gradient(gs, s.scalar_type()) : Rows3{};
-    const bool vectors = i[4], narrow = i[5] != i[6];
-    const auto vec = s.options().dtype(i[1] ? at::kFloat : at::kBFloat16);
+    const bool narrow = c.s_f32 != c.x_f32;
+    const auto vec = s.options().dtype(c.vectors_f32 ? at::kFloat : at::kBFloat16);
     Tensor ds = at::empty(s.sizes(), s.options()), dx = narrow ? at::empty(s.sizes(), s.options().dtype(at::kBFloat16)) : Tensor();
-    Tensor dw = vectors && i[2] ? at::empty(ctx->saved_data["wshape"].toIntVector(), vec) : Tensor();
-    Tensor db = vectors && i[3] ? at::empty(ctx->saved_data["bshape"].toIntVector(), vec) : Tensor();
+    Tensor dw = c.vectors && c.w ? at::empty(c.w_shape.get(), vec) : Tensor(), db = c.vectors && c.b ? at::empty(c.b_shape.get(), vec) : Tensor();
     const int64_t nws = dw.defined() || db.defined() ? mdattn_rms_norm_bwd_workspace_floats(r->groups, r->rows, (int)r->c) : 0;
     const Tensor ws = nws ? at::empty({nws}, s.options().dtype(at::kFloat)) : Tensor();
-    must(mdattn_rms_norm_bwd(stream(s), ptr(s), is_f32(s), ptr(g), is_f32(g), ptr(gs), mut(ds), mut(dx), ptr(w), mut(dw), mut(db), (int)i[1], r->groups, r->rows,
-                             (int)r->c, r->sg, r->sr, rg.sg, rg.sr, rs.sg, rs.sr, i[0], (float)f[0], (float)f[1], f32(ws), nws),
+    must(mdattn_rms_norm_bwd(stream(s), ptr(s), is_f32(s), ptr(g), is_f32(g), ptr(gs), mut(ds), mut(dx), ptr(w), mut(dw), mut(db), c.vectors_f32, r->groups,
+                             r->rows, (int)r->c, r->sg, r->sr, rg.sg, rg.sr, rs.sg, rs.sr, c.stride, (float)c.eps, (float)c.offset, f32(ws), nws),
          "mdattn_rms_norm_bwd");
-    return {narrow ? dx : ds, dw, db, i[7] ? ds : Tensor(), Tensor(), Tensor()};
+    return {narrow ? dx : ds, dw, db, c.residual ? ds : Tensor(), Tensor(), Tensor()};
   }
 };
 std::optional<variable_list> rms_norm(const Tensor& x, const OptTensor& w_, const OptTensor& b_, const OptTensor& res_, double eps, double offset) {
@@ -1019,7 +1051,10 @@ std::optional<variable_list> rms_norm(const Tensor& x, const OptTensor& w_, cons
   if (!x.is_cuda() || !float_on(x, x)) return std::nullopt;
   const auto r = as_rows(x);
   if (!r || !norm_vectors(x, *r, w, b, stride, f32) || !residual_rows(x, res, rr)) return std::nullopt;
-  if (wants_grad({&x, &w, &b, &res})) return unless_refused([&] { return RmsFn::apply(x, w_, b_, res_, eps, offset); });
+  if (wants_grad({&x, &w, &b, &res})) {
+    if (x.dim() > 8) return std::nullopt;
+    return unless_refused([&] { return RmsFn::apply(x, w_, b_, res_, eps, offset); });
+  }
   at::NoGradGuard guard;
   variable_list out = rms_run(x, *r, w, b, res, rr, stride, f32, eps, offset);
   if (out.empty()) return std::nullopt;
