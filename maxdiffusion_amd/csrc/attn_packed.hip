@@ -101,6 +101,16 @@ __device__ __forceinline__ void soft_block(const f32x16& S, float c, RowState& s
   st.l += sum;
 }
 
+// A row's fragments straight from memory, waited for here, with what is on its way into LDS: in the loop behind, the compiler would wait for them in
+// every block of keys, and with that for the keys requested since (16,384 tokens x 32 heads 1,895 -> @@ us).
+template <int NJ, bool PADDED>
+__device__ __forceinline__ void load_row(bf16x8 (&f)[NJ], const __bf16* p, int hh, int D) {
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) f[j] = !PADDED || j * 16 + hh * 8 < D ? *reinterpret_cast<const bf16x8*>(p + j * 16) : __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) asm volatile("" : "+v"(f[j]));
+}
+
 // A wave's 32 rows from row r0 of the sequence on, normalised, rounded and stored as whole rows through `stage` (32 rows of kOutRow bytes that
 // nobody else touches any more): as the accumulators lie, a store would touch 16 bytes of each of 32 rows.
 template <int ND>
@@ -209,14 +219,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     for (int i = tid * 16; i < SLOTS * F::Slot; i += 4096) *reinterpret_cast<uint4*>(smem + i) = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
   }
-  bf16x8 qf[NJ];
-  {
-    const __bf16* p = a.q + (int64_t)(s.q0 + token) * a.qs.row + (int64_t)(head * G + r - token * G) * a.qs.head + hh * 8;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      qf[j] = !PADDED || j * 16 + hh * 8 < a.D ? *reinterpret_cast<const bf16x8*>(p + j * 16) : __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
-  }
-
+  for (int t = 0; t < SLOTS - 1; ++t)
+    if (t < nt) request(t, t);
+  bf16x8 qf[NJ];
+  load_row<NJ, PADDED>(qf, a.q + (int64_t)(s.q0 + token) * a.qs.row + (int64_t)(head * G + r - token * G) * a.qs.head + hh * 8, hh, a.D);
   f32x16 O[ND];
 #pragma unroll
   for (int db = 0; db < ND; ++db)
@@ -280,9 +287,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     __builtin_amdgcn_s_setprio(0);
   };
 
-#pragma unroll
-  for (int t = 0; t < SLOTS - 1; ++t)
-    if (t < nt) request(t, t);
   int slot = 0, fill = SLOTS - 1;
   for (int t = 0; t < nt; ++t) {
     // this wave's share of slot t has landed (the SLOTS - 2 slots requested after it may be on their way), and everyone's; the slot
@@ -558,13 +562,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
         else lds_dma16(at, to + (unsigned)i * 1024u);
       }
     };
-    bf16x8 qf[NJ];
-    {
-      const __bf16* p = a.q + (int64_t)(s.q0 + token) * a.qs.row + (int64_t)(head * G + r - token * G) * a.qs.head + hh * 8;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        qf[j] = !PADDED || j * 16 + hh * 8 < a.D ? *reinterpret_cast<const bf16x8*>(p + j * 16) : __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
-    }
     if constexpr (PADDED) {  // chunks past the head dim: zeros that no load touches
       for (int i = lane * 16; i < 2 * T::Bytes; i += 1024) *reinterpret_cast<uint4*>(smem + wave * 2 * T::Bytes + i) = make_uint4(0u, 0u, 0u, 0u);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -573,6 +570,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
       request(kp, a.ks, mine, 0);
       request(vp, a.vs, mine + T::Bytes, 0);
     }
+    bf16x8 qf[NJ];
+    load_row<NJ, PADDED>(qf, a.q + (int64_t)(s.q0 + token) * a.qs.row + (int64_t)(head * G + r - token * G) * a.qs.head + hh * 8, hh, a.D);
     f32x16 O[ND];
 #pragma unroll
     for (int db = 0; db < ND; ++db)
@@ -668,33 +667,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 }
 
 // The pieces of the keys joined, in their order: a workgroup per row, lane p of each wave with the weight of piece p, each wave the sums of every
-// fourth piece.
+// fourth piece.  All loads go out at once, those of pieces without weight among them, whose rows are not used: 64 pieces of 32 rows 8.7 -> @@ us.
 constexpr int kMaxPieces = 64;
 __global__ __launch_bounds__(256) void packed_combine_kernel(PackedArgs a) {
   __shared__ float part[3][128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = blockIdx.x, group_rows = (int64_t)a.seqs.q_rows * a.group.d, rows = group_rows * a.kv_heads;
-  const int head = (int)(row / group_rows);
+  const int head = (int)(row / group_rows), c = 2 * lane;
   const unsigned rg = (unsigned)(row - head * group_rows), t = div_by(rg, a.group), h = head * a.group.d + rg - t * a.group.d;
-  if ((int)t < a.seqs.q_off[0] || (int)t >= a.seqs.q_off[a.seqs.count]) return;  // rows of no sequence: zeros already
-  const float2 u = lane < a.pieces ? a.ml[lane * rows + row] : make_float2(0.f, 0.f);
-  float top = u.y != 0.f ? u.x : -INFINITY;  // (a piece without weight carries no reference point)
+  const int first = a.seqs.q_off[0], last = a.seqs.q_off[a.seqs.count];
+  const float2 u = a.ml[min(lane, a.pieces - 1) * rows + row];
+  const float* p = a.part + row * a.D + (c < a.D ? c : 0);
+  float2 o[kMaxPieces / 4];
+#pragma unroll
+  for (int i = 0; i < kMaxPieces / 4; ++i)
+    if (4 * i + wave < a.pieces) o[i] = *reinterpret_cast<const float2*>(p + (4 * i + wave) * rows * a.D);
+  if ((int)t < first || (int)t >= last) return;  // rows of no sequence: zeros already
+  const bool has = lane < a.pieces && u.y != 0.f;
+  float top = has ? u.x : -INFINITY;  // (a piece without weight carries no reference point)
 #pragma unroll
   for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
-  const float x = u.y != 0.f ? __builtin_amdgcn_exp2f(u.x - top) : 0.f;
-  float sum = x * u.y;
+  const float x = has ? __builtin_amdgcn_exp2f(u.x - top) : 0.f;
+  float sum = has ? x * u.y : 0.f;
 #pragma unroll
   for (int i = 1; i < 64; i *= 2) sum += __shfl_xor(sum, i);
-  const int c = 2 * lane;
   float f0 = 0.f, f1 = 0.f;
-  const float* p = a.part + row * a.D + (c < a.D ? c : 0);
-#pragma unroll 8
-  for (int i = wave; i < a.pieces; i += 4) {
-    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), i));
+#pragma unroll
+  for (int i = 0; i < kMaxPieces / 4; ++i) {
+    if (4 * i + wave >= a.pieces) break;
+    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 4 * i + wave));
     if (w == 0.f) continue;  // (nothing may stand there; a weight that is not a number stays one)
-    const float2 o = *reinterpret_cast<const float2*>(p + i * rows * a.D);
-    f0 += w * o.x;
-    f1 += w * o.y;
+    f0 += w * o[i].x;
+    f1 += w * o[i].y;
   }
   if (wave) {
     part[wave - 1][c] = f0;
