@@ -12,7 +12,6 @@
 // Few rows (one or a few tokens) have a kernel of their own, bound by the keys' way from memory.
 // With few tiles the keys are cut into pieces besides; each leaves un-normalised f32 rows, joined by a third kernel in a fixed order.
 #include <algorithm>
-#include <type_traits>
 
 #include "attn_packed.h"
 
@@ -35,12 +34,13 @@ struct PackedArgs {
   float2* ml;   // [piece][kv_heads][q_rows * group]: reference point (log2 units) and sum of P
 };
 
-template <int HD>
+// KW: the waves that deal a slot's keys among them; 4 / KW waves of 32 rows.
+template <int HD, int KW>
 struct FwdShape {
-  static constexpr int NB = HD == 64 ? 2 : 1;      // blocks of 32 keys of a slot
-  static constexpr int SLOTS = HD == 64 ? 2 : 3;
-  static constexpr int Keys = 32 * NB, Half = NB * PackedBlock<HD>::Bytes, Slot = 2 * Half;
-  static constexpr int BM = 128;
+  static constexpr int NB = HD == 64 ? 2 : 1;               // blocks of 32 keys that a wave computes per slot
+  static constexpr int SLOTS = HD == 64 || KW == 2 ? 2 : 3;
+  static constexpr int Blocks = NB * KW, Keys = 32 * Blocks, Half = Blocks * PackedBlock<HD>::Bytes, Slot = 2 * Half;
+  static constexpr int BM = 128 / KW;
 };
 
 // rows of no sequence: tile `tile` of them
@@ -148,10 +148,11 @@ __device__ __forceinline__ void store_out(const PackedArgs& a, const SeqTile& s,
   }
 }
 
-template <int HD, int DC, bool PADDED>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 4 : 3, HD == 64 ? 4 : 3))) void packed_fwd_kernel(PackedArgs a) {
+template <int HD, int DC, bool PADDED, int KW>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KW == 2 ? 2 : HD == 64 ? 4 : 3, KW == 2 ? 2 : HD == 64 ? 4 : 3)))
+void packed_fwd_kernel(PackedArgs a) {
   using T = PackedBlock<HD>;
-  using F = FwdShape<HD>;
+  using F = FwdShape<HD, KW>;
   constexpr int NJ = DC / 16, ND = (DC + 31) / 32, NB = F::NB, SLOTS = F::SLOTS;
   constexpr int GPW = F::Keys / T::RPI / 4;  // row groups per wave, slot and tensor
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // (fragment addresses are formed by xor)
@@ -162,28 +163,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   const int rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
   const SeqTile s = find_tile<F::BM, false>(a.seqs, G, rank, lane);
   if (s.none) return;
-  const int64_t group_rows = (int64_t)a.seqs.q_rows * G;
-  const int tile = s.tile, rows = s.m * G, r0 = tile * F::BM + wave * 32;
-  const bool split = a.part != nullptr;
+  const int row_wave = KW == 1 ? wave : wave & 1, key_wave = KW == 1 ? 0 : wave >> 1;
+  const int tile = s.tile, rows = s.m * G, r0 = tile * F::BM + row_wave * 32;
   auto token_of = [&](int r) __attribute__((always_inline)) { return (int)div_by((unsigned)r, a.group); };
   if (s.gap) {
-    if (blockIdx.y == 0) fill_gap<F::BM, HD>(a, s, head, tid);
+    fill_gap<F::BM, HD>(a, s, head, tid);
     return;
   }
 
-  // keys that a row sees, of those of this piece
   const int r = min(r0 + l32, rows - 1);  // (rows past the end repeat the last one and are not stored)
   const int token = token_of(r);
-  const int piece = blockIdx.y, kb = piece * a.piece_keys;
-  const int ke = piece == a.pieces - 1 ? s.n : min(s.n, kb + a.piece_keys);
-  auto sees = [&](int t) __attribute__((always_inline)) { return min(ke, a.causal ? max(t + 1 + s.n - s.m, 0) : s.n) - kb; };
-  const int lim = sees(token);                                       // (may be negative)
+  auto sees = [&](int t) __attribute__((always_inline)) { return a.causal ? min(max(t + 1 + s.n - s.m, 0), s.n) : s.n; };
+  const int lim = sees(token);
   const int all = __builtin_amdgcn_readlane(lim, 0), some = __builtin_amdgcn_readlane(lim, 31);  // keys that all, some rows of the wave see
-  const int end = sees(token_of(min(tile * F::BM + F::BM, rows) - 1));  // some row of the workgroup
-  const int nt = (end + F::Keys - 1) / F::Keys;                        // slots visited; zero or less: none
+  const int end = sees(token_of(min(tile * F::BM + F::BM, rows) - 1));                           // some row of the workgroup
+  const int nt = (end + F::Keys - 1) / F::Keys;                                                   // slots visited
 
-  const __bf16* kp = a.k + (int64_t)(s.k0 + kb) * a.ks.row + head * a.ks.head;
-  const __bf16* vp = a.v + (int64_t)(s.k0 + kb) * a.vs.row + head * a.vs.head;
+  const __bf16* kp = a.k + (int64_t)s.k0 * a.ks.row + head * a.ks.head;
+  const __bf16* vp = a.v + (int64_t)s.k0 * a.vs.row + head * a.vs.head;
   const unsigned smem_addr = lds_addr_of(smem);
   const int grow = T::row(lane), col0 = T::chunk(lane, wave) * 8;  // (groups wave, wave + 4, ...: the swizzle sees the same)
   const int col = !PADDED || col0 < a.D ? col0 : 0;
@@ -193,10 +190,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     if constexpr (PADDED) lds_dma16(at..., mask);
     else lds_dma16(at...);
   };
-  const int n = s.n - kb;  // rows of k and v from kp on
   auto request = [&](int slot, int t) __attribute__((always_inline)) {
     const unsigned Ks = smem_addr + (unsigned)(slot * F::Slot), Vs = Ks + F::Half;
-    if (t * F::Keys + F::Keys <= n) {
+    if (t * F::Keys + F::Keys <= s.n) {
 #pragma unroll
       for (int i = 0; i < GPW; ++i) {
         const int g = wave + 4 * i;
@@ -208,7 +204,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 #pragma unroll
       for (int i = 0; i < GPW; ++i) {
         const int g = wave + 4 * i;
-        const int64_t row = min(t * F::Keys + T::RPI * g + grow, n - 1);
+        const int64_t row = min(t * F::Keys + T::RPI * g + grow, s.n - 1);
         load(kp + row * a.ks.row + col, Ks + (unsigned)g * 1024u);
         load(vp + row * a.vs.row + col, Vs + (unsigned)g * 1024u);
       }
@@ -233,7 +229,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   RowState st{-1e30f, -1e30f * c, 0.f};
   const unsigned row_at = T::row_at(lane), trans_at = T::trans_at(lane);
 
-  // a block of 32 keys, the first of them key `k0` of the piece, at `at` (its V a half slot on)
+  // a block of 32 keys, the first of them key k0 of the sequence, at `at` (its V a half slot on)
   auto block = [&](unsigned at, int k0) __attribute__((always_inline)) {
     constexpr int FPB = NJ + 2 * ND;
     auto frag = [&](int i) __attribute__((always_inline)) {
@@ -298,206 +294,47 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     const unsigned at = smem_addr + (unsigned)(slot * F::Slot);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int k0 = t * F::Keys + 32 * b;
-      if (k0 < some) block(at + (unsigned)(b * T::Bytes), k0);
+      const int i = key_wave * NB + b, k0 = t * F::Keys + 32 * i;
+      if (k0 < some) block(at + (unsigned)(i * T::Bytes), k0);
     }
     slot = slot == SLOTS - 1 ? 0 : slot + 1;
     fill = fill == SLOTS - 1 ? 0 : fill + 1;
   }
   __syncthreads();  // every wave has finished reading the ring, and no load into it is in flight: it now stages the output
-  const float l = xhalf_sum(st.l), mc = st.mc;
-
-  if (split) {
-    if (r0 + l32 >= rows) return;
-    const int64_t at = ((int64_t)piece * a.kv_heads + head) * group_rows + (int64_t)s.q0 * G + r0 + l32;
-    if (hh == 0) a.ml[at] = make_float2(mc, l);
-    if (nt <= 0) return;
-    float* p = a.part + at * a.D + 4 * hh;
+  float l = xhalf_sum(st.l), mc = st.mc;
+  if constexpr (KW == 2) {  // the second waves' shares to the first, by one reference point
+    constexpr int Ld = ND * 32 + 4;  // floats of a staged row
+    static_assert(2 * 32 * (Ld * 4 + 8) <= SLOTS * F::Slot, "the staged rows fit the ring");
+    float* to = reinterpret_cast<float*>(smem) + (row_wave * 32 + l32) * Ld + 4 * hh;
+    float2* ml = reinterpret_cast<float2*>(smem + 2 * 32 * Ld * 4) + row_wave * 32 + l32;
+    if (key_wave) {
+#pragma unroll
+      for (int db = 0; db < ND; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(to + db * 32 + 8 * g) = f32x4{O[db][4 * g], O[db][4 * g + 1], O[db][4 * g + 2], O[db][4 * g + 3]};
+      if (hh == 0) *ml = make_float2(mc, l);
+    }
+    __syncthreads();
+    if (key_wave) return;
+    const float2 u = *ml;
+    const float top = u.y == 0.f ? mc : l == 0.f ? u.x : fmaxf(mc, u.x);  // (a share without weight carries no reference point)
+    const float x = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(mc - top), y = u.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(u.x - top);
+    l = l * x + u.y * y;
+    mc = top;
 #pragma unroll
     for (int db = 0; db < ND; ++db)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (!PADDED || db * 32 + 8 * g < a.D)
-          *reinterpret_cast<f32x4*>(p + db * 32 + 8 * g) = f32x4{O[db][4 * g], O[db][4 * g + 1], O[db][4 * g + 2], O[db][4 * g + 3]};
-    return;
-  }
-  static_assert(4 * 32 * kOutRow<ND> <= SLOTS * F::Slot, "the staged rows fit the ring");
-  store_out<ND, DC, PADDED>(a, s, O, l, mc, head, r0, lane, smem + wave * 32 * kOutRow<ND>);
-}
-
-// ---------------------------------------------------------------------------------------------------------------------- pipelined
-// The same for head dim 128, software-pipelined inside the wave: one instruction stream holds the eight PV products of key block b - 1, the eight
-// score products of block b + 1 and the softmax of block b, with a share of the softmax behind each product and the LDS read of a
-// fragment one product of its kind ahead of its use.  64 keys per slot, K(t) beside V(t - 1), in a ring of four slots (128 KB, a
-// workgroup per CU), whose loads are two slots ahead of their use; one barrier per 64 keys.  Blocks in front of the first and behind the last are
-// masked whole (P = 0) and walked like the others.
-constexpr int kPipeSlot = 4 * PackedBlock<128>::Bytes, kPipeHalf = 2 * PackedBlock<128>::Bytes, kPipeBytes = 4 * kPipeSlot;
-
-__device__ const u32x4 kZeros = {0u, 0u, 0u, 0u};
-
-template <int NW>
-__global__ __launch_bounds__(NW * 64) void packed_pipe_kernel(PackedArgs a) {
-  using T = PackedBlock<128>;
-  constexpr int BM = NW * 32, GPW = 16 / NW;  // row groups per wave, slot and tensor
-  constexpr int kFirst = 2;                   // the product behind which the softmax starts: the scores' last one has left the pipe
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
-  const SeqTile s = find_tile<BM, false>(a.seqs, G, rank, lane);
-  if (s.none) return;
-  if (s.gap) {
-    if (tid < 256) fill_gap<BM, 128>(a, s, head, tid);
-    return;
-  }
-  const int rows = s.m * G, r0 = s.tile * BM + wave * 32;
-  auto token_of = [&](int r) __attribute__((always_inline)) { return (int)div_by((unsigned)r, a.group); };
-  const int r = min(r0 + l32, rows - 1), token = token_of(r);  // (rows past the end repeat the last one and are not stored)
-  auto sees = [&](int t) __attribute__((always_inline)) { return a.causal ? min(max(t + 1 + s.n - s.m, 0), s.n) : s.n; };
-  const int lim = sees(token), all = __builtin_amdgcn_readlane(lim, 0), some = __builtin_amdgcn_readlane(lim, 31);
-  const int nt = (sees(token_of(min(s.tile * BM + BM, rows) - 1)) + 63) / 64;  // slots that hold a key that some row of the workgroup sees
-
-  bf16x8 qf[8];
-  {
-    const __bf16* p = a.q + (int64_t)(s.q0 + token) * a.qs.row + (int64_t)(head * G + r - token * G) * a.qs.head + hh * 8;
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 o = *reinterpret_cast<const f32x4*>(to + db * 32 + 8 * g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) qf[j] = *reinterpret_cast<const bf16x8*>(p + j * 16);
-  }
-  const __bf16* kp = a.k + (int64_t)s.k0 * a.ks.row + head * a.ks.head;
-  const __bf16* vp = a.v + (int64_t)s.k0 * a.vs.row + head * a.vs.head;
-  const unsigned smem_addr = lds_addr_of(smem);
-  const int grow = T::row(lane), col = T::chunk(lane, wave) * 8;  // (groups wave, wave + 4, ...: the swizzle sees the same)
-  const unsigned kofs = (unsigned)(grow * (int)a.ks.row + col) * 2u, vofs = (unsigned)(grow * (int)a.vs.row + col) * 2u;
-  auto request = [&](int slot, int t) __attribute__((always_inline)) {
-    const unsigned Ks = smem_addr + (unsigned)(slot * kPipeSlot), Vs = Ks + kPipeHalf;
-    if (t >= 1 && t * 64 + 64 <= s.n) {
-#pragma unroll
-      for (int i = 0; i < GPW; ++i) {
-        const int g = wave + NW * i;
-        lds_dma16(kp + (int64_t)(t * 64 + 4 * g) * a.ks.row, kofs, Ks + (unsigned)g * 1024u);
-        lds_dma16(vp + (int64_t)(t * 64 - 64 + 4 * g) * a.vs.row, vofs, Vs + (unsigned)g * 1024u);
+        for (int e = 0; e < 4; ++e) O[db][4 * g + e] = O[db][4 * g + e] * x + o[e] * y;
       }
-    } else {  // keys past the sequence's end repeat its last one and meet masked logits; V's rows outside it are zeros, which P = 0 meets
-#pragma unroll
-      for (int i = 0; i < GPW; ++i) {
-        const int g = wave + NW * i, row = t * 64 + 4 * g + grow;
-        const __bf16* v = (unsigned)(row - 64) < (unsigned)s.n ? vp + (int64_t)(row - 64) * a.vs.row + col : reinterpret_cast<const __bf16*>(&kZeros);
-        lds_dma16(kp + (int64_t)min(row, s.n - 1) * a.ks.row + col, Ks + (unsigned)g * 1024u);
-        lds_dma16(v, Vs + (unsigned)g * 1024u);
-      }
-    }
-  };
-  if (nt > 0) {
-    request(0, 0);
-    request(1, 1);
-    request(2, 2);
   }
-  f32x16 O[4];
-#pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) O[db][i] = 0.f;
-  const float c = a.c;
-  RowState st{-1e30f, -1e30f * c, 0.f};
-  f32x16 Sa, Sb;        // logits of odd, even blocks
-  u32x4 Pa[2], Pb[2];   // probabilities of odd, even blocks as the PV product's operand
-  bf16x8 kf[2], vf[2];  // fragments read ahead
-#pragma unroll
-  for (int i = 0; i < 16; ++i) { Sa[i] = -INFINITY; Sb[i] = 0.f; }  // block -1
-#pragma unroll
-  for (int i = 0; i < 2; ++i) Pa[i] = Pb[i] = u32x4{0u, 0u, 0u, 0u};
 
-  const unsigned row_at = smem_addr + T::row_at(lane), trans_at = smem_addr + T::trans_at(lane);
-  // fragment j of K's block at byte `at` of the ring, jv of V's
-  auto k_frag = [&](int at, int j) __attribute__((always_inline)) { return read_row_frag((row_at ^ (unsigned)(32 * j)) + (unsigned)at); };
-  auto v_frag = [&](int at, int jv) __attribute__((always_inline)) {
-    const unsigned x = trans_at ^ (unsigned)(64 * (jv & 3));
-    return read_trans_frag(x + (unsigned)(at + (jv >> 2) * 16 * T::Row), (x ^ 32u) + (unsigned)(at + (8 + (jv >> 2) * 16) * T::Row));
-  };
-  // One block: the softmax of SC (block blk) into PC, the product of PP (blk - 1) with V at vc, the scores SN (blk + 1) from K at kc; kn, vn: the
-  // places of the next ones.
-  auto iter = [&](f32x16& SC, f32x16& SN, u32x4 (&PC)[2], u32x4 (&PP)[2], int kc, int kn, int vc, int vn, int blk) __attribute__((always_inline)) {
-    if (blk * 32 + 32 > all) {
-      asm volatile("" ::: "memory");  // keeps the branch
-      const int at0 = blk * 32 + 4 * hh;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (at0 + 8 * (i >> 2) + (i & 3) >= lim) SC[i] = -INFINITY;
-    }
-    float sum = 0.f, even = 0.f;
-#pragma unroll
-    for (int n = 0; n < 16; ++n) {
-      const int j = n >> 1;
-      if ((n & 1) == 0) {
-        O[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j & 1], __builtin_bit_cast(bf16x8, PP[j >> 2]), O[j & 3], 0, 0, 0);
-        vf[(j + 1) & 1] = j < 7 ? v_frag(vc, j + 1) : v_frag(vn, 0);
-      } else {
-        if (j == 0) {
-          f32x16 z;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) z[i] = 0.f;
-          SN = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[0], qf[0], z, 0, 0, 0);
-        } else {
-          SN = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j & 1], qf[j], SN, 0, 0, 0);
-        }
-        kf[(j + 1) & 1] = j < 7 ? k_frag(kc, j + 1) : k_frag(kn, 0);
-      }
-      const int e0 = n < kFirst ? 0 : (n - kFirst) * 16 / (16 - kFirst), e1 = n < kFirst ? 0 : (n + 1 - kFirst) * 16 / (16 - kFirst);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (e < e0 || e >= e1) continue;
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(SC[e], c, -st.mc));
-        if ((e & 1) == 0) {
-          even = x;
-          asm volatile("" : "+v"(even));  // pins the work behind its product
-        } else {
-          unsigned pk = pack2(even, x);
-          sum = e == 1 ? even + x : sum + (even + x);
-          asm volatile("" : "+v"(pk), "+v"(sum));
-          PC[e >> 3][(e >> 1) & 3] = pk;
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum <= kRange)) != 0, 0)) {  // (no product with V is on its way here)
-      bf16x8 P[2];
-      soft_block<4>(SC, c, st, O, P);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) PC[i] = __builtin_bit_cast(u32x4, P[i]);
-      sum = 0.f;
-    }
-    st.l += sum;
-  };
-
-  const int last = (some + 31) / 32;  // the block behind this wave's last: its iteration holds that one's product with V
-  auto period = [&](int t, auto slot) __attribute__((always_inline)) {
-    constexpr int cur = decltype(slot)::value * kPipeSlot, nxt = ((decltype(slot)::value + 1) & 3) * kPipeSlot, B = T::Bytes, H = kPipeHalf;
-    // slot t + 1 has landed, this wave's share and everyone's (the one requested after it may be on its way); slot t - 1 has been read
-    if (t + 2 <= nt) __builtin_amdgcn_s_waitcnt(0x0F70 | (2 * GPW));
-    else __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();
-    if (2 * t - 1 <= last) iter(Sa, Sb, Pa, Pb, cur, cur + B, cur + H, cur + H + B, 2 * t - 1);
-    // in the middle of the period, where not all waves queue for it
-    if (t + 3 <= nt) request((decltype(slot)::value + 3) & 3, t + 3);
-    if (2 * t <= last) iter(Sb, Sa, Pb, Pa, cur + B, nxt, cur + H + B, nxt + H, 2 * t);
-  };
-  if (nt > 0) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();
-    kf[0] = k_frag(0, 0);
-    vf[0] = v_frag(kPipeHalf, 0);
-    for (int t = 0; t <= nt; t += 4) {
-      period(t, std::integral_constant<int, 0>{});
-      if (t + 1 > nt) break;
-      period(t + 1, std::integral_constant<int, 1>{});
-      if (t + 2 > nt) break;
-      period(t + 2, std::integral_constant<int, 2>{});
-      if (t + 3 > nt) break;
-      period(t + 3, std::integral_constant<int, 3>{});
-    }
-  }
-  __syncthreads();  // every wave has finished reading the ring, and no load into it is in flight: it now stages the output
-  store_out<4, 128, false>(a, s, O, xhalf_sum(st.l), st.mc, head, r0, lane, smem + wave * 32 * kOutRow<4>);
+  constexpr int Behind = KW == 2 ? 2 * 32 * ((ND * 32 + 4) * 4 + 8) : 0;  // (the other wave's share may still be read)
+  static_assert(Behind + 4 / KW * 32 * kOutRow<ND> <= SLOTS * F::Slot, "the staged rows fit the ring");
+  store_out<ND, DC, PADDED>(a, s, O, l, mc, head, r0, lane, smem + Behind + row_wave * 32 * kOutRow<ND>);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- few rows
@@ -716,76 +553,49 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(PackedArgs a) {
   if (c == 0 && a.lse) a.lse[(int64_t)h * a.seqs.q_rows + t] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
 }
 
-// How a call is launched.
+// How a call is launched.  With few tiles a call's time is the longest walk over the keys by one wave: 0.72 us per block of 32 keys for a
+// workgroup alone on its CU with all waves in the rows' direction (flat), about half with two waves to share the keys (half), a quarter with
+// four (few); with many it is the CUs' work, which costs half 15 % more than flat, whose workgroups read each key for twice the rows, and few two
+// to three times as much.  us at head dim 128, few / half / flat: 512 tokens x 4 heads of k and v with groups of 4 (64 tiles) 11.0 / 11.7 / 15.8, 2,048 x 4
+// (256 tiles) 45 / 32 / 48, 4 x 1,024 x 4 (512 tiles) 62 / 33 / 29, causal 4,096 x 4 (512) 129 / 86 / 97, 8,192 x 4 (1,024) 440 / 300 / 257, not causal 4,096
+// x 4 210 / 149 / 131; 100 tokens at a time (256 tiles) 16 / 9.7 / 7.4.
+enum { kFew, kHalf, kFlat };
 struct FwdPlan {
   int kind, pieces, piece_keys;
-  int64_t floats, tiles;  // tiles: of 128 rows (few rows: 32), of all heads
-  void cut(const mdattn_packed* p, int64_t max_k, int64_t keys) {
-    keys = (std::max(keys, (max_k + kMaxPieces - 1) / kMaxPieces) + 127) / 128 * 128;
-    const int64_t n = (max_k + keys - 1) / keys;
-    if (n < 2) return;
-    pieces = (int)n;
-    piece_keys = (int)keys;
-    floats = n * p->q_rows * p->heads * (p->head_dim + 2);
-  }
+  int64_t floats, tiles;  // tiles: of 128 rows, of all heads
 };
-enum { kFew, kFlat, kPipe4, kPipe8 };
 FwdPlan fwd_plan(const mdattn_packed* p) {
   const int64_t group = p->heads / p->kv_heads;
   const int64_t max_q = p->max_q > 0 && p->max_q < p->q_rows ? p->max_q : p->q_rows, max_k = p->max_k > 0 && p->max_k < p->k_rows ? p->max_k : p->k_rows;
   FwdPlan f{kFlat, 1, 1 << 30, 0, 0};
-  // (the list of all tiles' pieces is counted in 31 bits)
-  if (max_q * group <= 32 && packed_tiles(p->q_rows * group, p->sequences, 32) * kMaxPieces * p->kv_heads < (1ll << 31)) f.kind = kFew;
-  const int bm = f.kind == kFew ? 32 : 128;
-  // tiles that there are: of the tokens, or of so many sequences of the longest one's
-  f.tiles = std::min((max_q * group + bm - 1) / bm * p->sequences, p->q_rows * group / bm + p->sequences) * p->kv_heads;
-  if (f.kind == kFew) {
-    const int64_t all = std::min(max_k * p->sequences, (int64_t)p->k_rows) * p->kv_heads;
-    if (max_k >= 512) f.cut(p, max_k, std::max<int64_t>(all / 2048, 256));
-    return f;
-  }
+  // tiles that there are: of the tokens, or of so many sequences of the longest one's; blocks of keys that the longest walk has
+  f.tiles = std::min((max_q * group + 127) / 128 * p->sequences, p->q_rows * group / 128 + p->sequences) * p->kv_heads;
   const int64_t blocks = (max_k + 31) / 32;
-  if (f.tiles > 256) {
-    // (tiles of 256 rows that fill their last round)
-    const int64_t rounds = (f.tiles + 511) / 512;
-    if (p->head_dim == 128 && !p->causal && blocks >= 128 && f.tiles >= rounds * 480) f.kind = kPipe8;
+  const bool one_tile = max_q * group <= 32, small = p->head_dim <= 64;
+  if (one_tile || (f.tiles <= 64 && blocks >= (small ? 4 : 12)) || (small && f.tiles <= 128 && blocks >= 32)) f.kind = kFew;
+  else if (f.tiles <= (p->causal && blocks >= 48 ? 512 : 256) && blocks >= (f.tiles <= 128 ? 4 : 8)) f.kind = kHalf;
+  if (f.kind != kFew) return f;
+  // (the list of all tiles' pieces is counted in 31 bits)
+  if (packed_tiles(p->q_rows * group, p->sequences, 32) * kMaxPieces * p->kv_heads >= (1ll << 31)) {
+    f.kind = kFlat;
     return f;
   }
-  const bool pipe = p->head_dim == 128;
-  if (pipe) f.kind = kPipe4;
-  // Alone on its CU a workgroup takes so many us per block of 32 keys; in n pieces, of the flat schedule, one n-th of them, and their rows go to
-  // memory and back, at some 4 TB/s, through a launch of 5 us.
-  const double row_us = (double)p->q_rows * p->heads * p->head_dim * 4 * 2 / 4e6 * (p->causal ? 0.6 : 1.0);
-  double best = 0.95 * blocks * (pipe ? 0.56 : 0.75);
-  int64_t pieces = 1;
-  for (int64_t n = 2; n <= 16 && blocks / n >= 16 && f.tiles * n <= 512; ++n) {
-    const double us = (double)blocks / n * (f.tiles * n <= 256 ? 0.75 : 1.06) + n * row_us + 5;
-    if (us < best) { best = us; pieces = n; }
-  }
-  if (pieces > 1) {
-    f.kind = kFlat;
-    f.cut(p, max_k, (max_k + pieces - 1) / pieces);
-  }
+  if (!one_tile || max_k < 512) return f;
+  const int64_t all = std::min(max_k * p->sequences, (int64_t)p->k_rows) * p->kv_heads;
+  const int64_t keys = (std::max({all / 2048, (int64_t)256, (max_k + kMaxPieces - 1) / kMaxPieces}) + 127) / 128 * 128;
+  f.pieces = (int)((max_k + keys - 1) / keys);
+  f.piece_keys = (int)keys;
+  f.floats = f.pieces * (int64_t)p->q_rows * p->heads * (p->head_dim + 2);
   return f;
-}
-
-template <int NW>
-int launch_pipe(hipStream_t st, const PackedArgs& a, int64_t grid) {
-  static LdsOptIn opted;
-  if (lds_opt_in(opted, reinterpret_cast<const void*>(packed_pipe_kernel<NW>), kPipeBytes) != MDATTN_OK) return MDATTN_E_LAUNCH;
-  MDATTN_LAUNCH(packed_pipe_kernel<NW>, dim3((unsigned)grid), dim3(NW * 64), kPipeBytes, st, a);
-  return launch_status();
 }
 
 template <int HD, int DC, bool PADDED>
 int launch(hipStream_t st, const PackedArgs& a, int kind, int64_t grid) {
-  if (kind == kFew) {
-    MDATTN_LAUNCH((packed_few_kernel<HD, DC, PADDED>), dim3((unsigned)grid), dim3(256), few_bytes<HD>(), st, a);
-  } else if (kind == kFlat || HD != 128 || PADDED) {
-    MDATTN_LAUNCH((packed_fwd_kernel<HD, DC, PADDED>), dim3((unsigned)grid, (unsigned)a.pieces), dim3(256), FwdShape<HD>::SLOTS * FwdShape<HD>::Slot, st, a);
-  } else {
-    return kind == kPipe4 ? launch_pipe<4>(st, a, grid) : launch_pipe<8>(st, a, grid);
-  }
+  using H = FwdShape<HD, 2>;
+  using F = FwdShape<HD, 1>;
+  if (kind == kFew) MDATTN_LAUNCH((packed_few_kernel<HD, DC, PADDED>), dim3((unsigned)grid), dim3(256), few_bytes<HD>(), st, a);
+  else if (kind == kHalf) MDATTN_LAUNCH((packed_fwd_kernel<HD, DC, PADDED, 2>), dim3((unsigned)grid), dim3(256), H::SLOTS * H::Slot, st, a);
+  else MDATTN_LAUNCH((packed_fwd_kernel<HD, DC, PADDED, 1>), dim3((unsigned)grid), dim3(256), F::SLOTS * F::Slot, st, a);
   return launch_status();
 }
 
@@ -810,7 +620,7 @@ extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, cons
       !packed_strides_ok(q_strides) || !packed_strides_ok(k_strides) || !packed_strides_ok(v_strides) || !packed_strides_ok(o_strides))
     return MDATTN_E_ALIGN;
   FwdPlan f = fwd_plan(p);
-  if (f.pieces > 1 && (!workspace || workspace_floats < f.floats)) {  // (flat or few rows)
+  if (f.pieces > 1 && (!workspace || workspace_floats < f.floats)) {
     f.pieces = 1;
     f.piece_keys = 1 << 30;
   } else if (f.pieces > 1 && !aligned16(workspace)) {
@@ -831,12 +641,12 @@ extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, cons
     a.part = workspace;
     a.ml = reinterpret_cast<float2*>(workspace + f.pieces * rows * a.D);
   }
-  int64_t grid = packed_tiles(group_rows, p->sequences, f.kind == kFew ? 32 : f.kind == kPipe8 ? 256 : 128) * p->kv_heads;
+  int64_t grid = packed_tiles(group_rows, p->sequences, f.kind == kFew ? 32 : f.kind == kHalf ? 64 : 128) * p->kv_heads;
   if (f.kind == kFew) {  // two per CU, in whole rounds of the heads, walk what there is
     const int64_t most = (512 + a.kv_heads - 1) / a.kv_heads * a.kv_heads;
     grid = grid * f.pieces < most ? grid * f.pieces : most;
   }
-  if (!grid_fits(grid, f.kind == kPipe8 ? 512 : 256) || (f.pieces > 1 && !grid_fits(rows, 256))) return MDATTN_E_UNSUPPORTED;
+  if (!grid_fits(grid, 256) || (f.pieces > 1 && !grid_fits(rows, 256))) return MDATTN_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   const int status = a.D == 64   ? launch<64, 64, false>(st, a, f.kind, grid)
                      : a.D < 64  ? launch<64, 64, true>(st, a, f.kind, grid)
