@@ -9,8 +9,9 @@
 // a lane holds 16 keys of one row and the accumulators are, packed to bf16, the B operand of O^T += V^T P^T.  The softmax keeps no running
 // maximum but a reference point per row, moved (in a rarely taken branch) when a sum of P leaves its range.  Keys that a row does not see get
 // s = -inf, in the blocks that hold such keys; blocks that no row of a wave sees are not computed.
-// Few rows (one or a few tokens) have a kernel of their own, bound by the keys' way from memory.
-// With few tiles the keys are cut into pieces besides; each leaves un-normalised f32 rows, joined by a third kernel in a fixed order.
+// Few tiles leave CUs idle: two waves then share the keys of 64 rows, or four waves those of 32 (a kernel of its own, that one token meets too).
+// Where a tile is all that a sequence has, its keys are cut into pieces besides; each leaves un-normalised f32 rows, joined by another kernel
+// in a fixed order.
 #include <algorithm>
 
 #include "attn_packed.h"
@@ -102,7 +103,7 @@ __device__ __forceinline__ void soft_block(const f32x16& S, float c, RowState& s
 }
 
 // A row's fragments straight from memory, waited for here, with what is on its way into LDS: in the loop behind, the compiler would wait for them in
-// every block of keys, and with that for the keys requested since (16,384 tokens x 32 heads 1,895 -> @@ us).
+// every block of keys, and with that for the keys requested since (16,384 tokens x 32 heads 1,895 -> 1,835 us).
 template <int NJ, bool PADDED>
 __device__ __forceinline__ void load_row(bf16x8 (&f)[NJ], const __bf16* p, int hh, int D) {
 #pragma unroll
@@ -504,7 +505,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 }
 
 // The pieces of the keys joined, in their order: a workgroup per row, lane p of each wave with the weight of piece p, each wave the sums of every
-// fourth piece.  All loads go out at once, those of pieces without weight among them, whose rows are not used: 64 pieces of 32 rows 8.7 -> @@ us.
+// fourth piece.  All loads go out at once, those of pieces without weight among them, whose rows are not used: 64 pieces of 32 rows 8.7 -> 4.7 us.
 constexpr int kMaxPieces = 64;
 __global__ __launch_bounds__(256) void packed_combine_kernel(PackedArgs a) {
   __shared__ float part[3][128];
@@ -629,7 +630,7 @@ extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   PackedArgs a{};
   a.q = static_cast<const __bf16*>(q); a.k = static_cast<const __bf16*>(k); a.v = static_cast<const __bf16*>(v);
   a.out = static_cast<__bf16*>(out); a.lse = lse;
-  a.seqs = {p->q_offsets, p->k_offsets, p->k_lengths, p->sequences, p->q_rows, p->k_rows, f.kind == kFew ? kAsTheyCome : packed_order(p, f.tiles), 256 / p->kv_heads};
+  a.seqs = {p->q_offsets, p->k_offsets, p->k_lengths, p->sequences, p->q_rows, p->k_rows, f.kind == kFew ? kAsTheyCome : packed_order(p, f.tiles * (f.kind == kHalf && p->causal ? 2 : 1)), 256 / p->kv_heads};
   a.group = divisor((unsigned)(p->heads / p->kv_heads));
   a.kv_heads = p->kv_heads; a.D = p->head_dim; a.causal = p->causal;
   a.qs = {q_strides->seq, q_strides->head}; a.ks = {k_strides->seq, k_strides->head};
