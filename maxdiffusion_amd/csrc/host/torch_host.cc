@@ -10,6 +10,7 @@
 // step become 91-108.
 #include <ATen/ATen.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -55,6 +56,19 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+// A leaf's node in the autograd graph belongs to the stream on which it was made and lives as long as any graph that leads to it.  A backward pass
+// captured on another stream would make that stream wait inside the capture, which ends the process: such a forward call is refused.
+void no_older_graph(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) {
+    if (!t->defined() || !t->is_cuda() || !t->requires_grad() || t->grad_fn()) continue;
+    const auto leaf = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto on = leaf ? leaf->stream() : std::nullopt;
+    if (!on || on->id() == c10::hip::getCurrentHIPStream(t->get_device()).id()) continue;
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+                "cannot capture a call that is to be differentiated: one of its inputs is still part of an autograd graph from another stream; drop the "
+                "outputs that hold that graph, or build it on the stream of the capture");
+  }
 }
 // A node's plain values as one entry of its saved_data (an entry each, boxed, cost a small backward call a few us)
 template <class T>
@@ -447,9 +461,11 @@ struct PackedFn : FirstOrder<PackedFn> {
 OptTensor flash_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qo, const OptTensor& ko_, const OptTensor& kl_, bool causal,
                        double scale, int64_t max_q, int64_t max_k) {
   const Tensor ko = ko_.has_value() ? *ko_ : qo, kl = value(kl_);
+  const bool grad = wants_grad({&q, &k, &v});
+  if (grad) no_older_graph({&q, &k, &v});
   mdattn_packed p;
   if (!packed_args(q, k, v, qo, ko, kl, causal, max_q, max_k, p)) return std::nullopt;
-  if (wants_grad({&q, &k, &v})) {
+  if (grad) {
     if (kl.defined()) return std::nullopt;
     return unless_refused([&] { return PackedFn::apply(q, k, v, qo, ko, causal, scale, max_q, max_k); });
   }
@@ -1048,10 +1064,12 @@ std::optional<variable_list> rms_norm(const Tensor& x, const OptTensor& w_, cons
   int64_t stride;
   int f32;
   Rows3 rr;
+  const bool grad = wants_grad({&x, &w, &b, &res});
+  if (grad) no_older_graph({&x, &w, &b, &res});
   if (!x.is_cuda() || !float_on(x, x)) return std::nullopt;
   const auto r = as_rows(x);
   if (!r || !norm_vectors(x, *r, w, b, stride, f32) || !residual_rows(x, res, rr)) return std::nullopt;
-  if (wants_grad({&x, &w, &b, &res})) {
+  if (grad) {
     if (x.dim() > 8) return std::nullopt;
     return unless_refused([&] { return RmsFn::apply(x, w_, b_, res_, eps, offset); });
   }
