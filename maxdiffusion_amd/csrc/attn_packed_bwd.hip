@@ -12,6 +12,12 @@
 // Blocks that no row of a wave sees, or no key of it is seen by, are not computed.
 // The dk / dv pass has a workgroup per 128 keys and head of k and v, of which the first ones of a causal sequence walk all of its tokens in every
 // head: these walks are cut into pieces, whose f32 sums a third kernel adds up in their order.
+// Roundings.  P and dS go into their products in bf16, and delta comes from the rounded out: at causal sequences of 600 tokens with a direction
+// that all logits share (so that sum(ds) = 0 cancels most of dq) each of the two costs dq 1.7e-3 of its size, as much as its own rounding.  dS in two
+// parts would cost a third more matrix products.
+// Bound.  A tile costs LDS as many cycles as the matrix pipes: 1 KB of fragments read per product of 32 cycles and wave, 128 bytes a cycle with
+// four waves.  100 to 4,096 tokens x 8 sequences, 32 heads on 8, causal: dq 221 us (1.05 PFLOP/s, pipes busy 50 % of the cycles), dk / dv 337 us
+// (0.92, 41 %), the pieces' sums 22 us.
 #include <algorithm>
 #include <cmath>
 

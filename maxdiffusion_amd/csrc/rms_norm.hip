@@ -7,7 +7,9 @@
 // and db stay in its registers while the rows pass by, the next row already on its way.  A row's one sum (two backward) takes one exchange
 // through LDS and one barrier.  h is formed from the f32 sum that s is rounded from; the backward pass has the rounded one, whose
 // roundings (2^-9 of an element on average) change a gradient by less than its own.
-// Bound by memory.
+// Bound by memory where rows are many: 75,600 rows of 5,120 in bf16, with a residual, scale and shift, 540 us (3.1 GB at 5.7 TB/s, above a copy's
+// 4.9: streaming stores); into e4m3, 4,096 x 4,096, 22 us (5.4 TB/s).  Few or odd rows wait for a row's way through memory and its sum: one row
+// 3.2 us, 2,674 of 1,001 with an f32 residual 9.2 us (3.5 TB/s), their backward pass 14.8 us (2.9 TB/s) and 4.1 for the sums of dw and db.
 #include "norm_rows.h"
 
 namespace mdattn {
