@@ -580,16 +580,18 @@ FwdPlan fwd_plan(const mdattn_packed* p) {
   else if (f.tiles <= (p->causal && blocks >= 48 ? 512 : 256) && blocks >= (f.tiles <= 128 ? 4 : 8)) f.kind = kHalf;
   if (f.kind != kFew) return f;
   // (the list of all tiles' pieces is counted in 31 bits)
-  if (packed_tiles(p->q_rows * group, p->sequences, 32) * kMaxPieces * p->kv_heads >= (1ll << 31)) {
+  if (packed_tiles(p->q_rows * group, p->sequences, 32) * kMaxPieces * p->kv_heads >= (1ll << 31) - (1 << 20)) {
     f.kind = kFlat;
     return f;
   }
   if (!one_tile || max_k < 512) return f;
-  const int64_t all = std::min(max_k * p->sequences, (int64_t)p->k_rows) * p->kv_heads;
-  const int64_t keys = (std::max({all / 2048, (int64_t)256, (max_k + kMaxPieces - 1) / kMaxPieces}) + 127) / 128 * 128;
+  // (256 MiB of rows at most, whatever the hints are)
+  const int64_t all = std::min(max_k * p->sequences, (int64_t)p->k_rows) * p->kv_heads, piece_floats = (int64_t)p->q_rows * p->heads * (p->head_dim + 2);
+  const int64_t most = std::max<int64_t>(std::min<int64_t>(kMaxPieces, (1 << 26) / std::max<int64_t>(piece_floats, 1)), 1);
+  const int64_t keys = (std::max({all / 2048, (int64_t)256, (max_k + most - 1) / most}) + 127) / 128 * 128;
   f.pieces = (int)((max_k + keys - 1) / keys);
   f.piece_keys = (int)keys;
-  f.floats = f.pieces * (int64_t)p->q_rows * p->heads * (p->head_dim + 2);
+  f.floats = f.pieces > 1 ? f.pieces * piece_floats : 0;
   return f;
 }
 

@@ -514,16 +514,23 @@ BwdPlan bwd_plan(const mdattn_packed* p) {
   b.aux_floats = ((int64_t)p->q_rows * p->heads * 2 + 3) & ~(int64_t)3;
   const int64_t tiles = (max_k + 127) / 128 * p->sequences, most = p->k_rows / 128 + p->sequences, walk = (max_q + 31) / 32 * group;
   b.tiles = (tiles < most ? tiles : most) * p->kv_heads;
-  // Of what a place on the chip (512: two workgroups per CU) has to walk, a part: with n parts the last places end some 0.3 / n of the time
-  // late, and each part costs its sums' way to memory and back, 130 KB in each of the 512 places, as much as 15 tiles.
+  // Where no walk is longer than what a place on the chip (512: two workgroups per CU) has to do, the walks are dealt as they are, long ones first.
+  // Else they are cut into parts of what a place has to do: with n parts the last places end some 0.3 / n of the time late, and each part
+  // costs its sums' way to memory and back, 130 KB in each of the 512 places, as much as 15 tiles.  us whole / in that many parts, at head dim
+  // 128, causal: 4 x 4,096 tokens, 32 heads on 8 (walks of 512 tiles, 512 to a place) 1,792 / 1,882 in 4; 16 on 16 (128, 256) 902 / 996 in 2; a
+  // sequence of 8,192, 32 on 8 (1,024, 512) 1,966 / 1,832 in 7; 8 on 1 (2,048, 128) 2,420 / 607 in 26.
   const double place = (double)b.tiles * walk / (p->causal ? 2 : 1) / 512;
-  int64_t piece = (int64_t)(place / std::max(1.0, std::sqrt(0.02 * place)));
-  if (piece < 16) piece = 16;
-  if (piece < walk) {
-    b.piece_tiles = (int)piece;
-    b.pieces = (int)((walk + piece - 1) / piece);
+  const int64_t sums = 2 * std::max<int64_t>((int64_t)p->k_rows * p->kv_heads * p->head_dim, 1);
+  if (walk > place) {
+    // (a GiB of sums at most, whatever the hints are)
+    const int64_t parts = std::max<int64_t>((1ll << 28) / sums, 1);
+    const int64_t piece = std::max({(int64_t)(place / std::max(1.0, std::sqrt(0.02 * place))), (int64_t)16, (walk + parts - 1) / parts});
+    if (piece < walk) {
+      b.piece_tiles = (int)piece;
+      b.pieces = (int)((walk + piece - 1) / piece);
+    }
   }
-  b.floats = b.aux_floats + (b.pieces > 1 ? (int64_t)b.pieces * 2 * p->k_rows * p->kv_heads * p->head_dim : 0);
+  b.floats = b.aux_floats + (b.pieces > 1 ? b.pieces * sums : 0);
   return b;
 }
 

@@ -98,3 +98,17 @@ def test_tensors_outside_the_device_are_refused(lib):
     attention_op.hip_flash_packed(q, q, q, o)
   with pytest.raises(ValueError, match="device memory"):
     ops.flash_attention_packed(q, q, q, o)
+
+
+def test_no_hint_makes_a_workspace_large(lib):
+  """Pieces' rows of 256 MiB and sums of a GiB at most, whatever the hints say; with less than two pieces none."""
+  for sizes in (dict(sequences=1, q_rows=1, k_rows=1 << 20), dict(sequences=512, q_rows=512, k_rows=1 << 21, heads=32, kv_heads=8),
+                dict(sequences=3, q_rows=100000, k_rows=100000, heads=32, kv_heads=8), dict(sequences=1, q_rows=1 << 20, k_rows=1 << 20, heads=64, kv_heads=1),
+                dict(sequences=1, q_rows=1 << 20, k_rows=1, heads=1024, kv_heads=1)):
+    for max_q in (0, 1, 33, 1 << 30):
+      for max_k in (0, 1, 700, 1 << 30):
+        p = packed(**sizes, max_q=max_q, max_k=max_k)
+        rows = p.q_rows * p.heads
+        assert 0 <= lib.mdattn_fwd_bf16_packed_workspace_floats(ctypes.byref(p)) <= 1 << 26
+        sums = lib.mdattn_bwd_bf16_packed_workspace_floats(ctypes.byref(p)) - (2 * rows + 3) // 4 * 4
+        assert sums == 0 or 4 * p.k_rows * p.kv_heads * p.head_dim <= sums <= max(1 << 28, 4 * p.k_rows * p.kv_heads * p.head_dim)
