@@ -276,7 +276,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   const SeqTile s = find_tile<BM, true>(a.seqs, G, rank, lane);
   if (s.none) return;
   const int key0 = (s.tiles - 1 - s.tile) * BM, w0 = key0 + wave * 32;  // (causal: the first keys meet the most tokens)
-  const int piece = blockIdx.y;
+  const int piece = gridDim.y - 1 - blockIdx.y;  // (the long walks' last pieces first, the short walks' only ones in the end)
   if (s.gap) {
     if (piece) return;
     for (int i = tid; i < BM * (HD / 8); i += 256) {
@@ -475,7 +475,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   });
 }
 
-// The pieces' sums of dk (blockIdx.y 0) and dv (1), added in their order, for the tiles of 128 keys whose rows were cut.
+// The pieces' sums of dk (blockIdx.y 0) and dv (1), added in their order, for the tiles of 128 keys whose rows were cut; a tile's elements to
+// gridDim.z workgroups where there are few.
 __global__ __launch_bounds__(256) void packed_reduce_kernel(PackedBwdArgs a) {
   const int lane = threadIdx.x & 63, rank = blockIdx.x / a.kv_heads, head = blockIdx.x - rank * a.kv_heads, G = a.group.d;
   const SeqTile s = find_tile<128, true>(a.seqs, G, rank, lane);
@@ -488,7 +489,7 @@ __global__ __launch_bounds__(256) void packed_reduce_kernel(PackedBwdArgs a) {
   const RowStrides st = blockIdx.y ? a.dvs : a.dks;
   __bf16* out = (blockIdx.y ? a.dv : a.dk) + (int64_t)(s.k0 + key0) * st.row + head * st.head;
   const int n = min(128, s.n - key0) * cpr;
-  for (int i = threadIdx.x; i < n; i += 256) {
+  for (int i = blockIdx.z * 256 + threadIdx.x; i < n; i += 256 * gridDim.z) {
     float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const f32x4* p = reinterpret_cast<const f32x4*>(part) + 2 * i;
 #pragma unroll 4
@@ -514,22 +515,30 @@ BwdPlan bwd_plan(const mdattn_packed* p) {
   b.aux_floats = ((int64_t)p->q_rows * p->heads * 2 + 3) & ~(int64_t)3;
   const int64_t tiles = (max_k + 127) / 128 * p->sequences, most = p->k_rows / 128 + p->sequences, walk = (max_q + 31) / 32 * group;
   b.tiles = (tiles < most ? tiles : most) * p->kv_heads;
-  // Where no walk is longer than what a place on the chip (512: two workgroups per CU) has to do, the walks are dealt as they are, long ones first.
-  // Else they are cut into parts of what a place has to do: with n parts the last places end some 0.3 / n of the time late, and each part
-  // costs its sums' way to memory and back, 130 KB in each of the 512 places, as much as 15 tiles.  us whole / in that many parts, at head dim
-  // 128, causal: 4 x 4,096 tokens, 32 heads on 8 (walks of 512 tiles, 512 to a place) 1,792 / 1,882 in 4; 16 on 16 (128, 256) 902 / 996 in 2; a
-  // sequence of 8,192, 32 on 8 (1,024, 512) 1,966 / 1,832 in 7; 8 on 1 (2,048, 128) 2,420 / 607 in 26.
-  const double place = (double)b.tiles * walk / (p->causal ? 2 : 1) / 512;
+  // The walks whole, long ones first, or in n parts, by what the last place on the chip (two workgroups per CU, three at head dims up to 64) then
+  // ends at, in tiles.  `place`: what each has to walk; of lengths that differ, known by their mean and their largest, some two thirds of what
+  // tiles that all met the longest would have.  A part costs its sums' way to memory and back, 130 KB in each of the places, as much as 15 tiles, parts
+  // at all another 25; with a part to each place (less a few: they do not fill evenly) the longest is waited for, with more (causal, or lengths that
+  // differ) half of one, else whole rounds.  us whole / in parts: 4 x 4,096 tokens, causal, 32 heads on 8 of 128, 1,782 / 1,792 in 2; 8 x 1,024
+  // 290 / 322 in 3; 8 from 100 to 4,096 1,179 / 1,106 in 4; one of 8,192 1,996 / 1,767 in 7; that, 8 on 1, 2,384 / 525 in 12; one of 2,048, no
+  // mask, 32 on 8, 378 / 235 in 4, 252 in 3, 248 in 6.
+  const int places = p->head_dim > 64 ? 512 : 768;
+  const double even = std::min(1.0, (double)p->k_rows / std::max(1.0, (double)max_k * p->sequences));
+  const double place = (double)b.tiles * walk / (p->causal ? 2 : 1) / places * (1 + even) / 2;
   const int64_t sums = 2 * std::max<int64_t>((int64_t)p->k_rows * p->kv_heads * p->head_dim, 1);
-  if (walk > place) {
-    // (a GiB of sums at most, whatever the hints are)
-    const int64_t parts = std::max<int64_t>((1ll << 28) / sums, 1);
-    const int64_t piece = std::max({(int64_t)(place / std::max(1.0, std::sqrt(0.02 * place))), (int64_t)16, (walk + parts - 1) / parts});
-    if (piece < walk) {
-      b.piece_tiles = (int)piece;
-      b.pieces = (int)((walk + piece - 1) / piece);
+  const int64_t most_parts = std::min({(int64_t)64, walk / 16, (int64_t)((1 << 28) / sums)});  // (a GiB of sums at most, whatever the hints are)
+  double best = 1.05 * std::max((double)walk, place);
+  for (int n = 2; n <= most_parts; ++n) {
+    const double part = (double)walk / n, parts = b.tiles * (p->causal ? 0.5 * (n + 1) : n);
+    const double end = 25 + (parts <= 0.95 * places || (!p->causal && parts <= places) ? part + 15
+                             : p->causal || even < 0.95                               ? place + 15 * parts / places + 0.5 * part
+                                                                                      : std::ceil(parts / places) * (part + 15));
+    if (end < best) {
+      best = end;
+      b.pieces = n;
     }
   }
+  if (b.pieces > 1) b.piece_tiles = (int)((walk + b.pieces - 1) / b.pieces);
   b.floats = b.aux_floats + (b.pieces > 1 ? b.pieces * sums : 0);
   return b;
 }
@@ -546,7 +555,8 @@ int launch(hipStream_t st, const PackedBwdArgs& a, int64_t dq_grid, int64_t dkv_
   MDATTN_LAUNCH((packed_dkv_kernel<HD, DC, PADDED>), dim3((unsigned)dkv_grid, (unsigned)a.pieces), dim3(256), bytes, st, a);
   const int rc = launch_status();
   if (rc != MDATTN_OK || a.pieces == 1) return rc;
-  MDATTN_LAUNCH(packed_reduce_kernel, dim3((unsigned)dkv_grid, 2), dim3(256), 0, st, a);
+  const unsigned share = dkv_grid < 32 ? 8 : dkv_grid < 256 ? (unsigned)(256 / dkv_grid) : 1;
+  MDATTN_LAUNCH(packed_reduce_kernel, dim3((unsigned)dkv_grid, 2, share), dim3(256), 0, st, a);
   return launch_status();
 }
 
@@ -595,7 +605,7 @@ extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   a.pieces = b.pieces; a.piece_tiles = b.piece_tiles;
   const int64_t dq_grid = p->q_rows ? packed_tiles((int64_t)p->q_rows * a.group.d, p->sequences, 128) * p->kv_heads : 0;
   const int64_t dkv_grid = p->k_rows ? packed_tiles(p->k_rows, p->sequences, 128) * p->kv_heads : 0;
-  if (!grid_fits(dq_grid, 256) || !grid_fits(dkv_grid, 256) || b.pieces > 65535) return MDATTN_E_UNSUPPORTED;
+  if (!grid_fits(dq_grid, 256) || !grid_fits(dkv_grid, 256)) return MDATTN_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   if (a.D == 64) return launch<64, 64, false>(st, a, dq_grid, dkv_grid);
   if (a.D < 64) return launch<64, 64, true>(st, a, dq_grid, dkv_grid);
