@@ -37,26 +37,27 @@ typedef struct {
 } mdattn_packed;
 
 /*
- * out = softmax(scale * q k^T) v over each sequence; bf16.  lse f32 [heads, q_rows], or NULL: the logarithm of each row's sum.  Rows
+ * out = softmax(scale * q k^T) v over each sequence; bf16.  rest, strided like out, or NULL: what the rounding of out left, rounded to bf16, for the
+ * backward pass (of rows of no sequence it is not written).  lse f32 [heads, q_rows], or NULL: the logarithm of each row's sum.  Rows
  * that see no key, and rows of no sequence: out 0, lse -inf.  Logits, softmax and sums in f32, P rounded to bf16 before its product.
  *   workspace     mdattn_fwd_bf16_packed_workspace_floats floats (0 where one is not needed), with which few rows against many keys are
  *                 split over the keys; with less they are not.  16-byte aligned.
  * A key or value that is infinite or NaN may spoil the rows of its sequence that do not see it.
  */
 int64_t mdattn_fwd_bf16_packed_workspace_floats(const mdattn_packed* p);
-int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, const void* q, const void* k, const void* v, void* out, float* lse,
-                           const mdattn_strides* q_strides, const mdattn_strides* k_strides, const mdattn_strides* v_strides,
+int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, const void* q, const void* k, const void* v, void* out, void* rest,
+                           float* lse, const mdattn_strides* q_strides, const mdattn_strides* k_strides, const mdattn_strides* v_strides,
                            const mdattn_strides* o_strides, float scale, float* workspace, int64_t workspace_floats);
 
 /*
- * Backward of mdattn_fwd_bf16_packed: dq, dk, dv (bf16, strided like q, k and v) from its inputs, out, lse and the gradient of
- * out (strided like it).  k_lengths has to be NULL.  Rows of no sequence get zeros.  Deterministic: sums over the rows and over the
+ * Backward of mdattn_fwd_bf16_packed: dq, dk, dv (bf16, strided like q, k and v) from its inputs, out, rest, lse and the
+ * gradient of out (strided like it, as rest is).  rest may be NULL, for gradients that are further off where a key has most of a row's weight.  k_lengths has to be NULL.  Rows of no sequence get zeros.  Deterministic: sums over the rows and over the
  * heads of a group are made in a fixed order.
  *   workspace     mdattn_bwd_bf16_packed_workspace_floats floats; 16-byte aligned
  */
 int64_t mdattn_bwd_bf16_packed_workspace_floats(const mdattn_packed* p);
-int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, const void* q, const void* k, const void* v, const void* out, const void* dout,
-                           const float* lse, void* dq, void* dk, void* dv, const mdattn_strides* q_strides, const mdattn_strides* k_strides,
+int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, const void* q, const void* k, const void* v, const void* out, const void* rest,
+                           const void* dout, const float* lse, void* dq, void* dk, void* dv, const mdattn_strides* q_strides, const mdattn_strides* k_strides,
                            const mdattn_strides* v_strides, const mdattn_strides* o_strides, const mdattn_strides* dq_strides,
                            const mdattn_strides* dk_strides, const mdattn_strides* dv_strides, float scale, float* workspace,
                            int64_t workspace_floats);

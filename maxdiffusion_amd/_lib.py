@@ -86,9 +86,9 @@ LAYER_SIGNATURES = {
 # symbol -> argtypes; every symbol include/mdpacked.h declares
 PACKED_SIGNATURES = {
     "mdattn_fwd_bf16_packed_workspace_floats": ([_K], _L),
-    "mdattn_fwd_bf16_packed": ([_P, _K, _P, _P, _P, _P, _P, _S, _S, _S, _S, _F, _P, _L], _I),
+    "mdattn_fwd_bf16_packed": ([_P, _K, _P, _P, _P, _P, _P, _P, _S, _S, _S, _S, _F, _P, _L], _I),
     "mdattn_bwd_bf16_packed_workspace_floats": ([_K], _L),
-    "mdattn_bwd_bf16_packed": ([_P, _K, _P, _P, _P, _P, _P, _P, _P, _P, _P, _S, _S, _S, _S, _S, _S, _S, _F, _P, _L], _I),
+    "mdattn_bwd_bf16_packed": ([_P, _K, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _S, _S, _S, _S, _S, _S, _S, _F, _P, _L], _I),
 }
 
 # what csrc/mdattn_host.h declares: entry points for this package's own host side

@@ -230,12 +230,13 @@ def _wants_grad(*ts) -> bool:
 
 
 class _HipFlashPacked(torch.autograd.Function):
-  """Saved for the backward: q, k, v, the offsets, out, lse."""
+  """Saved for the backward: q, k, v, the offsets, out, what its rounding left, lse."""
 
   @staticmethod
   def forward(ctx, q, k, v, q_offsets, k_offsets, causal, scale, max_q, max_k):
-    out, lse = ops.flash_attention_packed(q, k, v, q_offsets, k_offsets, causal=causal, scale=scale, max_q=max_q, max_k=max_k, return_lse=True)
-    ctx.save_for_backward(q, k, v, q_offsets, k_offsets, out, lse)
+    out, lse, rest = ops.flash_attention_packed(q, k, v, q_offsets, k_offsets, causal=causal, scale=scale, max_q=max_q, max_k=max_k, return_lse=True,
+                                                return_rest=True)
+    ctx.save_for_backward(q, k, v, q_offsets, k_offsets, out, lse, rest)
     ctx.cfg = dict(causal=causal, scale=scale, max_q=max_q, max_k=max_k)
     ctx.shapes = (q.shape, k.shape, q_offsets.shape)
     return out
@@ -243,10 +244,10 @@ class _HipFlashPacked(torch.autograd.Function):
   @staticmethod
   @_lib.first_order
   def backward(ctx, dout):
-    q, k, v, q_offsets, k_offsets, out, lse = ctx.saved_tensors
+    q, k, v, q_offsets, k_offsets, out, lse, rest = ctx.saved_tensors
     if (q.shape, k.shape, q_offsets.shape) != ctx.shapes:
       raise ValueError("a tensor saved for the backward pass came back from its hook with another dtype, shape or layout")
-    dq, dk, dv = ops.flash_attention_packed_backward(q, k, v, out, dout.to(torch.bfloat16), lse, q_offsets, k_offsets, **ctx.cfg)
+    dq, dk, dv = ops.flash_attention_packed_backward(q, k, v, out, dout.to(torch.bfloat16), lse, q_offsets, k_offsets, rest=rest, **ctx.cfg)
     return dq, dk, dv, None, None, None, None, None, None
 
 

@@ -26,7 +26,7 @@ constexpr float kRange = 16777216.f;  // a partial sum of P above 2^24 moves the
 
 struct PackedArgs {
   const __bf16 *q, *k, *v;
-  __bf16* out;
+  __bf16 *out, *rest;
   float* lse;
   PackedSeqs seqs;
   Divisor group;
@@ -115,6 +115,10 @@ __device__ __forceinline__ void load_row(bf16x8 (&f)[NJ], const __bf16* p, int h
   for (int j = 0; j < NJ; ++j) asm volatile("" : "+v"(f[j]));
 }
 
+// A pair of bf16 as floats
+__device__ __forceinline__ float low_half(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high_half(unsigned u) { return __uint_as_float(u & 0xFFFF0000u); }
+
 // A wave's 32 rows from row r0 of the sequence on, normalised, rounded and stored as whole rows through `stage` (32 rows of kOutRow bytes that
 // nobody else touches any more): as the accumulators lie, a store would touch 16 bytes of each of 32 rows.
 template <int ND>
@@ -130,26 +134,37 @@ __device__ __forceinline__ void store_out(const PackedArgs& a, const SeqTile& s,
     const int t = (int)div_by((unsigned)(r0 + l32), a.group);
     a.lse[(int64_t)(head * G + r0 + l32 - t * G) * a.seqs.q_rows + s.q0 + t] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * kLn2;
   }
-#pragma unroll
-  for (int db = 0; db < ND; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      uint2 u;
-      u.x = pack2(O[db][4 * g] * inv, O[db][4 * g + 1] * inv);
-      u.y = pack2(O[db][4 * g + 2] * inv, O[db][4 * g + 3] * inv);
-      *reinterpret_cast<uint2*>(stage + l32 * RowB + hh * 8 + (db * 32 + g * 8) * 2) = u;
-    }
-  // LDS accesses of one wave execute in order: the reads below see the writes above
   const int rr = lane / LPR, cc = lane % LPR;
-  if (cc * 8 >= (PADDED ? a.D : DC)) return;
+  auto put = [&](__bf16* out, bool rest) __attribute__((always_inline)) {
 #pragma unroll
-  for (int j = 0; j < 32 / RPI; ++j) {
-    const int row = r0 + j * RPI + rr;
-    if (row >= rows) break;
-    const int t = (int)div_by((unsigned)row, a.group);
-    st_nt(reinterpret_cast<uint4*>(a.out + (int64_t)(s.q0 + t) * a.os.row + (int64_t)(head * G + row - t * G) * a.os.head + cc * 8),
-          *reinterpret_cast<const uint4*>(stage + (j * RPI + rr) * RowB + cc * 16));
-  }
+    for (int db = 0; db < ND; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float f[4];
+        uint2 u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = O[db][4 * g + e] * inv;
+        u.x = pack2(f[0], f[1]);
+        u.y = pack2(f[2], f[3]);
+        if (rest) {
+          u.x = pack2(f[0] - low_half(u.x), f[1] - high_half(u.x));
+          u.y = pack2(f[2] - low_half(u.y), f[3] - high_half(u.y));
+        }
+        *reinterpret_cast<uint2*>(stage + l32 * RowB + hh * 8 + (db * 32 + g * 8) * 2) = u;
+      }
+    // LDS accesses of one wave execute in order: the reads below see the writes above, and those of another call the reads
+    if (cc * 8 >= (PADDED ? a.D : DC)) return;
+#pragma unroll
+    for (int j = 0; j < 32 / RPI; ++j) {
+      const int row = r0 + j * RPI + rr;
+      if (row >= rows) break;
+      const int t = (int)div_by((unsigned)row, a.group);
+      st_nt(reinterpret_cast<uint4*>(out + (int64_t)(s.q0 + t) * a.os.row + (int64_t)(head * G + row - t * G) * a.os.head + cc * 8),
+            *reinterpret_cast<const uint4*>(stage + (j * RPI + rr) * RowB + cc * 16));
+    }
+  };
+  put(a.out, false);
+  if (a.rest) put(a.rest, true);
 }
 
 template <int HD, int DC, bool PADDED, int KW>
@@ -500,7 +515,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] *= inv;
       const int t = token_of(row), h = head * G + row - t * G;
-      *reinterpret_cast<uint4*>(a.out + (int64_t)(s.q0 + t) * a.os.row + (int64_t)h * a.os.head + at) = pack8(f);
+      const int64_t to = (int64_t)(s.q0 + t) * a.os.row + (int64_t)h * a.os.head + at;
+      const uint4 u = pack8(f);
+      *reinterpret_cast<uint4*>(a.out + to) = u;
+      if (a.rest) {
+        float rounded[8];
+        unpack8(u, rounded);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] -= rounded[e];
+        *reinterpret_cast<uint4*>(a.rest + to) = pack8(f);
+      }
       if (at == 0 && a.lse) a.lse[(int64_t)h * a.seqs.q_rows + s.q0 + t] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
     }
     __syncthreads();  // the next piece's keys go where the rows were staged
@@ -553,7 +577,10 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(PackedArgs a) {
     f1 += part[w][c + 1];
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  *reinterpret_cast<unsigned*>(a.out + (int64_t)t * a.os.row + (int64_t)h * a.os.head + c) = pack2(f0 * inv, f1 * inv);
+  const int64_t to = (int64_t)t * a.os.row + (int64_t)h * a.os.head + c;
+  const unsigned both = pack2(f0 * inv, f1 * inv);
+  *reinterpret_cast<unsigned*>(a.out + to) = both;
+  if (a.rest) *reinterpret_cast<unsigned*>(a.rest + to) = pack2(f0 * inv - low_half(both), f1 * inv - high_half(both));
   if (c == 0 && a.lse) a.lse[(int64_t)h * a.seqs.q_rows + t] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
 }
 
@@ -591,7 +618,7 @@ FwdPlan fwd_plan(const mdattn_packed* p) {
   // some two workgroups per CU of caches that are half full, or, where the sequences alone are as many, small pieces that even them out: us in pieces of
   // 128 / 256 / 512 / 768 keys, 16 tokens with caches of up to 4,096 keys of 8 heads 18.8 / 15.0 / 14.1 / 16.0; 14 with 1,078 of 4 11.3 / 12.0 / 13.6 /
   // 15.4; 68 with 1,241 of 8 in pieces of 384 31.8, of 768 35.8
-  const int64_t share = (int64_t)p->sequences * p->kv_heads <= 256 ? 1024 : 2048;
+  const int64_t share = (int64_t)p->sequences * p->kv_heads <= 512 ? 1024 : 2048;
   const int64_t keys = (std::max({all / share, (int64_t)1, (max_k + most - 1) / most}) + 127) / 128 * 128;
   f.pieces = (int)((max_k + keys - 1) / keys);
   f.piece_keys = (int)keys;
@@ -618,15 +645,15 @@ extern "C" int64_t mdattn_fwd_bf16_packed_workspace_floats(const mdattn_packed* 
   return packed_sizes(p) == MDATTN_OK ? fwd_plan(p).floats : 0;
 }
 
-extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, const void* q, const void* k, const void* v, void* out, float* lse,
-                                      const mdattn_strides* q_strides, const mdattn_strides* k_strides, const mdattn_strides* v_strides,
+extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, const void* q, const void* k, const void* v, void* out, void* rest,
+                                      float* lse,                                      const mdattn_strides* q_strides, const mdattn_strides* k_strides, const mdattn_strides* v_strides,
                                       const mdattn_strides* o_strides, float scale, float* workspace, int64_t workspace_floats) {
   const int rc = packed_sizes(p);
   if (rc != MDATTN_OK) return rc;
   if (!(scale > 0.f) || !(scale < INFINITY) || !q_strides || !k_strides || !v_strides || !o_strides) return MDATTN_E_BADARG;
   if (p->q_rows == 0) return MDATTN_OK;  // nothing to be written
   if (!q || !out || (p->k_rows && (!k || !v))) return MDATTN_E_BADARG;
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !packed_aligned(p) || (reinterpret_cast<uintptr_t>(lse) & 3) ||
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(rest) || !packed_aligned(p) || (reinterpret_cast<uintptr_t>(lse) & 3) ||
       !packed_strides_ok(q_strides) || !packed_strides_ok(k_strides) || !packed_strides_ok(v_strides) || !packed_strides_ok(o_strides))
     return MDATTN_E_ALIGN;
   FwdPlan f = fwd_plan(p);
@@ -638,7 +665,7 @@ extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   }
   PackedArgs a{};
   a.q = static_cast<const __bf16*>(q); a.k = static_cast<const __bf16*>(k); a.v = static_cast<const __bf16*>(v);
-  a.out = static_cast<__bf16*>(out); a.lse = lse;
+  a.out = static_cast<__bf16*>(out); a.rest = static_cast<__bf16*>(rest); a.lse = lse;
   a.seqs = {p->q_offsets, p->k_offsets, p->k_lengths, p->sequences, p->q_rows, p->k_rows, f.kind == kFew ? kAsTheyCome : packed_order(p, f.tiles * (f.kind == kHalf && p->causal ? 2 : 1)), 256 / p->kv_heads};
   a.group = divisor((unsigned)(p->heads / p->kv_heads));
   a.kv_heads = p->kv_heads; a.D = p->head_dim; a.causal = p->causal;

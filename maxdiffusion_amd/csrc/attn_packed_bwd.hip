@@ -12,9 +12,10 @@
 // Blocks that no row of a wave sees, or no key of it is seen by, are not computed.
 // The dk / dv pass has a workgroup per 128 keys and head of k and v, of which the first ones of a causal sequence walk all of its tokens in every
 // head: these walks are cut into pieces, whose f32 sums a third kernel adds up in their order.
-// Roundings.  P and dS go into their products in bf16, and delta comes from the rounded out: at causal sequences of 600 tokens with a direction
-// that all logits share (so that sum(ds) = 0 cancels most of dq) each of the two costs dq 1.7e-3 of its size, as much as its own rounding.  dS in two
-// parts would cost a third more matrix products.
+// Roundings.  P and dS go into their products in bf16.  delta takes out and what its rounding left (rest): dS = p (dp - delta) is small beside both
+// where a key has most of a row's weight, and with the rounded out alone dq of sequences of 3, 8, 64 and 600 tokens, causal, with a direction that all
+// logits share, is off by 8.1, 6.3, 3.9 and 2.8e-3 of its size, with rest by 2.5, 2.5, 2.4 and 2.4 (its own rounding 1.7).  dS in two parts would
+// bring that to 1.7, for a third more matrix products.
 // Bound.  A tile costs LDS as many cycles as the matrix pipes: 1 KB of fragments read per product of 32 cycles and wave, 128 bytes a cycle with
 // four waves.  100 to 4,096 tokens x 8 sequences, 32 heads on 8, causal: dq 221 us (1.05 PFLOP/s, pipes busy 50 % of the cycles), dk / dv 337 us
 // (0.92, 41 %), the pieces' sums 22 us.
@@ -27,7 +28,7 @@ namespace mdattn {
 namespace {
 
 struct PackedBwdArgs {
-  const __bf16 *q, *k, *v, *out, *dout;
+  const __bf16 *q, *k, *v, *out, *rest, *dout;
   const float* lse;
   __bf16 *dq, *dk, *dv;
   float* aux;  // [2][heads][q_rows]: -lse / scale, -delta
@@ -171,6 +172,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
       const bf16x8 of = load_frag<PADDED>(po, j * 16 + hh * 8, a.D);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ndelta = __builtin_fmaf(-(float)of[e], (float)gf[j][e], ndelta);
+    }
+    if (a.rest) {
+      const __bf16* pr = a.rest + row * a.os.row + h * a.os.head;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const bf16x8 rf = load_frag<PADDED>(pr, j * 16 + hh * 8, a.D);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ndelta = __builtin_fmaf(-(float)rf[e], (float)gf[j][e], ndelta);
+      }
     }
   }
   ndelta = xhalf_sum(ndelta);
@@ -570,7 +580,7 @@ extern "C" int64_t mdattn_bwd_bf16_packed_workspace_floats(const mdattn_packed* 
 }
 
 extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, const void* q, const void* k, const void* v, const void* out,
-                                      const void* dout, const float* lse, void* dq, void* dk, void* dv, const mdattn_strides* q_strides,
+                                      const void* rest, const void* dout, const float* lse, void* dq, void* dk, void* dv, const mdattn_strides* q_strides,
                                       const mdattn_strides* k_strides, const mdattn_strides* v_strides, const mdattn_strides* o_strides,
                                       const mdattn_strides* dq_strides, const mdattn_strides* dk_strides, const mdattn_strides* dv_strides,
                                       float scale, float* workspace, int64_t workspace_floats) {
@@ -583,7 +593,7 @@ extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, cons
     if (!packed_strides_ok(s, s == q_strides || s == o_strides ? p->heads / p->kv_heads : 0)) return MDATTN_E_ALIGN;
   }
   if ((p->q_rows && (!q || !out || !dout || !lse || !dq)) || (p->k_rows && (!k || !v || !dk || !dv))) return MDATTN_E_BADARG;
-  for (const void* t : {q, k, v, out, dout, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)workspace})
+  for (const void* t : {q, k, v, out, rest, dout, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)workspace})
     if (!aligned16(t)) return MDATTN_E_ALIGN;
   if (!packed_aligned(p) || (reinterpret_cast<uintptr_t>(lse) & 3)) return MDATTN_E_ALIGN;
   if (p->q_rows == 0 && p->k_rows == 0) return MDATTN_OK;
@@ -591,7 +601,7 @@ extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   if (!workspace || workspace_floats < b.floats) return MDATTN_E_BADARG;
   PackedBwdArgs a{};
   a.q = static_cast<const __bf16*>(q); a.k = static_cast<const __bf16*>(k); a.v = static_cast<const __bf16*>(v);
-  a.out = static_cast<const __bf16*>(out); a.dout = static_cast<const __bf16*>(dout); a.lse = lse;
+  a.out = static_cast<const __bf16*>(out); a.rest = static_cast<const __bf16*>(rest); a.dout = static_cast<const __bf16*>(dout); a.lse = lse;
   a.dq = static_cast<__bf16*>(dq); a.dk = static_cast<__bf16*>(dk); a.dv = static_cast<__bf16*>(dv);
   a.aux = workspace;
   a.part = workspace + b.aux_floats;

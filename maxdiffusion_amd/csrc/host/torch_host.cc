@@ -411,12 +411,14 @@ bool packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
        (int)k.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), causal, hint(max_q), hint(max_k)};
   return true;
 }
-int packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const mdattn_packed& p, double scale, const Tensor& out, const Tensor& lse) {
+int packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const mdattn_packed& p, double scale, const Tensor& out, const Tensor& rest,
+               const Tensor& lse) {
   const int64_t nws = mdattn_fwd_bf16_packed_workspace_floats(&p);
   const Tensor ws = nws ? at::empty({nws}, q.options().dtype(at::kFloat)) : Tensor();
   const mdattn_strides sq = row_strides(q), sk = row_strides(k), sv = row_strides(v), so = row_strides(out);
-  return mdattn_fwd_bf16_packed(stream(q), &p, ptr(q), ptr(k), ptr(v), mut(out), f32(lse), &sq, &sk, &sv, &so, (float)scale, f32(ws), nws);
+  return mdattn_fwd_bf16_packed(stream(q), &p, ptr(q), ptr(k), ptr(v), mut(out), mut(rest), f32(lse), &sq, &sk, &sv, &so, (float)scale, f32(ws), nws);
 }
+bool dense_like(const Tensor& t, const Tensor& q) { return bf16_on(t, q) && t.is_contiguous() && t.sizes() == q.sizes() && aligned(t); }
 struct PackedFn : FirstOrder<PackedFn> {
   struct Values {
     double scale;
@@ -429,19 +431,20 @@ struct PackedFn : FirstOrder<PackedFn> {
                         double scale, int64_t max_q, int64_t max_k) {
     mdattn_packed p;
     packed_args(q, k, v, qo, ko, Tensor(), causal, max_q, max_k, p);
-    Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
-    if (packed_fwd(q, k, v, p, scale, out, lse) != MDATTN_OK) throw Refused{};
-    ctx->save_for_backward({q, k, v, qo, ko, out, lse});
+    Tensor out = at::empty(q.sizes(), q.options()), rest = at::empty(q.sizes(), q.options()),
+           lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+    if (packed_fwd(q, k, v, p, scale, out, rest, lse) != MDATTN_OK) throw Refused{};
+    ctx->save_for_backward({q, k, v, qo, ko, out, lse, rest});
     keep(ctx, Values{scale, causal, max_q, max_k, Shape8(q), Shape8(k), qo.size(0)});
     return out;
   }
   static variable_list gradients(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Values c = kept<Values>(ctx);
-    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &qo = saved[3], &ko = saved[4], &out = saved[5], &lse = saved[6];
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &qo = saved[3], &ko = saved[4], &out = saved[5], &lse = saved[6], &rest = saved[7];
     mdattn_packed p;
-    unpacked(packed_args(q, k, v, qo, ko, Tensor(), c.causal, c.max_q, c.max_k, p) && q.sizes() == c.q.get() && k.sizes() == c.k.get() && qo.size(0) == c.offsets && bf16_on(out, q) && out.is_contiguous() && out.sizes() == q.sizes() &&
-             aligned(out) && lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+    unpacked(packed_args(q, k, v, qo, ko, Tensor(), c.causal, c.max_q, c.max_k, p) && q.sizes() == c.q.get() && k.sizes() == c.k.get() && qo.size(0) == c.offsets &&
+             dense_like(out, q) && dense_like(rest, q) && lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
              lse.numel() == q.size(0) * q.size(1));
     Tensor dout = grads[0];
     if (dout.scalar_type() != at::kBFloat16) dout = dout.to(at::kBFloat16);
@@ -452,7 +455,7 @@ struct PackedFn : FirstOrder<PackedFn> {
     const int64_t nws = mdattn_bwd_bf16_packed_workspace_floats(&p);
     const Tensor ws = at::empty({nws}, lse.options());
     const mdattn_strides sq = row_strides(q), sk = row_strides(k), sv = row_strides(v), so = row_strides(out), dqs = row_strides(dq), dks = row_strides(dk);
-    must(mdattn_bwd_bf16_packed(stream(q), &p, ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), f32(lse), mut(dq), mut(dk), mut(dv), &sq, &sk, &sv, &so, &dqs, &dks,
+    must(mdattn_bwd_bf16_packed(stream(q), &p, ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(dout), f32(lse), mut(dq), mut(dk), mut(dv), &sq, &sk, &sv, &so, &dqs, &dks,
                                 &dks, (float)c.scale, f32(ws), nws),
          "mdattn_bwd_bf16_packed");
     return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
@@ -471,7 +474,7 @@ OptTensor flash_packed(const Tensor& q, const Tensor& k, const Tensor& v, const 
   }
   at::NoGradGuard guard;
   Tensor out = at::empty(q.sizes(), q.options());
-  if (packed_fwd(q, k, v, p, scale, out, Tensor()) != MDATTN_OK) return std::nullopt;
+  if (packed_fwd(q, k, v, p, scale, out, Tensor(), Tensor()) != MDATTN_OK) return std::nullopt;
   return out;
 }
 

@@ -641,7 +641,7 @@ def _packed(q, k, v, q_offsets, k_offsets, k_lengths, causal, max_q, max_k) -> _
 
 
 def flash_attention_packed(q, k, v, q_offsets, k_offsets=None, *, k_lengths=None, causal: bool = True, scale: float | None = None,
-                           max_q: int | None = None, max_k: int | None = None, return_lse: bool = False):
+                           max_q: int | None = None, max_k: int | None = None, return_lse: bool = False, return_rest: bool = False):
   """softmax(scale * q k^T) v over sequences that lie one behind the other.  q [Tq, H, D], k, v [Tk, Hkv, D], bf16, any strides of rows and heads;
   H a multiple of Hkv (head h of q meets head h // (H // Hkv)), D a multiple of 8 up to 128.
 
@@ -650,30 +650,33 @@ def flash_attention_packed(q, k, v, q_offsets, k_offsets=None, *, k_lengths=None
   sequence with m queries and n keys, query i sees the keys up to i + n - m.  max_q, max_k: the longest sequence's queries and keys, if the
   caller knows them; they choose how the work is cut and no result depends on them but for its roundings.
 
-  Returns out [Tq, H, D] and, if asked, lse f32 [H, Tq] (natural log).  Rows that see no key and rows of no sequence: 0 and -inf."""
+  Returns out [Tq, H, D] and, if asked, lse f32 [H, Tq] (natural log) and what the rounding of out left (bf16, for the backward pass; rows of no
+  sequence undefined).  Rows that see no key and rows of no sequence: 0 and -inf."""
   k_offsets = q_offsets if k_offsets is None else k_offsets
   p = _packed(q, k, v, q_offsets, k_offsets, k_lengths, causal, max_q, max_k)
   q, k, v = (_packed_rows(t) for t in (q, k, v))
   out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
   lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if return_lse else None
+  rest = torch.empty_like(out) if return_rest else None
   lib = _lib.load()
   nws = lib.mdattn_fwd_bf16_packed_workspace_floats(ctypes.byref(p))
   ws = torch.empty(nws, dtype=torch.float32, device=q.device) if nws else None
   st = [ctypes.byref(_row_strides(t)) for t in (q, k, v, out)]
-  rc = lib.mdattn_fwd_bf16_packed(_stream(), ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), *st,
+  rc = lib.mdattn_fwd_bf16_packed(_stream(), ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(lse), *st,
                                   float(q.shape[2]**-0.5 if scale is None else scale), _ptr(ws), nws)
   _lib.check(rc, "mdattn_fwd_bf16_packed")
-  return (out, lse) if return_lse else out
+  results = (out, *(t for t in (lse, rest) if t is not None))
+  return results if len(results) > 1 else out
 
 
-def flash_attention_packed_backward(q, k, v, out, dout, lse, q_offsets, k_offsets=None, *, causal: bool = True, scale: float | None = None,
+def flash_attention_packed_backward(q, k, v, out, dout, lse, q_offsets, k_offsets=None, *, rest=None, causal: bool = True, scale: float | None = None,
                                     max_q: int | None = None, max_k: int | None = None):
-  """Backward of `flash_attention_packed`: its inputs, its out and lse, and the gradient of out (bf16).  Returns (dq, dk, dv), bf16, dense; rows
-  of no sequence get zeros."""
+  """Backward of `flash_attention_packed`: its inputs, its out, lse and rest (None: gradients are further off where a key has most of a row's
+  weight), and the gradient of out (bf16).  Returns (dq, dk, dv), bf16, dense; rows of no sequence get zeros."""
   k_offsets = q_offsets if k_offsets is None else k_offsets
   p = _packed(q, k, v, q_offsets, k_offsets, None, causal, max_q, max_k)
-  _check_dev(q, out, dout, lse)
-  for name, t in (("out", out), ("dout", dout)):
+  _check_dev(q, out, dout, lse, rest)
+  for name, t in (("out", out), ("dout", dout), *((("rest", rest),) if rest is not None else ())):
     if t.shape != q.shape or t.dtype != torch.bfloat16:
       raise ValueError(f"{name} must be bf16 and shaped like q, {tuple(q.shape)}, got {tuple(t.shape)} {t.dtype}")
   if lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[1], q.shape[0]) or not lse.is_contiguous():
@@ -681,14 +684,15 @@ def flash_attention_packed_backward(q, k, v, out, dout, lse, q_offsets, k_offset
   group = q.shape[1] // k.shape[1]
   q, k, v = _packed_rows(q, group), _packed_rows(k), _packed_rows(v)
   out, dout = _packed_rows(out, group), _packed_rows(dout, group)
-  if _packed_strides(out) != _packed_strides(dout):
-    out, dout = out.contiguous(), dout.contiguous()
+  rest = rest if rest is None else _packed_rows(rest, group)
+  if any(t is not None and _packed_strides(t) != _packed_strides(out) for t in (dout, rest)):
+    out, dout, rest = (t if t is None else t.contiguous() for t in (out, dout, rest))
   dq, dk, dv = (torch.empty(t.shape, dtype=torch.bfloat16, device=q.device) for t in (q, k, v))
   lib = _lib.load()
   nws = lib.mdattn_bwd_bf16_packed_workspace_floats(ctypes.byref(p))
   ws = torch.empty(max(nws, 4), dtype=torch.float32, device=q.device)
   st = [ctypes.byref(_row_strides(t)) for t in (q, k, v, out, dq, dk, dv)]
-  rc = lib.mdattn_bwd_bf16_packed(_stream(), ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), _ptr(lse), _ptr(dq), _ptr(dk),
+  rc = lib.mdattn_bwd_bf16_packed(_stream(), ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(dout), _ptr(lse), _ptr(dq), _ptr(dk),
                                   _ptr(dv), *st, float(q.shape[2]**-0.5 if scale is None else scale), _ptr(ws), nws)
   _lib.check(rc, "mdattn_bwd_bf16_packed")
   return dq, dk, dv

@@ -11,9 +11,10 @@ def spans(offsets, rows):
   return [(a, b) for a, b in zip(offsets, offsets[1:])]
 
 
-def attention(q, k, v, q_off, k_off, k_len=None, causal=True, scale=None, dout=None):
+def attention(q, k, v, q_off, k_off, k_len=None, causal=True, scale=None, dout=None, rest=True):
   """q [Tq,H,D], k, v [Tk,Hkv,D] (any type), offsets as lists -> dict of results in 64 bits and of the errors that the kernels' roundings may make:
-  P and dS rounded to bf16 in front of their products, outputs rounded to bf16, everything else in f32."""
+  P and dS rounded to bf16 in front of their products, outputs rounded to bf16, everything else in f32; delta from out and, with `rest`, what
+  out's rounding left (rounded in its turn: U squared)."""
   q, k, v = (t.detach().double() for t in (q, k, v))
   tq, h, d = q.shape
   hkv = k.shape[1]
@@ -46,8 +47,8 @@ def attention(q, k, v, q_off, k_off, k_len=None, causal=True, scale=None, dout=N
         continue
       G = g[a:b, j]
       ds = p * (G @ V.T - (G * o).sum(1, keepdim=True))
-      # dS is rounded, and delta comes from the rounded out
-      ds_err = U * ds.abs() + p * (G.abs() * o_err).sum(1, keepdim=True)
+      # dS is rounded, and delta comes from an out made with rounded P, itself rounded
+      ds_err = U * ds.abs() + p * (G.abs() * (U * (p @ V.abs()) + U * (U if rest else 1) * o.abs())).sum(1, keepdim=True)
       r["dv"][c:e, kv] += p.T @ G
       r["dv_err"][c:e, kv] += U * (p.T @ G.abs())
       r["dq"][a:b, j] = scale * ds @ K

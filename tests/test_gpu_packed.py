@@ -66,8 +66,8 @@ def test_backward(dev, batch, h, hkv, d):
   for causal in (True, False):
     print(batch, h, hkv, d, causal, flush=True)
     want = attention(q, k, v, qo, ko, causal=causal, dout=g)
-    out, lse = ops.flash_attention_packed(q, k, v, ints(dev, qo), ints(dev, ko), causal=causal, return_lse=True)
+    out, lse, rest = ops.flash_attention_packed(q, k, v, ints(dev, qo), ints(dev, ko), causal=causal, return_lse=True, return_rest=True)
     for hint in (None, 1):
-      got = ops.flash_attention_packed_backward(q, k, v, out, g, lse, ints(dev, qo), ints(dev, ko), causal=causal, max_q=hint, max_k=hint)
+      got = ops.flash_attention_packed_backward(q, k, v, out, g, lse, ints(dev, qo), ints(dev, ko), rest=rest, causal=causal, max_q=hint, max_k=hint)
       for name, t in zip(("dq", "dk", "dv"), got):
         assert_within(t, want[name], want[name + "_err"], f"{name} {batch} {h} {hkv} {d} {causal} {hint}")

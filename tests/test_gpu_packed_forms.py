@@ -39,10 +39,10 @@ def test_forms(dev, form, d):
   for causal in (True, False):
     print(form, d, causal, flush=True)
     want = attention(q, k, v, o, o, causal=causal, dout=g)
-    out, lse = ops.flash_attention_packed(q, k, v, offsets, causal=causal, max_q=max_q, max_k=max_k, return_lse=True)
+    out, lse, rest = ops.flash_attention_packed(q, k, v, offsets, causal=causal, max_q=max_q, max_k=max_k, return_lse=True, return_rest=True)
     assert_within(out, want["out"], want["out_err"], f"out {form} {d} {causal}")
     assert (lse - want["lse"]).abs().max() <= 1e-4  # f32 logits up to some 20
-    for name, t in zip(("dq", "dk", "dv"), ops.flash_attention_packed_backward(q, k, v, out, g, lse, offsets, causal=causal, max_q=max_q, max_k=max_k)):
+    for name, t in zip(("dq", "dk", "dv"), ops.flash_attention_packed_backward(q, k, v, out, g, lse, offsets, rest=rest, causal=causal, max_q=max_q, max_k=max_k)):
       assert_within(t, want[name], want[name + "_err"], f"{name} {form} {d} {causal}")
 
 
@@ -55,10 +55,10 @@ def test_other_lengths_of_the_keys_in_each_order(dev):
     for causal in (True, False):
       print(h, hkv, d, causal, flush=True)
       want = attention(q, k, v, qo, ko, causal=causal, dout=g)
-      out, lse = ops.flash_attention_packed(q, k, v, ints(dev, qo), ints(dev, ko), causal=causal, return_lse=True)
+      out, lse, rest = ops.flash_attention_packed(q, k, v, ints(dev, qo), ints(dev, ko), causal=causal, return_lse=True, return_rest=True)
       assert_within(out, want["out"], want["out_err"], f"out {h} {causal}")
       assert torch.equal(lse == -math.inf, want["lse"] == -math.inf)
-      for name, t in zip(("dq", "dk", "dv"), ops.flash_attention_packed_backward(q, k, v, out, g, lse, ints(dev, qo), ints(dev, ko), causal=causal)):
+      for name, t in zip(("dq", "dk", "dv"), ops.flash_attention_packed_backward(q, k, v, out, g, lse, ints(dev, qo), ints(dev, ko), rest=rest, causal=causal)):
         assert_within(t, want[name], want[name + "_err"], f"{name} {h} {causal}")
 
 

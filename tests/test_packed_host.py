@@ -40,14 +40,14 @@ def strides(seq=1024, head=128):
   return ctypes.byref(_lib.Strides(0, seq, head))
 
 
-def fwd(lib, p=None, q=FAKE, out=FAKE, st=None, scale=0.1, ws=None, nws=0):
+def fwd(lib, p=None, q=FAKE, out=FAKE, rest=None, st=None, scale=0.1, ws=None, nws=0):
   s = st or strides()
-  return lib.mdattn_fwd_bf16_packed(None, ctypes.byref(p or packed()), q, FAKE, FAKE, out, None, s, strides(), strides(), strides(), scale, ws, nws)
+  return lib.mdattn_fwd_bf16_packed(None, ctypes.byref(p or packed()), q, FAKE, FAKE, out, rest, None, s, strides(), strides(), strides(), scale, ws, nws)
 
 
-def bwd(lib, p=None, lse=FAKE, dq=FAKE, st=None, scale=0.1, ws=FAKE, nws=1 << 40):
+def bwd(lib, p=None, rest=None, lse=FAKE, dq=FAKE, st=None, scale=0.1, ws=FAKE, nws=1 << 40):
   s = strides()
-  return lib.mdattn_bwd_bf16_packed(None, ctypes.byref(p or packed()), FAKE, FAKE, FAKE, FAKE, FAKE, lse, dq, FAKE, FAKE, st or s, s, s, s, s, s, s, scale, ws, nws)
+  return lib.mdattn_bwd_bf16_packed(None, ctypes.byref(p or packed()), FAKE, FAKE, FAKE, FAKE, rest, FAKE, lse, dq, FAKE, FAKE, st or s, s, s, s, s, s, s, scale, ws, nws)
 
 
 @pytest.mark.parametrize("call", [fwd, bwd])
@@ -70,7 +70,7 @@ def test_bad_arguments_are_rejected_on_the_host(lib, call):
 
 def test_the_forms_own_refusals(lib):
   assert fwd(lib, q=None) == fwd(lib, out=None) == _lib.E_BADARG
-  assert fwd(lib, q=ODD) == _lib.E_ALIGN
+  assert fwd(lib, q=ODD) == fwd(lib, rest=ODD) == bwd(lib, rest=ODD) == _lib.E_ALIGN
   assert fwd(lib, packed(q_rows=0), q=None, out=None) == _lib.E_OK  # nothing to be done
   assert bwd(lib, packed(k_lengths=0x1000)) == _lib.E_BADARG
   assert bwd(lib, dq=None) == bwd(lib, lse=None) == bwd(lib, ws=None) == bwd(lib, nws=3) == _lib.E_BADARG
