@@ -81,6 +81,8 @@ int mdattn_rms_norm_e4m3(void* stream, const void* x, int x_is_f32, const void* 
  * Backward of mdattn_rms_norm.  With a = g * (w_offset + w) and h = s r:
  *   ds = r (a - h mean(a h)) + gs,  dw = sum of g h,  db = sum of g, over the rows that share w and b; x's gradient and the residual's are ds.
  *   s             the forward's sum (x, where it had no residual), bf16 or f32; r is computed again
+ *   residual      or NULL; beside an s in bf16 only: s is x, in bf16, to which it is added again, for gradients without s's rounding (dw in f32); its
+ *                 own strides
  *   g             gradient of y, bf16 or f32; of s's type, or bf16 beside an f32 s
  *   gs            gradient of s, of its type, or NULL
  *   ds            of s's type;  dx: the same rounded to bf16, where g is bf16 and s f32, or NULL
@@ -89,9 +91,9 @@ int mdattn_rms_norm_e4m3(void* stream, const void* x, int x_is_f32, const void* 
  * ds and dx are dense [groups, rows, C].  Deterministic.
  */
 int64_t mdattn_rms_norm_bwd_workspace_floats(int64_t groups, int64_t rows, int C);
-int mdattn_rms_norm_bwd(void* stream, const void* s, int s_is_f32, const void* g, int g_is_f32, const void* gs, void* ds, void* dx, const void* w,
-                        void* dw, void* db, int wb_is_f32, int64_t groups, int64_t rows, int C, int64_t s_stride_group, int64_t s_stride_row,
-                        int64_t g_stride_group, int64_t g_stride_row, int64_t gs_stride_group, int64_t gs_stride_row, int64_t wb_stride, float eps,
+int mdattn_rms_norm_bwd(void* stream, const void* s, int s_is_f32, const void* residual, const void* g, int g_is_f32, const void* gs, void* ds, void* dx,
+                        const void* w, void* dw, void* db, int wb_is_f32, int64_t groups, int64_t rows, int C, int64_t s_stride_group,
+                        int64_t s_stride_row, int64_t r_stride_group, int64_t r_stride_row, int64_t g_stride_group, int64_t g_stride_row, int64_t gs_stride_group, int64_t gs_stride_row, int64_t wb_stride, float eps,
                         float w_offset, float* workspace, int64_t workspace_floats);
 
 /*

@@ -76,7 +76,7 @@ LAYER_SIGNATURES = {
     "mdattn_rms_norm": ([_P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _L, _L, _I, _L, _L, _L, _L, _L, _L, _L, _L, _L, _F, _F], _I),
     "mdattn_rms_norm_e4m3": ([_P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _I, _L, _L, _I, _L, _L, _L, _L, _L, _L, _L, _F, _F], _I),
     "mdattn_rms_norm_bwd_workspace_floats": ([_L, _L, _I], _L),
-    "mdattn_rms_norm_bwd": ([_P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _L, _L, _I, _L, _L, _L, _L, _L, _L, _L, _F, _F, _P, _L], _I),
+    "mdattn_rms_norm_bwd": ([_P, _P, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _L, _L, _I, _L, _L, _L, _L, _L, _L, _L, _L, _L, _F, _F, _P, _L], _I),
     "mdattn_quant_block_e4m3": ([_P, _P, _I, _L, _L, _L, _I, _P, _P, _P, _P, _P], _I),
     "mdattn_sum_rows": ([_P, _P, _L, _L, _P, _I], _I),
     "mdattn_matmul_fp8_block_workspace_floats": ([_L, _L, _L], _L),

@@ -1005,13 +1005,14 @@ variable_list rms_run(const Tensor& x, const Rows3& r, const Tensor& w, const Te
     return {};
   return s.defined() ? variable_list{y, s} : variable_list{y};
 }
-// Saved for the backward: s (x, without a residual) and w; of b only its shape and type.
+// Saved for the backward: s (x, without a residual) and w; of b only its shape and type.  Where the gradient of an f32 w is wanted beside an s in bf16,
+// whose rounding it would show: x and the residual in place of s.
 struct RmsFn : FirstOrder<RmsFn> {
   struct Values {
     double eps, offset;
     int64_t stride;
     int vectors_f32, s_f32, x_f32;
-    bool w, b, vectors, residual;  // which there are; whether the vectors' gradients are wanted
+    bool w, b, vectors, residual, again;  // which there are; whether the vectors' gradients are wanted; whether s is added up again
     Shape8 x, w_shape, b_shape;
   };
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w_, const OptTensor& b_, const OptTensor& res_, double eps, double offset) {
@@ -1025,9 +1026,10 @@ struct RmsFn : FirstOrder<RmsFn> {
     variable_list out = rms_run(x, r, w, b, res, rr, stride, f32, eps, offset);
     if (out.empty()) throw Refused{};
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({res.defined() ? out[1] : x, w});
+    const bool again = res.defined() && !is_f32(res) && w.defined() && is_f32(w) && w.requires_grad();
+    ctx->save_for_backward({res.defined() && !again ? out[1] : x, w, again ? res : Tensor()});
     keep(ctx, Values{eps, offset, stride, f32, is_f32(res.defined() ? res : x), is_f32(x), w.defined(), b.defined(),
-                     (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()), res.defined(), Shape8(x), Shape8(w), Shape8(b)});
+                     (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()), res.defined(), again, Shape8(x), Shape8(w), Shape8(b)});
     return out;
   }
   // a gradient as rows of the wanted type
@@ -1043,9 +1045,10 @@ struct RmsFn : FirstOrder<RmsFn> {
   static variable_list gradients(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Values c = kept<Values>(ctx);
-    const Tensor &s = saved[0], &w = saved[1];
+    const Tensor &s = saved[0], &w = saved[1], &res = saved[2];
     const auto r = as_rows(s);
-    unpacked(r && float_on(s, s) && is_f32(s) == c.s_f32 && s.sizes() == c.x.get() && w.defined() == c.w &&
+    Rows3 rr{};
+    unpacked(r && res.defined() == c.again && residual_rows(s, res, rr) && (!c.again || !is_f32(res)) && float_on(s, s) && is_f32(s) == c.s_f32 && s.sizes() == c.x.get() && w.defined() == c.w &&
              (!c.w || (float_on(w, s) && is_f32(w) == c.vectors_f32 && w.is_contiguous() && w.sizes() == c.w_shape.get())));
     const auto g_type = c.x_f32 ? at::kFloat : at::kBFloat16;
     Tensor g = grads[0].defined() ? grads[0] : at::zeros(s.sizes(), s.options().dtype(g_type)), gs = c.residual ? grads[1] : Tensor();
@@ -1056,8 +1059,8 @@ struct RmsFn : FirstOrder<RmsFn> {
     Tensor dw = c.vectors && c.w ? at::empty(c.w_shape.get(), vec) : Tensor(), db = c.vectors && c.b ? at::empty(c.b_shape.get(), vec) : Tensor();
     const int64_t nws = dw.defined() || db.defined() ? mdattn_rms_norm_bwd_workspace_floats(r->groups, r->rows, (int)r->c) : 0;
     const Tensor ws = nws ? at::empty({nws}, s.options().dtype(at::kFloat)) : Tensor();
-    must(mdattn_rms_norm_bwd(stream(s), ptr(s), is_f32(s), ptr(g), is_f32(g), ptr(gs), mut(ds), mut(dx), ptr(w), mut(dw), mut(db), c.vectors_f32, r->groups,
-                             r->rows, (int)r->c, r->sg, r->sr, rg.sg, rg.sr, rs.sg, rs.sr, c.stride, (float)c.eps, (float)c.offset, f32(ws), nws),
+    must(mdattn_rms_norm_bwd(stream(s), ptr(s), is_f32(s), ptr(res), ptr(g), is_f32(g), ptr(gs), mut(ds), mut(dx), ptr(w), mut(dw), mut(db), c.vectors_f32, r->groups,
+                             r->rows, (int)r->c, r->sg, r->sr, rr.sg, rr.sr, rg.sg, rg.sr, rs.sg, rs.sr, c.stride, (float)c.eps, (float)c.offset, f32(ws), nws),
          "mdattn_rms_norm_bwd");
     return {narrow ? dx : ds, dw, db, c.residual ? ds : Tensor(), Tensor(), Tensor()};
   }

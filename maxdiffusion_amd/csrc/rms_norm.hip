@@ -5,8 +5,9 @@
 //
 // As the layer norm: a team of threads owns whole rows, a thread the same few chunks of 8 channels in each of its rows; w, b and the sums of dw
 // and db stay in its registers while the rows pass by, the next row already on its way.  A row's one sum (two backward) takes one exchange
-// through LDS and one barrier.  h is formed from the f32 sum that s is rounded from; the backward pass has the rounded one, whose
-// roundings (2^-9 of an element on average) change a gradient by less than its own.
+// through LDS and one barrier.  h is formed from the f32 sum that s is rounded from.  The backward pass has the rounded one, whose roundings (2^-9 of an
+// element on average) change a gradient in bf16 by less than its own; where w, and with it dw, is f32 beside an s in bf16, x and the residual
+// take its place, one more read of a row.
 // Bound by memory where rows are many: 75,600 rows of 5,120 in bf16, with a residual, scale and shift, 540 us (3.1 GB at 5.7 TB/s, above a copy's
 // 4.9: streaming stores); into e4m3, 4,096 x 4,096, 22 us (5.4 TB/s).  Few or odd rows wait for a row's way through memory and its sum: one row
 // 3.2 us, 2,674 of 1,001 with an f32 residual 9.2 us (3.5 TB/s), their backward pass 14.8 us (2.9 TB/s) and 4.1 for the sums of dw and db.
@@ -109,11 +110,11 @@ __global__ __launch_bounds__(MAXT) void rms_norm_kernel(RmsArgs a) {
 }
 
 struct RmsBwdArgs {
-  const void *s, *g, *gs, *w;
+  const void *s, *res, *g, *gs, *w;  // res: added to s, of its type (bf16)
   void *ds, *dx;
   float* part;  // [workgroup][2][C]: its rows' dw and db; null: neither is wanted
   int64_t rows, wb_stride;
-  int64_t s_sg, s_sr, g_sg, g_sr, gs_sg, gs_sr;
+  int64_t s_sg, s_sr, r_sg, r_sr, g_sg, g_sr, gs_sg, gs_sr;
   int C, wb_f32, blocks, team;  // workgroups of a group; threads of a team
   float eps, offset;
 };
@@ -129,15 +130,21 @@ __global__ __launch_bounds__(MAXT) void rms_norm_bwd_kernel(RmsBwdArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave / waves, first_wave = mine * waves;
   const Deal<NV, TAIL> deal(a.C, threadIdx.x - first_wave * 64, a.team);
   const R* s = static_cast<const R*>(a.s) + group * a.s_sg;
+  [[maybe_unused]] const R* res = a.res ? static_cast<const R*>(a.res) + group * a.r_sg : nullptr;
   const T* g = static_cast<const T*>(a.g) + group * a.g_sg;
   const R* gs = a.gs ? static_cast<const R*>(a.gs) + group * a.gs_sg : nullptr;
   const int64_t out = (int64_t)group * a.rows * a.C;
   const int64_t step = (int64_t)a.blocks * teams;
   int64_t row = (int64_t)block * teams + mine;
+  constexpr bool Narrow = sizeof(R) == 2;
   Chunk<R> sn[NV], un[NV];
+  [[maybe_unused]] Chunk<R> rn[NV];
   Chunk<T> gn[NV];
   auto load = [&](int64_t at) __attribute__((always_inline)) {
     deal.load(sn, s + at * a.s_sr);
+    if constexpr (Narrow) {
+      if (res) deal.load(rn, res + at * a.r_sr);
+    }
     deal.load(gn, g + at * a.g_sr);
     if (gs) deal.load(un, gs + at * a.gs_sr);
   };
@@ -159,6 +166,14 @@ __global__ __launch_bounds__(MAXT) void rms_norm_bwd_kernel(RmsBwdArgs a) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       sn[j].get(f[j]);
+      if constexpr (Narrow) {
+        if (res) {
+          float r[8];
+          rn[j].get(r);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[j][e] += r[e];
+        }
+      }
       gn[j].get(q[j]);
       if (gs) {
         un[j].get(u[j]);
@@ -333,25 +348,26 @@ extern "C" int64_t mdattn_rms_norm_bwd_workspace_floats(int64_t groups, int64_t 
   return (apart > merged ? apart : merged) * 2 * C;
 }
 
-extern "C" int mdattn_rms_norm_bwd(void* stream, const void* s, int s_is_f32, const void* g, int g_is_f32, const void* gs, void* ds, void* dx,
+extern "C" int mdattn_rms_norm_bwd(void* stream, const void* s, int s_is_f32, const void* residual, const void* g, int g_is_f32, const void* gs, void* ds, void* dx,
                                    const void* w, void* dw, void* db, int wb_is_f32, int64_t groups, int64_t rows, int C, int64_t s_stride_group,
-                                   int64_t s_stride_row, int64_t g_stride_group, int64_t g_stride_row, int64_t gs_stride_group, int64_t gs_stride_row,
+                                   int64_t s_stride_row, int64_t r_stride_group, int64_t r_stride_row, int64_t g_stride_group, int64_t g_stride_row, int64_t gs_stride_group, int64_t gs_stride_row,
                                    int64_t wb_stride, float eps, float w_offset, float* workspace, int64_t workspace_floats) {
   if (!s || !g || !ds || !sizes_ok(groups, rows, C) || !(eps >= 0.f) || !(w_offset == w_offset) || (dw && !w)) return MDATTN_E_BADARG;
-  if (C > kMaxC || (g_is_f32 && !s_is_f32) || (dx && g_is_f32)) return MDATTN_E_UNSUPPORTED;
+  if (C > kMaxC || (g_is_f32 && !s_is_f32) || (dx && g_is_f32) || (residual && s_is_f32)) return MDATTN_E_UNSUPPORTED;
   const bool sums = dw || db;
   if (sums && (!workspace || workspace_floats < mdattn_rms_norm_bwd_workspace_floats(groups, rows, C))) return MDATTN_E_BADARG;
-  if (!elem_aligned(s, s_is_f32) || !elem_aligned(gs, s_is_f32) || !elem_aligned(ds, s_is_f32) || !elem_aligned(g, g_is_f32) || !elem_aligned(dx, 0) ||
+  if (!elem_aligned(s, s_is_f32) || !elem_aligned(residual, 0) || !elem_aligned(gs, s_is_f32) || !elem_aligned(ds, s_is_f32) || !elem_aligned(g, g_is_f32) || !elem_aligned(dx, 0) ||
       !elem_aligned(w, wb_is_f32) || !elem_aligned(dw, wb_is_f32) || !elem_aligned(db, wb_is_f32) || !elem_aligned(workspace, 1))
     return MDATTN_E_ALIGN;
   RmsBwdArgs a{};
-  a.s = s; a.g = g; a.gs = gs; a.w = w; a.ds = ds; a.dx = dx; a.part = sums ? workspace : nullptr;
+  a.s = s; a.res = residual; a.g = g; a.gs = gs; a.w = w; a.ds = ds; a.dx = dx; a.part = sums ? workspace : nullptr;
   a.rows = rows; a.wb_stride = wb_stride; a.C = C; a.wb_f32 = wb_is_f32; a.eps = eps; a.offset = w ? w_offset : 0.f;
-  a.s_sg = s_stride_group; a.s_sr = s_stride_row; a.g_sg = g_stride_group; a.g_sr = g_stride_row; a.gs_sg = gs_stride_group; a.gs_sr = gs_stride_row;
+  a.s_sg = s_stride_group; a.s_sr = s_stride_row; a.r_sg = r_stride_group; a.r_sr = r_stride_row; a.g_sg = g_stride_group; a.g_sr = g_stride_row; a.gs_sg = gs_stride_group; a.gs_sr = gs_stride_row;
   int64_t none_g = a.s_sg, none_r = a.s_sr;
-  const Strides us = gs ? Strides{&a.gs_sg, &a.gs_sr} : Strides{&none_g, &none_r};
-  merge_groups(groups, a.rows, wb_stride, {{&a.s_sg, &a.s_sr}, {&a.g_sg, &a.g_sr}, us});
-  const BwdShape b = bwd_shape(groups, a.rows, C, (int64_t)C * ((s_is_f32 ? 4 : 2) * (gs ? 2 : 1) + (g_is_f32 ? 4 : 2)));
+  int64_t no_res_g = a.s_sg, no_res_r = a.s_sr;
+  const Strides us = gs ? Strides{&a.gs_sg, &a.gs_sr} : Strides{&none_g, &none_r}, rs = residual ? Strides{&a.r_sg, &a.r_sr} : Strides{&no_res_g, &no_res_r};
+  merge_groups(groups, a.rows, wb_stride, {{&a.s_sg, &a.s_sr}, {&a.g_sg, &a.g_sr}, us, rs});
+  const BwdShape b = bwd_shape(groups, a.rows, C, (int64_t)C * ((s_is_f32 ? 4 : 2) * (1 + (gs != nullptr) + (residual != nullptr)) + (g_is_f32 ? 4 : 2)));
   a.blocks = b.blocks;
   a.team = b.s.threads;
   const int64_t grid = groups * a.blocks, sum_groups = wb_stride ? groups : 1;

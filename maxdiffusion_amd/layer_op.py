@@ -74,27 +74,31 @@ def hip_layer_norm(x, weight=None, bias=None, eps: float = 1e-6, weight_offset: 
 
 
 class _HipRmsNorm(torch.autograd.Function):
-  """Saved for the backward: s (x, without a residual) and the vectors; the rows' statistics are computed again."""
+  """Saved for the backward: s (x, without a residual; x and the residual, both bf16, where the gradient of an f32 weight is wanted, which s's rounding
+  would show in) and the vectors; the rows' statistics are computed again."""
 
   @staticmethod
   def forward(ctx, x, weight, bias, residual, eps, weight_offset):
     ctx.set_materialize_grads(False)
     out = ops.rms_norm(x, weight, bias, residual, eps, weight_offset)
-    s = x if residual is None else out[1]
-    ctx.save_for_backward(s, weight, bias)
-    ctx.cfg, ctx.forms = (eps, weight_offset), _forms(s, weight, bias)
+    again = residual is not None and residual.dtype == torch.bfloat16 and weight is not None and weight.dtype == torch.float32 and ctx.needs_input_grad[1]
+    s = x if residual is None or again else out[1]
+    saved = (s, weight, bias, residual if again else None)
+    ctx.save_for_backward(*saved)
+    ctx.cfg, ctx.forms = (eps, weight_offset), _forms(*saved)
     ctx.narrow, ctx.g_dtype, ctx.has_residual = s.dtype != x.dtype, x.dtype, residual is not None
     return out
 
   @staticmethod
   @_lib.first_order
   def backward(ctx, g, gs=None):
-    s, weight, bias = ctx.saved_tensors
-    if _forms(s, weight, bias) != ctx.forms:
+    s, weight, bias, residual = ctx.saved_tensors
+    if _forms(s, weight, bias, residual) != ctx.forms:
       raise ValueError("a tensor saved for the backward pass came back from its hook with another dtype, shape or device")
     g = torch.zeros(s.shape, dtype=ctx.g_dtype, device=s.device) if g is None else _rows(g.to(ctx.g_dtype))
     gs = None if gs is None else _rows(gs.to(s.dtype))
-    ds, dx, dw, db = ops.rms_norm_backward(_rows(s), weight, bias, g, gs, *ctx.cfg, needs_vectors=any(ctx.needs_input_grad[1:3]), narrow=ctx.narrow)
+    ds, dx, dw, db = ops.rms_norm_backward(_rows(s), weight, bias, g, gs, *ctx.cfg, needs_vectors=any(ctx.needs_input_grad[1:3]), narrow=ctx.narrow,
+                                        residual=None if residual is None else _rows(residual))
     return ds if dx is None else dx, dw, db, ds if ctx.has_residual else None, None, None
 
 

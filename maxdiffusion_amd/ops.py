@@ -857,12 +857,14 @@ def rms_norm_quant(x, weight=None, bias=None, residual=None, eps: float = 1e-6, 
   return q if residual is None else (q, s)
 
 
-def rms_norm_backward(s, weight, bias, g, gs=None, eps: float = 1e-6, weight_offset: float = 0.0, needs_vectors: bool = True, narrow: bool = False):
-  """Backward of `rms_norm`: s as the forward returned it (x, where there was no residual), weight and bias as it had them (of bias only
+def rms_norm_backward(s, weight, bias, g, gs=None, eps: float = 1e-6, weight_offset: float = 0.0, needs_vectors: bool = True, narrow: bool = False,
+                      residual=None):
+  """Backward of `rms_norm`: s as the forward returned it (x, where there was no residual; or x beside the forward's `residual`, both bf16, for
+  gradients without s's rounding), weight and bias as it had them (of bias only
   whether there is one, its shape and dtype), g and gs the gradients of y and s (gs None: none), g in s's dtype or bf16 beside an f32 s.  Returns (ds, dx,
   dweight, dbias): the gradient of the residual, and of x, in s's dtype; the same in bf16 where `narrow` (x was bf16 beside an f32
   residual), else None; None for what there is not, or for the last two with needs_vectors False."""
-  _check_dev(s, weight, bias, g, gs)
+  _check_dev(s, weight, bias, g, gs, residual)
   s_f32, g_f32 = _float_kind(s, "s"), _float_kind(g, "g")
   groups, rows, c, sg, sr = _norm_rows(s)
   stride, wb_f32 = _norm_vectors(weight, bias, groups, c)
@@ -871,6 +873,10 @@ def rms_norm_backward(s, weight, bias, g, gs=None, eps: float = 1e-6, weight_off
                      f"{g.dtype} for {s.dtype}")
   if gs is not None and (gs.shape != s.shape or gs.dtype != s.dtype):
     raise ValueError(f"gs must be shaped and typed like s, {tuple(s.shape)} {s.dtype}, got {tuple(gs.shape)} {gs.dtype}")
+  if residual is not None and (s_f32 or residual.shape != s.shape or residual.dtype != s.dtype):
+    raise ValueError(f"residual must be bf16 and shaped like s, which has to be bf16 beside it, got {tuple(residual.shape)} {residual.dtype} for "
+                     f"{tuple(s.shape)} {s.dtype}")
+  rg, rr = (0, 0) if residual is None else _norm_rows(residual, "residual")[3:]
   gg, gr = _norm_rows(g, "g")[3:]
   ug, ur = (0, 0) if gs is None else _norm_rows(gs, "gs")[3:]
   ds = torch.empty(s.shape, dtype=s.dtype, device=s.device)
@@ -882,8 +888,8 @@ def rms_norm_backward(s, weight, bias, g, gs=None, eps: float = 1e-6, weight_off
   lib = _lib.load()
   nws = lib.mdattn_rms_norm_bwd_workspace_floats(groups, rows, c) if dw is not None or db is not None else 0
   ws = torch.empty(nws, dtype=torch.float32, device=s.device) if nws else None
-  rc = lib.mdattn_rms_norm_bwd(_stream(), _ptr(s), s_f32, _ptr(g), g_f32, _ptr(gs), _ptr(ds), _ptr(dx), _ptr(weight), _ptr(dw), _ptr(db), wb_f32, groups, rows,
-                               c, sg, sr, gg, gr, ug, ur, stride, float(eps), float(weight_offset), _ptr(ws), nws)
+  rc = lib.mdattn_rms_norm_bwd(_stream(), _ptr(s), s_f32, _ptr(residual), _ptr(g), g_f32, _ptr(gs), _ptr(ds), _ptr(dx), _ptr(weight), _ptr(dw), _ptr(db), wb_f32,
+                               groups, rows, c, sg, sr, rg, rr, gg, gr, ug, ur, stride, float(eps), float(weight_offset), _ptr(ws), nws)
   _lib.check(rc, "mdattn_rms_norm_bwd")
   return ds, dx, dw, db
 

@@ -65,12 +65,15 @@ def test_backward(dev, shape, xt, rt, wt, per_batch, off):
   g, gs = rand(dev, *shape, seed=5, dtype=xt), rand(dev, *shape, seed=6, dtype=st)
   s = x if res is None else ops.rms_norm(x, w, v, res, 1e-6, off)[1]
   narrow = st != xt
-  v_s = 0.0 if res is None else HALF[st]
   _, _, h, r, m, _ = rms64(x, res, w, v, 1e-6, off)
   a = g.double() * m
   mean, size = (a * h).mean(-1, keepdim=True), (a * h).abs().mean(-1, keepdim=True)
-  for up in (None, gs):
-    ds, dx, dw, db = ops.rms_norm_backward(s, w, v, g, up, 1e-6, off, narrow=narrow)
+  # from s as it was rounded, and from x and the residual where both are bf16
+  for up, again in ((None, False), (gs, False), *(((None, True), (gs, True)) if rt == BF16 else ())):
+    v_s = 0.0 if res is None or again else HALF[st]
+    inputs = dict(s=x, residual=res) if again else dict(s=s)
+    call = lambda: ops.rms_norm_backward(weight=w, bias=v, g=g, gs=up, eps=1e-6, weight_offset=off, narrow=narrow, **inputs)
+    ds, dx, dw, db = call()
     want = r * (a - h * mean) + (0 if up is None else up.double())
     err = 32 * U * (r * (a.abs() + h.abs() * size) + (0 if up is None else up.double().abs()))
     err = err + v_s * (r * (a - h * mean)).abs() + 1.02 * r * h.abs() * (2 * v_s * mean.abs() + 2 * v_s * size)
@@ -81,8 +84,8 @@ def test_backward(dev, shape, xt, rt, wt, per_batch, off):
     want_w, want_b = (g.double() * h).sum(over), g.double().sum(over)
     close(dw, want_w, half_ulp(want_w, wt) + (2 * v_s * 1.02 + (2 * math.sqrt(terms) + 32) * U) * gh.sum(over), f"dw {shape}")
     close(db, want_b, half_ulp(want_b, wt) + (2 * math.sqrt(terms) + 16) * U * g.double().abs().sum(over), f"db {shape}")
-    again = ops.rms_norm_backward(s, w, v, g, up, 1e-6, off, narrow=narrow)
-    assert all(p is q or torch.equal(p, q) for p, q in zip((ds, dx, dw, db), again))
+    assert all(p is q or torch.equal(p, q) for p, q in zip((ds, dx, dw, db), call()))
+  ds, dx, dw, db = ops.rms_norm_backward(s, w, v, g, gs, 1e-6, off, narrow=narrow)
   alone = ops.rms_norm_backward(s, w, v, g, gs, 1e-6, off, needs_vectors=False, narrow=narrow)
   assert torch.equal(alone[0], ds) and alone[2] is None and alone[3] is None
   only = ops.rms_norm_backward(s, None, v, g, gs, 1e-6, off, narrow=narrow)
@@ -177,7 +180,9 @@ def test_autograd(dev, xt, rt, python):
   narrow = xt != rt
 
   def want(g, gs):
-    ds, dx, dw, db = ops.rms_norm_backward(s, w.detach(), b.detach(), torch.zeros_like(x) if g is None else g, gs, narrow=narrow)
+    again = rt == BF16 and w.dtype == F32  # x and the residual are kept, in place of s
+    ds, dx, dw, db = ops.rms_norm_backward(x.detach() if again else s, w.detach(), b.detach(), torch.zeros_like(x) if g is None else g, gs, narrow=narrow,
+                                           residual=res.detach() if again else None)
     return (ds if dx is None else dx, dw, db, ds)
 
   for up in ((g, None), (None, gs), (g, gs)):
@@ -216,6 +221,10 @@ def test_outputs_changed_in_place(dev):
   for p, q in zip(torch.autograd.grad(y.sum(), (x, w)), want):
     assert torch.equal(p, q)
   y, s = L.hip_rms_norm(x, w, b, res)
+  s += 1.0
+  if w.dtype == F32:  # (x and the residual are kept, in place of s)
+    assert torch.equal(torch.autograd.grad(y.sum(), x)[0], want[0])
+  y, s = L.hip_rms_norm(x, w.to(BF16), b.to(BF16), res)
   s += 1.0
   with pytest.raises(RuntimeError, match="modified by an inplace operation"):
     torch.autograd.grad(y.sum(), x)

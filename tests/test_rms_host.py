@@ -25,13 +25,13 @@ def test_backward_refuses(lib):
   n = lib.mdattn_rms_norm_bwd_workspace_floats(2, 100, 64)
   assert n > 0 and n % (2 * 64) == 0
   assert lib.mdattn_rms_norm_bwd_workspace_floats(0, 100, 64) == lib.mdattn_rms_norm_bwd_workspace_floats(1, 1, 16385) == 0
-  f = lambda s=FAKE, sf=0, g=FAKE, gf=0, gs=FAKE, ds=FAKE, dx=None, w=FAKE, dw=FAKE, db=FAKE, ws=FAKE, nws=n, c=64, eps=1e-6: lib.mdattn_rms_norm_bwd(
-      None, s, sf, g, gf, gs, ds, dx, w, dw, db, 1, 2, 100, c, 6400, c, 6400, c, 6400, c, 0, eps, 0.0, ws, nws)
+  f = lambda s=FAKE, sf=0, g=FAKE, gf=0, gs=FAKE, ds=FAKE, dx=None, w=FAKE, dw=FAKE, db=FAKE, ws=FAKE, nws=n, c=64, eps=1e-6, res=None: lib.mdattn_rms_norm_bwd(
+      None, s, sf, res, g, gf, gs, ds, dx, w, dw, db, 1, 2, 100, c, 6400, c, 6400, c, 6400, c, 6400, c, 0, eps, 0.0, ws, nws)
   assert f(s=None) == f(g=None) == f(ds=None) == f(eps=-1.0) == _lib.E_BADARG
   assert f(w=None) == _lib.E_BADARG  # a weight's gradient without the weight
   assert f(ws=None) == f(nws=n - 1) == _lib.E_BADARG
-  assert f(c=20000) == f(gf=1) == f(sf=1, gf=1, dx=FAKE) == _lib.E_UNSUPPORTED
-  assert f(s=ODD) == f(g=ODD) == f(gs=ODD) == f(ds=ODD) == f(sf=1, dx=ODD) == f(dw=P(0x1002)) == f(ws=P(0x1002)) == _lib.E_ALIGN
+  assert f(c=20000) == f(gf=1) == f(sf=1, gf=1, dx=FAKE) == f(sf=1, res=FAKE) == _lib.E_UNSUPPORTED
+  assert f(s=ODD) == f(g=ODD) == f(gs=ODD) == f(ds=ODD) == f(sf=1, dx=ODD) == f(dw=P(0x1002)) == f(ws=P(0x1002)) == f(res=P(0x1001)) == _lib.E_ALIGN
 
 
 def test_grids_past_2_32_threads_are_refused_before_a_launch(lib):
@@ -41,7 +41,7 @@ def test_grids_past_2_32_threads_are_refused_before_a_launch(lib):
   def backward(groups, c, vectors):
     nws = lib.mdattn_rms_norm_bwd_workspace_floats(groups, 1, c)
     d = FAKE if vectors else None
-    return lib.mdattn_rms_norm_bwd(None, FAKE, 1, FAKE, 1, None, FAKE, None, FAKE, d, d, 1, groups, 1, c, c, c, c, c, c, c, c, 1e-6, 0.0, FAKE, nws)
+    return lib.mdattn_rms_norm_bwd(None, FAKE, 1, None, FAKE, 1, None, FAKE, None, FAKE, d, d, 1, groups, 1, c, c, c, c, c, c, c, c, c, c, 1e-6, 0.0, FAKE, nws)
 
   assert backward(2**32 // 1024, 64, True) == backward(2**32 // 256, 1, False) == _lib.E_UNSUPPORTED
 
