@@ -619,6 +619,7 @@ extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   hipStream_t st = (hipStream_t)stream;
   if (a.D == 64) return launch<64, 64, false>(st, a, dq_grid, dkv_grid);
   if (a.D < 64) return launch<64, 64, true>(st, a, dq_grid, dkv_grid);
+  if (a.D <= 80) return launch<128, 80, true>(st, a, dq_grid, dkv_grid);
   if (a.D <= 96) return launch<128, 96, true>(st, a, dq_grid, dkv_grid);
   if (a.D < 128) return launch<128, 128, true>(st, a, dq_grid, dkv_grid);
   return launch<128, 128, false>(st, a, dq_grid, dkv_grid);
