@@ -390,10 +390,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   }
   const float c = a.c;
 
+  int from = 0, before = 0;  // (the items' ranks rise)
   for (int item = blockIdx.x;; item += gridDim.x) {
     const int rank = item / a.kv_heads, head = item - rank * a.kv_heads;
     int piece;
-    const SeqTile s = find_piece(a.seqs, G, rank, lane, a.piece_keys, a.pieces, piece);
+    const SeqTile s = find_piece(a.seqs, G, rank, lane, a.piece_keys, a.pieces, from, before, piece);
     if (s.none) return;
     if (s.gap) {
       fill_gap<32, HD>(a, s, head, tid);

@@ -89,3 +89,25 @@ def test_a_capture_beside_an_older_graph_of_the_same_leaves_is_refused(dev):
       torch.cuda.synchronize()
       for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_thousands_of_sequences(dev):
+  """More sequences than a workgroup looks through at once: short ones, and single tokens against caches of which a few are long."""
+  gen = torch.Generator().manual_seed(5)
+  m = torch.randint(0, 4, (4500,), generator=gen).tolist()
+  m[4400] = 150
+  o = starts(m)
+  q, k, v, g = make(dev, o[-1], o[-1], 2, 1, 64, seed=6, lean=0.5)
+  want = attention(q, k, v, o, o, dout=g)
+  for hints in ({}, dict(max_q=1, max_k=1), dict(max_q=150, max_k=150)):
+    out, lse, rest = ops.flash_attention_packed(q, k, v, ints(dev, o), return_lse=True, return_rest=True, **hints)
+    assert_within(out, want["out"], want["out_err"], f"out {hints}")
+    for name, t in zip(("dq", "dk", "dv"), ops.flash_attention_packed_backward(q, k, v, out, g, lse, ints(dev, o), rest=rest, **hints)):
+      assert_within(t, want[name], want[name + "_err"], f"{name} {hints}")
+  n = [1 + i % 3 for i in range(1500)]
+  n[7], n[700], n[1499] = 5000, 2000, 900
+  one, ko = list(range(len(n) + 1)), starts(n)
+  q, k, v, _ = make(dev, len(n), ko[-1], 2, 1, 128, seed=7)
+  want = attention(q, k, v, one, ko)
+  out = ops.flash_attention_packed(q, k, v, ints(dev, one), ints(dev, ko), max_q=1, max_k=5000)
+  assert_within(out, want["out"], want["out_err"], "tokens")
