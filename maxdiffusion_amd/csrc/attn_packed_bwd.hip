@@ -97,6 +97,16 @@ __device__ __forceinline__ bf16x8 load_frag(const __bf16* p, int col, int D) {
   return !PADDED || col < D ? *reinterpret_cast<const bf16x8*>(p + col) : __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
 }
 
+// A wave in its products goes before the other in its softmax (one sequence of 4,096 to 8,192 tokens 1 to 2.5 % faster; at head dim 64, where three share
+// the pipes, short calls 5 % slower: left out).
+template <int HD>
+__device__ __forceinline__ void priority(int high) {
+  if constexpr (HD == 128) {
+    if (high) __builtin_amdgcn_s_setprio(1);
+    else __builtin_amdgcn_s_setprio(0);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------- dq
 template <int HD, int DC, bool PADDED>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : 2, HD == 64 ? 3 : 2))) void packed_dq_kernel(PackedBwdArgs a) {
@@ -214,6 +224,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     bf16x8 win[LA];
 #pragma unroll
     for (int n = 0; n < LA; ++n) win[n] = frag(n);
+    priority<HD>(1);
 #pragma unroll
     for (int n = 0; n < 2 * NJ; ++n) {
       if (n < NJ) S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(win[n % LA], qf[n % NJ], S, 0, 0, 0);
@@ -221,6 +232,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
       win[n % LA] = frag(n + LA);
       __builtin_amdgcn_sched_barrier(0);
     }
+    priority<HD>(0);
     if (k0 + 32 > all) {
       asm volatile("" ::: "memory");  // keeps the branch
       const int at0 = k0 + 4 * hh;
@@ -239,12 +251,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
       }
       W[hb] = __builtin_bit_cast(bf16x8, u32x4{pk[0], pk[1], pk[2], pk[3]});
     }
+    priority<HD>(1);
 #pragma unroll
     for (int jv = 0; jv < 2 * ND; ++jv) {
       acc[jv % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(win[(2 * NJ + jv) % LA], W[jv / ND], acc[jv % ND], 0, 0, 0);
       if (jv + LA < 2 * ND) win[(2 * NJ + jv) % LA] = frag(2 * NJ + jv + LA);
       __builtin_amdgcn_sched_barrier(0);
     }
+    priority<HD>(0);
   };
   for (int t = 0; t < nt; ++t) {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's share of tile t has landed
@@ -398,6 +412,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
         dP[4 * g + e] = u1[e];
       }
     }
+    priority<HD>(1);
     if constexpr (LA1 > 0) {
       bf16x8 win[LA1];
 #pragma unroll
@@ -415,6 +430,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 #pragma unroll
       for (int j = 0; j < NJ; ++j) dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(NJ + j), vf[j], dP, 0, 0, 0);
     }
+    priority<HD>(0);
     if (token0 < all_from || token0 + 32 > s.m) {  // tokens that do not see the key, and what is behind the last
       asm volatile("" ::: "memory");  // keeps the branch
       const int at0 = token0 + 4 * hh;
@@ -437,6 +453,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
       W[hb] = __builtin_bit_cast(bf16x8, u32x4{wpk[0], wpk[1], wpk[2], wpk[3]});
       P[hb] = __builtin_bit_cast(bf16x8, u32x4{ppk[0], ppk[1], ppk[2], ppk[3]});
     }
+    priority<HD>(1);
     if constexpr (LA3 > 0) {
       bf16x8 win[LA3];
 #pragma unroll
@@ -456,6 +473,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
         dv[jv % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag3(2 * jv + 1), P[jv / ND], dv[jv % ND], 0, 0, 0);
       }
     }
+    priority<HD>(0);
   };
   for (int t = 0; t < nt; ++t) {
     __builtin_amdgcn_s_waitcnt(0x0F70);
