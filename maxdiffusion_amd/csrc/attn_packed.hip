@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "attn_packed.h"
+#include "mdattn_host.h"
 
 namespace mdattn {
 namespace {
@@ -33,7 +34,7 @@ struct PackedArgs {
   int kv_heads, D, causal;
   RowStrides qs, ks, vs, os;
   float c;  // scale * log2(e)
-  int pieces, piece_keys;
+  int pieces, piece_keys, items;  // items: see packed_few_kernel
   float* part;  // [piece][kv_heads][q_rows * group][D]
   float2* ml;   // [piece][kv_heads][q_rows * group]: reference point (log2 units) and sum of P
 };
@@ -361,7 +362,9 @@ void packed_fwd_kernel(PackedArgs a) {
 // workgroup at a time; in a piece the waves take blocks of 32 keys in turn, each through buffers of its own in LDS, one for K and one for V, so that no
 // wave waits for another: the next K is requested once the scores of this one are formed, the next V once its product is.  Four waves and
 // two workgroups per CU keep some 64 to 128 KB of keys on their way, what 256 CUs need at 8 TB/s.  The waves' sums are joined through LDS,
-// the pieces' by packed_combine_kernel.  The workgroups walk the list of pieces, whose length is known on the device only.
+// the pieces' by packed_combine_kernel.  The workgroups walk the list of pieces, whose length is known on the device only, up to a.items of them:
+// as many as offsets that do not decrease can make.  Offsets that go back and forth name rows many times over; their list would be as much longer, and
+// its ranks pass 31 bits.
 template <int HD>
 constexpr int few_bytes() {
   constexpr int ring = 8 * PackedBlock<HD>::Bytes, stage = (4 * 32 * 68 + 4 * 32 * 2) * 4;
@@ -391,7 +394,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
   const float c = a.c;
 
   int from = 0, before = 0;  // (the items' ranks rise)
-  for (int item = blockIdx.x;; item += gridDim.x) {
+  for (unsigned item = blockIdx.x; item < (unsigned)a.items; item += gridDim.x) {
     const int rank = item / a.kv_heads, head = item - rank * a.kv_heads;
     int piece;
     const SeqTile s = find_piece(a.seqs, G, rank, lane, a.piece_keys, a.pieces, from, before, piece);
@@ -595,6 +598,11 @@ enum { kFew, kHalf, kFlat };
 struct FwdPlan {
   int kind, pieces, piece_keys;
   int64_t floats, tiles;  // tiles: of 128 rows, of all heads
+  int order(const mdattn_packed* p) const { return kind == kFew ? kAsTheyCome : packed_order(p, tiles * (kind == kHalf && p->causal ? 2 : 1)); }
+  // tiles with their pieces, of all heads, that the call has at most (few: below 2^31)
+  int64_t items(const mdattn_packed* p) const {
+    return packed_tiles((int64_t)p->q_rows * (p->heads / p->kv_heads), p->sequences, kind == kFew ? 32 : kind == kHalf ? 64 : 128) * pieces * p->kv_heads;
+  }
 };
 FwdPlan fwd_plan(const mdattn_packed* p) {
   const int64_t group = p->heads / p->kv_heads;
@@ -646,8 +654,16 @@ extern "C" int64_t mdattn_fwd_bf16_packed_workspace_floats(const mdattn_packed* 
   return packed_sizes(p) == MDATTN_OK ? fwd_plan(p).floats : 0;
 }
 
+extern "C" int mdattn_host_packed_fwd_plan(const mdattn_packed* p, mdattn_host_packed_plan* plan) {
+  const int rc = packed_sizes(p);
+  if (rc != MDATTN_OK) return rc;
+  const FwdPlan f = fwd_plan(p);
+  *plan = {f.kind == kFew ? 4 : f.kind == kHalf ? 2 : 1, f.order(p), f.pieces, f.piece_keys, f.items(p)};
+  return MDATTN_OK;
+}
+
 extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, const void* q, const void* k, const void* v, void* out, void* rest,
-                                      float* lse,                                      const mdattn_strides* q_strides, const mdattn_strides* k_strides, const mdattn_strides* v_strides,
+                                      float* lse, const mdattn_strides* q_strides, const mdattn_strides* k_strides, const mdattn_strides* v_strides,
                                       const mdattn_strides* o_strides, float scale, float* workspace, int64_t workspace_floats) {
   const int rc = packed_sizes(p);
   if (rc != MDATTN_OK) return rc;
@@ -667,22 +683,22 @@ extern "C" int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, cons
   PackedArgs a{};
   a.q = static_cast<const __bf16*>(q); a.k = static_cast<const __bf16*>(k); a.v = static_cast<const __bf16*>(v);
   a.out = static_cast<__bf16*>(out); a.rest = static_cast<__bf16*>(rest); a.lse = lse;
-  a.seqs = {p->q_offsets, p->k_offsets, p->k_lengths, p->sequences, p->q_rows, p->k_rows, f.kind == kFew ? kAsTheyCome : packed_order(p, f.tiles * (f.kind == kHalf && p->causal ? 2 : 1)), 256 / p->kv_heads};
+  a.seqs = {p->q_offsets, p->k_offsets, p->k_lengths, p->sequences, p->q_rows, p->k_rows, f.order(p), 256 / p->kv_heads};
   a.group = divisor((unsigned)(p->heads / p->kv_heads));
   a.kv_heads = p->kv_heads; a.D = p->head_dim; a.causal = p->causal;
   a.qs = {q_strides->seq, q_strides->head}; a.ks = {k_strides->seq, k_strides->head};
   a.vs = {v_strides->seq, v_strides->head}; a.os = {o_strides->seq, o_strides->head};
   a.c = scale * kLog2e;
   a.pieces = f.pieces; a.piece_keys = f.piece_keys;
-  const int64_t rows = (int64_t)p->q_rows * p->heads, group_rows = (int64_t)p->q_rows * a.group.d;
+  const int64_t rows = (int64_t)p->q_rows * p->heads;
   if (f.pieces > 1) {
     a.part = workspace;
     a.ml = reinterpret_cast<float2*>(workspace + f.pieces * rows * a.D);
   }
-  int64_t grid = packed_tiles(group_rows, p->sequences, f.kind == kFew ? 32 : f.kind == kHalf ? 64 : 128) * p->kv_heads;
+  int64_t grid = f.items(p);
   if (f.kind == kFew) {  // two per CU, in whole rounds of the heads, walk what there is
-    const int64_t most = (512 + a.kv_heads - 1) / a.kv_heads * a.kv_heads;
-    grid = grid * f.pieces < most ? grid * f.pieces : most;
+    a.items = (int)grid;
+    grid = std::min(grid, (512 + (int64_t)a.kv_heads - 1) / a.kv_heads * a.kv_heads);
   }
   if (!grid_fits(grid, 256) || (f.pieces > 1 && !grid_fits(rows, 256))) return MDATTN_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
