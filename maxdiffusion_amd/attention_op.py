@@ -258,7 +258,7 @@ def hip_flash_packed(q, k, v, q_offsets, k_offsets=None, *, k_lengths=None, caus
 
   The arguments are those of `ops.flash_attention_packed`.  Differentiable in q, k and v (not with k_lengths): where autograd is recording and one
   of them requires a gradient, all three products' gradients come from the HIP backward pass."""
-  scale = float(q.shape[-1]**-0.5 if scale is None else scale) if q.dim() else 1.0
+  scale = float(q.shape[-1]**-0.5 if scale is None else scale) if q.dim() and q.shape[-1] else 1.0  # (refused below)
   grad = _wants_grad(q, k, v)
   if q.is_cuda and not (grad and k_lengths is not None):
     out = _lib.host().flash_packed(q, k, v, q_offsets, k_offsets, k_lengths, bool(causal), scale, int(max_q or 0), int(max_k or 0))

@@ -1,8 +1,11 @@
-"""How calls of packed attention are launched, as the library plans it on the host: no GPU needed."""
+"""How calls of packed attention are launched, as the library plans it on the host, and what its Python entry points refuse: no GPU needed."""
 import ctypes
 import random
 
-from maxdiffusion_amd import _lib
+import pytest
+import torch
+
+from maxdiffusion_amd import _lib, attention_op, ops
 
 
 class Plan(ctypes.Structure):
@@ -69,3 +72,10 @@ def test_plans_of_sizes_that_are_refused(lib):
   plan = Plan()
   assert lib.mdattn_host_packed_fwd_plan(None, ctypes.byref(plan)) == _lib.E_BADARG
   assert lib.mdattn_host_packed_fwd_plan(ctypes.byref(packed(head_dim=100)), ctypes.byref(plan)) == _lib.E_UNSUPPORTED
+
+
+def test_an_empty_head_dim_is_refused_as_others_are(lib):
+  q, o = torch.zeros(4, 2, 0, dtype=torch.bfloat16), torch.tensor([0, 4], dtype=torch.int32)
+  for call in (attention_op.hip_flash_packed, ops.flash_attention_packed):
+    with pytest.raises(ValueError):
+      call(q, q, q, o)
