@@ -37,8 +37,8 @@ typedef struct {
 } mdattn_packed;
 
 /*
- * out = softmax(scale * q k^T) v over each sequence; bf16.  rest, strided like out, or NULL: what the rounding of out left, rounded to bf16, for the
- * backward pass (of rows of no sequence it is not written).  lse f32 [heads, q_rows], or NULL: the logarithm of each row's sum.  Rows
+ * out = softmax(scale * q k^T) v over each sequence; bf16; scale positive and finite.  rest, strided like out, or NULL: what the rounding of out
+ * left, rounded to bf16, for the backward pass (of rows of no sequence it is not written).  lse f32 [heads, q_rows], or NULL: the logarithm of each row's sum.  Rows
  * that see no key, and rows of no sequence: out 0, lse -inf.  Logits, softmax and sums in f32, P rounded to bf16 before its product.
  *   workspace     mdattn_fwd_bf16_packed_workspace_floats floats (0 where one is not needed), with which few rows against many keys are
  *                 split over the keys; with less they are not.  16-byte aligned.
@@ -51,8 +51,9 @@ int mdattn_fwd_bf16_packed(void* stream, const mdattn_packed* p, const void* q, 
 
 /*
  * Backward of mdattn_fwd_bf16_packed: dq, dk, dv (bf16, strided like q, k and v) from its inputs, out, rest, lse and the
- * gradient of out (strided like it, as rest is).  rest may be NULL, for gradients that are further off where a key has most of a row's weight.  k_lengths has to be NULL.  Rows of no sequence get zeros.  Deterministic: sums over the rows and over the
- * heads of a group are made in a fixed order.
+ * gradient of out (strided like it, as rest is).  rest may be NULL, for gradients that are further off where a key has most of a row's weight.
+ * k_lengths has to be NULL, and scale 1e-30 at least (lse is divided by it).  Rows of no sequence get zeros.  Deterministic: sums over the rows and
+ * over the heads of a group are made in a fixed order.
  *   workspace     mdattn_bwd_bf16_packed_workspace_floats floats; 16-byte aligned
  */
 int64_t mdattn_bwd_bf16_packed_workspace_floats(const mdattn_packed* p);

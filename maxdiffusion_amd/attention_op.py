@@ -229,6 +229,9 @@ def _wants_grad(*ts) -> bool:
   return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+_MIN_GRAD_SCALE = 1e-30  # the backward pass divides by it (mdattn_bwd_bf16_packed)
+
+
 class _HipFlashPacked(torch.autograd.Function):
   """Saved for the backward: q, k, v, the offsets, out, what its rounding left, lse."""
 
@@ -256,8 +259,8 @@ def hip_flash_packed(q, k, v, q_offsets, k_offsets=None, *, k_lengths=None, caus
   """Attention over packed sequences: a prompt encoder's, causal, with grouped heads, its prompts one behind the other without padding (the
   reference's masked form: models/qwen3_flax.py:285), or images of several sizes.  q [Tq, H, D], k, v [Tk, Hkv, D] -> [Tq, H, D], bf16.
 
-  The arguments are those of `ops.flash_attention_packed`.  Differentiable in q, k and v (not with k_lengths): where autograd is recording and one
-  of them requires a gradient, all three products' gradients come from the HIP backward pass."""
+  The arguments are those of `ops.flash_attention_packed`.  Differentiable in q, k and v (not with k_lengths, nor with a scale below 1e-30): where
+  autograd is recording and one of them requires a gradient, all three products' gradients come from the HIP backward pass."""
   scale = float(q.shape[-1]**-0.5 if scale is None else scale) if q.dim() and q.shape[-1] else 1.0  # (refused below)
   grad = _wants_grad(q, k, v)
   if q.is_cuda and not (grad and k_lengths is not None):
@@ -269,6 +272,8 @@ def hip_flash_packed(q, k, v, q_offsets, k_offsets=None, *, k_lengths=None, caus
   if grad:
     if k_lengths is not None:
       raise NotImplementedError("hip_flash_packed has no gradient with k_lengths: call it under torch.no_grad()")
+    if 0 < scale < _MIN_GRAD_SCALE:
+      raise ValueError(f"scale={scale} is too small for a gradient: {_MIN_GRAD_SCALE} at least, or a call under torch.no_grad()")
     return _HipFlashPacked.apply(q, k, v, q_offsets, q_offsets if k_offsets is None else k_offsets, bool(causal), scale, max_q, max_k)
   return ops.flash_attention_packed(q, k, v, q_offsets, k_offsets, k_lengths=k_lengths, causal=causal, scale=scale, max_q=max_q, max_k=max_k)
 

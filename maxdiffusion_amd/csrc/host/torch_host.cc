@@ -469,7 +469,7 @@ OptTensor flash_packed(const Tensor& q, const Tensor& k, const Tensor& v, const 
   mdattn_packed p;
   if (!packed_args(q, k, v, qo, ko, kl, causal, max_q, max_k, p)) return std::nullopt;
   if (grad) {
-    if (kl.defined()) return std::nullopt;
+    if (kl.defined() || !(scale >= 1e-30)) return std::nullopt;  // (which the backward pass would refuse)
     return unless_refused([&] { return PackedFn::apply(q, k, v, qo, ko, causal, scale, max_q, max_k); });
   }
   at::NoGradGuard guard;

@@ -15,3 +15,16 @@ def test_an_empty_head_dim_is_refused(dev):
     for call in (A.hip_flash_packed, ops.flash_attention_packed):
       with pytest.raises(ValueError, match="head_dim=0"):
         call(q.detach().requires_grad_(grad), k, v, ints(dev, [0, 64]))
+
+
+def test_a_scale_that_the_backward_pass_refuses_is_refused_by_the_forward(dev):
+  q, k, v, g = make(dev, 64, 64, 4, 2, 64)
+  o = ints(dev, [0, 64])
+  leaf = q.clone().requires_grad_(True)
+  for t in (leaf, torch.cat((leaf, leaf), 2)[..., :64].transpose(0, 1).contiguous().transpose(0, 1)):
+    with pytest.raises(ValueError, match="scale"):
+      A.hip_flash_packed(t, k, v, o, scale=1e-31)
+  with torch.no_grad():
+    A.hip_flash_packed(leaf, k, v, o, scale=1e-31)
+  y = A.hip_flash_packed(leaf, k, v, o, scale=1e-30)
+  assert bool(torch.isfinite(torch.autograd.grad(y, leaf, g)[0]).all())
