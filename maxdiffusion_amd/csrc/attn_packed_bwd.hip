@@ -23,6 +23,7 @@
 #include <cmath>
 
 #include "attn_packed.h"
+#include "mdattn_host.h"
 
 namespace mdattn {
 namespace {
@@ -595,6 +596,14 @@ using namespace mdattn;
 
 extern "C" int64_t mdattn_bwd_bf16_packed_workspace_floats(const mdattn_packed* p) {
   return packed_sizes(p) == MDATTN_OK ? bwd_plan(p).floats : 0;
+}
+
+extern "C" int mdattn_host_packed_bwd_plan(const mdattn_packed* p, mdattn_host_packed_plan* plan) {
+  const int rc = packed_sizes(p);
+  if (rc != MDATTN_OK) return rc;
+  const BwdPlan b = bwd_plan(p);
+  *plan = {1, packed_order(p, b.tiles), b.pieces, b.piece_tiles, packed_tiles(p->k_rows, p->sequences, 128) * b.pieces * p->kv_heads};
+  return MDATTN_OK;
 }
 
 extern "C" int mdattn_bwd_bf16_packed(void* stream, const mdattn_packed* p, const void* q, const void* k, const void* v, const void* out,

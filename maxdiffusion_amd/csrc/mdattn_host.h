@@ -68,14 +68,15 @@ int mdattn_host_bwd_bf16(void* stream, const void* q, const void* k, const void*
                          const mdattn_strides* o_strides, float scale, const float* key_bias, int64_t bias_stride, const int* tiles,
                          const mdattn_host_bwd_plan* plan);
 
-/* How mdattn_fwd_bf16_packed launches a call, given the workspace that it asks for: the waves that share the keys of their rows (1, 2 or 4),
- * the order of the tiles (0: as they come, 1: by their number, 2: by what they meet), the pieces of the keys and the keys of each, and the tiles with
- * their pieces, of all heads, that it works on at most. */
+/* How mdattn_fwd_bf16_packed, and the dk / dv pass of mdattn_bwd_bf16_packed, launch a call, given the workspace that it asks for: the waves that
+ * share the keys of their rows (1, 2 or 4), the order of the tiles (0: as they come, 1: by their number, 2: by what they meet), the pieces of the walks
+ * at most and the keys (tiles of 32 tokens) of each, and the tiles with their pieces, of all heads, that it works on at most. */
 typedef struct {
   int waves, order, pieces, each;
   int64_t items;
 } mdattn_host_packed_plan;
 int mdattn_host_packed_fwd_plan(const mdattn_packed* p, mdattn_host_packed_plan* plan);
+int mdattn_host_packed_bwd_plan(const mdattn_packed* p, mdattn_host_packed_plan* plan);
 
 /* The prologue and its backward with the rotary table in the layout the model made it in:
  *   PLANES    cos, sin f32 [S, D/2] (the layout of mdattn.h's entry points)
