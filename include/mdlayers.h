@@ -91,10 +91,11 @@ int mdattn_rms_norm_e4m3(void* stream, const void* x, int x_is_f32, const void* 
  * ds and dx are dense [groups, rows, C].  Deterministic.
  */
 int64_t mdattn_rms_norm_bwd_workspace_floats(int64_t groups, int64_t rows, int C);
-int mdattn_rms_norm_bwd(void* stream, const void* s, int s_is_f32, const void* residual, const void* g, int g_is_f32, const void* gs, void* ds, void* dx,
-                        const void* w, void* dw, void* db, int wb_is_f32, int64_t groups, int64_t rows, int C, int64_t s_stride_group,
-                        int64_t s_stride_row, int64_t r_stride_group, int64_t r_stride_row, int64_t g_stride_group, int64_t g_stride_row, int64_t gs_stride_group, int64_t gs_stride_row, int64_t wb_stride, float eps,
-                        float w_offset, float* workspace, int64_t workspace_floats);
+int mdattn_rms_norm_bwd(void* stream, const void* s, int s_is_f32, const void* residual, const void* g, int g_is_f32, const void* gs, void* ds,
+                        void* dx, const void* w, void* dw, void* db, int wb_is_f32, int64_t groups, int64_t rows, int C, int64_t s_stride_group,
+                        int64_t s_stride_row, int64_t r_stride_group, int64_t r_stride_row, int64_t g_stride_group, int64_t g_stride_row,
+                        int64_t gs_stride_group, int64_t gs_stride_row, int64_t wb_stride, float eps, float w_offset, float* workspace,
+                        int64_t workspace_floats);
 
 /*
  * Quantisation of x [R, C] to e4m3 with one power-of-two scale per block of block_rows x 128 (block_rows 1 or 128).  Over a block,

@@ -21,8 +21,10 @@ extern "C" {
  * int32 in device memory and are read by the kernels: a captured graph follows what they hold when it is replayed.  They
  * must not decrease; whatever they hold, no row outside the tensors is touched.  Rows of q in front of the first sequence and behind the last
  * belong to none.
- *   q_strides, k_strides, v_strides, o_strides   elements between tokens (.seq) and heads (.head); .batch unused; head dim contiguous
- *   max_q, max_k   hints, the longest sequence's rows: they choose how the work is cut, and nothing else depends on them
+ *   q_strides, k_strides, v_strides, o_strides   elements between tokens (.seq, below 2^23) and heads (.head, below 2^40; in the backward
+ *                  pass, of q and out, below 2^29 * kv_heads / heads), multiples of 8; .batch unused; head dim contiguous
+ *   max_q, max_k   hints, the longest sequence's rows: they choose how the work is cut, and nothing else depends on them.  Without them (0) a call
+ *                  is planned for one sequence of all rows: single tokens against several caches are then not cut over their keys.
  */
 typedef struct {
   const int* q_offsets;

@@ -227,7 +227,8 @@ struct RowStrides {
   int64_t row, head;
 };
 
-// A few rows' strides are added up in 32 bits; heads' are not, but for q and dout in the dk / dv pass (`group` heads of them).
+// A few rows' strides are added up in 32 bits; heads' are not.  group: heads of q and out in the backward pass, whose strides the interface limits in
+// sum (no count in the kernels needs it).
 inline bool packed_strides_ok(const mdattn_strides* s, int64_t group = 0) {
   return s && s->seq % 8 == 0 && s->head % 8 == 0 && s->seq >= 0 && s->head >= 0 && s->seq < (1 << 23) && s->head < (1ll << 40) &&
          group * s->head < (1 << 29);

@@ -12,9 +12,12 @@
 // Few tiles leave CUs idle: two waves then share the keys of 64 rows, or four waves those of 32 (a kernel of its own, that one token meets too).
 // Where a tile is all that a sequence has, its keys are cut into pieces besides; each leaves un-normalised f32 rows, joined by another kernel
 // in a fixed order.
-// Bound: by the matrix pipes and LDS alike with long sequences (16,384 tokens, 32 heads on 8, causal: 1,835 us, 1.20 PFLOP/s, pipes busy 71 % of the
-// cycles; a library's product of 8,192^3 reaches 1.16); by the keys' way from memory with one token (131,072 keys of 8 heads 104 us, 5.2 TB/s); by one
-// tile's chain of products and softmax in between (prompts of up to 512 tokens 17 us).
+// Roundings.  Logits, softmax and sums are f32; P goes into its product in bf16, 2^-9 of an element on average, because the matrix pipes take f32 at a
+// sixteenth of the rate, and in two parts of bf16 P V would be twice the work: out is off by 1.1 to 1.5 times what its own rounding makes.
+// Bound: by the matrix pipes and LDS alike with long sequences (16,384 tokens, 32 heads on 8, causal: 1,895 us, 1.16 PFLOP/s, pipes busy 71 % of the
+// cycles; a library's product of 8,192^3 reaches 1.16; other machines 1,811 to 1,885); head dim 64, where a product has half the softmax's work beside
+// it, 1,107 us, 0.99; by the keys' way from memory with one token (131,072 keys of 8 heads 101 us, 5.3 TB/s); by the longest walk of a tile, products and
+// softmax in turn (prompts of up to 512 tokens 17 us; 4 x 512 tokens against 5,000 to 16,384 keys by two waves 477 us, 0.71 PFLOP/s).
 #include <algorithm>
 
 #include "attn_packed.h"

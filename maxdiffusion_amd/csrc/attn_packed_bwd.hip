@@ -17,8 +17,8 @@
 // logits share, is off by 8.1, 6.3, 3.9 and 2.8e-3 of its size, with rest by 2.5, 2.5, 2.4 and 2.4 (its own rounding 1.7).  dS in two parts would
 // bring that to 1.7, for a third more matrix products.
 // Bound.  A tile costs LDS as many cycles as the matrix pipes: 1 KB of fragments read per product of 32 cycles and wave, 128 bytes a cycle with
-// four waves.  100 to 4,096 tokens x 8 sequences, 32 heads on 8, causal: dq 221 us (1.05 PFLOP/s, pipes busy 50 % of the cycles), dk / dv 337 us
-// (0.92, 41 %), the pieces' sums 22 us.
+// four waves.  100 to 4,096 tokens x 8 sequences, 32 heads on 8, causal: dq 229 us (1.01 PFLOP/s, pipes busy 50 % of the cycles), dk / dv 358 us
+// (0.86, 41 %), the pieces' sums 32 us; 8,192 tokens at head dim 64 385, 594 and 34 us (1.07 and 0.93 PFLOP/s).
 #include <algorithm>
 #include <cmath>
 

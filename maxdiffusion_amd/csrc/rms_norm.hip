@@ -10,7 +10,10 @@
 // take its place, one more read of a row.
 // Bound by memory where rows are many: 75,600 rows of 5,120 in bf16, with a residual, scale and shift, 540 us (3.1 GB at 5.7 TB/s, above a copy's
 // 4.9: streaming stores); into e4m3, 4,096 x 4,096, 22 us (5.4 TB/s).  Few or odd rows wait for a row's way through memory and its sum: one row
-// 3.2 us, 2,674 of 1,001 with an f32 residual 9.2 us (3.5 TB/s), their backward pass 14.8 us (2.9 TB/s) and 4.1 for the sums of dw and db.
+// 3.1 us, 2,674 of 1,001 with an f32 residual 8.9 us (3.6 TB/s), their backward pass 14.6 us (2.9 TB/s) and 3.9 for the sums of dw and db.
+// Backward in bf16: 75,600 rows of 5,120 551 us (5.6 TB/s), from x and the residual 654 (5.9); 4,096 x 4,096 27 and 30 us (5.0, 5.6), the sums 4.
+// Above 12,288 channels 1,024 threads have 128 registers each, and 50 to 328 values of theirs are spilled (124 to 320 bytes of scratch a lane; f32 rows of
+// 8,193 to 12,288 spill 8 to 24 bytes): 4,096 x 16,384 in bf16 196 us (2.7 TB/s; 12,288 5.3), from x and the residual 262, in f32 426 (2.5; 12,288 4.7).
 #include "norm_rows.h"
 
 namespace mdattn {
@@ -348,10 +351,11 @@ extern "C" int64_t mdattn_rms_norm_bwd_workspace_floats(int64_t groups, int64_t 
   return (apart > merged ? apart : merged) * 2 * C;
 }
 
-extern "C" int mdattn_rms_norm_bwd(void* stream, const void* s, int s_is_f32, const void* residual, const void* g, int g_is_f32, const void* gs, void* ds, void* dx,
-                                   const void* w, void* dw, void* db, int wb_is_f32, int64_t groups, int64_t rows, int C, int64_t s_stride_group,
-                                   int64_t s_stride_row, int64_t r_stride_group, int64_t r_stride_row, int64_t g_stride_group, int64_t g_stride_row, int64_t gs_stride_group, int64_t gs_stride_row,
-                                   int64_t wb_stride, float eps, float w_offset, float* workspace, int64_t workspace_floats) {
+extern "C" int mdattn_rms_norm_bwd(void* stream, const void* s, int s_is_f32, const void* residual, const void* g, int g_is_f32, const void* gs,
+                                   void* ds, void* dx, const void* w, void* dw, void* db, int wb_is_f32, int64_t groups, int64_t rows, int C,
+                                   int64_t s_stride_group, int64_t s_stride_row, int64_t r_stride_group, int64_t r_stride_row,
+                                   int64_t g_stride_group, int64_t g_stride_row, int64_t gs_stride_group, int64_t gs_stride_row, int64_t wb_stride,
+                                   float eps, float w_offset, float* workspace, int64_t workspace_floats) {
   if (!s || !g || !ds || !sizes_ok(groups, rows, C) || !(eps >= 0.f) || !(w_offset == w_offset) || (dw && !w)) return MDATTN_E_BADARG;
   if (C > kMaxC || (g_is_f32 && !s_is_f32) || (dx && g_is_f32) || (residual && s_is_f32)) return MDATTN_E_UNSUPPORTED;
   const bool sums = dw || db;

@@ -605,7 +605,7 @@ def finalize(o_run: torch.Tensor) -> torch.Tensor:
 # ------------------------------------------------------------------------------------------------ attention over packed sequences
 def _packed_rows(t: torch.Tensor, group: int = 0) -> torch.Tensor:
   """t [rows, heads, D] as the kernels walk it (whole 16-byte pieces; strides below 2^23 between rows), copied if it is not.  group: heads of q
-  or dout whose strides the backward pass adds up in 32 bits."""
+  or out whose strides the backward entry limits in sum."""
   row, head = _packed_strides(t)
   ok = (t.stride(2) == 1 or t.shape[2] == 1) and row % 8 == 0 and head % 8 == 0 and row < 1 << 23 and group * head < 1 << 29 and t.data_ptr() % 16 == 0
   return t if ok else t.clone(memory_format=torch.contiguous_format)
@@ -648,7 +648,8 @@ def flash_attention_packed(q, k, v, q_offsets, k_offsets=None, *, k_lengths=None
   q_offsets, k_offsets: int32 [B + 1] on the device, not decreasing: sequence i is the rows q_offsets[i] .. q_offsets[i + 1] of q and those of
   k_offsets (None: the same) of k and v.  k_lengths int32 [B]: only the first k_lengths[i] of them are keys (a cache with room).  causal: of a
   sequence with m queries and n keys, query i sees the keys up to i + n - m.  max_q, max_k: the longest sequence's queries and keys, if the
-  caller knows them; they choose how the work is cut and no result depends on them but for its roundings.
+  caller knows them; they choose how the work is cut and no result depends on them but for its roundings.  Without them a call is planned for one
+  sequence of all rows: 16 single tokens against caches of up to 4,096 keys, whose keys are cut only by the hints, take 49 us for 15.
 
   Returns out [Tq, H, D] and, if asked, lse f32 [H, Tq] (natural log) and what the rounding of out left (bf16, for the backward pass; rows of no
   sequence undefined).  Rows that see no key and rows of no sequence: 0 and -inf."""
