@@ -58,16 +58,17 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 // A leaf's node in the autograd graph belongs to the stream on which it was made and lives as long as any graph that leads to it.  A backward pass
-// captured on another stream would make that stream wait inside the capture, which ends the process: such a forward call is refused.
+// captured on another stream makes that stream wait inside the capture: a stream of a program's own joins it, the default stream cannot be captured,
+// and the failure ends the process.  A forward call that would lead there is refused.
 void no_older_graph(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts) {
     if (!t->defined() || !t->is_cuda() || !t->requires_grad() || t->grad_fn()) continue;
     const auto leaf = torch::autograd::impl::try_get_grad_accumulator(*t);
     const auto on = leaf ? leaf->stream() : std::nullopt;
-    if (!on || on->id() == c10::hip::getCurrentHIPStream(t->get_device()).id()) continue;
+    if (!on || on->id() != c10::hip::getDefaultHIPStream(t->get_device()).id()) continue;
     TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
-                "cannot capture a call that is to be differentiated: one of its inputs is still part of an autograd graph from another stream; drop the "
-                "outputs that hold that graph, or build it on the stream of the capture");
+                "cannot capture a call that is to be differentiated: one of its inputs is still part of an autograd graph from another stream, the default "
+                "stream, which a capture cannot wait for; drop the outputs that hold that graph, or build it on a stream of its own");
   }
 }
 // A node's plain values as one entry of its saved_data (an entry each, boxed, cost a small backward call a few us)
